@@ -17,9 +17,22 @@ VARIANT_NAMES = {v: k for k, v in VARIANTS.items()}
 DINO_DTYPE = {"float16": 1, "float32": 2, "bfloat16": 6}
 ACTIVATIONS = {"silu": 1, "fast_gelu": 2}
 DEQUANT_DTYPE = {"float32": 0, "float16": 1, "bfloat16": 2}
+KV_TYPE = {"int8": 1, "float8_e4m3fn": 2}
 
 _lib = None
 _binding = None
+
+
+class KvCache(ctypes.Structure):
+    """DinoB200KvCache (include/dinoml_b200_decoder.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("type", ctypes.c_int),
+                ("blocks", ctypes.c_int), ("kv_heads", ctypes.c_int), ("block_size", ctypes.c_int), ("head_dim", ctypes.c_int)]
+
+
+class KvBatch(ctypes.Structure):
+    """DinoB200KvBatch (include/dinoml_b200_decoder.h)."""
+    _fields_ = [("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("table_blocks", ctypes.c_int), ("lengths", ctypes.c_void_p),
+                ("starts", ctypes.c_void_p), ("sequences", ctypes.c_int), ("rows", ctypes.c_int)]
 
 
 def variant_code(variant) -> int:
@@ -81,6 +94,15 @@ def lib() -> ctypes.CDLL:
     L.dinoml_b200_peer_pull_ctr.restype = ci
     L.dinoml_b200_peer_enable_access.argtypes = [ci]
     L.dinoml_b200_peer_enable_access.restype = ci
+    cache, batch = ctypes.POINTER(KvCache), ctypes.POINTER(KvBatch)
+    L.dinoml_b200_kv_cache_write.argtypes = [cache, batch, vp, vp, ci, i64, i64, i64, i64, vp]
+    L.dinoml_b200_kv_cache_write.restype = ci
+    L.dinoml_b200_kv_cache_read.argtypes = [cache, batch, vp, vp, vp, ci, vp]
+    L.dinoml_b200_kv_cache_read.restype = ci
+    L.dinoml_b200_kv_cache_attention.argtypes = [cache, batch, vp, vp, ci, ci, i64, i64, cf, ci, vp]
+    L.dinoml_b200_kv_cache_attention.restype = ci
+    L.dinoml_b200_rms_norm.argtypes = [vp, vp, vp, vp, vp, ci, ci, ci, ci, cf, ci, vp]
+    L.dinoml_b200_rms_norm.restype = ci
     _lib = L
     return L
 

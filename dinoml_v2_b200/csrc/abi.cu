@@ -23,6 +23,7 @@ int stream_device_status();
 bool gemm_umma_supports(int qtype, int dtype, int m, int n, int k);
 size_t gemm_umma_workspace(int qtype, int dtype, int m, int n, int k);
 int umma_device_status();
+int kv_device_status();
 int peer_device_status();
 int peer_enable_access(int peer_device);
 struct PeerOut { void* ptr[8]; int count; int act; };   // layout of gemv_mma_common.cuh
@@ -231,10 +232,11 @@ size_t dinoml_b200_gguf_prealloc_scratch_bytes(void) { return gemm_umma_static_s
 
 int dinoml_b200_gguf_device_status(void) {
   if (cudaDeviceSynchronize() != cudaSuccess) return -1;
-  const int peer = peer_device_status();   // read all three so that all are cleared
+  const int peer = peer_device_status();   // read all four so that all are cleared
+  const int cache = kv_device_status();
   const int gemm = umma_device_status();
   const int gemv = stream_device_status();
-  return gemm != 0 ? gemm : gemv != 0 ? gemv : peer;
+  return gemm != 0 ? gemm : gemv != 0 ? gemv : peer != 0 ? peer : cache;
 }
 
 int dinoml_b200_gguf_gemv_rcr_scatter(const void* a, const void* b_quant, const void* bias, void* c, void* const* peer_c, int n_peers,

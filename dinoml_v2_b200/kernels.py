@@ -1,6 +1,9 @@
 """Tensor-level wrappers over the C-ABI kernels (torch is used for device memory and streams only)."""
 from __future__ import annotations
 
+import ctypes
+from typing import NamedTuple
+
 import torch
 
 from . import _native
@@ -177,6 +180,188 @@ def variant_supports(variant: str, qtype, dtype: str, m: int, n: int, k: int) ->
 def variant_configs(variant: str) -> int:
     """Number of tuning configurations of a variant family (valid: "family:1" .. "family:N")."""
     return int(_native.lib().dinoml_b200_gguf_variant_configs(_native.variant_code(variant) & 0xff))
+
+
+class KVCache(NamedTuple):
+    """A paged cache of keys and values in 8 bits: k, v [blocks, kv_heads, block_size, head_dim] (int8 or float8_e4m3fn), k_scale, v_scale [blocks, kv_heads]
+    (float32).  A stored value stands for q * scale of its block and head.  Any sequence of four such tensors is a cache to the calls below."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+
+_KV_DTYPE = {"int8": torch.int8, "float8_e4m3fn": torch.float8_e4m3fn}
+_KV_TYPE = {torch.int8: 1, torch.float8_e4m3fn: 2}
+_KV_BLOCK_SIZES, _KV_HEAD_DIMS = (16, 32, 64, 128), (64, 128, 256)
+
+
+def kv_cache(blocks: int, kv_heads: int, block_size: int, head_dim: int, dtype: str = "int8", device="cuda") -> KVCache:
+    """An empty cache of `blocks` blocks of `block_size` tokens (16, 32, 64 or 128), head_dim 64, 128 or 256, values in int8 or float8_e4m3fn.  Small blocks
+    have a scale of their own for fewer tokens, large ones are fewer copies and table entries."""
+    if dtype not in _KV_DTYPE:
+        raise ValueError(f"cache dtype must be one of {sorted(_KV_DTYPE)}, got {dtype!r}")
+    if block_size not in _KV_BLOCK_SIZES or head_dim not in _KV_HEAD_DIMS or blocks < 1 or kv_heads < 1:
+        raise ValueError(f"a cache has blocks of {_KV_BLOCK_SIZES} tokens and heads of {_KV_HEAD_DIMS} values, got {block_size} and {head_dim}")
+    shape = (blocks, kv_heads, block_size, head_dim)
+    k, v = (torch.zeros(shape, dtype=torch.uint8, device=device).view(_KV_DTYPE[dtype]) for _ in range(2))
+    return KVCache(k, v, *(torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2)))
+
+
+def _kv_struct(cache) -> _native.KvCache:
+    k, v, k_scale, v_scale = cache
+    for name, t in (("cache.k", k), ("cache.v", v), ("cache.k_scale", k_scale), ("cache.v_scale", v_scale)):
+        _require_cuda(t, name)
+        if t.device != k.device:
+            raise ValueError("the tensors of a cache must be on one device")
+    if k.dtype not in _KV_TYPE or k.dim() != 4 or v.dtype != k.dtype or v.shape != k.shape:
+        raise ValueError("cache.k and cache.v must be int8 or float8_e4m3fn [blocks, kv_heads, block_size, head_dim] of one shape")
+    if k.shape[2] not in _KV_BLOCK_SIZES or k.shape[3] not in _KV_HEAD_DIMS or k.shape[0] < 1 or k.shape[1] < 1:
+        raise ValueError(f"a cache has blocks of {_KV_BLOCK_SIZES} tokens and heads of {_KV_HEAD_DIMS} values, got {tuple(k.shape)}")
+    for t in (k_scale, v_scale):
+        if t.dtype != torch.float32 or t.shape != k.shape[:2]:
+            raise ValueError(f"cache scales must be float32 {tuple(k.shape[:2])}")
+    return _native.KvCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), _KV_TYPE[k.dtype], *k.shape)
+
+
+def _kv_ints(t: torch.Tensor, name: str, count: int, device) -> int:
+    _require_cuda(t, name)
+    if t.dtype != torch.int32 or t.shape != (count,) or t.device != device:
+        raise ValueError(f"{name} must be int32 [{count}] on the device of the cache")
+    return t.data_ptr()
+
+
+def _kv_batch(cache, block_table: torch.Tensor, lengths, starts, rows: int) -> _native.KvBatch:
+    device = cache[0].device
+    if not block_table.is_cuda or block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.device != device or block_table.shape[1] < 1 \
+            or block_table.stride(1) != 1 or (block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]):
+        raise ValueError("block_table must be int32 [sequences, blocks] on the device of the cache, its rows contiguous")
+    sequences = block_table.shape[0]
+    if starts is None and rows != sequences:
+        raise ValueError(f"without starts there is one row per sequence: {rows} rows, {sequences} sequences")
+    return _native.KvBatch(block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+                           None if lengths is None else _kv_ints(lengths, "lengths", sequences, device),
+                           None if starts is None else _kv_ints(starts, "starts", sequences + 1, device), sequences, rows)
+
+
+def _kv_rows(t: torch.Tensor, name: str, device, heads, head_dim: int) -> None:
+    if not t.is_cuda or t.device != device:
+        raise ValueError(f"{name} must be a CUDA tensor on the device of the cache")
+    if t.dim() != 3 or t.dtype not in _DTYPE_NAME or t.shape[2] != head_dim or (heads is not None and t.shape[1] != heads) or t.stride(2) != 1:
+        raise ValueError(f"{name} must be [rows, {heads or 'heads'}, {head_dim}] in {sorted(_TORCH_DTYPE)}, its last dimension contiguous")
+
+
+def kv_cache_write(cache, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor | None = None, *,
+                   stream=None):
+    """Quantizes new tokens into the cache, in place, and returns it.  k, v: [rows, kv_heads, head_dim], any row and head strides.  Rows are packed:
+    sequence b has rows starts[b] .. starts[b + 1] - 1 (None: one row each) and `lengths[b]` tokens, these among them; position p of it is in slot
+    p % block_size of block block_table[b, p // block_size].  A block's scale grows with its largest value; the tokens that are there already
+    are brought to it.  Idle slots of a batch have length 0.  A non-finite value makes its block and head read as NaN."""
+    struct = _kv_struct(cache)
+    device, heads, dim = cache[0].device, struct.kv_heads, struct.head_dim
+    _kv_rows(k, "k", device, heads, dim)
+    _kv_rows(v, "v", device, heads, dim)
+    if v.dtype != k.dtype or v.shape != k.shape:
+        raise ValueError("k and v must have one shape and dtype")
+    batch = _kv_batch(cache, block_table, lengths, starts, k.shape[0])
+    if k.shape[0] and batch.sequences:
+        rc = _native.lib().dinoml_b200_kv_cache_write(
+            ctypes.byref(struct), ctypes.byref(batch), k.data_ptr(), v.data_ptr(), _native.DINO_DTYPE[_DTYPE_NAME[k.dtype]], k.stride(0), k.stride(1),
+            v.stride(0), v.stride(1), _stream_ptr(stream))
+        _native.check(rc, "dinoml_b200_kv_cache_write")
+    return cache
+
+
+def kv_cache_read(cache, block_table: torch.Tensor, starts: torch.Tensor | None, rows: int, dtype: str = "bfloat16", *, begins: torch.Tensor | None = None,
+                  out=None, stream=None):
+    """Dense (k, v), each [rows, kv_heads, head_dim]: row starts[b] + j is position begins[b] + j of sequence b (begins None: from the first token; starts
+    None: one row each).  `out`: two such tensors to fill."""
+    struct = _kv_struct(cache)
+    device, shape = cache[0].device, (int(rows), struct.kv_heads, struct.head_dim)
+    if dtype not in _TORCH_DTYPE:
+        raise ValueError(f"dtype must be one of {sorted(_TORCH_DTYPE)}, got {dtype!r}")
+    batch = _kv_batch(cache, block_table, None, starts, shape[0])
+    begins_ptr = None if begins is None else _kv_ints(begins, "begins", batch.sequences, device)
+    if out is None:
+        out = tuple(torch.empty(shape, dtype=_TORCH_DTYPE[dtype], device=device) for _ in range(2))
+    k, v = out
+    for t in (k, v):
+        _require_cuda(t, "out")
+        if t.shape != shape or t.dtype != _TORCH_DTYPE[dtype] or t.device != device:
+            raise ValueError(f"out must be two {dtype} tensors {shape} on the device of the cache")
+    if shape[0] and batch.sequences:
+        rc = _native.lib().dinoml_b200_kv_cache_read(ctypes.byref(struct), ctypes.byref(batch), begins_ptr, k.data_ptr(), v.data_ptr(),
+                                                     _native.DINO_DTYPE[dtype], _stream_ptr(stream))
+        _native.check(rc, "dinoml_b200_kv_cache_read")
+    return k, v
+
+
+def kv_cache_attention(q: torch.Tensor, cache, block_table: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor | None = None, *, scale: float | None = None,
+                       window: int = 0, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """softmax(scale * q K^T) V over the cache, causal: a row at position p of its sequence sees positions max(0, p - window + 1) .. p (window 0: all up to p).
+    q [rows, heads, head_dim], any row and head strides; heads is a multiple of kv_heads, head h reads cached head h // (heads // kv_heads); rows, lengths and
+    starts as for `kv_cache_write`, whose tokens have to be in the cache.  scale None: head_dim ** -0.5.  A row that sees nothing is zero."""
+    struct = _kv_struct(cache)
+    device = cache[0].device
+    _kv_rows(q, "q", device, None, struct.head_dim)
+    if q.shape[1] < 1 or q.shape[1] % struct.kv_heads:
+        raise ValueError(f"q has {q.shape[1]} heads: a multiple of the cache's {struct.kv_heads} is wanted")
+    if window < 0 or window > 0x7fffffff:
+        raise ValueError("window must not be negative (0: none)")
+    batch = _kv_batch(cache, block_table, lengths, starts, q.shape[0])
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    _require_cuda(out, "out")
+    if out.shape != q.shape or out.dtype != q.dtype or out.device != device:
+        raise ValueError("out must have the shape and dtype of q")
+    if q.shape[0] and batch.sequences:
+        rc = _native.lib().dinoml_b200_kv_cache_attention(
+            ctypes.byref(struct), ctypes.byref(batch), q.data_ptr(), out.data_ptr(), _native.DINO_DTYPE[_DTYPE_NAME[q.dtype]], q.shape[1], q.stride(0),
+            q.stride(1), struct.head_dim ** -0.5 if scale is None else float(scale), int(window), _stream_ptr(stream))
+        _native.check(rc, "dinoml_b200_kv_cache_attention")
+    return out
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, residual: torch.Tensor | None = None, q8_0: bool = False,
+             out: torch.Tensor | None = None, total: torch.Tensor | None = None, stream=None):
+    """(y, total): total = x + residual, y = total / sqrt(mean(total^2) + eps) * weight over the last dimension, in float32 with one rounding at the end.
+    weight [width] is float32 (as GGUF files hold it) or of x's dtype.  Without a residual total is None.  q8_0: y is uint8 [rows, width / 32 * 34], GGUF Q8_0
+    blocks (`dequantize_rows` reads them).  `total` may be `residual` or x: the sum is then written in place."""
+    _require_cuda(x, "x")
+    _require_cuda(weight, "weight")
+    if x.dtype not in _DTYPE_NAME or x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x must be [..., width] in {sorted(_TORCH_DTYPE)}")
+    width = x.shape[-1]
+    rows = x.numel() // width
+    if weight.shape != (width,) or weight.dtype not in (torch.float32, x.dtype) or weight.device != x.device:
+        raise ValueError(f"weight must be [{width}] in float32 or the dtype of x, on its device")
+    if residual is not None:
+        _require_cuda(residual, "residual")
+        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
+            raise ValueError("residual must have the shape and dtype of x")
+        if total is None:
+            total = torch.empty_like(x)
+    elif total is not None:
+        raise ValueError("total is the sum with a residual: none is given")
+    if total is not None:
+        _require_cuda(total, "total")
+        if total.shape != x.shape or total.dtype != x.dtype or total.device != x.device:
+            raise ValueError("total must have the shape and dtype of x")
+    if q8_0 and width % 32:
+        raise ValueError(f"Q8_0 blocks hold 32 values: width {width} is no multiple")
+    shape, dtype = ((rows, width // 32 * 34), torch.uint8) if q8_0 else (x.shape, x.dtype)
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=x.device)
+    _require_cuda(out, "out")
+    if out.shape != shape or out.dtype != dtype or out.device != x.device:
+        raise ValueError(f"out must be {dtype} {tuple(shape)}")
+    if rows:
+        rc = _native.lib().dinoml_b200_rms_norm(
+            x.data_ptr(), residual.data_ptr() if residual is not None else None, weight.data_ptr(), out.data_ptr(),
+            total.data_ptr() if total is not None else None, _native.DINO_DTYPE[_DTYPE_NAME[x.dtype]], _native.DINO_DTYPE[_DTYPE_NAME[weight.dtype]], rows, width,
+            float(eps), int(q8_0), _stream_ptr(stream))
+        _native.check(rc, "dinoml_b200_rms_norm")
+    return out, total
 
 
 def device_status() -> int:
