@@ -19,6 +19,7 @@
 #include <memory>
 #include <vector>
 
+#include "../../include/dinoml_b200_decoder.h"
 #include "../../include/dinoml_b200_gguf.h"
 #include "../../include/dinoml_b200_runtime.h"
 
@@ -188,6 +189,192 @@ PyObject* py_dequantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
+// ---- the operators between the linears.  A cache is a tuple of four tensors; the checks are those of kernels.py.
+bool kv_cache_of(PyObject* o, DinoB200KvCache* out, const at::Tensor** first) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return false;
+  const at::Tensor* t[4];
+  for (int i = 0; i < 4; ++i) {
+    t[i] = cuda_tensor(PyTuple_GET_ITEM(o, i));
+    if (t[i] == nullptr || t[i]->device() != t[0]->device()) return false;
+  }
+  const at::ScalarType type = t[0]->scalar_type();
+  if ((type != at::kChar && type != at::kFloat8_e4m3fn) || t[1]->scalar_type() != type || t[0]->dim() != 4 || t[1]->sizes() != t[0]->sizes()) return false;
+  for (int i = 2; i < 4; ++i)
+    if (t[i]->scalar_type() != at::kFloat || t[i]->sizes() != t[0]->sizes().slice(0, 2)) return false;
+  const auto size = t[0]->sizes();
+  for (int64_t n : size)
+    if (n < 1 || n > INT_MAX) return false;
+  if ((size[2] != 16 && size[2] != 32 && size[2] != 64 && size[2] != 128) || (size[3] != 64 && size[3] != 128 && size[3] != 256)) return false;
+  *out = {t[0]->data_ptr(), t[1]->data_ptr(), static_cast<float*>(t[2]->data_ptr()), static_cast<float*>(t[3]->data_ptr()),
+          type == at::kChar ? DINOML_B200_KV_INT8 : DINOML_B200_KV_E4M3, int(size[0]), int(size[1]), int(size[2]), int(size[3])};
+  *first = t[0];
+  return true;
+}
+
+bool kv_ints(PyObject* o, int64_t count, const at::Tensor& like, const int** out) {
+  const at::Tensor* t = cuda_tensor(o);
+  if (t == nullptr || t->scalar_type() != at::kInt || t->dim() != 1 || t->size(0) != count || t->device() != like.device()) return false;
+  *out = static_cast<const int*>(t->const_data_ptr());
+  return true;
+}
+
+// lengths: null if the call has none.
+bool kv_batch_of(PyObject* table, PyObject* lengths, PyObject* starts, int64_t rows, const at::Tensor& like, DinoB200KvBatch* out) {
+  if (!THPVariable_Check(table)) return false;
+  const at::Tensor& t = THPVariable_Unpack(table);
+  if (!t.defined() || t.layout() != at::kStrided || t.scalar_type() != at::kInt || t.dim() != 2 || t.device() != like.device() || t.size(0) < 1 || t.size(1) < 1 ||
+      t.size(0) > INT_MAX || t.size(1) > INT_MAX || t.stride(1) != 1 || (t.size(0) > 1 && t.stride(0) < t.size(1)) || rows < 1 || rows > INT_MAX)
+    return false;
+  *out = {static_cast<const int*>(t.const_data_ptr()), t.stride(0), int(t.size(1)), nullptr, nullptr, int(t.size(0)), int(rows)};
+  if (lengths != nullptr && !kv_ints(lengths, t.size(0), like, &out->lengths)) return false;
+  if (starts == Py_None) return rows == t.size(0);
+  return kv_ints(starts, t.size(0) + 1, like, &out->starts);
+}
+
+// [rows, heads, head_dim] with any row and head strides, or null.
+const at::Tensor* kv_rows(PyObject* o, const at::Tensor& like, int head_dim) {
+  if (!THPVariable_Check(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  return t.defined() && t.device() == like.device() && t.layout() == at::kStrided && t.dim() == 3 && t.size(0) >= 1 && t.size(1) >= 1 && t.size(2) == head_dim &&
+                 t.stride(2) == 1 && dino_dtype(t.scalar_type()) != 0
+             ? &t
+             : nullptr;
+}
+
+// kv_write(cache, k, v, block_table, lengths, starts, stream) -> cache
+PyObject* py_kv_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 7) { PyErr_SetString(PyExc_TypeError, "kv_write takes 7 arguments"); return nullptr; }
+  return guarded([&]() -> PyObject* {
+    DinoB200KvCache cache;
+    DinoB200KvBatch batch;
+    const at::Tensor* like = nullptr;
+    void* stream = nullptr;
+    if (!kv_cache_of(args[0], &cache, &like)) Py_RETURN_NONE;
+    const at::Tensor *k = kv_rows(args[1], *like, cache.head_dim), *v = kv_rows(args[2], *like, cache.head_dim);
+    if (k == nullptr || v == nullptr || k->size(1) != cache.kv_heads || v->sizes() != k->sizes() || v->scalar_type() != k->scalar_type()) Py_RETURN_NONE;
+    if (!kv_batch_of(args[3], args[4], args[5], k->size(0), *like, &batch) || !stream_of(args[6], &stream)) Py_RETURN_NONE;
+    const int dtype = dino_dtype(k->scalar_type());
+    const void *kp = k->const_data_ptr(), *vp = v->const_data_ptr();
+    const int64_t strides[4] = {k->stride(0), k->stride(1), v->stride(0), v->stride(1)};
+    int rc = 0;
+    Py_BEGIN_ALLOW_THREADS
+    rc = dinoml_b200_kv_cache_write(&cache, &batch, kp, vp, dtype, strides[0], strides[1], strides[2], strides[3], stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) return PyLong_FromLong(rc);
+    Py_INCREF(args[0]);
+    return args[0];
+  });
+}
+
+// kv_read(cache, block_table, starts, rows, dtype name, begins, stream) -> (k, v), new tensors
+PyObject* py_kv_read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 7) { PyErr_SetString(PyExc_TypeError, "kv_read takes 7 arguments"); return nullptr; }
+  return guarded([&]() -> PyObject* {
+    DinoB200KvCache cache;
+    DinoB200KvBatch batch;
+    const at::Tensor* like = nullptr;
+    const int* begins = nullptr;
+    void* stream = nullptr;
+    if (!kv_cache_of(args[0], &cache, &like) || !PyLong_CheckExact(args[3]) || !PyUnicode_Check(args[4])) Py_RETURN_NONE;
+    const int64_t rows = PyLong_AsLongLong(args[3]);
+    if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+    at::ScalarType type = at::kFloat;
+    if (PyUnicode_CompareWithASCIIString(args[4], "bfloat16") == 0) type = at::kBFloat16;
+    else if (PyUnicode_CompareWithASCIIString(args[4], "float16") == 0) type = at::kHalf;
+    else if (PyUnicode_CompareWithASCIIString(args[4], "float32") != 0) Py_RETURN_NONE;
+    if (!kv_batch_of(args[1], nullptr, args[2], rows, *like, &batch) || !stream_of(args[6], &stream)) Py_RETURN_NONE;
+    if (args[5] != Py_None && !kv_ints(args[5], batch.sequences, *like, &begins)) Py_RETURN_NONE;
+    const auto options = like->options().dtype(type);
+    const at::Tensor k = at::empty({rows, cache.kv_heads, cache.head_dim}, options), v = at::empty({rows, cache.kv_heads, cache.head_dim}, options);
+    void *kp = k.mutable_data_ptr(), *vp = v.mutable_data_ptr();
+    int rc = 0;
+    Py_BEGIN_ALLOW_THREADS
+    rc = dinoml_b200_kv_cache_read(&cache, &batch, begins, kp, vp, dino_dtype(type), stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) return PyLong_FromLong(rc);
+    PyObject *pk = THPVariable_Wrap(k), *pv = THPVariable_Wrap(v), *both = pk != nullptr && pv != nullptr ? PyTuple_Pack(2, pk, pv) : nullptr;
+    Py_XDECREF(pk);
+    Py_XDECREF(pv);
+    return both;
+  });
+}
+
+// kv_attention(q, cache, block_table, lengths, starts, scale, window, out, stream) -> out
+PyObject* py_kv_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 9) { PyErr_SetString(PyExc_TypeError, "kv_attention takes 9 arguments"); return nullptr; }
+  return guarded([&]() -> PyObject* {
+    DinoB200KvCache cache;
+    DinoB200KvBatch batch;
+    const at::Tensor *like = nullptr, *given = nullptr;
+    void* stream = nullptr;
+    if (!kv_cache_of(args[1], &cache, &like)) Py_RETURN_NONE;
+    const at::Tensor* q = kv_rows(args[0], *like, cache.head_dim);
+    if (q == nullptr || q->size(1) % cache.kv_heads != 0 || q->size(1) > INT_MAX) Py_RETURN_NONE;
+    if (!kv_batch_of(args[2], args[3], args[4], q->size(0), *like, &batch) || !stream_of(args[8], &stream)) Py_RETURN_NONE;
+    double scale = 0.;
+    if (args[5] == Py_None) scale = cache.head_dim == 64 ? 0.125 : cache.head_dim == 256 ? 0.0625 : 0.08838834764831845;
+    else if (PyFloat_CheckExact(args[5])) scale = PyFloat_AS_DOUBLE(args[5]);
+    else Py_RETURN_NONE;
+    if (!PyLong_CheckExact(args[6])) Py_RETURN_NONE;
+    const long window = PyLong_AsLong(args[6]);
+    if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+    if (window < 0 || window > INT_MAX) Py_RETURN_NONE;
+    if (args[7] != Py_None) {
+      given = cuda_tensor(args[7]);
+      if (given == nullptr || given->sizes() != q->sizes() || given->scalar_type() != q->scalar_type() || given->device() != q->device()) Py_RETURN_NONE;
+    }
+    const at::Tensor made = given != nullptr ? at::Tensor() : at::empty(q->sizes(), q->options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+    const void* qp = q->const_data_ptr();
+    void* out = (given != nullptr ? *given : made).mutable_data_ptr();
+    const int dtype = dino_dtype(q->scalar_type()), heads = int(q->size(1));
+    const int64_t row_stride = q->stride(0), head_stride = q->stride(1);
+    int rc = 0;
+    Py_BEGIN_ALLOW_THREADS
+    rc = dinoml_b200_kv_cache_attention(&cache, &batch, qp, out, dtype, heads, row_stride, head_stride, float(scale), int(window), stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) return PyLong_FromLong(rc);
+    if (given != nullptr) { Py_INCREF(args[7]); return args[7]; }
+    return THPVariable_Wrap(made);
+  });
+}
+
+// rms_norm(x, weight, eps, residual, q8_0, stream) -> (y, total or None), new tensors
+PyObject* py_rms_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 6) { PyErr_SetString(PyExc_TypeError, "rms_norm takes 6 arguments"); return nullptr; }
+  return guarded([&]() -> PyObject* {
+    const at::Tensor *x = cuda_tensor(args[0]), *weight = cuda_tensor(args[1]), *residual = nullptr;
+    void* stream = nullptr;
+    if (x == nullptr || weight == nullptr || !PyFloat_CheckExact(args[2]) || !PyBool_Check(args[4]) || !stream_of(args[5], &stream)) Py_RETURN_NONE;
+    const int dtype = dino_dtype(x->scalar_type()), weight_dtype = dino_dtype(weight->scalar_type());
+    const bool q8_0 = args[4] == Py_True;
+    if (dtype == 0 || x->dim() < 1 || x->size(-1) < 1 || (weight_dtype != dtype && weight_dtype != DINO_DTYPE_FLOAT32)) Py_RETURN_NONE;
+    const int64_t width = x->size(-1), rows = x->numel() / width;
+    if (rows < 1 || rows > INT_MAX || width > INT_MAX || weight->dim() != 1 || weight->size(0) != width || weight->device() != x->device() || (q8_0 && width % 32)) Py_RETURN_NONE;
+    if (args[3] != Py_None) {
+      residual = cuda_tensor(args[3]);
+      if (residual == nullptr || residual->sizes() != x->sizes() || residual->scalar_type() != x->scalar_type() || residual->device() != x->device()) Py_RETURN_NONE;
+    }
+    const auto options = x->options().requires_grad(false);
+    const at::Tensor y = q8_0 ? at::empty({rows, width / 32 * 34}, options.dtype(at::kByte)) : at::empty(x->sizes(), options);
+    const at::Tensor total = residual != nullptr ? at::empty(x->sizes(), options) : at::Tensor();
+    const void *xp = x->const_data_ptr(), *wp = weight->const_data_ptr(), *rp = residual != nullptr ? residual->const_data_ptr() : nullptr;
+    void *yp = y.mutable_data_ptr(), *tp = residual != nullptr ? total.mutable_data_ptr() : nullptr;
+    const float eps = float(PyFloat_AS_DOUBLE(args[2]));
+    int rc = 0;
+    Py_BEGIN_ALLOW_THREADS
+    rc = dinoml_b200_rms_norm(xp, rp, wp, yp, tp, dtype, weight_dtype, int(rows), int(width), eps, q8_0 ? 1 : 0, stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) return PyLong_FromLong(rc);
+    PyObject* py = THPVariable_Wrap(y);
+    PyObject* pt = Py_None;
+    if (residual != nullptr) pt = THPVariable_Wrap(total); else Py_INCREF(pt);
+    PyObject* both = py != nullptr && pt != nullptr ? PyTuple_Pack(2, py, pt) : nullptr;
+    Py_XDECREF(py);
+    Py_XDECREF(pt);
+    return both;
+  });
+}
+
 // ---- sessions.  A Runner carries what Session.run_torch needs of the artifact: the names and dtypes of its inputs and outputs,
 // the output shapes as a walk over the nodes (a node's result is its input's shape with `columns` as the last dimension), and the
 // run entry of the library the artifact loaded (an artifact may carry its own copy).
@@ -326,6 +513,10 @@ PyMethodDef kMethods[] = {
     {"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear)), METH_FASTCALL, nullptr},
     {"gated", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_gated)), METH_FASTCALL, nullptr},
     {"dequantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_dequantize)), METH_FASTCALL, nullptr},
+    {"kv_write", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_kv_write)), METH_FASTCALL, nullptr},
+    {"kv_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_kv_read)), METH_FASTCALL, nullptr},
+    {"kv_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_kv_attention)), METH_FASTCALL, nullptr},
+    {"rms_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_rms_norm)), METH_FASTCALL, nullptr},
     {"make_runner", py_make_runner, METH_VARARGS, nullptr},
     {"run_torch", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_run_torch)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

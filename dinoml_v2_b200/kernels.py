@@ -257,6 +257,11 @@ def kv_cache_write(cache, k: torch.Tensor, v: torch.Tensor, block_table: torch.T
     sequence b has rows starts[b] .. starts[b + 1] - 1 (None: one row each) and `lengths[b]` tokens, these among them; position p of it is in slot
     p % block_size of block block_table[b, p // block_size].  A block's scale grows with its largest value; the tokens that are there already
     are brought to it.  Idle slots of a batch have length 0.  A non-finite value makes its block and head read as NaN."""
+    done = _native_call("kv_write")(cache, k, v, block_table, lengths, starts, stream)
+    if done is not None:                                                                  # None: not the plain case, checked below
+        if type(done) is int:
+            _native.check(done, "dinoml_b200_kv_cache_write")
+        return done
     struct = _kv_struct(cache)
     device, heads, dim = cache[0].device, struct.kv_heads, struct.head_dim
     _kv_rows(k, "k", device, heads, dim)
@@ -276,6 +281,11 @@ def kv_cache_read(cache, block_table: torch.Tensor, starts: torch.Tensor | None,
                   out=None, stream=None):
     """Dense (k, v), each [rows, kv_heads, head_dim]: row starts[b] + j is position begins[b] + j of sequence b (begins None: from the first token; starts
     None: one row each).  `out`: two such tensors to fill."""
+    done = _native_call("kv_read")(cache, block_table, starts, rows, dtype, begins, stream) if out is None else None
+    if done is not None:                                                                  # None: not the plain case, checked below
+        if type(done) is int:
+            _native.check(done, "dinoml_b200_kv_cache_read")
+        return done
     struct = _kv_struct(cache)
     device, shape = cache[0].device, (int(rows), struct.kv_heads, struct.head_dim)
     if dtype not in _TORCH_DTYPE:
@@ -301,6 +311,11 @@ def kv_cache_attention(q: torch.Tensor, cache, block_table: torch.Tensor, length
     """softmax(scale * q K^T) V over the cache, causal: a row at position p of its sequence sees positions max(0, p - window + 1) .. p (window 0: all up to p).
     q [rows, heads, head_dim], any row and head strides; heads is a multiple of kv_heads, head h reads cached head h // (heads // kv_heads); rows, lengths and
     starts as for `kv_cache_write`, whose tokens have to be in the cache.  scale None: head_dim ** -0.5.  A row that sees nothing is zero."""
+    done = _native_call("kv_attention")(q, cache, block_table, lengths, starts, scale, window, out, stream)
+    if done is not None:                                                                  # None: not the plain case, checked below
+        if type(done) is int:
+            _native.check(done, "dinoml_b200_kv_cache_attention")
+        return done
     struct = _kv_struct(cache)
     device = cache[0].device
     _kv_rows(q, "q", device, None, struct.head_dim)
@@ -327,6 +342,11 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, residu
     """(y, total): total = x + residual, y = total / sqrt(mean(total^2) + eps) * weight over the last dimension, in float32 with one rounding at the end.
     weight [width] is float32 (as GGUF files hold it) or of x's dtype.  Without a residual total is None.  q8_0: y is uint8 [rows, width / 32 * 34], GGUF Q8_0
     blocks (`dequantize_rows` reads them).  `total` may be `residual` or x: the sum is then written in place."""
+    done = _native_call("rms_norm")(x, weight, eps, residual, q8_0, stream) if out is None and total is None else None
+    if done is not None:                                                                  # None: not the plain case, checked below
+        if type(done) is int:
+            _native.check(done, "dinoml_b200_rms_norm")
+        return done
     _require_cuda(x, "x")
     _require_cuda(weight, "weight")
     if x.dtype not in _DTYPE_NAME or x.dim() < 1 or x.shape[-1] < 1:
