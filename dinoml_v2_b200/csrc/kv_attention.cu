@@ -44,6 +44,13 @@ float* attention_scratch(size_t floats, int ctas, cudaStream_t s, int** arrived)
   return set.partial;
 }
 
+void attention_reset() {
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess) return;
+  std::lock_guard<std::mutex> lock(g_sets.mutex);
+  g_sets.for_each(dev, [](AttnScratch& set) { set.empty(nullptr); });
+}
+
 int cache_attention(const DinoB200KvCache* cache, const DinoB200KvBatch* batch, const void* q, void* out, int dtype, int heads, int64_t q_row_stride,
                     int64_t q_head_stride, float scale, int window, cudaStream_t s) {
   AttnParams a = {};
@@ -68,7 +75,7 @@ int cache_attention(const DinoB200KvCache* cache, const DinoB200KvBatch* batch, 
   a.min_rows = 0;
   a.max_rows = INT32_MAX;
   const int64_t rows = (int64_t(a.p.rows) + a.p.sequences - 1) / a.p.sequences * a.group;
-  const int tiles = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  const int tiles = rows <= 8 ? 1 : 2;
   return cache->type == DINOML_B200_KV_INT8 ? attention_few_int8(a, tiles, s) : attention_few_e4m3(a, tiles, s);
 }
 

@@ -65,7 +65,7 @@ __device__ __forceinline__ int tiles_of(const Item& it, int log2) { return it.hi
 // item at an end of a range is finished by whoever of its CTAs comes last.
 struct Walk {
   int b, row_tile, head, tile;               // the next unit
-  int workers;
+  int workers, per, more;                    // units of a worker, and how many of `workers` parts of one more unit
   int64_t units, start;                      // of the launch; the first one of this CTA's range
   int64_t unit, stop;                        // number of the next unit, and the end of the range
   int64_t item_unit;                         // number of the item's first unit
@@ -91,8 +91,11 @@ struct Walk {
     }
     open(a, log2);
   }
-  __device__ __forceinline__ int64_t start_of(int worker) const { return int64_t(worker) * units / workers; }
-  __device__ __forceinline__ int owner(int64_t u) const { return int(((u + 1) * workers - 1) / units); }
+  __device__ __forceinline__ int64_t start_of(int worker) const { return int64_t(worker) * per + worker * more / workers; }      // worker * units / workers
+  __device__ __forceinline__ int owner(int64_t u) const {
+    if (units < int64_t(1) << 21) return int((uint32_t(u + 1) * uint32_t(workers) - 1u) / uint32_t(units));      // (at most 1024 workers)
+    return int(((u + 1) * workers - 1) / units);
+  }
 };
 
 // Block-wide: the range of this CTA and where it begins; at least `least` units for every worker.  NT threads; `shared`: 2 + NT / 32 words of 8 bytes.
@@ -123,7 +126,10 @@ __device__ __forceinline__ Walk walk_of(const AttnParams& a, int log2, int least
   }
   Walk k;
   k.units = total;
-  k.workers = int(max(int64_t(1), min(int64_t(gridDim.x), total / least)));
+  const bool small = total < int64_t(1) << 31;                      // 64-bit divisions are slow
+  k.workers = int(max(int64_t(1), min(int64_t(gridDim.x), small ? int64_t(uint32_t(total) / uint32_t(least)) : total / least)));
+  k.per = small ? int(uint32_t(total) / uint32_t(k.workers)) : int(total / k.workers);
+  k.more = int(total - int64_t(k.per) * k.workers);
   k.start = k.unit = k.start_of(min(int(blockIdx.x), k.workers));
   k.stop = k.start_of(min(int(blockIdx.x) + 1, k.workers));
   int64_t at = before + sum - mine;
@@ -149,31 +155,40 @@ __device__ __forceinline__ Walk walk_of(const AttnParams& a, int log2, int least
     ++k.row_tile;
     k.open(a, log2);
   }
-  k.head = int((k.unit - k.item_unit) / k.tiles);
+  k.head = k.unit - k.item_unit < int64_t(1) << 31 ? int(uint32_t(k.unit - k.item_unit) / uint32_t(k.tiles)) : int((k.unit - k.item_unit) / k.tiles);
   k.item_unit += int64_t(k.head) * k.tiles;
   k.tile = int(k.unit - k.item_unit);
   return k;
 }
 
-// Two bytes of a cached word as two float16: times 1 for int8, times 2^-8 for e4m3 (the exponent field is moved as it is; it keeps denormals, and
-// the type's NaN codes become 480 * 2^-8 - bytes behind a sequence's last token may be anything, and zero times anything has to be zero).
+// Two bytes of a cached word as two float16, exactly.
 template <int TYPE> struct Half2Of;
 template <> struct Half2Of<DINOML_B200_KV_INT8> {
-  static constexpr float kFactor = 1.f;
-  static __device__ __forceinline__ uint32_t word(uint32_t w) { return w ^ 0x80808080u; }          // value + 128, unsigned
-  template <int LO, int HI> static __device__ __forceinline__ uint32_t pair(uint32_t w) {          // 1024 + 128 + value, then the value: exact
+  static constexpr float kBias = 1152.f;                            // 1024 + value + 128 has the value + 128 in its last byte
+  template <bool BIASED, int LO, int HI> static __device__ __forceinline__ uint32_t pair(uint32_t w) {
     const uint32_t m = __byte_perm(w, 0x64646464u, 0x4040 | LO | (HI << 8));
+    if (BIASED) return m;
     const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&m), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t*>(&v);
   }
+  // bytes 0, 1 and 2, 3 (BIASED: + kBias); bytes 0, 2 and 1, 3
+  template <bool BIASED> static __device__ __forceinline__ void along(uint32_t w, uint32_t& a, uint32_t& b) {
+    w ^= 0x80808080u;
+    a = pair<BIASED, 0, 1>(w);
+    b = pair<BIASED, 2, 3>(w);
+  }
+  static __device__ __forceinline__ void across(uint32_t w, uint32_t& a, uint32_t& b) {
+    w ^= 0x80808080u;
+    a = pair<false, 0, 2>(w);
+    b = pair<false, 1, 3>(w);
+  }
 };
 template <> struct Half2Of<DINOML_B200_KV_E4M3> {
-  static constexpr float kFactor = 256.f;
-  static __device__ __forceinline__ uint32_t word(uint32_t w) { return w; }
-  template <int LO, int HI> static __device__ __forceinline__ uint32_t pair(uint32_t w) {
-    const uint32_t m = __byte_perm(w, 0u, 0x0404 | (LO << 4) | (HI << 12));
-    return ((m >> 1) & 0x3f803f80u) | (m & 0x80008000u);
+  static constexpr float kBias = 0.f;
+  template <bool> static __device__ __forceinline__ void along(uint32_t w, uint32_t& a, uint32_t& b) {
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}\n" : "=r"(a), "=r"(b) : "r"(w));
   }
+  static __device__ __forceinline__ void across(uint32_t w, uint32_t& a, uint32_t& b) { along<false>(__byte_perm(w, w, 0x3120), a, b); }
 };
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -184,6 +199,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
 
 int attention_few_int8(AttnParams& a, int tiles, cudaStream_t s);
 int attention_few_e4m3(AttnParams& a, int tiles, cudaStream_t s);
+void attention_reset();                      // counters of the current device, after a launch that gave up
 float* attention_scratch(size_t floats, int ctas, cudaStream_t s, int** arrived);
 
 }  // namespace kv

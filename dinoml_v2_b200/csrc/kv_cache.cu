@@ -1,8 +1,7 @@
 // Write and read of the 8-bit cache of keys and values (layout: kv_cache.cuh).
 #include <mutex>
 
-#include "gemv_mma_common.cuh"
-#include "kv_cache.cuh"
+#include "kv_attention.cuh"
 
 namespace b200gguf {
 namespace kv {
@@ -236,6 +235,7 @@ int kv_device_status() {
   int* p = kv::status_ptr();
   if (p == nullptr || cudaMemcpy(&value, p, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return 0;
   if (value != 0) cudaMemset(p, 0, sizeof(int));
+  if (value == kv::ST_KV_TIMEOUT) kv::attention_reset();
   return value;
 }
 
