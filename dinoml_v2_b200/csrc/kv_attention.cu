@@ -61,6 +61,7 @@ int cache_attention(const DinoB200KvCache* cache, const DinoB200KvBatch* batch, 
   if (dtype != DINO_F16 && dtype != DINO_BF16 && dtype != DINO_F32) return RC_DTYPE;
   if ((reinterpret_cast<uintptr_t>(q) & (dtype == DINO_F32 ? 3 : 1)) != 0 || (reinterpret_cast<uintptr_t>(out) & 15) != 0) return RC_ALIGN;
   a.group = heads / a.c.heads;
+  a.by_group.set(uint32_t(a.group));
   if ((int64_t(a.c.blocks) * a.c.heads) << a.c.block_log2 > INT32_MAX) return RC_RANGE;      // rows of the copies' coordinates
   if (int rc = batch_view(batch, true, &a.p)) return rc;
   if (int64_t(a.p.rows) * a.group > INT32_MAX) return RC_RANGE;

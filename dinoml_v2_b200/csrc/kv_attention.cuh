@@ -12,6 +12,19 @@ namespace kv {
 constexpr float kLog2e = 1.4426950408889634f;
 enum : int { ST_KV_TIMEOUT = 11 };          // device status: a copy of cache bytes never arrived
 
+// n / d for 0 <= n < 2^31: the quotient is (mulhi(n, m) + n) >> s with s = ceil(log2 d), m = floor(2^32 (2^s - d) / d) + 1 (Granlund and Montgomery).
+struct Divisor {
+  uint32_t m, s;
+  void set(uint32_t d) {
+    s = 0;
+    while ((uint64_t(1) << s) < d) ++s;
+    m = uint32_t((((uint64_t(1) << s) - d) << 32) / d) + 1u;
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ int operator()(int n) const { return int((__umulhi(uint32_t(n), m) + uint32_t(n)) >> s); }
+#endif
+};
+
 struct AttnParams {
   Cache c;
   Batch p;
@@ -20,7 +33,8 @@ struct AttnParams {
   int64_t row_stride, head_stride;           // of q, in elements
   float scale;                               // of the scores, times log2(e)
   int window, heads, group, dtype;
-  int row_tile;                              // rows (token x head of the group) of an item
+  Divisor by_group;
+  int row_tile, row_tile_log2;               // rows (token x head of the group) of an item
   int min_rows, max_rows;                    // sequences with fewer or more rows (tokens x group) are another launch's
   float* partial;                            // two cut pieces per CTA
   int* arrived;                              // a counter per CTA, zero between launches
@@ -50,13 +64,13 @@ __device__ __forceinline__ Item item_at(const AttnParams& a, const Sequence& s, 
   Item it;
   it.r0 = row_tile * a.row_tile;
   it.r1 = min(it.r0 + a.row_tile, s.count * a.group);
-  const int first = s.first + it.r0 / a.group, last = s.first + (it.r1 - 1) / a.group;
+  const int first = s.first + a.by_group(it.r0), last = s.first + a.by_group(it.r1 - 1);
   it.high = max(0, min(last + 1, s.end));
   it.low = a.window > 0 ? max(0, first - a.window + 1) : 0;
   if (it.low > it.high) it.low = it.high;
   return it;
 }
-__device__ __forceinline__ int row_tiles(const AttnParams& a, const Sequence& s) { return (s.count * a.group + a.row_tile - 1) / a.row_tile; }
+__device__ __forceinline__ int row_tiles(const AttnParams& a, const Sequence& s) { return (s.count * a.group + a.row_tile - 1) >> a.row_tile_log2; }
 // Tiles of `size` positions (a power of two) that an item covers; one that sees nothing still has its rows to write.
 __device__ __forceinline__ int tiles_of(const Item& it, int log2) { return it.high > it.low ? ((it.high - 1) >> log2) - (it.low >> log2) + 1 : 1; }
 

@@ -26,7 +26,7 @@ namespace b200gguf {
 namespace kv {
 namespace few {
 
-constexpr int kCtasPerSm = 2, kSegments = 8;
+constexpr int kCtasPerSm = 2, kSegments = 4;
 
 template <int D_, int NT_, int PARTS_> struct Shape {
   static constexpr int D = D_, NT = NT_, PARTS = PARTS_;
@@ -43,7 +43,7 @@ template <int D_, int NT_, int PARTS_> struct Shape {
   static constexpr int kQ = KS * NT * PARTS * 32 * 8;                      // q as operand fragments
   static constexpr int kMergeCh = D < 128 ? D : 128, kPitch = kMergeCh + 4;
   static constexpr int kMerge = W * 8 * kPitch * 4;                        // sums of 8 rows and kMergeCh channels of every warp
-  static constexpr int kFixed = 1024 + kMerge + 2 * kQ, kStatic = 1800 + W * R * 8 + 40 * R;
+  static constexpr int kFixed = 1024 + kMerge + 2 * kQ, kStatic = 2000 + W * R * 8 + 40 * R;
   static constexpr int kRoom = (113 * 1024 - kFixed - kStatic) / (2 * kHalf);
   static constexpr int kStages = kRoom < 10 ? kRoom : 10;
   static constexpr int kRing = kStages * 2 * kHalf;
@@ -154,11 +154,12 @@ template <class S> struct Shared {
   uint64_t described[kSegments], closed[kSegments];               // of a segment: the copying warp's account of it is there, is no longer needed
   uint64_t opened[2], written[2];                                 // of a segment: q is there, its results are written
   uint64_t together, merged;                                      // of the computing warps: their sums are there, have been read
+  uint64_t ended;                                                 // it is known which items this CTA joins
   float4 boxes[S::kStages][S::kTile / 16];     // of every 16 tokens: their block's scales of K and V, whether there is one
-  Segment segments[kSegments];
+  Segment segments[kSegments], to_join[2];
   Rows8<S> rows[2];
   int64_t walk[4 + S::W];
-  int lost;                                    // a wait gave up
+  int joins, lost;                             // items to join; a wait gave up
   float2 ml[S::W][S::R];                       // every warp's maxima and sums
 };
 
@@ -265,95 +266,86 @@ __device__ __forceinline__ void copy_tiles(const AttnParams& a, Shared<S>& sh, c
   }
 }
 
-// ---- the opening warp.  Rows of an item: q as operand fragments, what their scores are multiplied by, what they see.
+// ---- the opening warp.  Rows of an item: q as operand fragments, what their scores are multiplied by, what they see.  Lane (g, t) has the fragments of
+// row g, 16 t .. 16 t + 15 of every 64 values, so it reads them, and eight rows are made at once.
 template <int TYPE, class S> __device__ __forceinline__ void open_rows(const AttnParams& a, Rows8<S>& out, const Segment& sg, uint2* qfrag) {
   using H = Half2Of<TYPE>;
-  constexpr int D = S::D, NT = S::NT, PARTS = S::PARTS, kSteps = (D + 127) / 128, kAtOnce = kSteps == 1 ? 4 : 2;
-  const int lane = threadIdx.x & 31, rows = sg.item.r1 - sg.item.r0;
+  constexpr int D = S::D, NT = S::NT, PARTS = S::PARTS;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, rows = sg.item.r1 - sg.item.r0;
   const int size = a.dtype == DINO_F32 ? 4 : 2;
   const bool wide = ((reinterpret_cast<uintptr_t>(a.q) | uint64_t(a.row_stride * size) | uint64_t(a.head_stride * size)) & uint64_t(4 * size - 1)) == 0;
-  float my_down = 0.f, my_total = 0.f;                                  // of row `lane`
-  for (int r0 = 0; r0 < rows; r0 += kAtOnce) {                          // (rows that the item has not stay zeros, or what an item before had there)
-    float x[kAtOnce][kSteps][4];
+  for (int n = 0; n < NT; ++n) {
+    const int r = 8 * n + g, token = a.by_group(sg.item.r0 + r), head = sg.head * a.group + (sg.item.r0 + r) - token * a.group;
+    const int64_t at = int64_t(sg.s.row + token) * a.row_stride + int64_t(head) * a.head_stride + 16 * t;
+    float x[D / 16][4];
+    uint32_t largest = 0;
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      const int r = r0 + k, token = (sg.item.r0 + r) / a.group, head = sg.head * a.group + (sg.item.r0 + r) - token * a.group;
-      const int64_t at = int64_t(sg.s.row + token) * a.row_stride + int64_t(head) * a.head_stride;
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const int e = 128 * i + 4 * lane;
-        if (r < rows && e < D) load_q4(a, at + e, wide, x[k][i]);
-        else x[k][i][0] = x[k][i][1] = x[k][i][2] = x[k][i][3] = 0.f;
-      }
+    for (int i = 0; i < D / 16; ++i) {
+      if (r < rows) load_q4(a, at + 64 * (i / 4) + 4 * (i % 4), wide, x[i]);
+      else x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
     }
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      const int r = r0 + k;
-      uint32_t largest = 0;
+    for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i)
+      for (int j = 0; j < 4; ++j) largest = max(largest, __float_as_uint(x[i][j]) & 0x7fffffffu);
+    largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+    largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+    // 2^12 <= |largest| up < 2^13; zeros, denormals, infinities and NaN as they are
+    const uint32_t e = largest >> 23;
+    const bool plain = e == 0 || e == 255;
+    const int shift = plain ? 0 : min(max(127 + 12 - int(e), -126), 126);
+    const float up = __uint_as_float(uint32_t(127 + shift) << 23), down = __uint_as_float(uint32_t(127 - shift) << 23);
+    float total = 0.f;                                                  // of the row's first terms
 #pragma unroll
-        for (int j = 0; j < 4; ++j) largest = max(largest, __float_as_uint(x[k][i][j]) & 0x7fffffffu);
-      largest = __reduce_max_sync(0xffffffffu, largest);
-      // 2^12 <= |largest| up < 2^13; zeros, denormals, infinities and NaN as they are
-      const uint32_t e = largest >> 23;
-      const bool plain = e == 0 || e == 255;
-      const int shift = plain ? 0 : min(max(127 + 12 - int(e), -126), 126);
-      const float up = __uint_as_float(uint32_t(127 + shift) << 23), down = __uint_as_float(uint32_t(127 - shift) << 23);
-      float total = 0.f;                                                // of the row's first terms
+    for (int i = 0; i < D / 16; ++i) {
+      float v[4];
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const int e0 = 128 * i + 4 * lane;
-        if (e0 < D) {
-          const int ks = (e0 / 64) * 4 + (e0 % 16) / 4, tt = (e0 % 64) / 16;
-          float v[4];
+      for (int j = 0; j < 4; ++j) v[j] = x[i][j] * up;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = x[k][i][j] * up;
-#pragma unroll
-          for (int part = 0; part < PARTS; ++part) {
-            const uint32_t lo = pack_half(v[0], v[1]), hi = pack_half(v[2], v[3]);
-            qfrag[((ks * NT + (r >> 3)) * PARTS + part) * 32 + (r & 7) * 4 + tt] = make_uint2(lo, hi);
-            const float2 l = __half22float2(*reinterpret_cast<const __half2*>(&lo)), h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-            if (part == 0) total += (l.x + l.y) + (h.x + h.y);
-            v[0] -= l.x; v[1] -= l.y; v[2] -= h.x; v[3] -= h.y;
-          }
-        }
+      for (int part = 0; part < PARTS; ++part) {
+        const uint32_t lo = pack_half(v[0], v[1]), hi = pack_half(v[2], v[3]);
+        qfrag[((i * NT + n) * PARTS + part) * 32 + lane] = make_uint2(lo, hi);
+        const float2 l = __half22float2(*reinterpret_cast<const __half2*>(&lo)), h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        if (part == 0) total += (l.x + l.y) + (h.x + h.y);
+        v[0] -= l.x; v[1] -= l.y; v[2] -= h.x; v[3] -= h.y;
       }
-      if (H::kBias != 0.f && PARTS == 1) {
-#pragma unroll
-        for (int i = 16; i > 0; i >>= 1) total += __shfl_xor_sync(0xffffffffu, total, i);
-      }
-      if (lane == r) { my_down = down; my_total = total; }
     }
-  }
-  if (lane < S::R) {
-    const int position = sg.s.first + (sg.item.r0 + lane) / a.group;
-    out.bias[lane] = -H::kBias * my_total;
-    out.factor[lane] = a.scale * my_down;
-    out.high[lane] = lane < rows ? min(position + 1, sg.s.end) : 0;
-    out.low[lane] = a.window > 0 ? max(0, position - a.window + 1) : 0;
+    total += __shfl_xor_sync(0xffffffffu, total, 1);
+    total += __shfl_xor_sync(0xffffffffu, total, 2);
+    if (t == 0) {
+      const int position = sg.s.first + token;
+      out.bias[r] = H::kBias != 0.f ? -H::kBias * total : 0.f;
+      out.factor[r] = a.scale * down;
+      out.high[r] = r < rows ? min(position + 1, sg.s.end) : 0;
+      out.low[r] = a.window > 0 ? max(0, position - a.window + 1) : 0;
+    }
   }
 }
 
 // Channels d .. d + 3 of row r.
 __device__ __forceinline__ void finish(const AttnParams& a, const Segment& sg, int dim, int r, int d, float4 v, float sum) {
   const float f = sum == 0.f ? 0.f : 1.f / sum;
-  const int token = (sg.item.r0 + r) / a.group, head = sg.head * a.group + (sg.item.r0 + r) - token * a.group;
+  const int token = a.by_group(sg.item.r0 + r), head = sg.head * a.group + (sg.item.r0 + r) - token * a.group;
   store4(a, (int64_t(sg.s.row + token) * a.heads + head) * dim + d, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
 }
 
 // A cut item, whose piece of this CTA is written: pieces are those of workers c0 .. c1, and the one that arrives last adds them up, in order.  The counter is
 // that of c0, whose range is the only one that this item leaves at its end.
-template <class S> __device__ __forceinline__ void join_pieces(const AttnParams& a, const Segment& sg) {
-  constexpr int D = S::D, kPiece = S::R * (D + 2);
-  const int count = sg.c1 - sg.c0 + 1, rows = sg.item.r1 - sg.item.r0, lane = threadIdx.x & 31;
+__device__ __forceinline__ bool arrives_last(const AttnParams& a, const Segment& sg) {
+  const int lane = threadIdx.x & 31;
   int before = 0;
   if (lane == 0) asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;\n" : "=r"(before) : "l"(a.arrived + sg.c0) : "memory");
-  if (__shfl_sync(0xffffffffu, before, 0) != count - 1) return;
-  if (lane == 0) a.arrived[sg.c0] = 0;
+  const bool last = __shfl_sync(0xffffffffu, before, 0) == sg.c1 - sg.c0;
+  if (last && lane == 0) a.arrived[sg.c0] = 0;
   __syncwarp();                                                         // all lanes behind the first one's acquire
-  constexpr int U = 4, P = 4;                                           // places and pieces under way at a time
-  for (int i0 = lane; i0 < rows * (D / 4); i0 += 32 * U) {
+  return last;
+}
+// By threads `from`, `from + step` and so on.
+template <class S> __device__ __forceinline__ void join_pieces(const AttnParams& a, const Segment& sg, int from, int step) {
+  constexpr int D = S::D, kPiece = S::R * (D + 2);
+  const int count = sg.c1 - sg.c0 + 1, rows = sg.item.r1 - sg.item.r0;
+  constexpr int U = 2, P = 8;                                           // places and pieces under way at a time
+  for (int i0 = from; i0 < rows * (D / 4); i0 += step * U) {
     float top[U], sum[U];
     float4 v[U];
 #pragma unroll
@@ -367,7 +359,7 @@ template <class S> __device__ __forceinline__ void join_pieces(const AttnParams&
       float4 y[U][P];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int i = i0 + 32 * u, r = i / (D / 4), d = i % (D / 4) * 4;
+        const int i = i0 + step * u, r = i / (D / 4), d = i % (D / 4) * 4;
 #pragma unroll
         for (int x = 0; x < P; ++x)
           if (r < rows && c + x < count) {
@@ -398,42 +390,54 @@ template <class S> __device__ __forceinline__ void join_pieces(const AttnParams&
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = i0 + 32 * u, r = i / (D / 4), d = i % (D / 4) * 4;
+      const int i = i0 + step * u, r = i / (D / 4), d = i % (D / 4) * 4;
       if (r < rows) finish(a, sg, D, r, d, v[u], sum[u]);
     }
   }
 }
 
-template <class S> __device__ __forceinline__ void close_segment(const AttnParams& a, Shared<S>& sh, int segment) {
+constexpr int kFewPieces = 4;
+
+// The items that a CTA joins are left to its end, where all warps do it, but for those of few pieces, which this warp does beside the others' work.
+template <class S> __device__ __forceinline__ void close_segment(const AttnParams& a, Shared<S>& sh, int segment, bool at_end) {
+  const int lane = threadIdx.x & 31;
   const Segment& sg = sh.segments[segment & (kSegments - 1)];
-  if (sg.piece >= 0) join_pieces<S>(a, sg);
+  if (sg.piece >= 0 && arrives_last(a, sg)) {
+    if (at_end || sg.c1 - sg.c0 >= kFewPieces) {
+      if (lane == 0) sh.to_join[sh.joins++] = sg;                       // (a CTA has two cut items at most)
+    } else {
+      join_pieces<S>(a, sg, lane, 32);
+    }
+  }
   __syncwarp();
-  if ((threadIdx.x & 31) == 0) umma::mbar_arrive(umma::smem_u32(&sh.closed[segment & (kSegments - 1)]));
+  if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.closed[segment & (kSegments - 1)]));
+}
+template <class S> __device__ __forceinline__ void join_at_end(const AttnParams& a, Shared<S>& sh, int from) {
+  for (int i = 0; i < sh.joins; ++i) join_pieces<S>(a, sh.to_join[i], from, (S::W + 1) * 32);
 }
 
 template <int TYPE, class S>
 __device__ __forceinline__ void open_and_close(const AttnParams& a, Shared<S>& sh, uint2* qfrag) {
   const int lane = threadIdx.x & 31;
-  int left = -1;                                                        // a segment that is written and not yet joined
   for (int segment = 0;; ++segment) {
     const int slot = segment & (kSegments - 1);
     if (!warp_wait(a, sh, &sh.described[slot], uint32_t(segment / kSegments) & 1u)) return;
     const bool done = sh.segments[slot].tile0 == sh.segments[slot].tile1;
-    if (segment >= 2) {                                                 // its place is that of the one before the last
-      if (!warp_wait(a, sh, &sh.written[segment & 1], uint32_t((segment - 2) >> 1) & 1u)) return;
-      left = segment - 2;
-    }
+    if (segment >= 2 && !warp_wait(a, sh, &sh.written[segment & 1], uint32_t((segment - 2) >> 1) & 1u)) return;      // its place is free
     if (!done) open_rows<TYPE, S>(a, sh.rows[segment & 1], sh.segments[slot], qfrag + (segment & 1) * (S::kQ / 8));
     __syncwarp();
     if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.opened[segment & 1]));
-    if (done && segment >= 1) {                                         // the last two
-      if (left >= 0) close_segment<S>(a, sh, left);
-      if (!warp_wait(a, sh, &sh.written[(segment - 1) & 1], uint32_t((segment - 1) >> 1) & 1u)) return;
-      left = segment - 1;
+    if (segment >= 2) close_segment(a, sh, segment - 2, done);
+    if (done) {
+      if (segment >= 1) {
+        if (!warp_wait(a, sh, &sh.written[(segment - 1) & 1], uint32_t((segment - 1) >> 1) & 1u)) return;
+        close_segment(a, sh, segment - 1, true);
+      }
+      __syncwarp();
+      if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.ended));
+      join_at_end(a, sh, S::W * 32 + lane);
+      return;
     }
-    if (left >= 0) close_segment<S>(a, sh, left);
-    left = -1;
-    if (done) return;
   }
 }
 
@@ -467,7 +471,8 @@ __global__ void __launch_bounds__(S::kThreads, kCtasPerSm) attention_few_kernel(
     }
     umma::mbar_init(umma::smem_u32(&sh.together), W);
     umma::mbar_init(umma::smem_u32(&sh.merged), W);
-    sh.lost = 0;
+    umma::mbar_init(umma::smem_u32(&sh.ended), 1);
+    sh.lost = sh.joins = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   for (int i = tid; i < 2 * S::kQ / 8; i += S::kThreads) qfrag[i] = make_uint2(0u, 0u);
@@ -493,12 +498,16 @@ __global__ void __launch_bounds__(S::kThreads, kCtasPerSm) attention_few_kernel(
     const Rows8<S>& of = sh.rows[segment & 1];
     const uint2* const qf = qfrag + (segment & 1) * (S::kQ / 8) + lane;
     const int tile0 = sg.tile0, tile1 = sg.tile1;
-    if (tile0 == tile1) return;
+    if (tile0 == tile1) {
+      if (!warp_wait(a, sh, &sh.ended, 0)) break;
+      join_at_end(a, sh, tid);
+      return;
+    }
     const int rows = sg.item.r1 - sg.item.r0;
     const int token_base = (sg.item.low >> S::kLog2) * S::kTile + (warp & 1) * TK, number = sg.number - tile0;
     // positions that every row sees: the first row ends first, the last one begins last
-    const int all_high = min(sg.s.first + sg.item.r0 / a.group + 1, sg.s.end);
-    const int all_low = a.window > 0 ? max(0, sg.s.first + (sg.item.r1 - 1) / a.group - a.window + 1) : 0;
+    const int all_high = min(sg.s.first + a.by_group(sg.item.r0) + 1, sg.s.end);
+    const int all_low = a.window > 0 ? max(0, sg.s.first + a.by_group(sg.item.r1 - 1) - a.window + 1) : 0;
     float factor[NT][2], begin[NT][2], m[NT][2], l[NT][2], o[S::DC][NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -793,6 +802,7 @@ inline bool cache_map(CUtensorMap* map, const void* data, const Cache& c, int to
 template <int TYPE, int D, int NT, int PARTS> int launch(AttnParams& a, cudaStream_t s) {
   using S = Shape<D, NT, PARTS>;
   a.row_tile = S::R;
+  a.row_tile_log2 = S::NT == 1 ? 3 : 4;
   const int tokens = S::kTile < (1 << a.c.block_log2) ? S::kTile : 1 << a.c.block_log2;
   CUtensorMap k_map, v_map;
   if (!cache_map(&k_map, a.c.data[0], a.c, tokens) || !cache_map(&v_map, a.c.data[1], a.c, tokens)) return RC_LAUNCH;
