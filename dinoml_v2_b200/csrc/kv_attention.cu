@@ -21,6 +21,7 @@ struct AttnScratch {
   static constexpr int kMaxWorkers = 1024;
 };
 static ScratchSets<AttnScratch> g_sets;
+constexpr int kFewRows = 64;
 
 // Allocates outside of stream capture only: callers run a shape once before capturing a graph.
 float* attention_scratch(size_t floats, int ctas, cudaStream_t s, int** arrived) {
@@ -73,11 +74,20 @@ int cache_attention(const DinoB200KvCache* cache, const DinoB200KvBatch* batch, 
   a.window = window;
   a.heads = heads;
   a.dtype = dtype;
+  // Sequences with few rows go to one kernel, those with many to the other; which there are only the device knows, so a call with rows enough is both.
+  const int64_t all_rows = int64_t(a.p.rows) * a.group, rows = (all_rows + a.p.sequences - 1) / a.p.sequences;
+  const bool tensor = dtype != DINO_F32 && a.c.dim != 256;
+  const int64_t most = a.p.starts == nullptr ? a.group : all_rows;          // rows of a sequence
   a.min_rows = 0;
-  a.max_rows = INT32_MAX;
-  const int64_t rows = (int64_t(a.p.rows) + a.p.sequences - 1) / a.p.sequences * a.group;
+  a.max_rows = tensor ? kFewRows : INT32_MAX;
   const int tiles = rows <= 8 ? 1 : 2;
-  return cache->type == DINOML_B200_KV_INT8 ? attention_few_int8(a, tiles, s) : attention_few_e4m3(a, tiles, s);
+  if (a.p.starts != nullptr || most <= a.max_rows) {
+    const int rc = cache->type == DINOML_B200_KV_INT8 ? attention_few_int8(a, tiles, s) : attention_few_e4m3(a, tiles, s);
+    if (rc != RC_OK || most <= a.max_rows) return rc;
+  }
+  a.min_rows = kFewRows + 1;
+  a.max_rows = INT32_MAX;
+  return attention_many(a, cache->type, s);
 }
 
 }  // namespace kv

@@ -10,7 +10,8 @@ namespace stream { int sm_count(); }             // gemv_stream.cu
 namespace kv {
 
 constexpr float kLog2e = 1.4426950408889634f;
-enum : int { ST_KV_TIMEOUT = 11 };          // device status: a copy of cache bytes never arrived
+enum : int { ST_KV_TIMEOUT = 11 };          // device status: a wait gave up
+constexpr uint32_t kPolls = 1u << 18;       // of a barrier before a wait gives up, a second or two: waits are within a CTA
 
 // n / d for 0 <= n < 2^31: the quotient is (mulhi(n, m) + n) >> s with s = ceil(log2 d), m = floor(2^32 (2^s - d) / d) + 1 (Granlund and Montgomery).
 struct Divisor {
@@ -211,6 +212,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+int attention_many(AttnParams& a, int type, cudaStream_t s);
 int attention_few_int8(AttnParams& a, int tiles, cudaStream_t s);
 int attention_few_e4m3(AttnParams& a, int tiles, cudaStream_t s);
 void attention_reset();                      // counters of the current device, after a launch that gave up

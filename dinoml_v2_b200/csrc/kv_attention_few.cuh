@@ -168,7 +168,7 @@ template <class S> __device__ __forceinline__ bool wait(const AttnParams& a, Sha
   const uint32_t at = umma::smem_u32(bar);
   volatile int* lost = &sh.lost;
   if (umma::mbar_test_wait(at, parity)) return true;
-  for (uint32_t i = 0; i < umma::kSpinLimit; ++i) {
+  for (uint32_t i = 0; i < kPolls; ++i) {
     if (umma::mbar_try_wait(at, parity)) return true;
     if ((i & 255u) == 255u && *lost) return false;
   }
