@@ -127,13 +127,38 @@ __device__ __forceinline__ void walk_items(const AttnParams& a, Shared& sh, Walk
   }
 }
 
-// ---- warps 8..11.  A warp has 32 tokens of every tile: in each of kCopies steps, rows of D / 16 lanes, 16 values a lane.
+// A lane's values of a tile, to[0] and to[1] being the places of its first 16.  BIASED: K of int8 stays 1152 too large (Half2Of), which the rows' scores take
+// off again.
+template <int TYPE, class S, bool BIASED, int COPIES> __device__ __forceinline__ void store_operand(const uint4 (&x)[COPIES], uint32_t smem, const uint32_t (&to)[2]) {
+  using H = Half2Of<TYPE>;
+  constexpr int kStep = 32 / COPIES;
+#pragma unroll
+  for (int i = 0; i < COPIES; ++i) {
+    uint32_t h[8];
+    H::template along<BIASED>(x[i].x, h[0], h[1]);
+    H::template along<BIASED>(x[i].y, h[2], h[3]);
+    H::template along<BIASED>(x[i].z, h[4], h[5]);
+    H::template along<BIASED>(x[i].w, h[6], h[7]);
+    const uint32_t turn = kStep == 4 && (i & 1) != 0 ? 64u : 0u;         // rows 4..7 of eight
+    const uint32_t at = smem + uint32_t(i * kStep * 128);
+    st_shared16((at + to[0]) ^ turn, h[0], h[1], h[2], h[3]);
+    st_shared16((at + to[1]) ^ turn, h[4], h[5], h[6], h[7]);
+  }
+  fence_async_smem();
+  __syncwarp();
+}
+
+// ---- warps 8..11.  A warp has 32 tokens of every tile, in kCopies steps of kStep tokens, 16 values a lane.
 template <int TYPE, class S>
 __device__ __forceinline__ void convert_tiles(const AttnParams& a, Shared& sh, uint32_t k_smem, uint32_t v_smem) {
-  using H = Half2Of<TYPE>;
   constexpr int kChunks = S::D / 16, kStep = 32 / kChunks, kCopies = 32 / kStep;
-  const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, chunk = lane % kChunks, row0 = 32 * warp + lane / kChunks;
+  const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, chunk = lane % kChunks;
+  // Where eight lanes have one row of 128 values, those of its second half take the neighbouring row instead: their stores go to the other banks.
+  const int row = lane / kChunks ^ (kChunks == 8 ? (lane >> 2) & 1 : 0);
   const int log2 = a.c.block_log2, mask = (1 << log2) - 1;
+  uint32_t to[2];                                                       // of a lane's two times 8 float16 in the first step
+#pragma unroll
+  for (int h = 0; h < 2; ++h) to[h] = operand_at(32 * warp + row, 2 * chunk + h);
   int n = 0;
   for (int segment = 0;; ++segment) {
     const int slot = segment % kSegments;
@@ -150,30 +175,16 @@ __device__ __forceinline__ void convert_tiles(const AttnParams& a, Shared& sh, u
     };
     uint4 raw[2][kCopies];
     auto load = [&](uint4 (&x)[kCopies], int which, int tile, int first_bh, int second_bh) {
+      const int token = base + tile * kTile + 32 * warp + row;           // (16 tokens from a multiple of 16 are in one block)
+      const uint8_t* const data = a.c.data[which] + chunk * 16;
+      const uint8_t *p0 = data + ((int64_t(first_bh) << log2) + (token & mask)) * S::D, *p1 = data + ((int64_t(second_bh) << log2) + ((token + 16) & mask)) * S::D - 16 * S::D;
 #pragma unroll
       for (int i = 0; i < kCopies; ++i) {
-        const int row = row0 + i * kStep, token = base + tile * kTile + row, bh = i * kStep < 16 ? first_bh : second_bh;
-        x[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (bh >= 0 && token >= low && token < high)
-          x[i] = __ldg(reinterpret_cast<const uint4*>(a.c.data[which] + ((int64_t(bh) << log2) + (token & mask)) * S::D + chunk * 16));
+        const bool first = i * kStep < 16;
+        x[i] = make_uint4(0u, 0u, 0u, 0u);                              // (what nobody sees has to be finite: zeros)
+        if ((first ? first_bh : second_bh) >= 0 && token + i * kStep >= low && token + i * kStep < high)
+          x[i] = __ldg(reinterpret_cast<const uint4*>((first ? p0 : p1) + i * kStep * S::D));
       }
-    };
-    auto store = [&](const uint4 (&x)[kCopies], uint32_t smem) {
-#pragma unroll
-      for (int i = 0; i < kCopies; ++i) {
-        uint32_t h[8];
-        H::template along<false>(x[i].x, h[0], h[1]);
-        H::template along<false>(x[i].y, h[2], h[3]);
-        H::template along<false>(x[i].z, h[4], h[5]);
-        H::template along<false>(x[i].w, h[6], h[7]);
-        const int row = row0 + i * kStep;
-        // (lanes of the second block of columns store their halves the other way round: eight lanes touch all banks)
-        const bool swap = (chunk & 4) != 0;
-        st_shared16(smem + operand_at(row, 2 * chunk + (swap ? 1 : 0)), swap ? h[4] : h[0], swap ? h[5] : h[1], swap ? h[6] : h[2], swap ? h[7] : h[3]);
-        st_shared16(smem + operand_at(row, 2 * chunk + (swap ? 0 : 1)), swap ? h[0] : h[4], swap ? h[1] : h[5], swap ? h[2] : h[6], swap ? h[3] : h[7]);
-      }
-      fence_async_smem();
-      __syncwarp();
     };
     int now = look_up(tile0);
     load(raw[0], 0, tile0, __shfl_sync(0xffffffffu, now, 0), __shfl_sync(0xffffffffu, now, 16));
@@ -192,11 +203,11 @@ __device__ __forceinline__ void convert_tiles(const AttnParams& a, Shared& sh, u
         const float v = vs < 0x1p-100f ? 0x1p-100f : vs;                // (a NaN stays)
         sh.scales[n % kScales][2 * warp + (lane >> 4)] = make_float4(ks, log2f(v), 1.f / v, now >= 0 ? 1.f : 0.f);
       }
-      store(raw[0], k_smem + uint32_t((n & 1) * S::kOperand));
+      store_operand<TYPE, S, true>(raw[0], k_smem + uint32_t((n & 1) * S::kOperand), to);
       if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.k_full[n & 1]));
       load(raw[0], 0, tile + 1, __shfl_sync(0xffffffffu, next, 0), __shfl_sync(0xffffffffu, next, 16));
       if (!wait(a, sh, &sh.v_empty[n & 1], lap ^ 1u)) return;
-      store(raw[1], v_smem + uint32_t((n & 1) * S::kOperand));
+      store_operand<TYPE, S, false>(raw[1], v_smem + uint32_t((n & 1) * S::kOperand), to);
       if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.v_full[n & 1]));
       now = next;
     }
@@ -261,8 +272,87 @@ __device__ __forceinline__ void issue_mmas(const AttnParams& a, Shared& sh, uint
   }
 }
 
+// Columns [32 c, 32 c + 32) of a tile's scores, in turn: f(c, registers), the next ones on their way meanwhile.
+template <typename F> __device__ __forceinline__ void for_columns(uint32_t tmem_s, F f) {
+  uint32_t r[2][32];
+  tmem_ld32(tmem_s, r[0]);
+  umma::tmem_ld_wait();
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    if (c < 3) tmem_ld32(tmem_s + uint32_t(32 * (c + 1)), r[(c + 1) & 1]);
+    f(c, r[c & 1]);
+    umma::tmem_ld_wait();
+  }
+}
+
+// A row's tile: the largest score, the sums so far brought to it if it has outgrown them, weights into the scores' place.  EVERY: the row sees
+// all of its columns, else those in [low, high) of blocks that are there.
+template <class S, bool EVERY>
+__device__ __forceinline__ void tile_weights(uint32_t tmem_s, uint32_t tmem_o, const float4* scales, float factor, float unbias, int low, int high, bool more,
+                                             float& ref, float& l) {
+  float top = -INFINITY;
+  for_columns(tmem_s, [&](int c, const uint32_t (&r)[32]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float4 x = scales[2 * c + h];
+      float m[4];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        float s = __uint_as_float(r[16 * h + k]);
+        if (!EVERY) s = x.w != 0.f && 32 * c + 16 * h + k >= low && 32 * c + 16 * h + k < high ? s : -INFINITY;
+        m[k & 3] = k < 4 ? s : fmaxf(m[k & 3], s);
+      }
+      const float best = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), f = x.x * factor;
+      if (EVERY || best != -INFINITY) top = fmaxf(top, fmaf(best - unbias, f, x.y));
+    }
+  });
+  const bool grow = top > ref + kGrow || (ref == -INFINITY && top != -INFINITY);
+  if (__any_sync(0xffffffffu, grow)) {
+    const float old = ref;
+    if (grow) ref = top;
+    if (more) {
+      const float keep = grow ? exp2_approx(old - ref) : 1.f;           // (nothing so far: 2^-inf)
+      l *= keep;
+#pragma unroll 1
+      for (int c = 0; c < S::D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(tmem_o + uint32_t(32 * c), o);
+        umma::tmem_ld_wait();
+#pragma unroll
+        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+        tmem_st32(tmem_o + uint32_t(32 * c), o);
+      }
+    }
+  }
+  const float bias = (ref == -INFINITY ? 0.f : -ref) + kUp;
+  for_columns(tmem_s, [&](int c, const uint32_t (&r)[32]) {
+    uint32_t p[16];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float4 x = scales[2 * c + h];
+      const float f = x.x * factor, add = fmaf(-unbias, f, x.y + bias);
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < 16; k += 2) {
+        float w[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          w[j] = exp2_approx(fmaf(__uint_as_float(r[16 * h + k + j]), f, add));
+          // what is not seen has no weight, whatever the block's scales are
+          if (!EVERY) w[j] = x.w != 0.f && 32 * c + 16 * h + k + j >= low && 32 * c + 16 * h + k + j < high ? w[j] : 0.f;
+          sum[j] += w[j];
+        }
+        p[8 * h + k / 2] = pack_half(w[0], w[1]);
+      }
+      const float both = sum[0] + sum[1];
+      if (EVERY || both != 0.f) l = fmaf(both, x.z, l);
+    }
+    umma::tmem_st16(tmem_s + uint32_t(16 * c), p);                           // (behind the columns that are still to be read)
+  });
+}
+
 // ---- warps 0..7: tile i of the item, a row per thread
-template <class S>
+template <int TYPE, class S>
 __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, uint32_t q_smem) {
   constexpr int D = S::D, kPiece = kItemRows * (D + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = warp >> 2, my_row = 32 * (warp & 3) + lane;
@@ -283,7 +373,7 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
     const bool mine = r < sg.item.r1;
     const int token = a.by_group(mine ? r : sg.item.r0), head = sg.head * a.group + (mine ? r : sg.item.r0) - token * a.group;
     const int64_t out_at = (int64_t(sg.s.row + token) * a.heads + head) * D;
-    float factor;
+    float factor, unbias = 0.f;
     {                                                                   // q of this row
       const int64_t at = int64_t(sg.s.row + token) * a.row_stride + int64_t(head) * a.head_stride;
       const bool wide = ((reinterpret_cast<uintptr_t>(a.q) | uint64_t(a.row_stride * 2) | uint64_t(a.head_stride * 2)) & 15) == 0;
@@ -327,9 +417,12 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
           if (f16) v = __half22float2(*reinterpret_cast<const __half2*>(&w));
           else v = make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
           h[k] = pack_half(v.x * sign, v.y * sign);
+          const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h[k]));
+          unbias += back.x + back.y;
         }
         st_shared16(q + operand_at(my_row, c), h[0], h[1], h[2], h[3]);
       }
+      unbias *= Half2Of<TYPE>::kBias;                                   // K's of int8 are that much too large
       fence_async_smem();
       __syncwarp();
       if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.q_ready));
@@ -343,76 +436,13 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
     for (int tile = tile0; tile < tile1; ++tile, ++n) {
       if (!wait(a, sh, &sh.s_full[i], uint32_t(n) & 1u)) { lost = true; break; }
       umma::tcgen05_fence_after();
-      uint32_t s[kTile];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(tmem_s + uint32_t(32 * c), s + 32 * c);
-      umma::tmem_ld_wait();
       const float4* const scales = sh.scales[n % kScales];
       const int token0 = base + tile * kTile;
       bool every = token0 >= all_low && token0 + kTile <= all_high;
 #pragma unroll
       for (int g = 0; g < kTile / 16; ++g) every = every && scales[g].w != 0.f;
-      if (!every) {
-#pragma unroll
-        for (int g = 0; g < kTile / 16; ++g) {
-          const bool there = scales[g].w != 0.f;
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const int at = token0 + 16 * g + k;
-            if (!there || at < low || at >= high) s[16 * g + k] = 0xff800000u;
-          }
-        }
-      }
-      float top = -INFINITY;
-#pragma unroll
-      for (int g = 0; g < kTile / 16; ++g) {
-        float m = __uint_as_float(s[16 * g]);
-#pragma unroll
-        for (int k = 1; k < 16; ++k) m = fmaxf(m, __uint_as_float(s[16 * g + k]));
-        top = fmaxf(top, m == -INFINITY ? m : fmaf(m, scales[g].x * factor, scales[g].y));
-      }
-      const bool grow = top > ref + kGrow || (ref == -INFINITY && top != -INFINITY);
-      if (__any_sync(0xffffffffu, grow)) {
-        const float old = ref;
-        if (grow) ref = top;
-        if (tile > tile0) {
-          const float keep = grow ? exp2_approx(old - ref) : 1.f;       // (nothing so far: 2^-inf)
-          l *= keep;
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(tmem_o + uint32_t(32 * c), o);
-            umma::tmem_ld_wait();
-#pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
-            tmem_st32(tmem_o + uint32_t(32 * c), o);
-          }
-        }
-      }
-      const float bias = (ref == -INFINITY ? 0.f : -ref) + kUp;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t p[32];
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const int g = 4 * c + h;
-          const float4 x = scales[g];
-          const float f = x.x * factor, add = x.y + bias;
-          float sum = 0.f;
-#pragma unroll
-          for (int k = 0; k < 16; k += 2) {
-            float u = exp2_approx(fmaf(__uint_as_float(s[16 * g + k]), f, add)), v = exp2_approx(fmaf(__uint_as_float(s[16 * g + k + 1]), f, add));
-            if (!every) {                                               // what is not seen has no weight, whatever the block's scales are
-              u = s[16 * g + k] == 0xff800000u ? 0.f : u;
-              v = s[16 * g + k + 1] == 0xff800000u ? 0.f : v;
-            }
-            sum += u + v;
-            p[8 * h + k / 2] = pack_half(u, v);
-          }
-          if (every || sum != 0.f) l = fmaf(sum, x.z, l);
-        }
-        tmem_st32(tmem_s + uint32_t(32 * c), p);
-      }
+      if (every) tile_weights<S, true>(tmem_s, tmem_o, scales, factor, unbias, 0, 0, tile > tile0, ref, l);
+      else tile_weights<S, false>(tmem_s, tmem_o, scales, factor, unbias, low - token0, high - token0, tile > tile0, ref, l);
       umma::tmem_st_wait();
       umma::tcgen05_fence_before();
       __syncwarp();
@@ -463,31 +493,51 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
       if (!meet()) return;
       if (sh.last) {
         const int rows = sg.item.r1 - sg.item.r0, count = sg.c1 - sg.c0 + 1;
-        for (int x = int(threadIdx.x); x < rows * (D / 4); x += 256) {
-          const int row = x / (D / 4), d = x % (D / 4) * 4;
-          float high_ref = -INFINITY, sum = 0.f;
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        constexpr int U = 4;                                            // places under way at a time
+        for (int x0 = int(threadIdx.x); x0 < rows * (D / 4); x0 += 256 * U) {
+          float high_ref[U], sum[U];
+          float4 v[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            high_ref[u] = -INFINITY;
+            sum[u] = 0.f;
+            v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          }
           for (int c = 0; c < count; ++c) {
             const float* src = a.partial + size_t(c == 0 ? sg.piece0 : 2 * (sg.c0 + c)) * kPiece;
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + kItemRows * D) + row);
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(src + size_t(row) * D + d));
-            const float next = fmaxf(high_ref, ml.x);
-            const float f0 = high_ref == -INFINITY ? 1.f : exp2_approx(high_ref - next), f1 = ml.x == -INFINITY ? 1.f : exp2_approx(ml.x - next);
-            sum = fmaf(ml.y, f1, sum * f0);
-            v = make_float4(fmaf(y.x, f1, v.x * f0), fmaf(y.y, f1, v.y * f0), fmaf(y.z, f1, v.z * f0), fmaf(y.w, f1, v.w * f0));
-            high_ref = next;
+            float2 ml[U];
+            float4 y[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              const int x = min(x0 + 256 * u, rows * (D / 4) - 1);
+              ml[u] = __ldcg(reinterpret_cast<const float2*>(src + kItemRows * D) + x / (D / 4));
+              y[u] = __ldcg(reinterpret_cast<const float4*>(src) + x);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              const float next = fmaxf(high_ref[u], ml[u].x);
+              const float f0 = high_ref[u] == -INFINITY ? 1.f : exp2_approx(high_ref[u] - next), f1 = ml[u].x == -INFINITY ? 1.f : exp2_approx(ml[u].x - next);
+              sum[u] = fmaf(ml[u].y, f1, sum[u] * f0);
+              v[u] = make_float4(fmaf(y[u].x, f1, v[u].x * f0), fmaf(y[u].y, f1, v[u].y * f0), fmaf(y[u].z, f1, v[u].z * f0), fmaf(y[u].w, f1, v[u].w * f0));
+              high_ref[u] = next;
+            }
           }
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          const int t = a.by_group(sg.item.r0 + row), hd = sg.head * a.group + sg.item.r0 + row - t * a.group;
-          const int64_t at = (int64_t(sg.s.row + t) * a.heads + hd) * D + d;
-          uint2 h;
-          if (a.dtype == DINO_F16) {
-            h = make_uint2(pack_half(v.x * inv, v.y * inv), pack_half(v.z * inv, v.w * inv));
-          } else {
-            const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x * inv, v.y * inv), hi = __floats2bfloat162_rn(v.z * inv, v.w * inv);
-            h = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int x = x0 + 256 * u, row = x / (D / 4), d = x % (D / 4) * 4;
+            if (row >= rows) continue;
+            const float inv = sum[u] == 0.f ? 0.f : 1.f / sum[u];
+            const int t = a.by_group(sg.item.r0 + row), hd = sg.head * a.group + sg.item.r0 + row - t * a.group;
+            const int64_t at = (int64_t(sg.s.row + t) * a.heads + hd) * D + d;
+            uint2 h;
+            if (a.dtype == DINO_F16) {
+              h = make_uint2(pack_half(v[u].x * inv, v[u].y * inv), pack_half(v[u].z * inv, v[u].w * inv));
+            } else {
+              const __nv_bfloat162 lo = __floats2bfloat162_rn(v[u].x * inv, v[u].y * inv), hi = __floats2bfloat162_rn(v[u].z * inv, v[u].w * inv);
+              h = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+            }
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = h;
           }
-          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = h;
         }
       }
     }
@@ -533,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_many_kernel(const __gri
   umma::tcgen05_fence_after();
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 176;\n");            // 2 x 176 + 96 + 64 = 4 x 128
-    softmax_rows<S>(a, sh, q_smem);
+    softmax_rows<TYPE, S>(a, sh, q_smem);
   } else if (warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
     convert_tiles<TYPE, S>(a, sh, k_smem, v_smem);
