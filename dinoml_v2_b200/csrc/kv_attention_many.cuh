@@ -1,8 +1,8 @@
 // Attention of many rows per cached head (prompts, chunks of them) over the 8-bit cache, on tcgen05: bound by the products and by the exponentials, which
-// take the same time (256 rows against 128 tokens, heads of 128: four MMAs of 512 cycles, 32768 exponentials at 16 a cycle).
+// take the same time (256 rows against 64 tokens, heads of 128: four MMAs of 256 cycles, 16384 exponentials at 16 a cycle).
 //
-// A CTA has 256 rows (token x head of the group, so a cached tile is read once for all heads that share it) as two tiles of 128, whose softmax and
-// MMAs alternate: while one tile's warps take exponentials, the other one's products run.
+// A CTA has 256 rows (token x head of the group, so a cached tile is read once for all heads that share it) as two tiles of 128.  The scores of a tile
+// have two places in tensor memory: the next ones are there when the softmax of a tile is done, which so never waits for products.
 //   * warps 0..3 and 4..7: softmax, a row of scores per thread, S_i from tensor memory, P_i back into the same columns;
 //   * warps 8..11: K and V of the next tiles, 8 bits in global memory to float16 in shared memory (swizzled as the MMA reads them);
 //   * warp 12: issues the MMAs, S_i = Q_i K^T from shared memory and O_i += P_i V with P_i from tensor memory; V stays [token][channel], an MN-major operand;
@@ -18,16 +18,17 @@ namespace b200gguf {
 namespace kv {
 namespace many {
 
-constexpr int kRows = 128, kItemRows = 2 * kRows, kTile = 128, kLog2 = 7;      // rows of an MMA, of an item; cached tokens of a tile
-constexpr int kThreads = 512, kSegments = 4, kScales = 4;
-constexpr uint32_t kTmem = 512, kS = 0, kO = 256;                             // columns: S_i at 128 i, O_i at 256 + D i
+constexpr int kRows = 128, kItemRows = 2 * kRows, kTile = 64, kLog2 = 6;       // rows of an MMA, of an item; cached tokens of a tile
+constexpr int kThreads = 512, kSegments = 4;
+constexpr int kStages = 4, kScales = 8;                                       // tiles of K and of V in shared memory; of scales (K runs two tiles ahead of V)
+constexpr uint32_t kTmem = 512, kO = 256;                                     // columns: S_i of even and odd tiles at 128 i and 128 i + 64, O_i at 256 + D i
 constexpr float kGrow = 8.f, kUp = 7.f;
+constexpr unsigned kPolynomial = 0x11;      // of eight pairs of exponentials, those that the FMA units take: the special function units are the bound
 
 template <int D_> struct Shape {
   static constexpr int D = D_;
-  static constexpr int kBlock = kRows * 128;                  // bytes of 128 rows of 64 float16
-  static constexpr int kOperand = kBlock * (D / 64);          // of a tile of Q, K or V
-  static constexpr size_t kSmem = 1024 + 6 * size_t(kOperand);
+  static constexpr int kQ = kRows * D * 2, kKv = kTile * D * 2;      // bytes of a tile of Q, of K or V
+  static constexpr size_t kSmem = 1024 + 2 * size_t(kQ) + 2 * kStages * size_t(kKv);
 };
 
 struct Segment {
@@ -39,9 +40,11 @@ struct Segment {
 
 struct Shared {
   uint64_t described[kSegments], closed[kSegments], q_ready;
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_full[2], together, drain;
+  uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
+  uint64_t s_full[2][2], p_ready[2][2], o_done[2], together, drain;            // of row tile i: scores and weights of even and odd tiles, every product with V
   Segment segments[kSegments];
   float4 scales[kScales][kTile / 16];         // of 16 tokens: K's scale, log2 of V's, 1 / V's, whether there is a block
+  int4 whole[kScales];                        // of 16 tokens each: whether there is a block
   int64_t walk[2 + kThreads / 32];
   uint32_t tmem;
   int last, lost;
@@ -96,9 +99,9 @@ __device__ __forceinline__ void st_shared16(uint32_t at, uint32_t x, uint32_t y,
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
-// Address of 16 bytes (8 float16) of an operand tile: K-major rows of 64 values with the 128-byte swizzle, blocks of 64 columns one after the other.
-__device__ __forceinline__ uint32_t operand_at(int row, int chunk) {
-  return uint32_t((chunk >> 3) * (kRows * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+// Address of 16 bytes (8 float16) of an operand tile of ROWS rows: rows of 64 values with the 128-byte swizzle, blocks of 64 columns one after the other.
+template <int ROWS> __device__ __forceinline__ uint32_t operand_at(int row, int chunk) {
+  return uint32_t((chunk >> 3) * (ROWS * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
 }
 
 // ---- warp 13
@@ -131,7 +134,7 @@ __device__ __forceinline__ void walk_items(const AttnParams& a, Shared& sh, Walk
 // off again.
 template <int TYPE, class S, bool BIASED, int COPIES> __device__ __forceinline__ void store_operand(const uint4 (&x)[COPIES], uint32_t smem, const uint32_t (&to)[2]) {
   using H = Half2Of<TYPE>;
-  constexpr int kStep = 32 / COPIES;
+  constexpr int kStep = 16 / COPIES;
 #pragma unroll
   for (int i = 0; i < COPIES; ++i) {
     uint32_t h[8];
@@ -148,17 +151,17 @@ template <int TYPE, class S, bool BIASED, int COPIES> __device__ __forceinline__
   __syncwarp();
 }
 
-// ---- warps 8..11.  A warp has 32 tokens of every tile, in kCopies steps of kStep tokens, 16 values a lane.
+// ---- warps 8..11.  A warp has 16 tokens of every tile, which are of one block, in kCopies steps of kStep tokens, 16 values a lane.
 template <int TYPE, class S>
 __device__ __forceinline__ void convert_tiles(const AttnParams& a, Shared& sh, uint32_t k_smem, uint32_t v_smem) {
-  constexpr int kChunks = S::D / 16, kStep = 32 / kChunks, kCopies = 32 / kStep;
+  constexpr int kChunks = S::D / 16, kStep = 32 / kChunks, kCopies = 16 / kStep;
   const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, chunk = lane % kChunks;
   // Where eight lanes have one row of 128 values, those of its second half take the neighbouring row instead: their stores go to the other banks.
   const int row = lane / kChunks ^ (kChunks == 8 ? (lane >> 2) & 1 : 0);
   const int log2 = a.c.block_log2, mask = (1 << log2) - 1;
   uint32_t to[2];                                                       // of a lane's two times 8 float16 in the first step
 #pragma unroll
-  for (int h = 0; h < 2; ++h) to[h] = operand_at(32 * warp + row, 2 * chunk + h);
+  for (int h = 0; h < 2; ++h) to[h] = operand_at<kTile>(16 * warp + row, 2 * chunk + h);
   int n = 0;
   for (int segment = 0;; ++segment) {
     const int slot = segment % kSegments;
@@ -166,50 +169,48 @@ __device__ __forceinline__ void convert_tiles(const AttnParams& a, Shared& sh, u
     const Segment& sg = sh.segments[slot];
     const int tile0 = sg.tile0, tile1 = sg.tile1, low = sg.item.low, high = sg.item.high, base = (low >> kLog2) << kLog2, b = sg.b, head = sg.head;
     if (tile0 == tile1) return;
-    // The block of this lane's half of the warp's tokens (lane / 16: the first or the last 16), as block x head, -1 if there is none.
-    auto look_up = [&](int tile) {
-      const int token = base + tile * kTile + 32 * warp + (lane & 16);
+    auto look_up = [&](int tile) {                                      // the warp's block, as block x head, -1 if there is none
+      const int token = base + tile * kTile + 16 * warp;
       if (tile >= tile1 || token >= high || token + 16 <= low) return -1;
       const int id = block_at(a.p, a.c.blocks, b, token >> log2);
       return id < 0 ? -1 : id * a.c.heads + head;
     };
     uint4 raw[2][kCopies];
-    auto load = [&](uint4 (&x)[kCopies], int which, int tile, int first_bh, int second_bh) {
-      const int token = base + tile * kTile + 32 * warp + row;           // (16 tokens from a multiple of 16 are in one block)
-      const uint8_t* const data = a.c.data[which] + chunk * 16;
-      const uint8_t *p0 = data + ((int64_t(first_bh) << log2) + (token & mask)) * S::D, *p1 = data + ((int64_t(second_bh) << log2) + ((token + 16) & mask)) * S::D - 16 * S::D;
+    auto load = [&](uint4 (&x)[kCopies], int which, int tile, int bh) {
+      const int token = base + tile * kTile + 16 * warp + row;
+      const uint8_t* const from = a.c.data[which] + chunk * 16 + ((int64_t(bh) << log2) + (token & mask)) * S::D;
 #pragma unroll
       for (int i = 0; i < kCopies; ++i) {
-        const bool first = i * kStep < 16;
         x[i] = make_uint4(0u, 0u, 0u, 0u);                              // (what nobody sees has to be finite: zeros)
-        if ((first ? first_bh : second_bh) >= 0 && token + i * kStep >= low && token + i * kStep < high)
-          x[i] = __ldg(reinterpret_cast<const uint4*>((first ? p0 : p1) + i * kStep * S::D));
+        if (bh >= 0 && token + i * kStep >= low && token + i * kStep < high) x[i] = __ldg(reinterpret_cast<const uint4*>(from + i * kStep * S::D));
       }
     };
-    int now = look_up(tile0);
-    load(raw[0], 0, tile0, __shfl_sync(0xffffffffu, now, 0), __shfl_sync(0xffffffffu, now, 16));
+    // Loads run two tiles ahead of what they are for: K of the next tile and V of this one are under way while K of this one is stored.
+    int now = look_up(tile0), next = look_up(tile0 + 1);
+    load(raw[0], 0, tile0, now);
     for (int tile = tile0; tile < tile1; ++tile, ++n) {
-      const int first_bh = __shfl_sync(0xffffffffu, now, 0), second_bh = __shfl_sync(0xffffffffu, now, 16);
-      const int next = look_up(tile + 1);
-      load(raw[1], 1, tile, first_bh, second_bh);
+      const int after = look_up(tile + 2), stage = n % kStages;
+      load(raw[1], 1, tile, now);
       float ks = 0.f, vs = 0.f;
       if (now >= 0) {
         ks = __ldg(a.c.scale[0] + now);
         vs = __ldg(a.c.scale[1] + now);
       }
-      const uint32_t lap = uint32_t(n >> 1) & 1u;
-      if (!wait(a, sh, &sh.k_empty[n & 1], lap ^ 1u)) return;
-      if ((lane & 15) == 0) {
+      const uint32_t lap = uint32_t(n / kStages) & 1u;
+      if (!wait(a, sh, &sh.k_empty[stage], lap ^ 1u)) return;
+      if (lane == 0) {
         const float v = vs < 0x1p-100f ? 0x1p-100f : vs;                // (a NaN stays)
-        sh.scales[n % kScales][2 * warp + (lane >> 4)] = make_float4(ks, log2f(v), 1.f / v, now >= 0 ? 1.f : 0.f);
+        sh.scales[n % kScales][warp] = make_float4(ks, log2f(v), 1.f / v, now >= 0 ? 1.f : 0.f);
+        reinterpret_cast<int*>(&sh.whole[n % kScales])[warp] = now >= 0;
       }
-      store_operand<TYPE, S, true>(raw[0], k_smem + uint32_t((n & 1) * S::kOperand), to);
-      if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.k_full[n & 1]));
-      load(raw[0], 0, tile + 1, __shfl_sync(0xffffffffu, next, 0), __shfl_sync(0xffffffffu, next, 16));
-      if (!wait(a, sh, &sh.v_empty[n & 1], lap ^ 1u)) return;
-      store_operand<TYPE, S, false>(raw[1], v_smem + uint32_t((n & 1) * S::kOperand), to);
-      if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.v_full[n & 1]));
+      store_operand<TYPE, S, true>(raw[0], k_smem + uint32_t(stage * S::kKv), to);
+      if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.k_full[stage]));
+      load(raw[0], 0, tile + 1, next);
+      if (!wait(a, sh, &sh.v_empty[stage], lap ^ 1u)) return;
+      store_operand<TYPE, S, false>(raw[1], v_smem + uint32_t(stage * S::kKv), to);
+      if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.v_full[stage]));
       now = next;
+      next = after;
     }
     if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.closed[slot]));
   }
@@ -222,48 +223,54 @@ __device__ __forceinline__ void issue_mmas(const AttnParams& a, Shared& sh, uint
   const uint32_t idesc_s = (1u << 4) | (uint32_t(kTile >> 3) << 17) | (uint32_t(kRows >> 4) << 24);                    // float16, float32 sums
   const uint32_t idesc_o = (1u << 4) | (1u << 16) | (uint32_t(S::D >> 3) << 17) | (uint32_t(kRows >> 4) << 24);        // B is MN-major
   int n = 0;
-  auto scores = [&](int i, int stage) {
+  auto scores = [&](int i, int tile) {                                  // S_i = Q_i K^T of a tile (numbered like n)
     if (umma::elect_one()) {
-      const uint64_t q = umma::smem_desc_sw128(q_smem + uint32_t(i * S::kOperand)), k = umma::smem_desc_sw128(k_smem + uint32_t(stage * S::kOperand));
+      const int stage = tile % kStages;
+      const uint64_t q = umma::smem_desc_sw128(q_smem + uint32_t(i * S::kQ)), k = umma::smem_desc_sw128(k_smem + uint32_t(stage * S::kKv));
 #pragma unroll
-      for (int s = 0; s < S::D / 16; ++s) {
-        const uint64_t off = uint64_t(((s >> 2) * S::kBlock + (s & 3) * 32) >> 4);
-        umma_f16_ss(tmem + kS + uint32_t(i * kTile), q + off, k + off, idesc_s, s != 0);
-      }
-      umma::umma_commit<false>(umma::smem_u32(&sh.s_full[i]), 0);
+      for (int s = 0; s < S::D / 16; ++s)
+        umma_f16_ss(tmem + uint32_t(i * 128 + (tile & 1) * 64), q + uint64_t(((s >> 2) * kRows * 128 + (s & 3) * 32) >> 4),
+                    k + uint64_t(((s >> 2) * kTile * 128 + (s & 3) * 32) >> 4), idesc_s, s != 0);
+      umma::umma_commit<false>(umma::smem_u32(&sh.s_full[i][tile & 1]), 0);
       if (i == 1) umma::umma_commit<false>(umma::smem_u32(&sh.k_empty[stage]), 0);
     }
     __syncwarp();
+  };
+  auto k_landed = [&](int tile) {
+    const bool ok = wait(a, sh, &sh.k_full[tile % kStages], uint32_t(tile / kStages) & 1u);
+    umma::tcgen05_fence_after();
+    return ok;
   };
   for (int segment = 0;; ++segment) {
     const int slot = segment % kSegments;
     if (!wait(a, sh, &sh.described[slot], uint32_t(segment / kSegments) & 1u)) return;
     const int tiles = sh.segments[slot].tile1 - sh.segments[slot].tile0;
     if (tiles == 0) return;
-    if (!wait(a, sh, &sh.q_ready, uint32_t(segment) & 1u) || !wait(a, sh, &sh.k_full[n & 1], uint32_t(n >> 1) & 1u)) return;
-    umma::tcgen05_fence_after();
-    scores(0, n & 1);
-    scores(1, n & 1);
+    if (!wait(a, sh, &sh.q_ready, uint32_t(segment) & 1u)) return;
+    for (int j = 0; j < min(2, tiles); ++j) {
+      if (!k_landed(n + j)) return;
+      scores(0, n + j);
+      scores(1, n + j);
+    }
     for (int j = 0; j < tiles; ++j, ++n) {
-      const int stage = n & 1;
-      if (!wait(a, sh, &sh.v_full[stage], uint32_t(n >> 1) & 1u)) return;
+      const int stage = n % kStages;
+      if (!wait(a, sh, &sh.v_full[stage], uint32_t(n / kStages) & 1u)) return;
       for (int i = 0; i < 2; ++i) {
-        if (!wait(a, sh, &sh.p_ready[i], uint32_t(n) & 1u)) return;
+        if (!wait(a, sh, &sh.p_ready[i][n & 1], uint32_t(n >> 1) & 1u)) return;
         umma::tcgen05_fence_after();
         if (umma::elect_one()) {
-          const uint64_t v = smem_desc_mn(v_smem + uint32_t(stage * S::kOperand), S::kBlock);
+          const uint64_t v = smem_desc_mn(v_smem + uint32_t(stage * S::kKv), kTile * 128);
 #pragma unroll
           for (int s = 0; s < kTile / 16; ++s)
-            umma::umma_f16_ts<false>(tmem + kO + uint32_t(i * S::D), tmem + kS + uint32_t(i * kTile + 8 * s), v + uint64_t((16 * 128 * s) >> 4), idesc_o,
+            umma::umma_f16_ts<false>(tmem + kO + uint32_t(i * S::D), tmem + uint32_t(i * 128 + (n & 1) * 64 + 8 * s), v + uint64_t((16 * 128 * s) >> 4), idesc_o,
                                      (j != 0 || s != 0) ? 1u : 0u);
+          umma::umma_commit<false>(umma::smem_u32(&sh.o_done[i]), 0);
           if (i == 1) umma::umma_commit<false>(umma::smem_u32(&sh.v_empty[stage]), 0);
-          if (j + 1 == tiles) umma::umma_commit<false>(umma::smem_u32(&sh.o_full[i]), 0);
         }
         __syncwarp();
-        if (j + 1 < tiles) {
-          if (i == 0 && !wait(a, sh, &sh.k_full[stage ^ 1], uint32_t((n + 1) >> 1) & 1u)) return;
-          umma::tcgen05_fence_after();
-          scores(i, stage ^ 1);
+        if (j + 2 < tiles) {                                            // into the place that the weights just read leave
+          if (i == 0 && !k_landed(n + 2)) return;
+          scores(i, n + 2);
         }
       }
     }
@@ -272,45 +279,80 @@ __device__ __forceinline__ void issue_mmas(const AttnParams& a, Shared& sh, uint
   }
 }
 
-// Columns [32 c, 32 c + 32) of a tile's scores, in turn: f(c, registers), the next ones on their way meanwhile.
-template <typename F> __device__ __forceinline__ void for_columns(uint32_t tmem_s, F f) {
-  uint32_t r[2][32];
-  tmem_ld32(tmem_s, r[0]);
-  umma::tmem_ld_wait();
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    if (c < 3) tmem_ld32(tmem_s + uint32_t(32 * (c + 1)), r[(c + 1) & 1]);
-    f(c, r[c & 1]);
-    umma::tmem_ld_wait();
-  }
+// Two float32 in a register pair.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ float2 halves_of(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float v;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+  return v;
+}
+
+// 2^x of two numbers below 2^7 without the special function unit: x = n + f with n the nearest integer (its bits are the last ones of x + 1.5 2^23), a
+// polynomial of degree four for 2^f on [-1/2, 1/2] (Remez exchange, relative error 2.6e-6), n added to its exponent.  Below 2^-126: 2^-126.
+__device__ __forceinline__ float2 exp2_pair(uint64_t x) {
+  const float2 raw = halves_of(x);
+  x = pair_of(fmaxf(raw.x, -126.f), fmaxf(raw.y, -126.f));
+  constexpr float kRound = 12582912.f;
+  const uint64_t t = add2(x, pair_of(kRound, kRound)), n = add2(t, pair_of(-kRound, -kRound)), f = fma2(n, pair_of(-1.f, -1.f), x);
+  uint64_t p = fma2(f, pair_of(0.009570102207362652f, 0.009570102207362652f), pair_of(0.05591785907745361f, 0.05591785907745361f));
+  p = fma2(p, f, pair_of(0.240247443318367f, 0.240247443318367f));
+  p = fma2(p, f, pair_of(0.6931217908859253f, 0.6931217908859253f));
+  p = fma2(p, f, pair_of(0.9999992847442627f, 0.9999992847442627f));
+  const float2 q = halves_of(p), e = halves_of(t);
+  return make_float2(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(e.x) << 23)), __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(e.y) << 23)));
 }
 
 // A row's tile: the largest score, the sums so far brought to it if it has outgrown them, weights into the scores' place.  EVERY: the row sees
-// all of its columns, else those in [low, high) of blocks that are there.
-template <class S, bool EVERY>
-__device__ __forceinline__ void tile_weights(uint32_t tmem_s, uint32_t tmem_o, const float4* scales, float factor, float unbias, int low, int high, bool more,
-                                             float& ref, float& l) {
+// all of its columns, else those in [low, high) of blocks that are there.  products_done: waits for the tile before to be in O; false where that gives up.
+template <class S, bool EVERY, typename Wait>
+__device__ __forceinline__ bool tile_weights(uint32_t tmem_s, uint32_t tmem_o, const float4* scales, float factor, float unbias, int low, int high, bool more,
+                                             float& ref, float& l, Wait products_done) {
+  uint32_t r[kTile];
+  tmem_ld32(tmem_s, r);
+  tmem_ld32(tmem_s + 32u, r + 32);
+  float4 x[kTile / 16];
+#pragma unroll
+  for (int g = 0; g < kTile / 16; ++g) x[g] = scales[g];
+  umma::tmem_ld_wait();
   float top = -INFINITY;
-  for_columns(tmem_s, [&](int c, const uint32_t (&r)[32]) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float4 x = scales[2 * c + h];
-      float m[4];
+  for (int g = 0; g < kTile / 16; ++g) {
+    float s[16];
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        float s = __uint_as_float(r[16 * h + k]);
-        if (!EVERY) s = x.w != 0.f && 32 * c + 16 * h + k >= low && 32 * c + 16 * h + k < high ? s : -INFINITY;
-        m[k & 3] = k < 4 ? s : fmaxf(m[k & 3], s);
-      }
-      const float best = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), f = x.x * factor;
-      if (EVERY || best != -INFINITY) top = fmaxf(top, fmaf(best - unbias, f, x.y));
+    for (int k = 0; k < 16; ++k) {
+      s[k] = __uint_as_float(r[16 * g + k]);
+      if (!EVERY) s[k] = x[g].w != 0.f && 16 * g + k >= low && 16 * g + k < high ? s[k] : -INFINITY;
     }
-  });
+    const float u = max3(max3(s[0], s[1], s[2]), s[3], s[4]), v = max3(max3(s[5], s[6], s[7]), s[8], s[9]), w = max3(max3(s[10], s[11], s[12]), s[13], s[14]);
+    const float best = max3(u, v, fmaxf(w, s[15])), f = x[g].x * factor;
+    if (EVERY || best != -INFINITY) top = fmaxf(top, fmaf(best - unbias, f, x[g].y));
+  }
   const bool grow = top > ref + kGrow || (ref == -INFINITY && top != -INFINITY);
   if (__any_sync(0xffffffffu, grow)) {
     const float old = ref;
     if (grow) ref = top;
     if (more) {
+      if (!products_done()) return false;
+      umma::tcgen05_fence_after();
       const float keep = grow ? exp2_approx(old - ref) : 1.f;           // (nothing so far: 2^-inf)
       l *= keep;
 #pragma unroll 1
@@ -325,30 +367,36 @@ __device__ __forceinline__ void tile_weights(uint32_t tmem_s, uint32_t tmem_o, c
     }
   }
   const float bias = (ref == -INFINITY ? 0.f : -ref) + kUp;
-  for_columns(tmem_s, [&](int c, const uint32_t (&r)[32]) {
-    uint32_t p[16];
+  uint32_t p[kTile / 2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float4 x = scales[2 * c + h];
-      const float f = x.x * factor, add = fmaf(-unbias, f, x.y + bias);
-      float sum[2] = {0.f, 0.f};
+  for (int g = 0; g < kTile / 16; ++g) {
+    const float f = x[g].x * factor, add = fmaf(-unbias, f, x[g].y + bias);
+    const uint64_t ff = pair_of(f, f), aa = pair_of(add, add);
+    uint64_t sum[2] = {0u, 0u};
 #pragma unroll
-      for (int k = 0; k < 16; k += 2) {
-        float w[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          w[j] = exp2_approx(fmaf(__uint_as_float(r[16 * h + k + j]), f, add));
-          // what is not seen has no weight, whatever the block's scales are
-          if (!EVERY) w[j] = x.w != 0.f && 32 * c + 16 * h + k + j >= low && 32 * c + 16 * h + k + j < high ? w[j] : 0.f;
-          sum[j] += w[j];
-        }
-        p[8 * h + k / 2] = pack_half(w[0], w[1]);
+    for (int k = 0; k < 16; k += 2) {
+      const uint64_t y = fma2(pair_of(__uint_as_float(r[16 * g + k]), __uint_as_float(r[16 * g + k + 1])), ff, aa);
+      float w[2];
+      if (EVERY && (kPolynomial >> (k / 2) & 1) != 0) {                 // (a NaN is lost there: the row's other columns of the block have it)
+        const float2 e = exp2_pair(y);
+        w[0] = e.x;
+        w[1] = e.y;
+      } else {
+        w[0] = exp2_approx(halves_of(y).x);
+        w[1] = exp2_approx(halves_of(y).y);
       }
-      const float both = sum[0] + sum[1];
-      if (EVERY || both != 0.f) l = fmaf(both, x.z, l);
+      if (!EVERY) {                                                     // what is not seen has no weight, whatever the block's scales are
+#pragma unroll
+        for (int j = 0; j < 2; ++j) w[j] = x[g].w != 0.f && 16 * g + k + j >= low && 16 * g + k + j < high ? w[j] : 0.f;
+      }
+      sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], pair_of(w[0], w[1]));
+      p[8 * g + k / 2] = pack_half(w[0], w[1]);
     }
-    umma::tmem_st16(tmem_s + uint32_t(16 * c), p);                           // (behind the columns that are still to be read)
-  });
+    const float2 both = halves_of(add2(sum[0], sum[1]));
+    if (EVERY || both.x + both.y != 0.f) l = fmaf(both.x + both.y, x[g].z, l);
+  }
+  tmem_st32(tmem_s, p);
+  return true;
 }
 
 // ---- warps 0..7: tile i of the item, a row per thread
@@ -356,7 +404,7 @@ template <int TYPE, class S>
 __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, uint32_t q_smem) {
   constexpr int D = S::D, kPiece = kItemRows * (D + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = warp >> 2, my_row = 32 * (warp & 3) + lane;
-  const uint32_t lanes = sh.tmem + (uint32_t(32 * (warp & 3)) << 16), tmem_s = lanes + kS + uint32_t(i * kTile), tmem_o = lanes + kO + uint32_t(i * D);
+  const uint32_t lanes = sh.tmem + (uint32_t(32 * (warp & 3)) << 16), tmem_s = lanes + uint32_t(i * 128), tmem_o = lanes + kO + uint32_t(i * D);
   int n = 0, meetings = 0;
   auto meet = [&] {
     __syncwarp();
@@ -406,7 +454,7 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
       const float up = __uint_as_float(uint32_t(127 + shift) << 23);
       const float sign = a.scale < 0.f ? -up : up;                      // scores' factors are not negative
       factor = fabsf(a.scale) * __uint_as_float(uint32_t(127 - shift) << 23);
-      const uint32_t q = q_smem + uint32_t(i * S::kOperand);
+      const uint32_t q = q_smem + uint32_t(i * S::kQ);
 #pragma unroll
       for (int c = 0; c < D / 8; ++c) {
         uint32_t h[4];
@@ -420,7 +468,7 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
           const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h[k]));
           unbias += back.x + back.y;
         }
-        st_shared16(q + operand_at(my_row, c), h[0], h[1], h[2], h[3]);
+        st_shared16(q + operand_at<kRows>(my_row, c), h[0], h[1], h[2], h[3]);
       }
       unbias *= Half2Of<TYPE>::kBias;                                   // K's of int8 are that much too large
       fence_async_smem();
@@ -434,22 +482,26 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
     float ref = -INFINITY, l = 0.f;
     bool lost = false;
     for (int tile = tile0; tile < tile1; ++tile, ++n) {
-      if (!wait(a, sh, &sh.s_full[i], uint32_t(n) & 1u)) { lost = true; break; }
+      if (!wait(a, sh, &sh.s_full[i][n & 1], uint32_t(n >> 1) & 1u)) { lost = true; break; }
       umma::tcgen05_fence_after();
       const float4* const scales = sh.scales[n % kScales];
       const int token0 = base + tile * kTile;
-      bool every = token0 >= all_low && token0 + kTile <= all_high;
-#pragma unroll
-      for (int g = 0; g < kTile / 16; ++g) every = every && scales[g].w != 0.f;
-      if (every) tile_weights<S, true>(tmem_s, tmem_o, scales, factor, unbias, 0, 0, tile > tile0, ref, l);
-      else tile_weights<S, false>(tmem_s, tmem_o, scales, factor, unbias, low - token0, high - token0, tile > tile0, ref, l);
+      const int4 whole = sh.whole[n % kScales];
+      const bool every = token0 >= all_low && token0 + kTile <= all_high && (whole.x & whole.y & whole.z & whole.w) != 0;
+      const uint32_t at = tmem_s + uint32_t((n & 1) * 64);
+      auto products_done = [&] { return wait(a, sh, &sh.o_done[i], uint32_t(n - 1) & 1u); };
+      if (!(every ? tile_weights<S, true>(at, tmem_o, scales, factor, unbias, 0, 0, tile > tile0, ref, l, products_done)
+                  : tile_weights<S, false>(at, tmem_o, scales, factor, unbias, low - token0, high - token0, tile > tile0, ref, l, products_done))) {
+        lost = true;
+        break;
+      }
       umma::tmem_st_wait();
       umma::tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.p_ready[i]));
+      if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.p_ready[i][n & 1]));
     }
     if (lost) return;
-    if (!wait(a, sh, &sh.o_full[i], uint32_t(segment) & 1u)) return;
+    if (!wait(a, sh, &sh.o_done[i], uint32_t(n - 1) & 1u)) return;
     umma::tcgen05_fence_after();
     const float f = l == 0.f ? 0.f : 1.f / l;
     float* const part = a.partial + size_t(max(sg.piece, 0)) * kPiece + size_t(i * kRows + my_row) * D;
@@ -551,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_many_kernel(const __gri
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared sh;
   const uint32_t smem = (umma::smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t q_smem = smem, k_smem = smem + 2 * S::kOperand, v_smem = smem + 4 * S::kOperand;
+  const uint32_t q_smem = smem, k_smem = smem + 2 * S::kQ, v_smem = k_smem + kStages * S::kKv;
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSegments; ++i) {
@@ -559,14 +611,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_many_kernel(const __gri
       umma::mbar_init(umma::smem_u32(&sh.closed[i]), 13);              // eight, four and one warps
     }
     umma::mbar_init(umma::smem_u32(&sh.q_ready), 8);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       umma::mbar_init(umma::smem_u32(&sh.k_full[i]), 4);
       umma::mbar_init(umma::smem_u32(&sh.v_full[i]), 4);
       umma::mbar_init(umma::smem_u32(&sh.k_empty[i]), 1);
       umma::mbar_init(umma::smem_u32(&sh.v_empty[i]), 1);
-      umma::mbar_init(umma::smem_u32(&sh.s_full[i]), 1);
-      umma::mbar_init(umma::smem_u32(&sh.p_ready[i]), 4);
-      umma::mbar_init(umma::smem_u32(&sh.o_full[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      for (int k = 0; k < 2; ++k) {
+        umma::mbar_init(umma::smem_u32(&sh.s_full[i][k]), 1);
+        umma::mbar_init(umma::smem_u32(&sh.p_ready[i][k]), 4);
+      }
+      umma::mbar_init(umma::smem_u32(&sh.o_done[i]), 1);
     }
     umma::mbar_init(umma::smem_u32(&sh.together), 8);
     umma::mbar_init(umma::smem_u32(&sh.drain), 1);
