@@ -20,7 +20,8 @@ namespace many {
 
 constexpr int kRows = 128, kItemRows = 2 * kRows, kTile = 64, kLog2 = 6;       // rows of an MMA, of an item; cached tokens of a tile
 constexpr int kThreads = 512, kSegments = 4;
-constexpr int kStages = 4, kScales = 8;                                       // tiles of K and of V in shared memory; of scales (K runs two tiles ahead of V)
+// A stage is V of a tile and K of the tile two behind it, which the MMAs read one after the other: one barrier for both.
+constexpr int kAhead = 2, kStages = 4, kScales = 8;                           // stages in shared memory; tiles whose scales are kept
 constexpr uint32_t kTmem = 512, kO = 256;                                     // columns: S_i of even and odd tiles at 128 i and 128 i + 64, O_i at 256 + D i
 constexpr float kGrow = 8.f, kUp = 7.f;
 constexpr unsigned kPolynomial = 0x11;      // of eight pairs of exponentials, those that the FMA units take: the special function units are the bound
@@ -40,8 +41,8 @@ struct Segment {
 
 struct Shared {
   uint64_t described[kSegments], closed[kSegments], q_ready;
-  uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-  uint64_t s_full[2][2], p_ready[2][2], o_done[2], together, drain;            // of row tile i: scores and weights of even and odd tiles, every product with V
+  uint64_t full[kStages], empty[kStages];
+  uint64_t s_full[2][2], p_ready[2][2], o_done[2][kAhead], together, drain;    // of row tile i: scores, weights of even and odd tiles, an item's last products with V
   Segment segments[kSegments];
   float4 scales[kScales][kTile / 16];         // of 16 tokens: K's scale, log2 of V's, 1 / V's, whether there is a block
   int4 whole[kScales];                        // of 16 tokens each: whether there is a block
@@ -147,8 +148,6 @@ template <int TYPE, class S, bool BIASED, int COPIES> __device__ __forceinline__
     st_shared16((at + to[0]) ^ turn, h[0], h[1], h[2], h[3]);
     st_shared16((at + to[1]) ^ turn, h[4], h[5], h[6], h[7]);
   }
-  fence_async_smem();
-  __syncwarp();
 }
 
 // ---- warps 8..11.  A warp has 16 tokens of every tile, which are of one block, in kCopies steps of kStep tokens, 16 values a lane.
@@ -162,7 +161,7 @@ __device__ __forceinline__ void convert_tiles(const AttnParams& a, Shared& sh, u
   uint32_t to[2];                                                       // of a lane's two times 8 float16 in the first step
 #pragma unroll
   for (int h = 0; h < 2; ++h) to[h] = operand_at<kTile>(16 * warp + row, 2 * chunk + h);
-  int n = 0;
+  int n = 0, first = 0;                                                 // stages so far; tiles before this item's
   for (int segment = 0;; ++segment) {
     const int slot = segment % kSegments;
     if (!wait(a, sh, &sh.described[slot], uint32_t(segment / kSegments) & 1u)) return;
@@ -185,33 +184,43 @@ __device__ __forceinline__ void convert_tiles(const AttnParams& a, Shared& sh, u
         if (bh >= 0 && token + i * kStep >= low && token + i * kStep < high) x[i] = __ldg(reinterpret_cast<const uint4*>(from + i * kStep * S::D));
       }
     };
-    // Loads run two tiles ahead of what they are for: K of the next tile and V of this one are under way while K of this one is stored.
-    int now = look_up(tile0), next = look_up(tile0 + 1);
-    load(raw[0], 0, tile0, now);
-    for (int tile = tile0; tile < tile1; ++tile, ++n) {
-      const int after = look_up(tile + 2), stage = n % kStages;
-      load(raw[1], 1, tile, now);
+    // Stage u of an item has K of tile u and V of tile u - kAhead.  What the next one is made of is on its way while this one is stored.
+    const int tiles = tile1 - tile0;
+    int bh[kAhead + 2];                                                 // of tiles u - kAhead .. u + 1
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) bh[i] = -1;
+    bh[kAhead] = look_up(tile0);
+    bh[kAhead + 1] = look_up(tile0 + 1);
+    load(raw[0], 0, tile0, bh[kAhead]);
+    for (int u = 0; u < tiles + kAhead; ++u, ++n) {
+      const int after = look_up(tile0 + u + 2), stage = n % kStages;
+      const bool has_k = u < tiles, has_v = u >= kAhead;
+      if (has_v) load(raw[1], 1, tile0 + u - kAhead, bh[0]);
       float ks = 0.f, vs = 0.f;
-      if (now >= 0) {
-        ks = __ldg(a.c.scale[0] + now);
-        vs = __ldg(a.c.scale[1] + now);
+      if (bh[kAhead] >= 0) {
+        ks = __ldg(a.c.scale[0] + bh[kAhead]);
+        vs = __ldg(a.c.scale[1] + bh[kAhead]);
       }
-      const uint32_t lap = uint32_t(n / kStages) & 1u;
-      if (!wait(a, sh, &sh.k_empty[stage], lap ^ 1u)) return;
-      if (lane == 0) {
-        const float v = vs < 0x1p-100f ? 0x1p-100f : vs;                // (a NaN stays)
-        sh.scales[n % kScales][warp] = make_float4(ks, log2f(v), 1.f / v, now >= 0 ? 1.f : 0.f);
-        reinterpret_cast<int*>(&sh.whole[n % kScales])[warp] = now >= 0;
+      if (!wait(a, sh, &sh.empty[stage], (uint32_t(n / kStages) & 1u) ^ 1u)) return;
+      if (has_k) {
+        const int at = (first + u) % kScales;
+        if (lane == 0) {
+          const float v = vs < 0x1p-100f ? 0x1p-100f : vs;              // (a NaN stays)
+          sh.scales[at][warp] = make_float4(ks, log2f(v), 1.f / v, bh[kAhead] >= 0 ? 1.f : 0.f);
+          reinterpret_cast<int*>(&sh.whole[at])[warp] = bh[kAhead] >= 0;
+        }
+        store_operand<TYPE, S, true>(raw[0], k_smem + uint32_t(stage * S::kKv), to);
       }
-      store_operand<TYPE, S, true>(raw[0], k_smem + uint32_t(stage * S::kKv), to);
-      if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.k_full[stage]));
-      load(raw[0], 0, tile + 1, next);
-      if (!wait(a, sh, &sh.v_empty[stage], lap ^ 1u)) return;
-      store_operand<TYPE, S, false>(raw[1], v_smem + uint32_t(stage * S::kKv), to);
-      if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.v_full[stage]));
-      now = next;
-      next = after;
+      load(raw[0], 0, tile0 + u + 1, bh[kAhead + 1]);
+      if (has_v) store_operand<TYPE, S, false>(raw[1], v_smem + uint32_t(stage * S::kKv), to);
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.full[stage]));
+#pragma unroll
+      for (int i = 0; i <= kAhead; ++i) bh[i] = bh[i + 1];
+      bh[kAhead + 1] = after;
     }
+    first += tiles;
     if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.closed[slot]));
   }
 }
@@ -222,24 +231,16 @@ __device__ __forceinline__ void issue_mmas(const AttnParams& a, Shared& sh, uint
   const uint32_t tmem = sh.tmem;
   const uint32_t idesc_s = (1u << 4) | (uint32_t(kTile >> 3) << 17) | (uint32_t(kRows >> 4) << 24);                    // float16, float32 sums
   const uint32_t idesc_o = (1u << 4) | (1u << 16) | (uint32_t(S::D >> 3) << 17) | (uint32_t(kRows >> 4) << 24);        // B is MN-major
-  int n = 0;
-  auto scores = [&](int i, int tile) {                                  // S_i = Q_i K^T of a tile (numbered like n)
-    if (umma::elect_one()) {
-      const int stage = tile % kStages;
-      const uint64_t q = umma::smem_desc_sw128(q_smem + uint32_t(i * S::kQ)), k = umma::smem_desc_sw128(k_smem + uint32_t(stage * S::kKv));
+  const uint64_t q0 = umma::smem_desc_sw128(q_smem), k0 = umma::smem_desc_sw128(k_smem), v0 = smem_desc_mn(v_smem, kTile * 128);
+  int n = 0, first = 0;                                                 // stages so far; tiles before this item's
+  // S_i = Q_i K^T of a tile (numbered over all items)
+  auto scores = [&](int i, int tile, int stage) {
+    const uint64_t q = q0 + uint64_t(uint32_t(i * S::kQ) >> 4), k = k0 + uint64_t(uint32_t(stage * S::kKv) >> 4);
 #pragma unroll
-      for (int s = 0; s < S::D / 16; ++s)
-        umma_f16_ss(tmem + uint32_t(i * 128 + (tile & 1) * 64), q + uint64_t(((s >> 2) * kRows * 128 + (s & 3) * 32) >> 4),
-                    k + uint64_t(((s >> 2) * kTile * 128 + (s & 3) * 32) >> 4), idesc_s, s != 0);
-      umma::umma_commit<false>(umma::smem_u32(&sh.s_full[i][tile & 1]), 0);
-      if (i == 1) umma::umma_commit<false>(umma::smem_u32(&sh.k_empty[stage]), 0);
-    }
-    __syncwarp();
-  };
-  auto k_landed = [&](int tile) {
-    const bool ok = wait(a, sh, &sh.k_full[tile % kStages], uint32_t(tile / kStages) & 1u);
-    umma::tcgen05_fence_after();
-    return ok;
+    for (int s = 0; s < S::D / 16; ++s)
+      umma_f16_ss(tmem + uint32_t(i * 128 + (tile & 1) * 64), q + uint64_t(((s >> 2) * kRows * 128 + (s & 3) * 32) >> 4),
+                  k + uint64_t(((s >> 2) * kTile * 128 + (s & 3) * 32) >> 4), idesc_s, s != 0);
+    umma::umma_commit<false>(umma::smem_u32(&sh.s_full[i][tile & 1]), 0);
   };
   for (int segment = 0;; ++segment) {
     const int slot = segment % kSegments;
@@ -247,33 +248,30 @@ __device__ __forceinline__ void issue_mmas(const AttnParams& a, Shared& sh, uint
     const int tiles = sh.segments[slot].tile1 - sh.segments[slot].tile0;
     if (tiles == 0) return;
     if (!wait(a, sh, &sh.q_ready, uint32_t(segment) & 1u)) return;
-    for (int j = 0; j < min(2, tiles); ++j) {
-      if (!k_landed(n + j)) return;
-      scores(0, n + j);
-      scores(1, n + j);
-    }
-    for (int j = 0; j < tiles; ++j, ++n) {
-      const int stage = n % kStages;
-      if (!wait(a, sh, &sh.v_full[stage], uint32_t(n / kStages) & 1u)) return;
+    for (int u = 0; u < tiles + kAhead; ++u, ++n) {                     // stage u: V of tile j = u - kAhead, K of tile u
+      const int j = u - kAhead, stage = n % kStages;
+      if (!wait(a, sh, &sh.full[stage], uint32_t(n / kStages) & 1u)) return;
       for (int i = 0; i < 2; ++i) {
-        if (!wait(a, sh, &sh.p_ready[i][n & 1], uint32_t(n >> 1) & 1u)) return;
+        const int tile = first + j;
+        if (j >= 0 && !wait(a, sh, &sh.p_ready[i][tile & 1], uint32_t(tile >> 1) & 1u)) return;
         umma::tcgen05_fence_after();
         if (umma::elect_one()) {
-          const uint64_t v = smem_desc_mn(v_smem + uint32_t(stage * S::kKv), kTile * 128);
+          if (j >= 0) {
+            const uint64_t v = v0 + uint64_t(uint32_t(stage * S::kKv) >> 4);
 #pragma unroll
-          for (int s = 0; s < kTile / 16; ++s)
-            umma::umma_f16_ts<false>(tmem + kO + uint32_t(i * S::D), tmem + uint32_t(i * 128 + (n & 1) * 64 + 8 * s), v + uint64_t((16 * 128 * s) >> 4), idesc_o,
-                                     (j != 0 || s != 0) ? 1u : 0u);
-          umma::umma_commit<false>(umma::smem_u32(&sh.o_done[i]), 0);
-          if (i == 1) umma::umma_commit<false>(umma::smem_u32(&sh.v_empty[stage]), 0);
+            for (int s = 0; s < kTile / 16; ++s)
+              umma::umma_f16_ts<false>(tmem + kO + uint32_t(i * S::D), tmem + uint32_t(i * 128 + (tile & 1) * 64 + 8 * s), v + uint64_t((16 * 128 * s) >> 4),
+                                       idesc_o, (j != 0 || s != 0) ? 1u : 0u);
+          }
+          // The scores of the tile two on take the place of the weights just read; the barrier also says that those are in O.
+          if (u < tiles) scores(i, first + u, stage);
+          else umma::umma_commit<false>(umma::smem_u32(&sh.o_done[i][u - tiles]), 0);
+          if (i == 1) umma::umma_commit<false>(umma::smem_u32(&sh.empty[stage]), 0);
         }
         __syncwarp();
-        if (j + 2 < tiles) {                                            // into the place that the weights just read leave
-          if (i == 0 && !k_landed(n + 2)) return;
-          scores(i, n + 2);
-        }
       }
     }
+    first += tiles;
     if (umma::elect_one()) umma::mbar_arrive(umma::smem_u32(&sh.closed[slot]));
     __syncwarp();
   }
@@ -489,7 +487,10 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
       const int4 whole = sh.whole[n % kScales];
       const bool every = token0 >= all_low && token0 + kTile <= all_high && (whole.x & whole.y & whole.z & whole.w) != 0;
       const uint32_t at = tmem_s + uint32_t((n & 1) * 64);
-      auto products_done = [&] { return wait(a, sh, &sh.o_done[i], uint32_t(n - 1) & 1u); };
+      // That the tile before is in O: the scores of the tile after this one come behind it, at the end of an item its own barrier does.
+      auto products_done = [&] {
+        return tile + 1 < tile1 ? wait(a, sh, &sh.s_full[i][(n + 1) & 1], uint32_t((n + 1) >> 1) & 1u) : wait(a, sh, &sh.o_done[i][kAhead - 2], uint32_t(segment) & 1u);
+      };
       if (!(every ? tile_weights<S, true>(at, tmem_o, scales, factor, unbias, 0, 0, tile > tile0, ref, l, products_done)
                   : tile_weights<S, false>(at, tmem_o, scales, factor, unbias, low - token0, high - token0, tile > tile0, ref, l, products_done))) {
         lost = true;
@@ -501,7 +502,7 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
       if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.p_ready[i][n & 1]));
     }
     if (lost) return;
-    if (!wait(a, sh, &sh.o_done[i], uint32_t(n - 1) & 1u)) return;
+    if (!wait(a, sh, &sh.o_done[i][kAhead - 1], uint32_t(segment) & 1u)) return;
     umma::tcgen05_fence_after();
     const float f = l == 0.f ? 0.f : 1.f / l;
     float* const part = a.partial + size_t(max(sg.piece, 0)) * kPiece + size_t(i * kRows + my_row) * D;
@@ -612,17 +613,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_many_kernel(const __gri
     }
     umma::mbar_init(umma::smem_u32(&sh.q_ready), 8);
     for (int i = 0; i < kStages; ++i) {
-      umma::mbar_init(umma::smem_u32(&sh.k_full[i]), 4);
-      umma::mbar_init(umma::smem_u32(&sh.v_full[i]), 4);
-      umma::mbar_init(umma::smem_u32(&sh.k_empty[i]), 1);
-      umma::mbar_init(umma::smem_u32(&sh.v_empty[i]), 1);
+      umma::mbar_init(umma::smem_u32(&sh.full[i]), 4);
+      umma::mbar_init(umma::smem_u32(&sh.empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       for (int k = 0; k < 2; ++k) {
         umma::mbar_init(umma::smem_u32(&sh.s_full[i][k]), 1);
         umma::mbar_init(umma::smem_u32(&sh.p_ready[i][k]), 4);
       }
-      umma::mbar_init(umma::smem_u32(&sh.o_done[i]), 1);
+      for (int k = 0; k < kAhead; ++k) umma::mbar_init(umma::smem_u32(&sh.o_done[i][k]), 1);
     }
     umma::mbar_init(umma::smem_u32(&sh.together), 8);
     umma::mbar_init(umma::smem_u32(&sh.drain), 1);
