@@ -20,7 +20,8 @@ namespace many {
 
 constexpr int kRows = 128, kItemRows = 2 * kRows, kTile = 64, kLog2 = 6;       // rows of an MMA, of an item; cached tokens of a tile
 constexpr int kThreads = 512, kSegments = 4;
-// A stage is V of a tile and K of the tile two behind it, which the MMAs read one after the other: one barrier for both.
+// A stage is V of a tile and K of the tile two behind it, which the MMAs read one after the other: one barrier for both.  Items begin at stage 0 (the
+// last ones of an item may be empty): addresses of the MMAs are constants, and S of a tile is in the place that its stage's number says.
 constexpr int kAhead = 2, kStages = 4, kScales = 8;                           // stages in shared memory; tiles whose scales are kept
 constexpr uint32_t kTmem = 512, kO = 256;                                     // columns: S_i of even and odd tiles at 128 i and 128 i + 64, O_i at 256 + D i
 constexpr float kGrow = 8.f, kUp = 7.f;
@@ -42,7 +43,7 @@ struct Segment {
 struct Shared {
   uint64_t described[kSegments], closed[kSegments], q_ready;
   uint64_t full[kStages], empty[kStages];
-  uint64_t s_full[2][2], p_ready[2][2], o_done[2][kAhead], together, drain;    // of row tile i: scores, weights of even and odd tiles, an item's last products with V
+  uint64_t s_full[2][2], p_ready[2][2], together, drain;    // of row tile i, even and odd stages: its MMAs are done, its weights are there
   Segment segments[kSegments];
   float4 scales[kScales][kTile / 16];         // of 16 tokens: K's scale, log2 of V's, 1 / V's, whether there is a block
   int4 whole[kScales];                        // of 16 tokens each: whether there is a block
@@ -50,6 +51,8 @@ struct Shared {
   uint32_t tmem;
   int last, lost;
 };
+
+__device__ __forceinline__ int stages_of(int tiles) { return (tiles + kAhead + kStages - 1) / kStages * kStages; }
 
 __device__ __forceinline__ bool wait(const AttnParams& a, Shared& sh, uint64_t* bar, uint32_t parity) {      // bounded; by a converged warp
   const uint32_t at = umma::smem_u32(bar);
@@ -84,9 +87,24 @@ __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t* r) {
       "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
-__device__ __forceinline__ void umma_f16_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d), "l"(desc_a),
-               "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+// MMAs whose operands lie A_OFF, B_OFF (in 16 bytes) behind a descriptor's address.  The sums are made beside each MMA: as constants of an unrolled loop
+// they become hundreds of registers, and the issuing warp, which everything waits for, spills.
+template <int A_OFF, int B_OFF> __device__ __forceinline__ void umma_f16_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tadd.s64 a, %1, %5;\n\tadd.s64 b, %2, %6;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(tmem_d),
+               "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "n"(A_OFF), "n"(B_OFF) : "memory");
+}
+template <int A_OFF, int B_OFF> __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t.reg .b32 a;\n\tadd.s32 a, %1, %5;\n\tadd.s64 b, %2, %6;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, p;\n\t}\n" ::"r"(tmem_d),
+               "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "n"(A_OFF), "n"(B_OFF) : "memory");
+}
+// O += P V and S = Q K^T of a stage, step by step of sixteen.
+template <class S, int I> __device__ __forceinline__ void issue_weights(uint32_t tmem_o, uint32_t tmem_p, uint64_t v, uint32_t idesc, bool more) {
+  umma_f16_ts<8 * I, (16 * 128 * I) / 16>(tmem_o, tmem_p, v, idesc, more || I != 0 ? 1u : 0u);
+  if constexpr (I + 1 < kTile / 16) issue_weights<S, I + 1>(tmem_o, tmem_p, v, idesc, more);
+}
+template <class S, int I> __device__ __forceinline__ void issue_scores(uint32_t tmem_s, uint64_t q, uint64_t k, uint32_t idesc) {
+  umma_f16_ss<((I >> 2) * kRows * 128 + (I & 3) * 32) / 16, ((I >> 2) * kTile * 128 + (I & 3) * 32) / 16>(tmem_s, q, k, idesc, I != 0);
+  if constexpr (I + 1 < S::D / 16) issue_scores<S, I + 1>(tmem_s, q, k, idesc);
 }
 // V as it lies: rows of tokens (K of the product), 64 channels (N) of 128 bytes, blocks of 64 channels one after the other.
 __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr, int block_bytes) {
@@ -184,35 +202,38 @@ __device__ __forceinline__ void convert_tiles(const AttnParams& a, Shared& sh, u
         if (bh >= 0 && token + i * kStep >= low && token + i * kStep < high) x[i] = __ldg(reinterpret_cast<const uint4*>(from + i * kStep * S::D));
       }
     };
-    // Stage u of an item has K of tile u and V of tile u - kAhead.  What the next one is made of is on its way while this one is stored.
+    // Stage u of an item has K of tile u and V of tile u - kAhead.  All that it is made of was asked for while the one before was stored.
     const int tiles = tile1 - tile0;
     int bh[kAhead + 2];                                                 // of tiles u - kAhead .. u + 1
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) bh[i] = -1;
     bh[kAhead] = look_up(tile0);
     bh[kAhead + 1] = look_up(tile0 + 1);
-    load(raw[0], 0, tile0, bh[kAhead]);
-    for (int u = 0; u < tiles + kAhead; ++u, ++n) {
-      const int after = look_up(tile0 + u + 2), stage = n % kStages;
-      const bool has_k = u < tiles, has_v = u >= kAhead;
-      if (has_v) load(raw[1], 1, tile0 + u - kAhead, bh[0]);
-      float ks = 0.f, vs = 0.f;
-      if (bh[kAhead] >= 0) {
-        ks = __ldg(a.c.scale[0] + bh[kAhead]);
-        vs = __ldg(a.c.scale[1] + bh[kAhead]);
+    float ks = 0.f, vs = 0.f;                                           // of tile u
+    auto load_k = [&](int tile, int at) {
+      load(raw[0], 0, tile, at);
+      ks = vs = 0.f;
+      if (at >= 0) {
+        ks = __ldg(a.c.scale[0] + at);
+        vs = __ldg(a.c.scale[1] + at);
       }
+    };
+    load_k(tile0, bh[kAhead]);
+    for (int u = 0; u < stages_of(tiles); ++u, ++n) {
+      const int after = look_up(tile0 + u + 2), stage = n % kStages;
       if (!wait(a, sh, &sh.empty[stage], (uint32_t(n / kStages) & 1u) ^ 1u)) return;
-      if (has_k) {
+      if (u < tiles) {
         const int at = (first + u) % kScales;
         if (lane == 0) {
           const float v = vs < 0x1p-100f ? 0x1p-100f : vs;              // (a NaN stays)
-          sh.scales[at][warp] = make_float4(ks, log2f(v), 1.f / v, bh[kAhead] >= 0 ? 1.f : 0.f);
+          sh.scales[at][warp] = make_float4(ks, __log2f(v), __fdividef(1.f, v), bh[kAhead] >= 0 ? 1.f : 0.f);
           reinterpret_cast<int*>(&sh.whole[at])[warp] = bh[kAhead] >= 0;
         }
         store_operand<TYPE, S, true>(raw[0], k_smem + uint32_t(stage * S::kKv), to);
       }
-      load(raw[0], 0, tile0 + u + 1, bh[kAhead + 1]);
-      if (has_v) store_operand<TYPE, S, false>(raw[1], v_smem + uint32_t(stage * S::kKv), to);
+      load_k(tile0 + u + 1, bh[kAhead + 1]);
+      if (u >= kAhead && u < tiles + kAhead) store_operand<TYPE, S, false>(raw[1], v_smem + uint32_t(stage * S::kKv), to);
+      if (u + 1 >= kAhead) load(raw[1], 1, tile0 + u + 1 - kAhead, bh[1]);
       fence_async_smem();
       __syncwarp();
       if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.full[stage]));
@@ -232,46 +253,33 @@ __device__ __forceinline__ void issue_mmas(const AttnParams& a, Shared& sh, uint
   const uint32_t idesc_s = (1u << 4) | (uint32_t(kTile >> 3) << 17) | (uint32_t(kRows >> 4) << 24);                    // float16, float32 sums
   const uint32_t idesc_o = (1u << 4) | (1u << 16) | (uint32_t(S::D >> 3) << 17) | (uint32_t(kRows >> 4) << 24);        // B is MN-major
   const uint64_t q0 = umma::smem_desc_sw128(q_smem), k0 = umma::smem_desc_sw128(k_smem), v0 = smem_desc_mn(v_smem, kTile * 128);
-  int n = 0, first = 0;                                                 // stages so far; tiles before this item's
-  // S_i = Q_i K^T of a tile (numbered over all items)
-  auto scores = [&](int i, int tile, int stage) {
-    const uint64_t q = q0 + uint64_t(uint32_t(i * S::kQ) >> 4), k = k0 + uint64_t(uint32_t(stage * S::kKv) >> 4);
-#pragma unroll
-    for (int s = 0; s < S::D / 16; ++s)
-      umma_f16_ss(tmem + uint32_t(i * 128 + (tile & 1) * 64), q + uint64_t(((s >> 2) * kRows * 128 + (s & 3) * 32) >> 4),
-                  k + uint64_t(((s >> 2) * kTile * 128 + (s & 3) * 32) >> 4), idesc_s, s != 0);
-    umma::umma_commit<false>(umma::smem_u32(&sh.s_full[i][tile & 1]), 0);
-  };
+  int n = 0;                                                            // stages so far, a multiple of kStages
+  uint32_t weights = 0;                                                 // phases of p_ready, a bit for even and one for odd stages
   for (int segment = 0;; ++segment) {
     const int slot = segment % kSegments;
     if (!wait(a, sh, &sh.described[slot], uint32_t(segment / kSegments) & 1u)) return;
     const int tiles = sh.segments[slot].tile1 - sh.segments[slot].tile0;
     if (tiles == 0) return;
     if (!wait(a, sh, &sh.q_ready, uint32_t(segment) & 1u)) return;
-    for (int u = 0; u < tiles + kAhead; ++u, ++n) {                     // stage u: V of tile j = u - kAhead, K of tile u
-      const int j = u - kAhead, stage = n % kStages;
+    for (int u = 0; u < stages_of(tiles); ++u, ++n) {
+      const int stage = u % kStages, j = u - kAhead;                    // K of tile u, V of tile j
+      const uint64_t k = k0 + uint64_t(uint32_t(stage * S::kKv) >> 4), v = v0 + uint64_t(uint32_t(stage * S::kKv) >> 4);
       if (!wait(a, sh, &sh.full[stage], uint32_t(n / kStages) & 1u)) return;
+#pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int tile = first + j;
-        if (j >= 0 && !wait(a, sh, &sh.p_ready[i][tile & 1], uint32_t(tile >> 1) & 1u)) return;
+        if (j >= 0 && j < tiles && !wait(a, sh, &sh.p_ready[i][u & 1], (weights >> (u & 1)) & 1u)) return;
         umma::tcgen05_fence_after();
         if (umma::elect_one()) {
-          if (j >= 0) {
-            const uint64_t v = v0 + uint64_t(uint32_t(stage * S::kKv) >> 4);
-#pragma unroll
-            for (int s = 0; s < kTile / 16; ++s)
-              umma::umma_f16_ts<false>(tmem + kO + uint32_t(i * S::D), tmem + uint32_t(i * 128 + (tile & 1) * 64 + 8 * s), v + uint64_t((16 * 128 * s) >> 4),
-                                       idesc_o, (j != 0 || s != 0) ? 1u : 0u);
-          }
-          // The scores of the tile two on take the place of the weights just read; the barrier also says that those are in O.
-          if (u < tiles) scores(i, first + u, stage);
-          else umma::umma_commit<false>(umma::smem_u32(&sh.o_done[i][u - tiles]), 0);
+          const uint32_t scores = tmem + uint32_t(i * 128 + (u & 1) * 64);
+          if (j >= 0 && j < tiles) issue_weights<S, 0>(tmem + kO + uint32_t(i * S::D), scores, v, idesc_o, j != 0);
+          if (u < tiles) issue_scores<S, 0>(scores, q0 + uint64_t((i * S::kQ) >> 4), k, idesc_s);      // into the place of the weights just read
+          umma::umma_commit<false>(umma::smem_u32(&sh.s_full[i][u & 1]), 0);
           if (i == 1) umma::umma_commit<false>(umma::smem_u32(&sh.empty[stage]), 0);
         }
         __syncwarp();
       }
+      if (j >= 0 && j < tiles) weights ^= 1u << (u & 1);
     }
-    first += tiles;
     if (umma::elect_one()) umma::mbar_arrive(umma::smem_u32(&sh.closed[slot]));
     __syncwarp();
   }
@@ -319,31 +327,65 @@ __device__ __forceinline__ float2 exp2_pair(uint64_t x) {
   return make_float2(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(e.x) << 23)), __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(e.y) << 23)));
 }
 
-// A row's tile: the largest score, the sums so far brought to it if it has outgrown them, weights into the scores' place.  EVERY: the row sees
-// all of its columns, else those in [low, high) of blocks that are there.  products_done: waits for the tile before to be in O; false where that gives up.
+// Weights of 32 columns (two blocks' scales), their sum over each block's V scale; the largest y = s + log2(vs) of them.
+// EVERY: the row sees all of its columns, else those in [low, high) of blocks that are there.
+template <bool EVERY>
+__device__ __forceinline__ void weights_of(const uint32_t (&r)[32], const float4 (&x)[2], float factor, float unbias, int low, int high, float bias, uint32_t (&p)[16],
+                                           float& l, float& top) {
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const float f = x[g].x * factor, add = fmaf(-unbias, f, x[g].y + bias);
+    const uint64_t ff = pair_of(f, f), aa = pair_of(add, add);
+    uint64_t sum[2] = {0u, 0u};
+    float best = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 16; k += 2) {
+      const float s[2] = {__uint_as_float(r[16 * g + k]), __uint_as_float(r[16 * g + k + 1])};
+      const uint64_t y = fma2(pair_of(s[0], s[1]), ff, aa);
+      float w[2];
+      if (EVERY && (kPolynomial >> (k / 2) & 1) != 0) {                 // (a NaN is lost there: the row's other columns of the block have it)
+        const float2 e = exp2_pair(y);
+        w[0] = e.x;
+        w[1] = e.y;
+      } else {
+        w[0] = exp2_approx(halves_of(y).x);
+        w[1] = exp2_approx(halves_of(y).y);
+      }
+      if (EVERY) {
+        best = max3(best, s[0], s[1]);
+      } else {                                                          // what is not seen has no weight, whatever the block's scales are
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const bool seen = x[g].w != 0.f && 16 * g + k + j >= low && 16 * g + k + j < high;
+          w[j] = seen ? w[j] : 0.f;
+          best = fmaxf(best, seen ? s[j] : -INFINITY);
+        }
+      }
+      sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], pair_of(w[0], w[1]));
+      p[8 * g + k / 2] = pack_half(w[0], w[1]);
+    }
+    const float2 both = halves_of(add2(sum[0], sum[1]));
+    if (EVERY || both.x + both.y != 0.f) l = fmaf(both.x + both.y, x[g].z, l);
+    if (EVERY || best != -INFINITY) top = fmaxf(top, fmaf(best - unbias, f, x[g].y));
+  }
+}
+
+// A row's tile: weights into the scores' place, their sum to l.  They are taken relative to what was the largest so far, at once, and again where the tile has
+// outgrown that (O is brought along then, once products_done() says that the tile before is in it; false where that gives up): the first tiles do.
 template <class S, bool EVERY, typename Wait>
 __device__ __forceinline__ bool tile_weights(uint32_t tmem_s, uint32_t tmem_o, const float4* scales, float factor, float unbias, int low, int high, bool more,
                                              float& ref, float& l, Wait products_done) {
-  uint32_t r[kTile];
-  tmem_ld32(tmem_s, r);
-  tmem_ld32(tmem_s + 32u, r + 32);
-  float4 x[kTile / 16];
+  uint32_t r[2][32], p[2][16];
+  tmem_ld32(tmem_s, r[0]);
+  float4 x[2][2];
 #pragma unroll
-  for (int g = 0; g < kTile / 16; ++g) x[g] = scales[g];
+  for (int g = 0; g < 4; ++g) x[g >> 1][g & 1] = scales[g];
   umma::tmem_ld_wait();
-  float top = -INFINITY;
-#pragma unroll
-  for (int g = 0; g < kTile / 16; ++g) {
-    float s[16];
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      s[k] = __uint_as_float(r[16 * g + k]);
-      if (!EVERY) s[k] = x[g].w != 0.f && 16 * g + k >= low && 16 * g + k < high ? s[k] : -INFINITY;
-    }
-    const float u = max3(max3(s[0], s[1], s[2]), s[3], s[4]), v = max3(max3(s[5], s[6], s[7]), s[8], s[9]), w = max3(max3(s[10], s[11], s[12]), s[13], s[14]);
-    const float best = max3(u, v, fmaxf(w, s[15])), f = x[g].x * factor;
-    if (EVERY || best != -INFINITY) top = fmaxf(top, fmaf(best - unbias, f, x[g].y));
-  }
+  tmem_ld32(tmem_s + 32u, r[1]);
+  float bias = (ref == -INFINITY ? 0.f : -ref) + kUp, sum = 0.f, top = -INFINITY;
+  weights_of<EVERY>(r[0], x[0], factor, unbias, low, high, bias, p[0], sum, top);
+  umma::tmem_ld_wait();
+  weights_of<EVERY>(r[1], x[1], factor, unbias, low - 32, high - 32, bias, p[1], sum, top);
   const bool grow = top > ref + kGrow || (ref == -INFINITY && top != -INFINITY);
   if (__any_sync(0xffffffffu, grow)) {
     const float old = ref;
@@ -363,37 +405,25 @@ __device__ __forceinline__ bool tile_weights(uint32_t tmem_s, uint32_t tmem_o, c
         tmem_st32(tmem_o + uint32_t(32 * c), o);
       }
     }
-  }
-  const float bias = (ref == -INFINITY ? 0.f : -ref) + kUp;
-  uint32_t p[kTile / 2];
+    bias = (ref == -INFINITY ? 0.f : -ref) + kUp;
+    sum = 0.f;
+    float again = -INFINITY;
+#pragma unroll 1
+    for (int c = 0; c < 2; ++c) {
+      uint32_t s[32], w[16];
+      tmem_ld32(tmem_s + uint32_t(32 * c), s);
+      float4 y[2] = {scales[2 * c], scales[2 * c + 1]};
+      umma::tmem_ld_wait();
+      weights_of<false>(s, y, factor, unbias, EVERY ? 0 : low - 32 * c, EVERY ? 32 : high - 32 * c, bias, w, sum, again);
 #pragma unroll
-  for (int g = 0; g < kTile / 16; ++g) {
-    const float f = x[g].x * factor, add = fmaf(-unbias, f, x[g].y + bias);
-    const uint64_t ff = pair_of(f, f), aa = pair_of(add, add);
-    uint64_t sum[2] = {0u, 0u};
-#pragma unroll
-    for (int k = 0; k < 16; k += 2) {
-      const uint64_t y = fma2(pair_of(__uint_as_float(r[16 * g + k]), __uint_as_float(r[16 * g + k + 1])), ff, aa);
-      float w[2];
-      if (EVERY && (kPolynomial >> (k / 2) & 1) != 0) {                 // (a NaN is lost there: the row's other columns of the block have it)
-        const float2 e = exp2_pair(y);
-        w[0] = e.x;
-        w[1] = e.y;
-      } else {
-        w[0] = exp2_approx(halves_of(y).x);
-        w[1] = exp2_approx(halves_of(y).y);
+      for (int k = 0; k < 16; ++k) {
+        if (c == 0) p[0][k] = w[k]; else p[1][k] = w[k];
       }
-      if (!EVERY) {                                                     // what is not seen has no weight, whatever the block's scales are
-#pragma unroll
-        for (int j = 0; j < 2; ++j) w[j] = x[g].w != 0.f && 16 * g + k + j >= low && 16 * g + k + j < high ? w[j] : 0.f;
-      }
-      sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], pair_of(w[0], w[1]));
-      p[8 * g + k / 2] = pack_half(w[0], w[1]);
     }
-    const float2 both = halves_of(add2(sum[0], sum[1]));
-    if (EVERY || both.x + both.y != 0.f) l = fmaf(both.x + both.y, x[g].z, l);
   }
-  tmem_st32(tmem_s, p);
+  l += sum;
+  umma::tmem_st16(tmem_s, p[0]);
+  umma::tmem_st16(tmem_s + 16u, p[1]);
   return true;
 }
 
@@ -403,7 +433,7 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
   constexpr int D = S::D, kPiece = kItemRows * (D + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = warp >> 2, my_row = 32 * (warp & 3) + lane;
   const uint32_t lanes = sh.tmem + (uint32_t(32 * (warp & 3)) << 16), tmem_s = lanes + uint32_t(i * 128), tmem_o = lanes + kO + uint32_t(i * D);
-  int n = 0, meetings = 0;
+  int n = 0, first = 0, meetings = 0;                                   // stages, tiles so far
   auto meet = [&] {
     __syncwarp();
     if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.together));
@@ -479,30 +509,32 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
     const int base = (sg.item.low >> kLog2) << kLog2;
     float ref = -INFINITY, l = 0.f;
     bool lost = false;
-    for (int tile = tile0; tile < tile1; ++tile, ++n) {
-      if (!wait(a, sh, &sh.s_full[i][n & 1], uint32_t(n >> 1) & 1u)) { lost = true; break; }
+    const int tiles = tile1 - tile0;
+    for (int u = 0; u < tiles; ++u) {
+      const int tile = tile0 + u;
+      if (!wait(a, sh, &sh.s_full[i][u & 1], uint32_t((n + u) >> 1) & 1u)) { lost = true; break; }
       umma::tcgen05_fence_after();
-      const float4* const scales = sh.scales[n % kScales];
+      const float4* const scales = sh.scales[(first + u) % kScales];
       const int token0 = base + tile * kTile;
-      const int4 whole = sh.whole[n % kScales];
+      const int4 whole = sh.whole[(first + u) % kScales];
       const bool every = token0 >= all_low && token0 + kTile <= all_high && (whole.x & whole.y & whole.z & whole.w) != 0;
-      const uint32_t at = tmem_s + uint32_t((n & 1) * 64);
-      // That the tile before is in O: the scores of the tile after this one come behind it, at the end of an item its own barrier does.
-      auto products_done = [&] {
-        return tile + 1 < tile1 ? wait(a, sh, &sh.s_full[i][(n + 1) & 1], uint32_t((n + 1) >> 1) & 1u) : wait(a, sh, &sh.o_done[i][kAhead - 2], uint32_t(segment) & 1u);
-      };
-      if (!(every ? tile_weights<S, true>(at, tmem_o, scales, factor, unbias, 0, 0, tile > tile0, ref, l, products_done)
-                  : tile_weights<S, false>(at, tmem_o, scales, factor, unbias, low - token0, high - token0, tile > tile0, ref, l, products_done))) {
+      const uint32_t at = tmem_s + uint32_t((u & 1) * 64);
+      auto products_done = [&] { return wait(a, sh, &sh.s_full[i][(u + 1) & 1], uint32_t((n + u + 1) >> 1) & 1u); };      // the MMAs of the stage after this one
+      if (!(every ? tile_weights<S, true>(at, tmem_o, scales, factor, unbias, 0, 0, u > 0, ref, l, products_done)
+                  : tile_weights<S, false>(at, tmem_o, scales, factor, unbias, low - token0, high - token0, u > 0, ref, l, products_done))) {
         lost = true;
         break;
       }
       umma::tmem_st_wait();
       umma::tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.p_ready[i][n & 1]));
+      if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.p_ready[i][u & 1]));
     }
     if (lost) return;
-    if (!wait(a, sh, &sh.o_done[i][kAhead - 1], uint32_t(segment) & 1u)) return;
+    for (int u = tiles; u < stages_of(tiles); ++u)                       // the last of the products among them
+      if (!wait(a, sh, &sh.s_full[i][u & 1], uint32_t((n + u) >> 1) & 1u)) return;
+    n += stages_of(tiles);
+    first += tiles;
     umma::tcgen05_fence_after();
     const float f = l == 0.f ? 0.f : 1.f / l;
     float* const part = a.partial + size_t(max(sg.piece, 0)) * kPiece + size_t(i * kRows + my_row) * D;
@@ -621,7 +653,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_many_kernel(const __gri
         umma::mbar_init(umma::smem_u32(&sh.s_full[i][k]), 1);
         umma::mbar_init(umma::smem_u32(&sh.p_ready[i][k]), 4);
       }
-      for (int k = 0; k < kAhead; ++k) umma::mbar_init(umma::smem_u32(&sh.o_done[i][k]), 1);
     }
     umma::mbar_init(umma::smem_u32(&sh.together), 8);
     umma::mbar_init(umma::smem_u32(&sh.drain), 1);
