@@ -117,6 +117,11 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
 __device__ __forceinline__ void st_shared16(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 // Address of 16 bytes (8 float16) of an operand tile of ROWS rows: rows of 64 values with the 128-byte swizzle, blocks of 64 columns one after the other.
 template <int ROWS> __device__ __forceinline__ uint32_t operand_at(int row, int chunk) {
@@ -427,6 +432,135 @@ __device__ __forceinline__ bool tile_weights(uint32_t tmem_s, uint32_t tmem_o, c
   return true;
 }
 
+// Where row r of an item stands among packed rows and heads, times head_dim.
+__device__ __forceinline__ int64_t place_of(const AttnParams& a, const Segment& sg, int r) {
+  const int token = a.by_group(sg.item.r0 + r), head = sg.head * a.group + sg.item.r0 + r - token * a.group;
+  return (int64_t(sg.s.row + token) * a.heads + head) * a.c.dim;
+}
+
+// q of a warp's 32 rows, from row r0 of the sequence, into its place in shared memory; factor, unbias: of the row of this lane.  D / 8 lanes have a row.
+template <int TYPE, class S>
+__device__ __forceinline__ void open_rows(const AttnParams& a, const Segment& sg, uint32_t q_smem, int r0, float& factor, float& unbias) {
+  constexpr int kLanes = S::D / 8, kStep = 32 / kLanes, kSteps = 32 / kStep;      // of a row; rows at once
+  const int lane = threadIdx.x & 31, chunk = lane % kLanes, sub = lane / kLanes, row0 = 32 * ((threadIdx.x >> 5) & 3);
+  const bool wide = ((reinterpret_cast<uintptr_t>(a.q) | uint64_t(a.row_stride * 2) | uint64_t(a.head_stride * 2)) & 15) == 0, f16 = a.dtype == DINO_F16;
+  uint4 x[kSteps];
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) {
+    const int r = r0 + kStep * k + sub, token = a.by_group(min(r, sg.item.r1 - 1)), head = sg.head * a.group + r - token * a.group;
+    const uint16_t* src = static_cast<const uint16_t*>(a.q) + int64_t(sg.s.row + token) * a.row_stride + int64_t(head) * a.head_stride + 8 * chunk;
+    x[k] = make_uint4(0u, 0u, 0u, 0u);
+    if (r < sg.item.r1) {
+      if (wide) {
+        x[k] = __ldg(reinterpret_cast<const uint4*>(src));
+      } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = uint32_t(src[2 * j]) | (uint32_t(src[2 * j + 1]) << 16);
+        x[k] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) {
+    // The largest of the 16-bit magnitudes, whose order is that of the values.
+    uint32_t largest = __vmaxu2(__vmaxu2(x[k].x & 0x7fff7fffu, x[k].y & 0x7fff7fffu), __vmaxu2(x[k].z & 0x7fff7fffu, x[k].w & 0x7fff7fffu));
+    largest = max(largest & 0xffffu, largest >> 16);
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+    const float top = f16 ? __half2float(__ushort_as_half(uint16_t(largest))) : __uint_as_float(largest << 16);
+    const uint32_t e = __float_as_uint(top) >> 23;
+    const bool plain = e == 0 || e == 255;
+    const int shift = plain ? 0 : min(max(127 + 12 - int(e), -126), 126);
+    const float up = __uint_as_float(uint32_t(127 + shift) << 23), down = __uint_as_float(uint32_t(127 - shift) << 23);
+    const float sign = a.scale < 0.f ? -up : up;                        // scores' factors are not negative
+    const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+    uint32_t h[4];
+    float total = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 v = f16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[j])) : make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+      h[j] = pack_half(v.x * sign, v.y * sign);
+      const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+      total += back.x + back.y;
+    }
+    st_shared16(q_smem + operand_at<kRows>(row0 + kStep * k + sub, chunk), h[0], h[1], h[2], h[3]);
+    if (Half2Of<TYPE>::kBias != 0.f) {                                  // K's of int8 are that much too large
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+#pragma unroll
+    for (int j = 0; j < kStep; ++j) {                                   // to the lanes of these rows
+      const float d = __shfl_sync(0xffffffffu, down, j * kLanes), t = __shfl_sync(0xffffffffu, total, j * kLanes);
+      if (lane == kStep * k + j) {
+        factor = fabsf(a.scale) * d;
+        unbias = Half2Of<TYPE>::kBias * t;
+      }
+    }
+  }
+  fence_async_smem();
+  __syncwarp();
+}
+
+// O of a warp's 32 rows (row0: the first one's number in the item): results, or float32 sums of a piece.  Through the place of q, which nobody reads any more:
+// 256 bytes a row there, chunks of 16 bytes turned by the row's number, so that rows leave in whole lines.
+template <class S>
+__device__ __forceinline__ void close_rows(const AttnParams& a, const Segment& sg, uint32_t q_smem, uint32_t tmem_o, int row0, float inverse) {
+  constexpr int D = S::D, kPiece = kItemRows * (D + 2);
+  const int lane = threadIdx.x & 31, rows = sg.item.r1 - sg.item.r0 - row0;      // of this warp's
+  const uint32_t mine = q_smem + uint32_t(((threadIdx.x >> 5) & 3) * 32 * D * 2);
+  auto at = [&](int row, int chunk) { return mine + uint32_t(row * D * 2) + uint32_t((chunk ^ (row & (D / 8 - 1))) << 4); };
+  if (sg.piece < 0) {
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      uint32_t o[32], h[16];
+      tmem_ld32(tmem_o + uint32_t(32 * c), o);
+      umma::tmem_ld_wait();
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const float u = __uint_as_float(o[2 * k]) * inverse, v = __uint_as_float(o[2 * k + 1]) * inverse;
+        if (a.dtype == DINO_F16) {
+          h[k] = pack_half(u, v);
+        } else {
+          const __nv_bfloat162 x = __floats2bfloat162_rn(u, v);
+          h[k] = *reinterpret_cast<const uint32_t*>(&x);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) st_shared16(at(lane, 4 * c + k), h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]);
+    }
+    __syncwarp();
+    constexpr int kLanes = D / 8, kStep = 32 / kLanes;
+#pragma unroll 4
+    for (int k = 0; k < 32; k += kStep) {
+      const int row = k + lane / kLanes, chunk = lane % kLanes;
+      if (row < rows) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + place_of(a, sg, row0 + row) + 8 * chunk) = lds128(at(row, chunk));
+    }
+    __syncwarp();
+    return;
+  }
+  float* const part = a.partial + size_t(sg.piece) * kPiece + size_t(row0) * D;
+#pragma unroll 1
+  for (int half = 0; half < 2; ++half) {                                // D / 2 columns at a time
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+      uint32_t o[32];
+      tmem_ld32(tmem_o + uint32_t(half * (D / 2) + 32 * c), o);
+      umma::tmem_ld_wait();
+#pragma unroll
+      for (int k = 0; k < 8; ++k) st_shared16(at(lane, 8 * c + k), o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+    }
+    __syncwarp();
+    constexpr int kLanes = D / 8, kStep = 32 / kLanes;
+#pragma unroll 4
+    for (int k = 0; k < 32; k += kStep) {
+      const int row = k + lane / kLanes, chunk = lane % kLanes;
+      if (row < rows) __stcg(reinterpret_cast<uint4*>(part + size_t(row) * D + half * (D / 2) + 4 * chunk), lds128(at(row, chunk)));
+    }
+    __syncwarp();
+  }
+}
+
 // ---- warps 0..7: tile i of the item, a row per thread
 template <int TYPE, class S>
 __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, uint32_t q_smem) {
@@ -447,62 +581,10 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
     if (tile0 == tile1) return;
     const int r = sg.item.r0 + i * kRows + my_row;
     const bool mine = r < sg.item.r1;
-    const int token = a.by_group(mine ? r : sg.item.r0), head = sg.head * a.group + (mine ? r : sg.item.r0) - token * a.group;
-    const int64_t out_at = (int64_t(sg.s.row + token) * a.heads + head) * D;
-    float factor, unbias = 0.f;
-    {                                                                   // q of this row
-      const int64_t at = int64_t(sg.s.row + token) * a.row_stride + int64_t(head) * a.head_stride;
-      const bool wide = ((reinterpret_cast<uintptr_t>(a.q) | uint64_t(a.row_stride * 2) | uint64_t(a.head_stride * 2)) & 15) == 0;
-      const uint16_t* src = static_cast<const uint16_t*>(a.q) + at;
-      uint32_t x[D / 2];
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (mine) {
-          if (wide) {
-            v = __ldg(reinterpret_cast<const uint4*>(src + 8 * c));
-          } else {
-            uint32_t w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = uint32_t(src[8 * c + 2 * k]) | (uint32_t(src[8 * c + 2 * k + 1]) << 16);
-            v = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-        x[4 * c] = v.x; x[4 * c + 1] = v.y; x[4 * c + 2] = v.z; x[4 * c + 3] = v.w;
-      }
-      uint32_t largest = 0;                                             // of the 16-bit magnitudes: their order is that of the values
-#pragma unroll
-      for (int k = 0; k < D / 2; ++k) largest = __vmaxu2(largest, x[k] & 0x7fff7fffu);
-      largest = max(largest & 0xffffu, largest >> 16);
-      const bool f16 = a.dtype == DINO_F16;
-      const float top = f16 ? __half2float(__ushort_as_half(uint16_t(largest))) : __uint_as_float(largest << 16);
-      const uint32_t e = __float_as_uint(top) >> 23;
-      const bool plain = e == 0 || e == 255;
-      const int shift = plain ? 0 : min(max(127 + 12 - int(e), -126), 126);
-      const float up = __uint_as_float(uint32_t(127 + shift) << 23);
-      const float sign = a.scale < 0.f ? -up : up;                      // scores' factors are not negative
-      factor = fabsf(a.scale) * __uint_as_float(uint32_t(127 - shift) << 23);
-      const uint32_t q = q_smem + uint32_t(i * S::kQ);
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        uint32_t h[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t w = x[4 * c + k];
-          float2 v;
-          if (f16) v = __half22float2(*reinterpret_cast<const __half2*>(&w));
-          else v = make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-          h[k] = pack_half(v.x * sign, v.y * sign);
-          const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h[k]));
-          unbias += back.x + back.y;
-        }
-        st_shared16(q + operand_at<kRows>(my_row, c), h[0], h[1], h[2], h[3]);
-      }
-      unbias *= Half2Of<TYPE>::kBias;                                   // K's of int8 are that much too large
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.q_ready));
-    }
+    const int token = a.by_group(mine ? r : sg.item.r0);
+    float factor = 0.f, unbias = 0.f;
+    open_rows<TYPE, S>(a, sg, q_smem + uint32_t(i * S::kQ), sg.item.r0 + i * kRows + 32 * (warp & 3), factor, unbias);
+    if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.q_ready));
     const int position = sg.s.first + token;
     const int high = mine ? min(position + 1, sg.s.end) : 0, low = a.window > 0 ? max(0, position - a.window + 1) : 0;
     const int all_high = __reduce_min_sync(0xffffffffu, mine ? high : INT32_MAX), all_low = __reduce_max_sync(0xffffffffu, mine ? low : 0);
@@ -536,35 +618,7 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
     n += stages_of(tiles);
     first += tiles;
     umma::tcgen05_fence_after();
-    const float f = l == 0.f ? 0.f : 1.f / l;
-    float* const part = a.partial + size_t(max(sg.piece, 0)) * kPiece + size_t(i * kRows + my_row) * D;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-      uint32_t o[32];
-      tmem_ld32(tmem_o + uint32_t(32 * c), o);
-      umma::tmem_ld_wait();
-      if (mine && sg.piece >= 0) {
-#pragma unroll
-        for (int k = 0; k < 32; k += 4)
-          __stcg(reinterpret_cast<uint4*>(part + 32 * c + k), make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]));
-      } else if (mine) {
-        uint32_t h[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float u = __uint_as_float(o[2 * k]) * f, v = __uint_as_float(o[2 * k + 1]) * f;
-          if (a.dtype == DINO_F16) {
-            h[k] = pack_half(u, v);
-          } else {
-            const __nv_bfloat162 x = __floats2bfloat162_rn(u, v);
-            h[k] = *reinterpret_cast<const uint32_t*>(&x);
-          }
-        }
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + out_at + 32 * c);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) dst[k] = make_uint4(h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]);
-      }
-      __syncwarp();
-    }
+    close_rows<S>(a, sg, q_smem + uint32_t(i * S::kQ), tmem_o, i * kRows + 32 * (warp & 3), l == 0.f ? 0.f : 1.f / l);
     umma::tcgen05_fence_before();
     if (sg.piece >= 0) {                                                // cut: the last of its CTAs to arrive adds the pieces up, in order
       if (mine) __stcg(reinterpret_cast<float2*>(a.partial + size_t(sg.piece) * kPiece + kItemRows * D) + (i * kRows + my_row), make_float2(ref, l));
@@ -578,7 +632,7 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
       if (!meet()) return;
       if (sh.last) {
         const int rows = sg.item.r1 - sg.item.r0, count = sg.c1 - sg.c0 + 1;
-        constexpr int U = 4;                                            // places under way at a time
+        constexpr int U = 4, P = 3;                                     // places and pieces under way at a time
         for (int x0 = int(threadIdx.x); x0 < rows * (D / 4); x0 += 256 * U) {
           float high_ref[U], sum[U];
           float4 v[U];
@@ -588,32 +642,38 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
             sum[u] = 0.f;
             v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
           }
-          for (int c = 0; c < count; ++c) {
-            const float* src = a.partial + size_t(c == 0 ? sg.piece0 : 2 * (sg.c0 + c)) * kPiece;
-            float2 ml[U];
-            float4 y[U];
+          for (int c = 0; c < count; c += P) {
+            float2 ml[P][U];
+            float4 y[P][U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-              const int x = min(x0 + 256 * u, rows * (D / 4) - 1);
-              ml[u] = __ldcg(reinterpret_cast<const float2*>(src + kItemRows * D) + x / (D / 4));
-              y[u] = __ldcg(reinterpret_cast<const float4*>(src) + x);
-            }
+            for (int k = 0; k < P; ++k)
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-              const float next = fmaxf(high_ref[u], ml[u].x);
-              const float f0 = high_ref[u] == -INFINITY ? 1.f : exp2_approx(high_ref[u] - next), f1 = ml[u].x == -INFINITY ? 1.f : exp2_approx(ml[u].x - next);
-              sum[u] = fmaf(ml[u].y, f1, sum[u] * f0);
-              v[u] = make_float4(fmaf(y[u].x, f1, v[u].x * f0), fmaf(y[u].y, f1, v[u].y * f0), fmaf(y[u].z, f1, v[u].z * f0), fmaf(y[u].w, f1, v[u].w * f0));
-              high_ref[u] = next;
-            }
+              for (int u = 0; u < U; ++u) {
+                const int x = min(x0 + 256 * u, rows * (D / 4) - 1);
+                ml[k][u] = make_float2(-INFINITY, 0.f);
+                y[k][u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (c + k < count) {
+                  const float* src = a.partial + size_t(c + k == 0 ? sg.piece0 : 2 * (sg.c0 + c + k)) * kPiece;
+                  ml[k][u] = __ldcg(reinterpret_cast<const float2*>(src + kItemRows * D) + x / (D / 4));
+                  y[k][u] = __ldcg(reinterpret_cast<const float4*>(src) + x);
+                }
+              }
+#pragma unroll
+            for (int k = 0; k < P; ++k)
+#pragma unroll
+              for (int u = 0; u < U; ++u) {
+                const float next = fmaxf(high_ref[u], ml[k][u].x);
+                const float f0 = high_ref[u] == -INFINITY ? 1.f : exp2_approx(high_ref[u] - next), f1 = ml[k][u].x == -INFINITY ? 1.f : exp2_approx(ml[k][u].x - next);
+                sum[u] = fmaf(ml[k][u].y, f1, sum[u] * f0);
+                v[u] = make_float4(fmaf(y[k][u].x, f1, v[u].x * f0), fmaf(y[k][u].y, f1, v[u].y * f0), fmaf(y[k][u].z, f1, v[u].z * f0), fmaf(y[k][u].w, f1, v[u].w * f0));
+                high_ref[u] = next;
+              }
           }
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             const int x = x0 + 256 * u, row = x / (D / 4), d = x % (D / 4) * 4;
             if (row >= rows) continue;
             const float inv = sum[u] == 0.f ? 0.f : 1.f / sum[u];
-            const int t = a.by_group(sg.item.r0 + row), hd = sg.head * a.group + sg.item.r0 + row - t * a.group;
-            const int64_t at = (int64_t(sg.s.row + t) * a.heads + hd) * D + d;
             uint2 h;
             if (a.dtype == DINO_F16) {
               h = make_uint2(pack_half(v[u].x * inv, v[u].y * inv), pack_half(v[u].z * inv, v[u].w * inv));
@@ -621,7 +681,7 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
               const __nv_bfloat162 lo = __floats2bfloat162_rn(v[u].x * inv, v[u].y * inv), hi = __floats2bfloat162_rn(v[u].z * inv, v[u].w * inv);
               h = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
             }
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = h;
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + place_of(a, sg, row) + d) = h;
           }
         }
       }
