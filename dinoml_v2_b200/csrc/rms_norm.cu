@@ -1,5 +1,9 @@
-// Root-mean-square norm with the residual's addition: t = x + residual, y = t / sqrt(mean(t^2) + eps) * weight, one CTA per row, in float32 with one
-// rounding at the end; y in the activation type or as Q8_0 blocks.
+// Root-mean-square norm with the residual's addition: t = x + residual, y = t / sqrt(mean(t^2) + eps) * weight, in float32 with one rounding at the
+// end; y in the activation type or as Q8_0 blocks.
+//
+// Bound by bytes: x and the residual in, t and y out.  A CTA has a row and a thread keeps its values of t in registers between the sum of squares and the
+// products, so each is read once; rows that registers do not hold are read a second time (from L2).  NT threads of V values, R rounds: as few threads as hold a row
+// in 16 bytes each, since a CTA of few warps starts and meets sooner.
 #include "kv_cache.cuh"
 
 namespace b200gguf {
@@ -8,38 +12,153 @@ namespace norm {
 using kv::from_float;
 using kv::to_float;
 
-template <typename T, typename W>
-__global__ void __launch_bounds__(256) rms_norm_kernel(const T* x, const T* residual, const W* weight, void* y, T* total, int width, float eps, bool q8_0) {
-  __shared__ float sums[8];
-  const int64_t row = blockIdx.x;
-  x += row * width;
-  auto value = [&](int i) { return to_float<T>(x[i]) + (residual != nullptr ? to_float<T>(residual[row * width + i]) : 0.f); };
-  float sum = 0.f;
-  for (int i = threadIdx.x; i < width; i += 256) {
-    const float t = value(i);
-    sum += t * t;
+// V values from or to memory: WIDE: at an address that is a multiple of 16, in accesses of 16 bytes.
+template <typename T, int N> struct alignas(sizeof(T) * N) Vec { T v[N]; };
+template <bool WIDE, int V, typename T> __device__ __forceinline__ void load_values(const T* p, float (&t)[V]) {
+  constexpr int N = !WIDE ? 1 : V * int(sizeof(T)) > 16 ? 16 / int(sizeof(T)) : V;
+#pragma unroll
+  for (int i = 0; i < V; i += N) {
+    const Vec<T, N> a = *reinterpret_cast<const Vec<T, N>*>(p + i);
+#pragma unroll
+    for (int j = 0; j < N; ++j) t[i + j] = to_float<T>(a.v[j]);
   }
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum;
-  __syncthreads();
-  sum = 0.f;
-  for (int i = 0; i < 8; ++i) sum += sums[i];
-  const float r = rsqrtf(sum / float(width) + eps);
-  for (int i = threadIdx.x; i < width; i += 256) {                // total may be x or residual: a value is read and written by one thread
-    const float t = value(i), v = t * r * to_float<W>(weight[i]);
-    if (total != nullptr) total[row * width + i] = from_float<T>(t);
-    if (!q8_0) {
-      static_cast<T*>(y)[row * width + i] = from_float<T>(v);
-    } else {                                                     // whole warps: width is a multiple of 32
-      const float largest = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu));
-      const __half d = __float2half_rn(__fmul_rn(largest, 1.0f / 127.0f));
-      const float scale = __half2float(d);
-      uint8_t* block = static_cast<uint8_t*>(y) + (row * width + i) / 32 * 34;
-      const int lane = threadIdx.x & 31;
-      block[2 + lane] = scale > 0.f ? uint8_t(__float2int_rn(fminf(fmaxf(__fdiv_rn(v, scale), -127.f), 127.f))) : 0;
-      if (lane == 0) *reinterpret_cast<__half*>(block) = d;
+}
+template <bool WIDE, int V, typename T> __device__ __forceinline__ void store_values(T* p, const float (&t)[V]) {
+  constexpr int N = WIDE ? V : 1;
+#pragma unroll
+  for (int i = 0; i < V; i += N) {
+    Vec<T, N> a;
+#pragma unroll
+    for (int j = 0; j < N; ++j) a.v[j] = from_float<T>(t[i + j]);
+    *reinterpret_cast<Vec<T, N>*>(p + i) = a;
+  }
+}
+
+template <typename T, typename W, int V, bool WIDE, int R, int NT, bool Q8>
+__global__ void __launch_bounds__(NT) rms_norm_kernel(const T* x, const T* residual, const W* weight, void* y, T* total, int width, float eps) {
+  __shared__ float sums[NT / 32 > 1 ? NT / 32 : 1];
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int64_t row = blockIdx.x;
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  x += row * width;
+  if (residual != nullptr) residual += row * width;
+  auto load = [&](int i, float (&t)[V]) {
+    load_values<WIDE, V>(x + i, t);
+    if (residual != nullptr) {
+      float u[V];
+      load_values<WIDE, V>(residual + i, u);
+#pragma unroll
+      for (int j = 0; j < V; ++j) t[j] += u[j];
+    }
+  };
+  const int first = tid * V, step = NT * V;
+  float t[R][V], sum = 0.f;
+  bool in[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    in[r] = first + r * step < width;
+    if (in[r]) {
+      load(first + r * step, t[r]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) t[r][j] = 0.f;
     }
   }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) s = fmaf(t[r][j], t[r][j], s);
+    sum += s;
+  }
+  for (int i = first + R * step; i < width; i += step) {                 // what registers do not hold
+    float u[V], s = 0.f;
+    load(i, u);
+#pragma unroll
+    for (int j = 0; j < V; ++j) s = fmaf(u[j], u[j], s);
+    sum += s;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (NT > 32) {
+    if (lane == 0) sums[tid >> 5] = sum;
+    __syncthreads();
+    sum = lane < NT / 32 ? sums[lane] : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  }
+  const float scale = rsqrtf(sum / float(width) + eps);
+  auto finish = [&](int i, const float (&u)[V], bool here) {             // (called by whole warps where there are blocks)
+    float v[V];
+    if (here) {
+      float w[V];
+      load_values<WIDE, V>(weight + i, w);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = u[j] * scale * w[j];
+      if (total != nullptr) store_values<WIDE, V>(total + row * width + i, u);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = 0.f;
+    }
+    if (!Q8) {
+      if (here) store_values<WIDE, V>(static_cast<T*>(y) + row * width + i, v);
+    } else {                                                             // 32 / V lanes have a block (a width of blocks: all of them or none)
+      uint32_t largest = 0;
+#pragma unroll
+      for (int j = 0; j < V; ++j) largest = max(largest, __float_as_uint(v[j]) & 0x7fffffffu);
+#pragma unroll
+      for (int o = 16 / V; o > 0; o >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+      if (!here) return;
+      const __half d = __float2half_rn(__fmul_rn(__uint_as_float(largest), 1.0f / 127.0f));
+      const float step8 = __half2float(d);
+      // blocks are multiples of two bytes
+      uint16_t* block = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(y) + (row * width + i) / 32 * 34);
+      if ((i & 31) == 0) block[0] = __half_as_ushort(d);
+      uint32_t q[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) q[j] = step8 > 0.f ? uint32_t(__float2int_rn(fminf(fmaxf(__fdiv_rn(v[j], step8), -127.f), 127.f))) & 0xffu : 0u;
+#pragma unroll
+      for (int j = 0; j + 1 < V; j += 2) block[1 + ((i & 31) + j) / 2] = uint16_t(q[j] | (q[j + 1] << 8));
+    }
+  };
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (!Q8 || first - lane * V + r * step < width) finish(first + r * step, t[r], in[r]);
+  for (int i = first + R * step; i - lane * V < width; i += step) {      // (total may be x or the residual: a value is read and written by one thread)
+    float u[V];
+    if (i < width) load(i, u);
+    finish(i, u, i < width);
+  }
+}
+
+template <typename T, typename W, int V, bool WIDE, int R, int NT, bool Q8>
+static int launch(const void* x, const void* residual, const void* weight, void* y, void* total, int rows, int width, float eps, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(rows));
+  cfg.blockDim = dim3(NT);
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, rms_norm_kernel<T, W, V, WIDE, R, NT, Q8>, static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<const W*>(weight), y,
+                            static_cast<T*>(total), width, eps) == cudaSuccess
+             ? RC_OK
+             : RC_LAUNCH;
+}
+
+// The same threads have the same values whatever the addresses are, so that results do not depend on those.
+template <typename T, typename W, bool Q8, bool WIDE>
+static int pick(const void* x, const void* residual, const void* weight, void* y, void* total, int rows, int width, float eps, cudaStream_t s) {
+  constexpr int V = 16 / int(sizeof(T));
+  if (width % V != 0) return launch<T, W, 1, false, 8, 1024, false>(x, residual, weight, y, total, rows, width, eps, s);
+  if (width <= 128 * V) return launch<T, W, V, WIDE, 1, 128, Q8>(x, residual, weight, y, total, rows, width, eps, s);
+  if (width <= 256 * V) return launch<T, W, V, WIDE, 1, 256, Q8>(x, residual, weight, y, total, rows, width, eps, s);
+  if (width <= 512 * V) return launch<T, W, V, WIDE, 1, 512, Q8>(x, residual, weight, y, total, rows, width, eps, s);
+  if (width <= 1024 * V) return launch<T, W, V, WIDE, 2, 512, Q8>(x, residual, weight, y, total, rows, width, eps, s);
+  return launch<T, W, V, WIDE, 4, 1024, Q8>(x, residual, weight, y, total, rows, width, eps, s);
 }
 
 int rms_norm(const void* x, const void* residual, const void* weight, void* y, void* total, int dtype, int weight_dtype, int rows, int width, float eps, int q8_0,
@@ -50,16 +169,16 @@ int rms_norm(const void* x, const void* residual, const void* weight, void* y, v
   if (weight_dtype != DINO_F32 && weight_dtype != dtype) return RC_DTYPE;
   return kv::with_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    const uintptr_t all = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) | reinterpret_cast<uintptr_t>(total);
-    if ((all & (sizeof(T) - 1)) != 0 || (reinterpret_cast<uintptr_t>(y) & (q8_0 ? 1 : sizeof(T) - 1)) != 0) return RC_ALIGN;
+    const uintptr_t all = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) | reinterpret_cast<uintptr_t>(total), out = reinterpret_cast<uintptr_t>(y);
+    if ((all & (sizeof(T) - 1)) != 0 || (out & (q8_0 ? 1 : sizeof(T) - 1)) != 0) return RC_ALIGN;
     if ((reinterpret_cast<uintptr_t>(weight) & (weight_dtype == DINO_F32 ? 3 : sizeof(T) - 1)) != 0) return RC_ALIGN;
-    if (weight_dtype == DINO_F32)
-      rms_norm_kernel<T, float><<<unsigned(rows), 256, 0, s>>>(static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<const float*>(weight), y,
-                                                               static_cast<T*>(total), width, eps, q8_0 != 0);
-    else
-      rms_norm_kernel<T, T><<<unsigned(rows), 256, 0, s>>>(static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<const T*>(weight), y,
-                                                           static_cast<T*>(total), width, eps, q8_0 != 0);
-    return cudaGetLastError() == cudaSuccess ? RC_OK : RC_LAUNCH;
+    const bool wide = ((all | reinterpret_cast<uintptr_t>(weight) | (q8_0 ? 0 : out) | uint64_t(width) * sizeof(T)) & 15) == 0;
+    auto go = [&](auto w) -> int {
+      using W = decltype(w);
+      if (q8_0) return wide ? pick<T, W, true, true>(x, residual, weight, y, total, rows, width, eps, s) : pick<T, W, true, false>(x, residual, weight, y, total, rows, width, eps, s);
+      return wide ? pick<T, W, false, true>(x, residual, weight, y, total, rows, width, eps, s) : pick<T, W, false, false>(x, residual, weight, y, total, rows, width, eps, s);
+    };
+    return weight_dtype == DINO_F32 ? go(float{}) : go(T{});
   });
 }
 
