@@ -49,7 +49,7 @@ struct Sequence {
 };
 __device__ __forceinline__ Sequence sequence_at(const AttnParams& a, int b) {
   const Rows rows = rows_of(a.p, b);
-  const int length = __ldg(a.p.lengths + b);
+  const int length = fetch(a.p.lengths + b);
   const int reach = int(min(int64_t(a.p.table_blocks) << a.c.block_log2, int64_t(INT32_MAX)));
   if (length > reach) flag_range(a.p.status);
   const int64_t total = int64_t(rows.count) * a.group;

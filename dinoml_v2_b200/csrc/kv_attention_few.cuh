@@ -86,7 +86,7 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float load_q(const AttnParams& a, int64_t at) {
-  if (a.dtype == DINO_F32) return __ldg(static_cast<const float*>(a.q) + at);
+  if (a.dtype == DINO_F32) return fetch(static_cast<const float*>(a.q) + at);
   if (a.dtype == DINO_F16) return __half2float(static_cast<const __half*>(a.q)[at]);
   return __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[at]);
 }
@@ -96,10 +96,10 @@ __device__ __forceinline__ void load_q4(const AttnParams& a, int64_t at, bool wi
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = load_q(a, at + i);
   } else if (a.dtype == DINO_F32) {
-    const float4 x = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at));
+    const float4 x = fetch(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at));
     v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
   } else {
-    const uint2 x = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.q) + at));
+    const uint2 x = fetch(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.q) + at));
     if (a.dtype == DINO_F16) {
       const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&x.x)), hi = __half22float2(*reinterpret_cast<const __half2*>(&x.y));
       v[0] = lo.x; v[1] = lo.y; v[2] = hi.x; v[3] = hi.y;
@@ -219,8 +219,8 @@ __device__ __forceinline__ void copy_tiles(const AttnParams& a, Shared<S>& sh, c
       if (id < 0) return x;
       const int bh = id * a.c.heads + w.head;                           // (rows of the cache are an int)
       x.row = (bh << a.c.block_log2) + (token & ((1 << a.c.block_log2) - 1));
-      x.k_scale = __ldg(a.c.scale[0] + bh);
-      x.v_scale = __ldg(a.c.scale[1] + bh);
+      x.k_scale = fetch(a.c.scale[0] + bh);
+      x.v_scale = fetch(a.c.scale[1] + bh);
       return x;
     };
     Box now = look_up(tile0), ahead = look_up(tile0 + per_look);

@@ -204,7 +204,7 @@ __device__ __forceinline__ void convert_tiles(const AttnParams& a, Shared& sh, u
 #pragma unroll
       for (int i = 0; i < kCopies; ++i) {
         x[i] = make_uint4(0u, 0u, 0u, 0u);                              // (what nobody sees has to be finite: zeros)
-        if (bh >= 0 && token + i * kStep >= low && token + i * kStep < high) x[i] = __ldg(reinterpret_cast<const uint4*>(from + i * kStep * S::D));
+        if (bh >= 0 && token + i * kStep >= low && token + i * kStep < high) x[i] = fetch(reinterpret_cast<const uint4*>(from + i * kStep * S::D));
       }
     };
     // Stage u of an item has K of tile u and V of tile u - kAhead.  All that it is made of was asked for while the one before was stored.
@@ -219,8 +219,8 @@ __device__ __forceinline__ void convert_tiles(const AttnParams& a, Shared& sh, u
       load(raw[0], 0, tile, at);
       ks = vs = 0.f;
       if (at >= 0) {
-        ks = __ldg(a.c.scale[0] + at);
-        vs = __ldg(a.c.scale[1] + at);
+        ks = fetch(a.c.scale[0] + at);
+        vs = fetch(a.c.scale[1] + at);
       }
     };
     load_k(tile0, bh[kAhead]);
@@ -452,7 +452,7 @@ __device__ __forceinline__ void open_rows(const AttnParams& a, const Segment& sg
     x[k] = make_uint4(0u, 0u, 0u, 0u);
     if (r < sg.item.r1) {
       if (wide) {
-        x[k] = __ldg(reinterpret_cast<const uint4*>(src));
+        x[k] = fetch(reinterpret_cast<const uint4*>(src));
       } else {
         uint32_t w[4];
 #pragma unroll

@@ -1,5 +1,6 @@
 // Write and read of the 8-bit cache of keys and values (layout: kv_cache.cuh).
 #include <mutex>
+#include <type_traits>
 
 #include "kv_attention.cuh"
 
@@ -45,10 +46,32 @@ int batch_view(const DinoB200KvBatch* b, bool needs_lengths, Batch* out) {
   return RC_OK;
 }
 
+// Both kernels are bound by bytes, and a short call by its chain of dependent reads (starts, length, table, data): every thread has all of its
+// reads of a step under way before it uses the first, and a launch starts while the one before it ends.
+
+// A launch that starts while the one before it in the stream ends; the kernel waits for that itself.
+template <typename... P, typename... A> static int start(void (*kernel)(P...), unsigned ctas, cudaStream_t s, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? RC_OK : RC_LAUNCH;
+}
+__device__ __forceinline__ void wait_for_launch_before() {
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+}
+
 // ---- write ------------------------------------------------------------------------------------------------------------------
 // A unit is the new tokens of one sequence in one block, for one head of K or of V: the only writer of that block and head, so the scale and the
-// tokens that are there already need no atomics.  NT threads work on a unit (a warp where a call brings a token or two, a CTA where it brings
-// whole blocks).
+// tokens that are there already need no atomics.  NT threads work on a unit: a warp where a call brings a token or two, a CTA where it brings
+// whole blocks.  A thread keeps the first kHeld pieces of 16 bytes that it has between the maximum and the rounding and reads the others again.
+constexpr int kHeld = 4;
 struct Source {
   const void* x[2];
   int64_t row_stride[2], head_stride[2];
@@ -68,9 +91,10 @@ __global__ void __launch_bounds__(256) kv_write_kernel(Cache c, Batch p, Source 
   using Q = Quant<TYPE>;
   constexpr int N = Pack<T>::N;
   __shared__ uint32_t shared[8];
+  wait_for_launch_before();
   const int tid = threadIdx.x % NT;
   const int64_t unit = int64_t(blockIdx.x) * (256 / NT) + threadIdx.x / NT;
-  const int which = int(unit & 1), bs = 1 << c.block_log2;
+  auto pick = [&](const auto& of) { return (unit & 1) == 0 ? of[0] : of[1]; };      // of K or V
   const int head = int((unit >> 1) % c.heads);
   const int64_t piece64 = (unit >> 1) / c.heads;
   if (piece64 >= pieces) return;
@@ -80,12 +104,12 @@ __global__ void __launch_bounds__(256) kv_write_kernel(Cache c, Batch p, Source 
   int b = piece, base = piece;
   if (p.starts != nullptr) {
     const int log2 = c.block_log2;
-    auto key = [&](int i) { return int64_t(__ldg(p.starts + i) >> log2) + 2 * i; };
+    auto key = [&](int i) { return int64_t(fetch(p.starts + i) >> log2) + 2 * i; };
     b = last_at_most(p.sequences, piece, key);
     base = int(key(b));
   }
   const Rows rows = rows_of(p, b);
-  const int length = __ldg(p.lengths + b);
+  const int length = fetch(p.lengths + b);
   const int first = length - rows.count;                       // position of the first new token
   const int block = (max(first, 0) >> c.block_log2) + (piece - base);
   const int low = max(max(first, 0), block << c.block_log2), high = int(min(int64_t(length), (int64_t(block) + 1) << c.block_log2));
@@ -93,45 +117,76 @@ __global__ void __launch_bounds__(256) kv_write_kernel(Cache c, Batch p, Source 
   const int id = block_at(p, c.blocks, b, block);
   if (id < 0) return;
 
-  const T* x = static_cast<const T*>(src.x[which]) + head * src.head_stride[which] + int64_t(rows.first + low - first) * src.row_stride[which];
-  const int64_t stride = src.row_stride[which];
-  const int per_row = c.dim / N, total = (high - low) * per_row;
-  uint32_t largest = 0;                                        // as bits: an infinity or a NaN is larger than every number
-  for (int i = tid; i < total; i += NT) {
-    Pack<T> v;
-    v.load(x + (i / per_row) * stride + (i % per_row) * N, src.wide);
-#pragma unroll
-    for (int j = 0; j < N; ++j) largest = max(largest, __float_as_uint(to_float<T>(v.v[j])) & 0x7fffffffu);
-  }
-  largest = unit_max<NT>(largest, shared);
-  float* scale = c.scale[which] + int64_t(id) * c.heads + head;
+  const T* x = static_cast<const T*>(pick(src.x)) + head * pick(src.head_stride) + int64_t(rows.first + low - first) * pick(src.row_stride);
+  const int64_t stride = pick(src.row_stride);
+  const int log2 = __ffs(c.dim / N) - 1, total = (high - low) << log2;
+  auto load = [&](int i, Pack<T>& v) { v.load(x + (i >> log2) * stride + (i & ((1 << log2) - 1)) * N, src.wide); };
+  float* scale = pick(c.scale) + int64_t(id) * c.heads + head;
   const int kept = low - (block << c.block_log2);              // tokens that were in the block before
   const float before = kept > 0 ? *scale : 0.f;
+  Pack<T> held[kHeld];
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (tid + k * NT < total) load(tid + k * NT, held[k]);
+  uint32_t largest = 0;                                        // as bits: an infinity or a NaN is larger than every number
+  auto meet = [&](const Pack<T>& v) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) largest = max(largest, __float_as_uint(to_float<T>(v.v[j])) & 0x7fffffffu);
+  };
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (tid + k * NT < total) meet(held[k]);
+  for (int i = tid + kHeld * NT; i < total; i += NT) {
+    Pack<T> v;
+    load(i, v);
+    meet(v);
+  }
+  largest = unit_max<NT>(largest, shared);
   const float wanted = largest < 0x7f800000u ? Q::wanted(__uint_as_float(largest)) : __uint_as_float(0x7fc00000u);
   const float after = before != before || wanted != wanted ? __uint_as_float(0x7fc00000u) : fmaxf(before, wanted);
-  uint8_t* dst = c.data[which] + ((int64_t(id) * c.heads + head) << c.block_log2) * c.dim;
+  uint8_t* dst = pick(c.data) + ((int64_t(id) * c.heads + head) << c.block_log2) * c.dim;
   if (NT > 32) __syncthreads(); else __syncwarp();             // everyone has read the scale
   if (tid == 0) *scale = after;
   if (kept > 0 && after != before && after == after) {
     const float ratio = __fdiv_rn(before, after);
-    for (int i = tid; i < kept * c.dim / 4; i += NT) {
-      const uint32_t q = reinterpret_cast<const uint32_t*>(dst)[i];
-      uint32_t r = 0;
+    uint4* old = reinterpret_cast<uint4*>(dst);
+    const int count = kept * c.dim / 16;
+    for (int i = tid; i < count; i += kHeld * NT) {
+      uint4 q[kHeld];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r |= Q::nearest(__fmul_rn(Q::up((q >> (8 * j)) & 0xffu), ratio)) << (8 * j);
-      reinterpret_cast<uint32_t*>(dst)[i] = r;
+      for (int k = 0; k < kHeld; ++k)
+        if (i + k * NT < count) q[k] = old[i + k * NT];
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k) {
+        if (i + k * NT >= count) break;
+        uint32_t* w = &q[k].x;
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          uint32_t r = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) r |= Q::nearest(__fmul_rn(Q::up((w[m] >> (8 * j)) & 0xffu), ratio)) << (8 * j);
+          w[m] = r;
+        }
+        old[i + k * NT] = q[k];
+      }
     }
   }
   dst += int64_t(kept) * c.dim;
   const typename Q::Down down(after);                          // a NaN scale: zeros
-  for (int i = tid; i < total; i += NT) {
-    Pack<T> v;
-    v.load(x + (i / per_row) * stride + (i % per_row) * N, src.wide);
+  auto store = [&](int i, const Pack<T>& v) {
     uint32_t w[N / 4];
 #pragma unroll
     for (int j = 0; j < N; j += 4) w[j / 4] = down(to_float<T>(v.v[j])) | down(to_float<T>(v.v[j + 1])) << 8 | down(to_float<T>(v.v[j + 2])) << 16 | down(to_float<T>(v.v[j + 3])) << 24;
+    if constexpr (N == 8) reinterpret_cast<uint2*>(dst)[i] = make_uint2(w[0], w[1]);
+    else reinterpret_cast<uint32_t*>(dst)[i] = w[0];
+  };
 #pragma unroll
-    for (int j = 0; j < N / 4; ++j) reinterpret_cast<uint32_t*>(dst)[i * (N / 4) + j] = w[j];
+  for (int k = 0; k < kHeld; ++k)
+    if (tid + k * NT < total) store(tid + k * NT, held[k]);
+  for (int i = tid + kHeld * NT; i < total; i += NT) {
+    Pack<T> v;
+    load(i, v);
+    store(i, v);
   }
 }
 
@@ -153,59 +208,63 @@ int cache_write(const DinoB200KvCache* cache, const DinoB200KvBatch* batch, cons
     const bool few = p.rows < 8 * int64_t(p.sequences);
     const int64_t ctas = few ? (units + 7) / 8 : units;
     if (pieces > INT32_MAX || ctas > INT32_MAX) return RC_RANGE;
-    auto launch = [&](auto kern) {
-      kern<<<unsigned(ctas), 256, 0, s>>>(c, p, src, int(pieces));
-      return cudaGetLastError() == cudaSuccess ? RC_OK : RC_LAUNCH;
-    };
+    auto launch = [&](auto kern) { return start(kern, unsigned(ctas), s, c, p, src, int(pieces)); };
     if (cache->type == DINOML_B200_KV_INT8) return few ? launch(kv_write_kernel<T, DINOML_B200_KV_INT8, 32>) : launch(kv_write_kernel<T, DINOML_B200_KV_INT8, 256>);
     return few ? launch(kv_write_kernel<T, DINOML_B200_KV_E4M3, 32>) : launch(kv_write_kernel<T, DINOML_B200_KV_E4M3, 256>);
   });
 }
 
 // ---- read -------------------------------------------------------------------------------------------------------------------
-constexpr int kReadRows = 8;         // rows of a CTA
+// A warp has one row of K and V: 512 bytes of the result at a time, kReadAhead of them under way.
+constexpr int kReadWarps = 8, kReadAhead = 4;
 
 template <typename T, int TYPE>
-__global__ void __launch_bounds__(256) kv_read_kernel(Cache c, Batch p, const int* begins, T* k_out, T* v_out) {
+__global__ void __launch_bounds__(32 * kReadWarps) kv_read_kernel(Cache c, Batch p, const int* begins, T* k_out, T* v_out) {
   using Q = Quant<TYPE>;
-  __shared__ int ids[kReadRows], slots[kReadRows];
-  const int row0 = blockIdx.x * kReadRows, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (row0 + warp < p.rows) {                                  // one warp finds one row's block
-    const int row = row0 + warp;
-    int b = row;
-    if (p.starts != nullptr) b = last_at_most(p.sequences, row, [&](int i) { return int64_t(__ldg(p.starts + i)); });
-    const Rows rows = rows_of(p, b);
-    const int64_t position = int64_t(row) - rows.first + (begins != nullptr ? __ldg(begins + b) : 0);
-    int id = -1;
-    if (row >= rows.first && row < rows.first + rows.count && position >= 0 && position <= INT32_MAX) id = block_at(p, c.blocks, b, int(position >> c.block_log2));
-    if (lane == 0) { ids[warp] = id; slots[warp] = int(position) & ((1 << c.block_log2) - 1); }
-  }
-  __syncthreads();
-  const int per_row = c.heads * c.dim / 16, rows = min(kReadRows, p.rows - row0);
-  for (int i = threadIdx.x; i < rows * per_row; i += 256) {
-    const int r = i / per_row, at = i % per_row, head = at * 16 / c.dim, column = at * 16 % c.dim;
-    const int id = ids[r];
+  constexpr int N = 16 / int(sizeof(T));                       // values of a lane: 4 or 8 bytes of the cache
+  using Raw = std::conditional_t<N == 8, uint2, uint32_t>;
+  wait_for_launch_before();
+  const int lane = threadIdx.x & 31;
+  const int64_t row64 = int64_t(blockIdx.x) * kReadWarps + (threadIdx.x >> 5);
+  if (row64 >= p.rows) return;
+  const int row = int(row64);
+  int b = row;
+  if (p.starts != nullptr) b = last_at_most(p.sequences, row, [&](int i) { return int64_t(fetch(p.starts + i)); });
+  const Rows rows = rows_of(p, b);
+  const int64_t position = int64_t(row) - rows.first + (begins != nullptr ? fetch(begins + b) : 0);
+  int id = -1;
+  if (row >= rows.first && row < rows.first + rows.count && position >= 0 && position <= INT32_MAX) id = block_at(p, c.blocks, b, int(position >> c.block_log2));
+  const int slot = int(position) & ((1 << c.block_log2) - 1), log2 = __ffs(c.dim) - 1, width = c.heads << log2;
+  const int64_t to = row64 * width;
+  for (int i = lane * N; i < width; i += 32 * N * kReadAhead) {
+    Raw raw[kReadAhead][2];
+    float scale[kReadAhead][2];
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      uint4 raw = make_uint4(0, 0, 0, 0);
-      float scale = 0.f;
-      if (id >= 0) {
-        const int64_t block = int64_t(id) * c.heads + head;
-        raw = *reinterpret_cast<const uint4*>(c.data[which] + ((block << c.block_log2) + slots[r]) * c.dim + column);
-        scale = c.scale[which][block];
+    for (int k = 0; k < kReadAhead; ++k) {
+      const int at = i + 32 * N * k;
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        raw[k][which] = Raw{};
+        scale[k][which] = 0.f;
+        if (at < width && id >= 0) {
+          const int64_t block = int64_t(id) * c.heads + (at >> log2);
+          raw[k][which] = fetch(reinterpret_cast<const Raw*>(c.data[which] + ((((block << c.block_log2) + slot) << log2) + (at & (c.dim - 1)))));
+          scale[k][which] = fetch(c.scale[which] + block);
+        }
       }
-      const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
-      constexpr int N = Pack<T>::N;
-      uint4* out = reinterpret_cast<uint4*>((which == 0 ? k_out : v_out) + (int64_t(row0) + r) * c.heads * c.dim + at * 16);
+    }
 #pragma unroll
-      for (int o = 0; o < 16 / N; ++o) {
+    for (int k = 0; k < kReadAhead; ++k) {
+      const int at = i + 32 * N * k;
+      if (at >= width) break;
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        uint32_t words[2];
+        if constexpr (N == 8) { words[0] = raw[k][which].x; words[1] = raw[k][which].y; } else { words[0] = raw[k][which]; }
         Pack<T> v;
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const int e = o * N + j;
-          v.v[j] = from_float<T>(__fmul_rn(Q::up((words[e / 4] >> (8 * (e % 4))) & 0xffu), scale));
-        }
-        out[o] = v.raw;
+        for (int j = 0; j < N; ++j) v.v[j] = from_float<T>(__fmul_rn(Q::up((words[j / 4] >> (8 * (j % 4))) & 0xffu), scale[k][which]));
+        *reinterpret_cast<uint4*>((which == 0 ? k_out : v_out) + to + at) = v.raw;
       }
     }
   }
@@ -220,10 +279,9 @@ int cache_read(const DinoB200KvCache* cache, const DinoB200KvBatch* batch, const
   if (int rc = batch_view(batch, false, &p)) return rc;
   return with_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    const unsigned ctas = unsigned((int64_t(p.rows) + kReadRows - 1) / kReadRows);
-    if (cache->type == DINOML_B200_KV_INT8) kv_read_kernel<T, DINOML_B200_KV_INT8><<<ctas, 256, 0, s>>>(c, p, begins, static_cast<T*>(k_out), static_cast<T*>(v_out));
-    else kv_read_kernel<T, DINOML_B200_KV_E4M3><<<ctas, 256, 0, s>>>(c, p, begins, static_cast<T*>(k_out), static_cast<T*>(v_out));
-    return cudaGetLastError() == cudaSuccess ? RC_OK : RC_LAUNCH;
+    const unsigned ctas = unsigned((int64_t(p.rows) + kReadWarps - 1) / kReadWarps);
+    auto launch = [&](auto kern) { return start(kern, ctas, s, c, p, begins, static_cast<T*>(k_out), static_cast<T*>(v_out)); };
+    return cache->type == DINOML_B200_KV_INT8 ? launch(kv_read_kernel<T, DINOML_B200_KV_INT8>) : launch(kv_read_kernel<T, DINOML_B200_KV_E4M3>);
   });
 }
 

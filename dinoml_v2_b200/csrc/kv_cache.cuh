@@ -30,12 +30,15 @@ int cache_view(const DinoB200KvCache* cache, Cache* out);
 int batch_view(const DinoB200KvBatch* batch, bool needs_lengths, Batch* out);
 
 #ifdef __CUDACC__
+// A plain read.  (A read as of constant data may be moved ahead of a kernel's wait for the launch before it.)
+template <typename T> __device__ __forceinline__ T fetch(const T* p) { return *p; }
+
 __device__ __forceinline__ void flag_range(int* status) { atomicCAS(status, 0, ST_KV_RANGE); }
 
 // Block j of sequence b, -1 if there is none.
 __device__ __forceinline__ int block_at(const Batch& p, int blocks, int b, int j) {
   int id = -1;
-  if (unsigned(j) < unsigned(p.table_blocks)) id = __ldg(p.table + int64_t(b) * p.table_stride + j);
+  if (unsigned(j) < unsigned(p.table_blocks)) id = fetch(p.table + int64_t(b) * p.table_stride + j);
   if (unsigned(id) < unsigned(blocks)) return id;
   flag_range(p.status);
   return -1;
@@ -47,7 +50,7 @@ struct Rows {
 // Packed rows of sequence b.
 __device__ __forceinline__ Rows rows_of(const Batch& p, int b) {
   if (p.starts == nullptr) return {b, b < p.rows ? 1 : 0};
-  const int s0 = __ldg(p.starts + b), s1 = __ldg(p.starts + b + 1);
+  const int s0 = fetch(p.starts + b), s1 = fetch(p.starts + b + 1);
   if (s0 < 0 || s1 < s0 || s1 > p.rows) {
     flag_range(p.status);
     return {0, 0};
@@ -128,7 +131,7 @@ template <typename T> struct Pack {
   __device__ __forceinline__ Pack() {}
   __device__ __forceinline__ void load(const T* p, bool wide) {
     if (wide) {
-      raw = __ldg(reinterpret_cast<const uint4*>(p));
+      raw = fetch(reinterpret_cast<const uint4*>(p));
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] = p[i];
