@@ -114,20 +114,20 @@ __global__ void __launch_bounds__(256) kv_write_kernel(Cache c, Batch p, Source 
   const int block = (max(first, 0) >> c.block_log2) + (piece - base);
   const int low = max(max(first, 0), block << c.block_log2), high = int(min(int64_t(length), (int64_t(block) + 1) << c.block_log2));
   if (piece < base || low >= high) return;
-  const int id = block_at(p, c.blocks, b, block);
-  if (id < 0) return;
 
   const T* x = static_cast<const T*>(pick(src.x)) + head * pick(src.head_stride) + int64_t(rows.first + low - first) * pick(src.row_stride);
   const int64_t stride = pick(src.row_stride);
   const int log2 = __ffs(c.dim / N) - 1, total = (high - low) << log2;
   auto load = [&](int i, Pack<T>& v) { v.load(x + (i >> log2) * stride + (i & ((1 << log2) - 1)) * N, src.wide); };
-  float* scale = pick(c.scale) + int64_t(id) * c.heads + head;
-  const int kept = low - (block << c.block_log2);              // tokens that were in the block before
-  const float before = kept > 0 ? *scale : 0.f;
   Pack<T> held[kHeld];
 #pragma unroll
   for (int k = 0; k < kHeld; ++k)
     if (tid + k * NT < total) load(tid + k * NT, held[k]);
+  const int id = block_at(p, c.blocks, b, block);
+  if (id < 0) return;
+  float* scale = pick(c.scale) + int64_t(id) * c.heads + head;
+  const int kept = low - (block << c.block_log2);              // tokens that were in the block before
+  const float before = kept > 0 ? *scale : 0.f;
   uint32_t largest = 0;                                        // as bits: an infinity or a NaN is larger than every number
   auto meet = [&](const Pack<T>& v) {
 #pragma unroll
