@@ -438,33 +438,37 @@ __device__ __forceinline__ int64_t place_of(const AttnParams& a, const Segment& 
   return (int64_t(sg.s.row + token) * a.heads + head) * a.c.dim;
 }
 
-// q of a warp's 32 rows, from row r0 of the sequence, into its place in shared memory; factor, unbias: of the row of this lane.  D / 8 lanes have a row.
+// q of a warp's 32 rows, from row r0 of the sequence, into its place in shared memory; factor, unbias: of the row of this lane.  D / 8 lanes have a row; a lane
+// copies its 16 bytes of every row there as they are and then works on them in place.  (What happens once an item is short loops: unrolled code is fetched
+// more slowly than it runs when nothing has run it for a while; 12800 cycles here when it was.)
 template <int TYPE, class S>
 __device__ __forceinline__ void open_rows(const AttnParams& a, const Segment& sg, uint32_t q_smem, int r0, float& factor, float& unbias) {
   constexpr int kLanes = S::D / 8, kStep = 32 / kLanes, kSteps = 32 / kStep;      // of a row; rows at once
   const int lane = threadIdx.x & 31, chunk = lane % kLanes, sub = lane / kLanes, row0 = 32 * ((threadIdx.x >> 5) & 3);
   const bool wide = ((reinterpret_cast<uintptr_t>(a.q) | uint64_t(a.row_stride * 2) | uint64_t(a.head_stride * 2)) & 15) == 0, f16 = a.dtype == DINO_F16;
-  uint4 x[kSteps];
-#pragma unroll
+#pragma unroll 2
   for (int k = 0; k < kSteps; ++k) {
     const int r = r0 + kStep * k + sub, token = a.by_group(min(r, sg.item.r1 - 1)), head = sg.head * a.group + r - token * a.group;
     const uint16_t* src = static_cast<const uint16_t*>(a.q) + int64_t(sg.s.row + token) * a.row_stride + int64_t(head) * a.head_stride + 8 * chunk;
-    x[k] = make_uint4(0u, 0u, 0u, 0u);
-    if (r < sg.item.r1) {
-      if (wide) {
-        x[k] = fetch(reinterpret_cast<const uint4*>(src));
-      } else {
-        uint32_t w[4];
+    const uint32_t to = q_smem + operand_at<kRows>(row0 + kStep * k + sub, chunk);
+    if (r >= sg.item.r1) {
+      st_shared16(to, 0u, 0u, 0u, 0u);
+    } else if (wide) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to), "l"(src) : "memory");
+    } else {
+      uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = uint32_t(src[2 * j]) | (uint32_t(src[2 * j + 1]) << 16);
-        x[k] = make_uint4(w[0], w[1], w[2], w[3]);
-      }
+      for (int j = 0; j < 4; ++j) w[j] = uint32_t(src[2 * j]) | (uint32_t(src[2 * j + 1]) << 16);
+      st_shared16(to, w[0], w[1], w[2], w[3]);
     }
   }
-#pragma unroll
+  asm volatile("cp.async.wait_all;\n" ::: "memory");
+#pragma unroll 2
   for (int k = 0; k < kSteps; ++k) {
+    const uint32_t to = q_smem + operand_at<kRows>(row0 + kStep * k + sub, chunk);
+    const uint4 x = lds128(to);
     // The largest of the 16-bit magnitudes, whose order is that of the values.
-    uint32_t largest = __vmaxu2(__vmaxu2(x[k].x & 0x7fff7fffu, x[k].y & 0x7fff7fffu), __vmaxu2(x[k].z & 0x7fff7fffu, x[k].w & 0x7fff7fffu));
+    uint32_t largest = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
     largest = max(largest & 0xffffu, largest >> 16);
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
@@ -474,7 +478,7 @@ __device__ __forceinline__ void open_rows(const AttnParams& a, const Segment& sg
     const int shift = plain ? 0 : min(max(127 + 12 - int(e), -126), 126);
     const float up = __uint_as_float(uint32_t(127 + shift) << 23), down = __uint_as_float(uint32_t(127 - shift) << 23);
     const float sign = a.scale < 0.f ? -up : up;                        // scores' factors are not negative
-    const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
     uint32_t h[4];
     float total = 0.f;
 #pragma unroll
@@ -484,7 +488,7 @@ __device__ __forceinline__ void open_rows(const AttnParams& a, const Segment& sg
       const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
       total += back.x + back.y;
     }
-    st_shared16(q_smem + operand_at<kRows>(row0 + kStep * k + sub, chunk), h[0], h[1], h[2], h[3]);
+    st_shared16(to, h[0], h[1], h[2], h[3]);
     if (Half2Of<TYPE>::kBias != 0.f) {                                  // K's of int8 are that much too large
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -511,7 +515,7 @@ __device__ __forceinline__ void close_rows(const AttnParams& a, const Segment& s
   const uint32_t mine = q_smem + uint32_t(((threadIdx.x >> 5) & 3) * 32 * D * 2);
   auto at = [&](int row, int chunk) { return mine + uint32_t(row * D * 2) + uint32_t((chunk ^ (row & (D / 8 - 1))) << 4); };
   if (sg.piece < 0) {
-#pragma unroll
+#pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
       uint32_t o[32], h[16];
       tmem_ld32(tmem_o + uint32_t(32 * c), o);
@@ -559,6 +563,88 @@ __device__ __forceinline__ void close_rows(const AttnParams& a, const Segment& s
     }
     __syncwarp();
   }
+}
+
+// The results of a cut item from its pieces, by 256 threads.  First a row's largest y and its sum by a thread each (kept in the place of q), then the sums of
+// all columns, kPlaces of four columns and kPieces pieces under way at a time.
+template <class S, typename Meet> __device__ __forceinline__ bool join_rows(const AttnParams& a, const Segment& sg, uint32_t q_smem, Meet meet) {
+  constexpr int D = S::D, kPiece = kItemRows * (D + 2), kPlaces = 8, kPieces = 2;
+  const int rows = sg.item.r1 - sg.item.r0, count = sg.c1 - sg.c0 + 1, tid = int(threadIdx.x);
+  auto piece = [&](int c) { return a.partial + size_t(c == 0 ? sg.piece0 : 2 * (sg.c0 + c)) * kPiece; };
+  auto weight = [](float ref, float top) { return ref == -INFINITY ? 0.f : exp2_approx(ref - top); };
+  if (tid < rows) {
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll 1
+    for (int c = 0; c < count; c += 4) {
+      float2 ml[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) ml[k] = c + k < count ? __ldcg(reinterpret_cast<const float2*>(piece(c + k) + kItemRows * D) + tid) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float next = fmaxf(top, ml[k].x);
+        sum = fmaf(ml[k].y, weight(ml[k].x, next), sum * weight(top, next));
+        top = next;
+      }
+    }
+    const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+    asm volatile("st.shared.v2.f32 [%0], {%1,%2};\n" ::"r"(q_smem + 8u * uint32_t(tid)), "f"(top), "f"(inverse) : "memory");
+  }
+  if (!meet()) return false;
+  auto stats = [&](int row) {
+    float2 v;
+    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];\n" : "=f"(v.x), "=f"(v.y) : "r"(q_smem + 8u * uint32_t(row)) : "memory");
+    return v;
+  };
+  const int last = rows * (D / 4) - 1;
+#pragma unroll 1
+  for (int x0 = tid; x0 <= last; x0 += 256 * kPlaces) {
+    float4 v[kPlaces];
+    float top[kPlaces];
+#pragma unroll
+    for (int u = 0; u < kPlaces; ++u) {
+      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      top[u] = stats(min(x0 + 256 * u, last) / (D / 4)).x;
+    }
+#pragma unroll 1
+    for (int c = 0; c < count; c += kPieces) {
+      float ref[kPieces][kPlaces];
+      float4 y[kPieces][kPlaces];
+#pragma unroll
+      for (int k = 0; k < kPieces; ++k) {
+        const float* const src = piece(min(c + k, count - 1));
+#pragma unroll
+        for (int u = 0; u < kPlaces; ++u) {
+          const int x = min(x0 + 256 * u, last);
+          y[k][u] = __ldcg(reinterpret_cast<const float4*>(src) + x);
+          ref[k][u] = __ldcg(src + kItemRows * D + 2 * (x / (D / 4)));
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kPieces; ++k) {
+        if (c + k >= count) break;
+#pragma unroll
+        for (int u = 0; u < kPlaces; ++u) {
+          const float f = weight(ref[k][u], top[u]);
+          v[u] = make_float4(fmaf(y[k][u].x, f, v[u].x), fmaf(y[k][u].y, f, v[u].y), fmaf(y[k][u].z, f, v[u].z), fmaf(y[k][u].w, f, v[u].w));
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kPlaces; ++u) {
+      const int x = x0 + 256 * u;
+      if (x > last) break;
+      const float inv = stats(x / (D / 4)).y;
+      uint2 h;
+      if (a.dtype == DINO_F16) {
+        h = make_uint2(pack_half(v[u].x * inv, v[u].y * inv), pack_half(v[u].z * inv, v[u].w * inv));
+      } else {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(v[u].x * inv, v[u].y * inv), hi = __floats2bfloat162_rn(v[u].z * inv, v[u].w * inv);
+        h = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+      }
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + place_of(a, sg, x / (D / 4)) + x % (D / 4) * 4) = h;
+    }
+  }
+  return meet();                                                        // (the next item's q goes where the rows' sums are)
 }
 
 // ---- warps 0..7: tile i of the item, a row per thread
@@ -631,59 +717,7 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
       }
       if (!meet()) return;
       if (sh.last) {
-        const int rows = sg.item.r1 - sg.item.r0, count = sg.c1 - sg.c0 + 1;
-        constexpr int U = 4, P = 3;                                     // places and pieces under way at a time
-        for (int x0 = int(threadIdx.x); x0 < rows * (D / 4); x0 += 256 * U) {
-          float high_ref[U], sum[U];
-          float4 v[U];
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            high_ref[u] = -INFINITY;
-            sum[u] = 0.f;
-            v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-          }
-          for (int c = 0; c < count; c += P) {
-            float2 ml[P][U];
-            float4 y[P][U];
-#pragma unroll
-            for (int k = 0; k < P; ++k)
-#pragma unroll
-              for (int u = 0; u < U; ++u) {
-                const int x = min(x0 + 256 * u, rows * (D / 4) - 1);
-                ml[k][u] = make_float2(-INFINITY, 0.f);
-                y[k][u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (c + k < count) {
-                  const float* src = a.partial + size_t(c + k == 0 ? sg.piece0 : 2 * (sg.c0 + c + k)) * kPiece;
-                  ml[k][u] = __ldcg(reinterpret_cast<const float2*>(src + kItemRows * D) + x / (D / 4));
-                  y[k][u] = __ldcg(reinterpret_cast<const float4*>(src) + x);
-                }
-              }
-#pragma unroll
-            for (int k = 0; k < P; ++k)
-#pragma unroll
-              for (int u = 0; u < U; ++u) {
-                const float next = fmaxf(high_ref[u], ml[k][u].x);
-                const float f0 = high_ref[u] == -INFINITY ? 1.f : exp2_approx(high_ref[u] - next), f1 = ml[k][u].x == -INFINITY ? 1.f : exp2_approx(ml[k][u].x - next);
-                sum[u] = fmaf(ml[k][u].y, f1, sum[u] * f0);
-                v[u] = make_float4(fmaf(y[k][u].x, f1, v[u].x * f0), fmaf(y[k][u].y, f1, v[u].y * f0), fmaf(y[k][u].z, f1, v[u].z * f0), fmaf(y[k][u].w, f1, v[u].w * f0));
-                high_ref[u] = next;
-              }
-          }
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const int x = x0 + 256 * u, row = x / (D / 4), d = x % (D / 4) * 4;
-            if (row >= rows) continue;
-            const float inv = sum[u] == 0.f ? 0.f : 1.f / sum[u];
-            uint2 h;
-            if (a.dtype == DINO_F16) {
-              h = make_uint2(pack_half(v[u].x * inv, v[u].y * inv), pack_half(v[u].z * inv, v[u].w * inv));
-            } else {
-              const __nv_bfloat162 lo = __floats2bfloat162_rn(v[u].x * inv, v[u].y * inv), hi = __floats2bfloat162_rn(v[u].z * inv, v[u].w * inv);
-              h = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-            }
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + place_of(a, sg, row) + d) = h;
-          }
-        }
+        if (!join_rows<S>(a, sg, q_smem, meet)) return;
       }
     }
     __syncwarp();
