@@ -36,6 +36,7 @@ struct AttnParams {
   int window, heads, group, dtype;
   Divisor by_group;
   int row_tile, row_tile_log2;               // rows (token x head of the group) of an item
+  int ends;                                  // what an item costs beside its tiles, in tiles
   int min_rows, max_rows;                    // sequences with fewer or more rows (tokens x group) are another launch's
   float* partial;                            // two cut pieces per CTA
   int* arrived;                              // a counter per CTA, zero between launches
@@ -75,28 +76,35 @@ __device__ __forceinline__ int row_tiles(const AttnParams& a, const Sequence& s)
 // Tiles of `size` positions (a power of two) that an item covers; one that sees nothing still has its rows to write.
 __device__ __forceinline__ int tiles_of(const Item& it, int log2) { return it.high > it.low ? ((it.high - 1) >> log2) - (it.low >> log2) + 1 : 1; }
 
-// The units of the launch are one line: sequences, their row tiles, the cached heads, tiles of cached positions.  Worker c of G (a CTA; those
-// beyond G have nothing to do) takes units [c W / G, (c + 1) W / G): the same work for every CTA whatever the lengths are, at the price that an
-// item at an end of a range is finished by whoever of its CTAs comes last.
+// The units of the launch are one line: sequences, their row tiles, the cached heads, and for each of these items `ends` units for its beginning and its end, in
+// which there is nothing to do, and its tiles of cached positions.  Worker c of G (a CTA; those beyond G have nothing to do) takes units
+// [c W / G, (c + 1) W / G): the same work for every CTA whatever the lengths are, at the price that an item that is cut is finished by whoever of its CTAs
+// comes last.
 struct Walk {
-  int b, row_tile, head, tile;               // the next unit
+  int b, row_tile, head, tile;               // the next tile
   int workers, per, more;                    // units of a worker, and how many of `workers` parts of one more unit
   int64_t units, start;                      // of the launch; the first one of this CTA's range
   int64_t unit, stop;                        // number of the next unit, and the end of the range
   int64_t item_unit;                         // number of the item's first unit
   Sequence s;
   Item item;
-  int tiles;                                 // of the item
+  int tiles, ends;                           // of the item
 
   __device__ __forceinline__ bool done() const { return unit >= stop; }
+  __device__ __forceinline__ int64_t first_tile() const { return item_unit + ends; }
+  __device__ __forceinline__ int end_tile() const { return int(min(int64_t(tiles), stop - first_tile())); }
+  // Numbers of the partial sums of this CTA's part of the item, and of the item's first part: a CTA has two at most, one of the item that its range begins in.
+  __device__ __forceinline__ int piece() const { return 2 * int(blockIdx.x) + (start >= item_unit ? 0 : 1); }
+  __device__ __forceinline__ int first_piece(int owner_of_it) const { return 2 * owner_of_it + (start_of(owner_of_it) >= item_unit ? 0 : 1); }
   __device__ __forceinline__ void open(const AttnParams& a, int log2) {
     item = item_at(a, s, row_tile);
     tiles = tiles_of(item, log2);
   }
   __device__ __forceinline__ void next_item(const AttnParams& a, int log2) {
-    unit = item_unit + tiles;
-    item_unit = unit;
+    unit = item_unit = first_tile() + tiles;
     tile = 0;
+    if (done()) return;
+    unit += ends;
     if (done() || ++head < a.c.heads) return;
     head = 0;
     if (++row_tile >= row_tiles(a, s)) {
@@ -120,7 +128,7 @@ __device__ __forceinline__ Walk walk_of(const AttnParams& a, int log2, int least
   const int per = (a.p.sequences + NT - 1) / NT;
   auto units_of = [&](const Sequence& s) {
     int64_t n = 0;
-    for (int t = row_tiles(a, s) - 1; t >= 0; --t) n += tiles_of(item_at(a, s, t), log2);
+    for (int t = row_tiles(a, s) - 1; t >= 0; --t) n += a.ends + tiles_of(item_at(a, s, t), log2);
     return n * a.c.heads;
   };
   int64_t mine = 0;
@@ -140,6 +148,7 @@ __device__ __forceinline__ Walk walk_of(const AttnParams& a, int log2, int least
     total += shared[2 + w];
   }
   Walk k;
+  k.ends = a.ends;
   k.units = total;
   const bool small = total < int64_t(1) << 31;                      // 64-bit divisions are slow
   k.workers = int(max(int64_t(1), min(int64_t(gridDim.x), small ? int64_t(uint32_t(total) / uint32_t(least)) : total / least)));
@@ -165,14 +174,16 @@ __device__ __forceinline__ Walk walk_of(const AttnParams& a, int log2, int least
   k.row_tile = 0;
   k.s = sequence_at(a, k.b);
   k.open(a, log2);
-  while (k.unit >= k.item_unit + int64_t(k.tiles) * a.c.heads) {
-    k.item_unit += int64_t(k.tiles) * a.c.heads;
+  while (k.unit >= k.item_unit + int64_t(k.ends + k.tiles) * a.c.heads) {
+    k.item_unit += int64_t(k.ends + k.tiles) * a.c.heads;
     ++k.row_tile;
     k.open(a, log2);
   }
-  k.head = k.unit - k.item_unit < int64_t(1) << 31 ? int(uint32_t(k.unit - k.item_unit) / uint32_t(k.tiles)) : int((k.unit - k.item_unit) / k.tiles);
-  k.item_unit += int64_t(k.head) * k.tiles;
-  k.tile = int(k.unit - k.item_unit);
+  const int each = k.ends + k.tiles;
+  k.head = k.unit - k.item_unit < int64_t(1) << 31 ? int(uint32_t(k.unit - k.item_unit) / uint32_t(each)) : int((k.unit - k.item_unit) / each);
+  k.item_unit += int64_t(k.head) * each;
+  k.unit = max(k.unit, k.first_tile());
+  k.tile = int(k.unit - k.first_tile());
   return k;
 }
 

@@ -24,6 +24,9 @@ constexpr int kThreads = 512, kSegments = 4;
 // last ones of an item may be empty): addresses of the MMAs are constants, and S of a tile is in the place that its stage's number says.
 constexpr int kAhead = 2, kStages = 4, kScales = 8;                           // stages in shared memory; tiles whose scales are kept
 constexpr uint32_t kTmem = 512, kO = 256;                                     // columns: S_i of even and odd tiles at 128 i and 128 i + 64, O_i at 256 + D i
+// An item's q, its results and, where it is cut, the pieces' way through memory take as long as some tiles do: counted as none a CTA with ends of many items was
+// the last one by far (chunks of up to 300 tokens in 8 sequences 126 us, with 4 to 12 tiles 113, 100, 104, 100; 2048 tokens after 6144 317, 308, 306, 306, 306).
+constexpr int kEnds = 8, kLeast = 12;          // in tiles; units that a CTA takes at least
 constexpr float kGrow = 8.f, kUp = 7.f;
 constexpr unsigned kPolynomial = 0x11;      // of eight pairs of exponentials, those that the FMA units take: the special function units are the bound
 
@@ -139,13 +142,13 @@ __device__ __forceinline__ void walk_items(const AttnParams& a, Shared& sh, Walk
       g.s = w.s; g.item = w.item;
       g.b = w.b; g.head = w.head; g.tiles = w.tiles;
       g.tile0 = done ? 0 : w.tile;
-      g.tile1 = done ? 0 : int(min(int64_t(w.tiles), w.stop - w.item_unit));
+      g.tile1 = done ? 0 : w.end_tile();
       g.piece = -1; g.c0 = g.c1 = g.piece0 = 0;
       if (!done && (g.tile0 != 0 || g.tile1 != w.tiles)) {
-        g.piece = 2 * int(blockIdx.x) + (w.item_unit + g.tile0 == w.start ? 0 : 1);
-        g.c0 = w.owner(w.item_unit);
-        g.c1 = w.owner(w.item_unit + w.tiles - 1);
-        g.piece0 = 2 * g.c0 + (w.start_of(g.c0) >= w.item_unit ? 0 : 1);
+        g.piece = w.piece();
+        g.c0 = w.owner(w.first_tile());
+        g.c1 = w.owner(w.first_tile() + w.tiles - 1);
+        g.piece0 = w.first_piece(g.c0);
       }
       sh.segments[slot] = g;
       umma::mbar_arrive(umma::smem_u32(&sh.described[slot]));
@@ -432,26 +435,30 @@ __device__ __forceinline__ bool tile_weights(uint32_t tmem_s, uint32_t tmem_o, c
   return true;
 }
 
-// Where row r of an item stands among packed rows and heads, times head_dim.
-__device__ __forceinline__ int64_t place_of(const AttnParams& a, const Segment& sg, int r) {
-  const int token = a.by_group(sg.item.r0 + r), head = sg.head * a.group + sg.item.r0 + r - token * a.group;
-  return (int64_t(sg.s.row + token) * a.heads + head) * a.c.dim;
-}
+// What the ends of an item need to know of it, in registers: every access to shared memory in between would have them read again.
+struct Ends {
+  int row, r0, r1, head, piece;               // packed row of the sequence's first token; rows [r0, r1); first head of the group; as in Segment
+  // Where row r of the item stands among packed rows and heads, times head_dim.
+  __device__ __forceinline__ int64_t place(const AttnParams& a, int r) const {
+    const int token = a.by_group(r0 + r);
+    return (int64_t(row + token) * a.heads + head + r0 + r - token * a.group) * a.c.dim;
+  }
+};
 
 // q of a warp's 32 rows, from row r0 of the sequence, into its place in shared memory; factor, unbias: of the row of this lane.  D / 8 lanes have a row; a lane
 // copies its 16 bytes of every row there as they are and then works on them in place.  (What happens once an item is short loops: unrolled code is fetched
 // more slowly than it runs when nothing has run it for a while; 12800 cycles here when it was.)
 template <int TYPE, class S>
-__device__ __forceinline__ void open_rows(const AttnParams& a, const Segment& sg, uint32_t q_smem, int r0, float& factor, float& unbias) {
-  constexpr int kLanes = S::D / 8, kStep = 32 / kLanes, kSteps = 32 / kStep;      // of a row; rows at once
+__device__ __forceinline__ void open_rows(const AttnParams& a, const Ends e, uint32_t q_smem, int r0, float& factor, float& unbias) {
+  constexpr int kLanes = S::D / 8, kStep = 32 / kLanes, kSteps = 32 / kStep, U = 4;      // of a row; rows at once; steps at once
   const int lane = threadIdx.x & 31, chunk = lane % kLanes, sub = lane / kLanes, row0 = 32 * ((threadIdx.x >> 5) & 3);
   const bool wide = ((reinterpret_cast<uintptr_t>(a.q) | uint64_t(a.row_stride * 2) | uint64_t(a.head_stride * 2)) & 15) == 0, f16 = a.dtype == DINO_F16;
-#pragma unroll 2
+#pragma unroll 4
   for (int k = 0; k < kSteps; ++k) {
-    const int r = r0 + kStep * k + sub, token = a.by_group(min(r, sg.item.r1 - 1)), head = sg.head * a.group + r - token * a.group;
-    const uint16_t* src = static_cast<const uint16_t*>(a.q) + int64_t(sg.s.row + token) * a.row_stride + int64_t(head) * a.head_stride + 8 * chunk;
+    const int r = r0 + kStep * k + sub, token = a.by_group(min(r, e.r1 - 1)), head = e.head + r - token * a.group;
+    const uint16_t* src = static_cast<const uint16_t*>(a.q) + int64_t(e.row + token) * a.row_stride + int64_t(head) * a.head_stride + 8 * chunk;
     const uint32_t to = q_smem + operand_at<kRows>(row0 + kStep * k + sub, chunk);
-    if (r >= sg.item.r1) {
+    if (r >= e.r1) {
       st_shared16(to, 0u, 0u, 0u, 0u);
     } else if (wide) {
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to), "l"(src) : "memory");
@@ -463,42 +470,62 @@ __device__ __forceinline__ void open_rows(const AttnParams& a, const Segment& sg
     }
   }
   asm volatile("cp.async.wait_all;\n" ::: "memory");
-#pragma unroll 2
-  for (int k = 0; k < kSteps; ++k) {
-    const uint32_t to = q_smem + operand_at<kRows>(row0 + kStep * k + sub, chunk);
-    const uint4 x = lds128(to);
-    // The largest of the 16-bit magnitudes, whose order is that of the values.
-    uint32_t largest = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
-    largest = max(largest & 0xffffu, largest >> 16);
+#pragma unroll 1
+  for (int k = 0; k < kSteps; k += U) {
+    uint32_t to[U], largest[U];
+    uint4 x[U];
+    float down[U], total[U];
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-    const float top = f16 ? __half2float(__ushort_as_half(uint16_t(largest))) : __uint_as_float(largest << 16);
-    const uint32_t e = __float_as_uint(top) >> 23;
-    const bool plain = e == 0 || e == 255;
-    const int shift = plain ? 0 : min(max(127 + 12 - int(e), -126), 126);
-    const float up = __uint_as_float(uint32_t(127 + shift) << 23), down = __uint_as_float(uint32_t(127 - shift) << 23);
-    const float sign = a.scale < 0.f ? -up : up;                        // scores' factors are not negative
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    uint32_t h[4];
-    float total = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 v = f16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[j])) : make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
-      h[j] = pack_half(v.x * sign, v.y * sign);
-      const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
-      total += back.x + back.y;
+    for (int u = 0; u < U; ++u) {
+      to[u] = q_smem + operand_at<kRows>(row0 + kStep * (k + u) + sub, chunk);
+      x[u] = lds128(to[u]);
     }
-    st_shared16(to, h[0], h[1], h[2], h[3]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {                                       // the largest of the 16-bit magnitudes, whose order is that of the values
+      const uint32_t m = __vmaxu2(__vmaxu2(x[u].x & 0x7fff7fffu, x[u].y & 0x7fff7fffu), __vmaxu2(x[u].z & 0x7fff7fffu, x[u].w & 0x7fff7fffu));
+      largest[u] = max(m & 0xffffu, m >> 16);
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) largest[u] = max(largest[u], __shfl_xor_sync(0xffffffffu, largest[u], o));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float top = f16 ? __half2float(__ushort_as_half(uint16_t(largest[u]))) : __uint_as_float(largest[u] << 16);
+      const uint32_t exponent = __float_as_uint(top) >> 23;
+      const bool plain = exponent == 0 || exponent == 255;
+      const int shift = plain ? 0 : min(max(127 + 12 - int(exponent), -126), 126);
+      const float up = __uint_as_float(uint32_t(127 + shift) << 23), sign = a.scale < 0.f ? -up : up;      // scores' factors are not negative
+      down[u] = __uint_as_float(uint32_t(127 - shift) << 23);
+      const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+      uint32_t h[4];
+      total[u] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 v = f16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[j])) : make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+        h[j] = pack_half(v.x * sign, v.y * sign);
+        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+        total[u] += back.x + back.y;
+      }
+      st_shared16(to[u], h[0], h[1], h[2], h[3]);
+    }
     if (Half2Of<TYPE>::kBias != 0.f) {                                  // K's of int8 are that much too large
 #pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      for (int o = kLanes / 2; o > 0; o >>= 1) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) total[u] += __shfl_xor_sync(0xffffffffu, total[u], o);
+      }
     }
 #pragma unroll
-    for (int j = 0; j < kStep; ++j) {                                   // to the lanes of these rows
-      const float d = __shfl_sync(0xffffffffu, down, j * kLanes), t = __shfl_sync(0xffffffffu, total, j * kLanes);
-      if (lane == kStep * k + j) {
-        factor = fabsf(a.scale) * d;
-        unbias = Half2Of<TYPE>::kBias * t;
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int j = 0; j < kStep; ++j) {                                 // to the lanes of these rows
+        const float d = __shfl_sync(0xffffffffu, down[u], j * kLanes), t = Half2Of<TYPE>::kBias != 0.f ? __shfl_sync(0xffffffffu, total[u], j * kLanes) : 0.f;
+        if (lane == kStep * (k + u) + j) {
+          factor = fabsf(a.scale) * d;
+          unbias = Half2Of<TYPE>::kBias * t;
+        }
       }
     }
   }
@@ -509,12 +536,12 @@ __device__ __forceinline__ void open_rows(const AttnParams& a, const Segment& sg
 // O of a warp's 32 rows (row0: the first one's number in the item): results, or float32 sums of a piece.  Through the place of q, which nobody reads any more:
 // 256 bytes a row there, chunks of 16 bytes turned by the row's number, so that rows leave in whole lines.
 template <class S>
-__device__ __forceinline__ void close_rows(const AttnParams& a, const Segment& sg, uint32_t q_smem, uint32_t tmem_o, int row0, float inverse) {
+__device__ __forceinline__ void close_rows(const AttnParams& a, const Ends e, uint32_t q_smem, uint32_t tmem_o, int row0, float inverse) {
   constexpr int D = S::D, kPiece = kItemRows * (D + 2);
-  const int lane = threadIdx.x & 31, rows = sg.item.r1 - sg.item.r0 - row0;      // of this warp's
+  const int lane = threadIdx.x & 31, rows = e.r1 - e.r0 - row0;      // of this warp's
   const uint32_t mine = q_smem + uint32_t(((threadIdx.x >> 5) & 3) * 32 * D * 2);
   auto at = [&](int row, int chunk) { return mine + uint32_t(row * D * 2) + uint32_t((chunk ^ (row & (D / 8 - 1))) << 4); };
-  if (sg.piece < 0) {
+  if (e.piece < 0) {
 #pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
       uint32_t o[32], h[16];
@@ -538,12 +565,12 @@ __device__ __forceinline__ void close_rows(const AttnParams& a, const Segment& s
 #pragma unroll 4
     for (int k = 0; k < 32; k += kStep) {
       const int row = k + lane / kLanes, chunk = lane % kLanes;
-      if (row < rows) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + place_of(a, sg, row0 + row) + 8 * chunk) = lds128(at(row, chunk));
+      if (row < rows) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + e.place(a, row0 + row) + 8 * chunk) = lds128(at(row, chunk));
     }
     __syncwarp();
     return;
   }
-  float* const part = a.partial + size_t(sg.piece) * kPiece + size_t(row0) * D;
+  float* const part = a.partial + size_t(e.piece) * kPiece + size_t(row0) * D;
 #pragma unroll 1
   for (int half = 0; half < 2; ++half) {                                // D / 2 columns at a time
 #pragma unroll
@@ -567,10 +594,10 @@ __device__ __forceinline__ void close_rows(const AttnParams& a, const Segment& s
 
 // The results of a cut item from its pieces, by 256 threads.  First a row's largest y and its sum by a thread each (kept in the place of q), then the sums of
 // all columns, kPlaces of four columns and kPieces pieces under way at a time.
-template <class S, typename Meet> __device__ __forceinline__ bool join_rows(const AttnParams& a, const Segment& sg, uint32_t q_smem, Meet meet) {
+template <class S, typename Meet> __device__ __forceinline__ bool join_rows(const AttnParams& a, const Ends e, int c0, int c1, int piece0, uint32_t q_smem, Meet meet) {
   constexpr int D = S::D, kPiece = kItemRows * (D + 2), kPlaces = 8, kPieces = 2;
-  const int rows = sg.item.r1 - sg.item.r0, count = sg.c1 - sg.c0 + 1, tid = int(threadIdx.x);
-  auto piece = [&](int c) { return a.partial + size_t(c == 0 ? sg.piece0 : 2 * (sg.c0 + c)) * kPiece; };
+  const int rows = e.r1 - e.r0, count = c1 - c0 + 1, tid = int(threadIdx.x);
+  auto piece = [&](int c) { return a.partial + size_t(c == 0 ? piece0 : 2 * (c0 + c)) * kPiece; };
   auto weight = [](float ref, float top) { return ref == -INFINITY ? 0.f : exp2_approx(ref - top); };
   if (tid < rows) {
     float top = -INFINITY, sum = 0.f;
@@ -641,7 +668,7 @@ template <class S, typename Meet> __device__ __forceinline__ bool join_rows(cons
         const __nv_bfloat162 lo = __floats2bfloat162_rn(v[u].x * inv, v[u].y * inv), hi = __floats2bfloat162_rn(v[u].z * inv, v[u].w * inv);
         h = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
       }
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + place_of(a, sg, x / (D / 4)) + x % (D / 4) * 4) = h;
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + e.place(a, x / (D / 4)) + x % (D / 4) * 4) = h;
     }
   }
   return meet();                                                        // (the next item's q goes where the rows' sums are)
@@ -665,11 +692,12 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
     const Segment& sg = sh.segments[slot];
     const int tile0 = sg.tile0, tile1 = sg.tile1;
     if (tile0 == tile1) return;
-    const int r = sg.item.r0 + i * kRows + my_row;
-    const bool mine = r < sg.item.r1;
-    const int token = a.by_group(mine ? r : sg.item.r0);
+    const Ends e = {sg.s.row, sg.item.r0, sg.item.r1, sg.head * a.group, sg.piece};
+    const int r = e.r0 + i * kRows + my_row;
+    const bool mine = r < e.r1;
+    const int token = a.by_group(mine ? r : e.r0);
     float factor = 0.f, unbias = 0.f;
-    open_rows<TYPE, S>(a, sg, q_smem + uint32_t(i * S::kQ), sg.item.r0 + i * kRows + 32 * (warp & 3), factor, unbias);
+    open_rows<TYPE, S>(a, e, q_smem + uint32_t(i * S::kQ), e.r0 + i * kRows + 32 * (warp & 3), factor, unbias);
     if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.q_ready));
     const int position = sg.s.first + token;
     const int high = mine ? min(position + 1, sg.s.end) : 0, low = a.window > 0 ? max(0, position - a.window + 1) : 0;
@@ -704,10 +732,10 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
     n += stages_of(tiles);
     first += tiles;
     umma::tcgen05_fence_after();
-    close_rows<S>(a, sg, q_smem + uint32_t(i * S::kQ), tmem_o, i * kRows + 32 * (warp & 3), l == 0.f ? 0.f : 1.f / l);
+    close_rows<S>(a, e, q_smem + uint32_t(i * S::kQ), tmem_o, i * kRows + 32 * (warp & 3), l == 0.f ? 0.f : 1.f / l);
     umma::tcgen05_fence_before();
-    if (sg.piece >= 0) {                                                // cut: the last of its CTAs to arrive adds the pieces up, in order
-      if (mine) __stcg(reinterpret_cast<float2*>(a.partial + size_t(sg.piece) * kPiece + kItemRows * D) + (i * kRows + my_row), make_float2(ref, l));
+    if (e.piece >= 0) {                                                 // cut: the last of its CTAs to arrive adds the pieces up, in order
+      if (mine) __stcg(reinterpret_cast<float2*>(a.partial + size_t(e.piece) * kPiece + kItemRows * D) + (i * kRows + my_row), make_float2(ref, l));
       if (!meet()) return;
       if (threadIdx.x == 0) {
         int before = 0;
@@ -717,7 +745,7 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
       }
       if (!meet()) return;
       if (sh.last) {
-        if (!join_rows<S>(a, sg, q_smem, meet)) return;
+        if (!join_rows<S>(a, e, sg.c0, sg.c1, sg.piece0, q_smem, meet)) return;
       }
     }
     __syncwarp();
@@ -758,7 +786,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_many_kernel(const __gri
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   asm volatile("griddepcontrol.wait;\n" ::: "memory");                // nothing of the launches before is read before this
   umma::tcgen05_fence_before();
-  const Walk first = walk_of<kThreads>(a, kLog2, 1, sh.walk);         // (its barriers: the inits and the allocation are visible)
+  const Walk first = walk_of<kThreads>(a, kLog2, kLeast, sh.walk);         // (its barriers: the inits and the allocation are visible)
   __syncthreads();
   umma::tcgen05_fence_after();
   if (warp < 8) {
@@ -794,6 +822,7 @@ template <int TYPE, int D> int launch(AttnParams& a, cudaStream_t s) {
   using S = Shape<D>;
   a.row_tile = kItemRows;
   a.row_tile_log2 = 8;
+  a.ends = kEnds;
   const int ctas = stream::sm_count();
   a.partial = attention_scratch(size_t(ctas) * 2 * kItemRows * (D + 2), ctas, s, &a.arrived);
   if (a.partial == nullptr) return RC_LAUNCH;
