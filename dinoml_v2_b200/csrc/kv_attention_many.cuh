@@ -445,12 +445,12 @@ struct Ends {
   }
 };
 
-// q of a warp's 32 rows, from row r0 of the sequence, into its place in shared memory; factor, unbias: of the row of this lane.  D / 8 lanes have a row; a lane
-// copies its 16 bytes of every row there as they are and then works on them in place.  (What happens once an item is short loops: unrolled code is fetched
-// more slowly than it runs when nothing has run it for a while; 12800 cycles here when it was.)
+// q of a warp's 32 rows, from row r0 of the sequence, into its place in shared memory; factor, unbias: of the row of this lane.  It is copied there as it is
+// (D / 8 lanes have a row) and worked on in place by a thread a row: eight lanes' chunks lie in different banks by the swizzle, and nothing is shuffled (4000
+// to 5700 cycles an item went into shuffles).  What happens once an item is short loops: unrolled code is fetched more slowly than it runs.
 template <int TYPE, class S>
 __device__ __forceinline__ void open_rows(const AttnParams& a, const Ends e, uint32_t q_smem, int r0, float& factor, float& unbias) {
-  constexpr int kLanes = S::D / 8, kStep = 32 / kLanes, kSteps = 32 / kStep, U = 4;      // of a row; rows at once; steps at once
+  constexpr int kLanes = S::D / 8, kStep = 32 / kLanes, kSteps = 32 / kStep;      // of a row; rows at once
   const int lane = threadIdx.x & 31, chunk = lane % kLanes, sub = lane / kLanes, row0 = 32 * ((threadIdx.x >> 5) & 3);
   const bool wide = ((reinterpret_cast<uintptr_t>(a.q) | uint64_t(a.row_stride * 2) | uint64_t(a.head_stride * 2)) & 15) == 0, f16 = a.dtype == DINO_F16;
 #pragma unroll 4
@@ -470,65 +470,37 @@ __device__ __forceinline__ void open_rows(const AttnParams& a, const Ends e, uin
     }
   }
   asm volatile("cp.async.wait_all;\n" ::: "memory");
-#pragma unroll 1
-  for (int k = 0; k < kSteps; k += U) {
-    uint32_t to[U], largest[U];
-    uint4 x[U];
-    float down[U], total[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      to[u] = q_smem + operand_at<kRows>(row0 + kStep * (k + u) + sub, chunk);
-      x[u] = lds128(to[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {                                       // the largest of the 16-bit magnitudes, whose order is that of the values
-      const uint32_t m = __vmaxu2(__vmaxu2(x[u].x & 0x7fff7fffu, x[u].y & 0x7fff7fffu), __vmaxu2(x[u].z & 0x7fff7fffu, x[u].w & 0x7fff7fffu));
-      largest[u] = max(m & 0xffffu, m >> 16);
-    }
-#pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) largest[u] = max(largest[u], __shfl_xor_sync(0xffffffffu, largest[u], o));
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const float top = f16 ? __half2float(__ushort_as_half(uint16_t(largest[u]))) : __uint_as_float(largest[u] << 16);
-      const uint32_t exponent = __float_as_uint(top) >> 23;
-      const bool plain = exponent == 0 || exponent == 255;
-      const int shift = plain ? 0 : min(max(127 + 12 - int(exponent), -126), 126);
-      const float up = __uint_as_float(uint32_t(127 + shift) << 23), sign = a.scale < 0.f ? -up : up;      // scores' factors are not negative
-      down[u] = __uint_as_float(uint32_t(127 - shift) << 23);
-      const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-      uint32_t h[4];
-      total[u] = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 v = f16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[j])) : make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
-        h[j] = pack_half(v.x * sign, v.y * sign);
-        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
-        total[u] += back.x + back.y;
-      }
-      st_shared16(to[u], h[0], h[1], h[2], h[3]);
-    }
-    if (Half2Of<TYPE>::kBias != 0.f) {                                  // K's of int8 are that much too large
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) total[u] += __shfl_xor_sync(0xffffffffu, total[u], o);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int j = 0; j < kStep; ++j) {                                 // to the lanes of these rows
-        const float d = __shfl_sync(0xffffffffu, down[u], j * kLanes), t = Half2Of<TYPE>::kBias != 0.f ? __shfl_sync(0xffffffffu, total[u], j * kLanes) : 0.f;
-        if (lane == kStep * (k + u) + j) {
-          factor = fabsf(a.scale) * d;
-          unbias = Half2Of<TYPE>::kBias * t;
-        }
-      }
-    }
+  __syncwarp();
+  uint32_t largest = 0;                                                 // of the 16-bit magnitudes, whose order is that of the values
+#pragma unroll 4
+  for (int c = 0; c < S::D / 8; ++c) {
+    const uint4 x = lds128(q_smem + operand_at<kRows>(row0 + lane, c));
+    largest = __vmaxu2(largest, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
   }
+  largest = max(largest & 0xffffu, largest >> 16);
+  const float top = f16 ? __half2float(__ushort_as_half(uint16_t(largest))) : __uint_as_float(largest << 16);
+  const uint32_t exponent = __float_as_uint(top) >> 23;
+  const bool plain = exponent == 0 || exponent == 255;
+  const int shift = plain ? 0 : min(max(127 + 12 - int(exponent), -126), 126);
+  const float up = __uint_as_float(uint32_t(127 + shift) << 23), sign = a.scale < 0.f ? -up : up;      // scores' factors are not negative
+  float total[2] = {0.f, 0.f};
+#pragma unroll 2
+  for (int c = 0; c < S::D / 8; ++c) {
+    const uint32_t at = q_smem + operand_at<kRows>(row0 + lane, c);
+    const uint4 x = lds128(at);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    uint32_t h[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 v = f16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[j])) : make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+      h[j] = pack_half(v.x * sign, v.y * sign);
+      const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+      total[j & 1] += back.x + back.y;
+    }
+    st_shared16(at, h[0], h[1], h[2], h[3]);
+  }
+  factor = fabsf(a.scale) * __uint_as_float(uint32_t(127 - shift) << 23);
+  unbias = Half2Of<TYPE>::kBias * (total[0] + total[1]);                // K's of int8 are that much too large
   fence_async_smem();
   __syncwarp();
 }
