@@ -281,7 +281,8 @@ __device__ __forceinline__ void issue_mmas(const AttnParams& a, Shared& sh, uint
           const uint32_t scores = tmem + uint32_t(i * 128 + (u & 1) * 64);
           if (j >= 0 && j < tiles) issue_weights<S, 0>(tmem + kO + uint32_t(i * S::D), scores, v, idesc_o, j != 0);
           if (u < tiles) issue_scores<S, 0>(scores, q0 + uint64_t((i * S::kQ) >> 4), k, idesc_s);      // into the place of the weights just read
-          umma::umma_commit<false>(umma::smem_u32(&sh.s_full[i][u & 1]), 0);
+          // (Not at the empty stages behind an item's last products: nothing there waits for the softmax, so that a phase of the barrier could pass it by.)
+          if (j < tiles) umma::umma_commit<false>(umma::smem_u32(&sh.s_full[i][u & 1]), 0);
           if (i == 1) umma::umma_commit<false>(umma::smem_u32(&sh.empty[stage]), 0);
         }
         __syncwarp();
@@ -652,7 +653,8 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
   constexpr int D = S::D, kPiece = kItemRows * (D + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = warp >> 2, my_row = 32 * (warp & 3) + lane;
   const uint32_t lanes = sh.tmem + (uint32_t(32 * (warp & 3)) << 16), tmem_s = lanes + uint32_t(i * 128), tmem_o = lanes + kO + uint32_t(i * D);
-  int n = 0, first = 0, meetings = 0;                                   // stages, tiles so far
+  int first = 0, meetings = 0;                                          // tiles so far
+  uint32_t scores = 0;                                                  // phases of s_full, a bit for even and one for odd stages
   auto meet = [&] {
     __syncwarp();
     if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.together));
@@ -680,14 +682,15 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
     const int tiles = tile1 - tile0;
     for (int u = 0; u < tiles; ++u) {
       const int tile = tile0 + u;
-      if (!wait(a, sh, &sh.s_full[i][u & 1], uint32_t((n + u) >> 1) & 1u)) { lost = true; break; }
+      if (!wait(a, sh, &sh.s_full[i][u & 1], (scores >> (u & 1)) & 1u)) { lost = true; break; }
+      scores ^= 1u << (u & 1);
       umma::tcgen05_fence_after();
       const float4* const scales = sh.scales[(first + u) % kScales];
       const int token0 = base + tile * kTile;
       const int4 whole = sh.whole[(first + u) % kScales];
       const bool every = token0 >= all_low && token0 + kTile <= all_high && (whole.x & whole.y & whole.z & whole.w) != 0;
       const uint32_t at = tmem_s + uint32_t((u & 1) * 64);
-      auto products_done = [&] { return wait(a, sh, &sh.s_full[i][(u + 1) & 1], uint32_t((n + u + 1) >> 1) & 1u); };      // the MMAs of the stage after this one
+      auto products_done = [&] { return wait(a, sh, &sh.s_full[i][(u + 1) & 1], (scores >> ((u + 1) & 1)) & 1u); };      // the MMAs of the stage after this one
       if (!(every ? tile_weights<S, true>(at, tmem_o, scales, factor, unbias, 0, 0, u > 0, ref, l, products_done)
                   : tile_weights<S, false>(at, tmem_o, scales, factor, unbias, low - token0, high - token0, u > 0, ref, l, products_done))) {
         lost = true;
@@ -699,9 +702,10 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
       if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.p_ready[i][u & 1]));
     }
     if (lost) return;
-    for (int u = tiles; u < stages_of(tiles); ++u)                       // the last of the products among them
-      if (!wait(a, sh, &sh.s_full[i][u & 1], uint32_t((n + u) >> 1) & 1u)) return;
-    n += stages_of(tiles);
+    for (int u = tiles; u < tiles + kAhead; ++u) {                       // the last products
+      if (!wait(a, sh, &sh.s_full[i][u & 1], (scores >> (u & 1)) & 1u)) return;
+      scores ^= 1u << (u & 1);
+    }
     first += tiles;
     umma::tcgen05_fence_after();
     close_rows<S>(a, e, q_smem + uint32_t(i * S::kQ), tmem_o, i * kRows + 32 * (warp & 3), l == 0.f ? 0.f : 1.f / l);
