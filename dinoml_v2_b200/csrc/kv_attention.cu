@@ -79,7 +79,7 @@ int cache_attention(const DinoB200KvCache* cache, const DinoB200KvBatch* batch, 
   a.dtype = dtype;
   // Sequences with few rows go to one kernel, those with many to the other; which there are only the device knows, so a call with rows enough is both.
   const int64_t all_rows = int64_t(a.p.rows) * a.group, rows = (all_rows + a.p.sequences - 1) / a.p.sequences;
-  const bool tensor = dtype != DINO_F32 && a.c.dim != 256;
+  const bool tensor = dtype != DINO_F32 || a.c.dim != 256;                   // (two terms of 256 values do not fit into shared memory)
   const int64_t most = a.p.starts == nullptr ? a.group : all_rows;          // rows of a sequence
   a.min_rows = 0;
   a.max_rows = tensor ? kFewRows : INT32_MAX;

@@ -12,17 +12,19 @@
 // what V is multiplied by, and the softmax's sum takes P / vs in float32.  ref is the row's largest y when it was last set; O is rescaled only when y
 // outgrows it by 2^8, so that P stays below 2^15 and loses bits (as a float16 denormal) only below 2^-21 of that.
 #pragma once
+#include <type_traits>
+
 #include "kv_attention.cuh"
 
 namespace b200gguf {
 namespace kv {
 namespace many {
 
-constexpr int kRows = 128, kItemRows = 2 * kRows, kTile = 64, kLog2 = 6;       // rows of an MMA, of an item; cached tokens of a tile
+constexpr int kRows = 128, kTile = 64, kLog2 = 6;                             // rows of an MMA; cached tokens of a tile
 constexpr int kThreads = 512, kSegments = 4;
 // A stage is V of a tile and K of the tile two behind it, which the MMAs read one after the other: one barrier for both.  Items begin at stage 0 (the
 // last ones of an item may be empty): addresses of the MMAs are constants, and S of a tile is in the place that its stage's number says.
-constexpr int kAhead = 2, kStages = 4, kScales = 8;                           // stages in shared memory; tiles whose scales are kept
+constexpr int kAhead = 2, kMostStages = 4, kScales = 8;                       // stages in shared memory; tiles whose scales are kept
 constexpr uint32_t kTmem = 512, kO = 256;                                     // columns: S_i of even and odd tiles at 128 i and 128 i + 64, O_i at 256 + D i
 // An item's q, its results and, where it is cut, the pieces' way through memory take as long as some tiles do: counted as none a CTA with ends of many items was
 // the last one by far (chunks of up to 300 tokens in 8 sequences 126 us, with 4 to 12 tiles 113, 100, 104, 100; 2048 tokens after 6144 317, 308, 306, 306, 306).
@@ -30,10 +32,14 @@ constexpr int kEnds = 8, kLeast = 12;          // in tiles; units that a CTA tak
 constexpr float kGrow = 8.f, kUp = 7.f;
 constexpr unsigned kPolynomial = 0x11;      // of eight pairs of exponentials, those that the FMA units take: the special function units are the bound
 
-template <int D_> struct Shape {
-  static constexpr int D = D_;
-  static constexpr int kQ = kRows * D * 2, kKv = kTile * D * 2;      // bytes of a tile of Q, of K or V
-  static constexpr size_t kSmem = 1024 + 2 * size_t(kQ) + 2 * kStages * size_t(kKv);
+// PARTS: float16 terms of a q and of a weight, 2 for float32 activations.  Shared memory has room for two tiles of rows where q takes 256 bytes a row, for
+// one tile beyond; the warps that had the other one are converters then.
+template <int D_, int PARTS_> struct Shape {
+  static constexpr int D = D_, PARTS = PARTS_;
+  static constexpr int kTiles = PARTS == 1 && D <= 128 ? 2 : 1, kStages = D <= 128 ? kMostStages : 2, kConverters = kTiles == 2 ? 4 : 8;
+  static constexpr int kItemRows = kTiles * kRows, kPiece = kItemRows * (D + 2);      // rows of an item; floats of a piece
+  static constexpr int kQ = kRows * D * PARTS * 2, kKv = kTile * D * 2;               // bytes of a tile of Q, of K or V
+  static constexpr size_t kSmem = 1024 + size_t(kTiles) * kQ + 2 * kStages * size_t(kKv);
 };
 
 struct Segment {
@@ -45,7 +51,7 @@ struct Segment {
 
 struct Shared {
   uint64_t described[kSegments], closed[kSegments], q_ready;
-  uint64_t full[kStages], empty[kStages];
+  uint64_t full[kMostStages], empty[kMostStages];
   uint64_t s_full[2][2], p_ready[2][2], together, drain;    // of row tile i, even and odd stages: its MMAs are done, its weights are there
   Segment segments[kSegments];
   float4 scales[kScales][kTile / 16];         // of 16 tokens: K's scale, log2 of V's, 1 / V's, whether there is a block
@@ -55,7 +61,7 @@ struct Shared {
   int last, lost;
 };
 
-__device__ __forceinline__ int stages_of(int tiles) { return (tiles + kAhead + kStages - 1) / kStages * kStages; }
+template <class S> __device__ __forceinline__ int stages_of(int tiles) { return (tiles + kAhead + S::kStages - 1) / S::kStages * S::kStages; }
 
 __device__ __forceinline__ bool wait(const AttnParams& a, Shared& sh, uint64_t* bar, uint32_t parity) {      // bounded; by a converged warp
   const uint32_t at = umma::smem_u32(bar);
@@ -100,14 +106,15 @@ template <int A_OFF, int B_OFF> __device__ __forceinline__ void umma_f16_ts(uint
   asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t.reg .b32 a;\n\tadd.s32 a, %1, %5;\n\tadd.s64 b, %2, %6;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, p;\n\t}\n" ::"r"(tmem_d),
                "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "n"(A_OFF), "n"(B_OFF) : "memory");
 }
-// O += P V and S = Q K^T of a stage, step by step of sixteen.
+// O += P V and S = Q K^T of a stage, step by step of sixteen.  Terms: those of the weights lie one after the other, those of q step by step.
 template <class S, int I> __device__ __forceinline__ void issue_weights(uint32_t tmem_o, uint32_t tmem_p, uint64_t v, uint32_t idesc, bool more) {
-  umma_f16_ts<8 * I, (16 * 128 * I) / 16>(tmem_o, tmem_p, v, idesc, more || I != 0 ? 1u : 0u);
-  if constexpr (I + 1 < kTile / 16) issue_weights<S, I + 1>(tmem_o, tmem_p, v, idesc, more);
+  umma_f16_ts<8 * I, (16 * 128 * (I % (kTile / 16))) / 16>(tmem_o, tmem_p, v, idesc, more || I != 0 ? 1u : 0u);
+  if constexpr (I + 1 < S::PARTS * kTile / 16) issue_weights<S, I + 1>(tmem_o, tmem_p, v, idesc, more);
 }
 template <class S, int I> __device__ __forceinline__ void issue_scores(uint32_t tmem_s, uint64_t q, uint64_t k, uint32_t idesc) {
-  umma_f16_ss<((I >> 2) * kRows * 128 + (I & 3) * 32) / 16, ((I >> 2) * kTile * 128 + (I & 3) * 32) / 16>(tmem_s, q, k, idesc, I != 0);
-  if constexpr (I + 1 < S::D / 16) issue_scores<S, I + 1>(tmem_s, q, k, idesc);
+  constexpr int J = I / S::PARTS;
+  umma_f16_ss<((I >> 2) * kRows * 128 + (I & 3) * 32) / 16, ((J >> 2) * kTile * 128 + (J & 3) * 32) / 16>(tmem_s, q, k, idesc, I != 0);
+  if constexpr (I + 1 < S::PARTS * S::D / 16) issue_scores<S, I + 1>(tmem_s, q, k, idesc);
 }
 // V as it lies: rows of tokens (K of the product), 64 channels (N) of 128 bytes, blocks of 64 channels one after the other.
 __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr, int block_bytes) {
@@ -176,17 +183,18 @@ template <int TYPE, class S, bool BIASED, int COPIES> __device__ __forceinline__
   }
 }
 
-// ---- warps 8..11.  A warp has 16 tokens of every tile, which are of one block, in kCopies steps of kStep tokens, 16 values a lane.
+// ---- the converters, up to warp 11.  A warp has 16 tokens of every tile, which are of one block, and kChannels of their channels, in kCopies steps of kStep
+// tokens, 16 values a lane.
 template <int TYPE, class S>
 __device__ __forceinline__ void convert_tiles(const AttnParams& a, Shared& sh, uint32_t k_smem, uint32_t v_smem) {
-  constexpr int kChunks = S::D / 16, kStep = 32 / kChunks, kCopies = 16 / kStep;
-  const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, chunk = lane % kChunks;
+  constexpr int kStages = S::kStages, kChannels = 4 * S::D / S::kConverters, kChunks = kChannels / 16, kStep = 32 / kChunks, kCopies = 16 / kStep;
+  const int warp = (threadIdx.x >> 5) & 3, part = (threadIdx.x >> 5) - (12 - S::kConverters) >= 4, lane = threadIdx.x & 31, chunk = lane % kChunks;
   // Where eight lanes have one row of 128 values, those of its second half take the neighbouring row instead: their stores go to the other banks.
   const int row = lane / kChunks ^ (kChunks == 8 ? (lane >> 2) & 1 : 0);
   const int log2 = a.c.block_log2, mask = (1 << log2) - 1;
   uint32_t to[2];                                                       // of a lane's two times 8 float16 in the first step
 #pragma unroll
-  for (int h = 0; h < 2; ++h) to[h] = operand_at<kTile>(16 * warp + row, 2 * chunk + h);
+  for (int h = 0; h < 2; ++h) to[h] = operand_at<kTile>(16 * warp + row, part * (kChannels / 8) + 2 * chunk + h);
   int n = 0, first = 0;                                                 // stages so far; tiles before this item's
   for (int segment = 0;; ++segment) {
     const int slot = segment % kSegments;
@@ -203,7 +211,7 @@ __device__ __forceinline__ void convert_tiles(const AttnParams& a, Shared& sh, u
     uint4 raw[2][kCopies];
     auto load = [&](uint4 (&x)[kCopies], int which, int tile, int bh) {
       const int token = base + tile * kTile + 16 * warp + row;
-      const uint8_t* const from = a.c.data[which] + chunk * 16 + ((int64_t(bh) << log2) + (token & mask)) * S::D;
+      const uint8_t* const from = a.c.data[which] + part * kChannels + chunk * 16 + ((int64_t(bh) << log2) + (token & mask)) * S::D;
 #pragma unroll
       for (int i = 0; i < kCopies; ++i) {
         x[i] = make_uint4(0u, 0u, 0u, 0u);                              // (what nobody sees has to be finite: zeros)
@@ -227,17 +235,17 @@ __device__ __forceinline__ void convert_tiles(const AttnParams& a, Shared& sh, u
       }
     };
     load_k(tile0, bh[kAhead]);
-    for (int u = 0; u < stages_of(tiles); ++u, ++n) {
+    for (int u = 0; u < stages_of<S>(tiles); ++u, ++n) {
       const int after = look_up(tile0 + u + 2), stage = n % kStages;
       if (!wait(a, sh, &sh.empty[stage], (uint32_t(n / kStages) & 1u) ^ 1u)) return;
       if (u < tiles) {
         const int at = (first + u) % kScales;
-        if (lane == 0) {
+        if (lane == 0 && part == 0) {
           const float v = vs < 0x1p-100f ? 0x1p-100f : vs;              // (a NaN stays)
           sh.scales[at][warp] = make_float4(ks, __log2f(v), __fdividef(1.f, v), bh[kAhead] >= 0 ? 1.f : 0.f);
           reinterpret_cast<int*>(&sh.whole[at])[warp] = bh[kAhead] >= 0;
         }
-        store_operand<TYPE, S, true>(raw[0], k_smem + uint32_t(stage * S::kKv), to);
+        store_operand<TYPE, S, S::PARTS == 1>(raw[0], k_smem + uint32_t(stage * S::kKv), to);
       }
       load_k(tile0 + u + 1, bh[kAhead + 1]);
       if (u >= kAhead && u < tiles + kAhead) store_operand<TYPE, S, false>(raw[1], v_smem + uint32_t(stage * S::kKv), to);
@@ -269,12 +277,12 @@ __device__ __forceinline__ void issue_mmas(const AttnParams& a, Shared& sh, uint
     const int tiles = sh.segments[slot].tile1 - sh.segments[slot].tile0;
     if (tiles == 0) return;
     if (!wait(a, sh, &sh.q_ready, uint32_t(segment) & 1u)) return;
-    for (int u = 0; u < stages_of(tiles); ++u, ++n) {
-      const int stage = u % kStages, j = u - kAhead;                    // K of tile u, V of tile j
+    for (int u = 0; u < stages_of<S>(tiles); ++u, ++n) {
+      const int stage = u % S::kStages, j = u - kAhead;                 // K of tile u, V of tile j
       const uint64_t k = k0 + uint64_t(uint32_t(stage * S::kKv) >> 4), v = v0 + uint64_t(uint32_t(stage * S::kKv) >> 4);
-      if (!wait(a, sh, &sh.full[stage], uint32_t(n / kStages) & 1u)) return;
+      if (!wait(a, sh, &sh.full[stage], uint32_t(n / S::kStages) & 1u)) return;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < S::kTiles; ++i) {
         if (j >= 0 && j < tiles && !wait(a, sh, &sh.p_ready[i][u & 1], (weights >> (u & 1)) & 1u)) return;
         umma::tcgen05_fence_after();
         if (umma::elect_one()) {
@@ -283,7 +291,7 @@ __device__ __forceinline__ void issue_mmas(const AttnParams& a, Shared& sh, uint
           if (u < tiles) issue_scores<S, 0>(scores, q0 + uint64_t((i * S::kQ) >> 4), k, idesc_s);      // into the place of the weights just read
           // (Not at the empty stages behind an item's last products: nothing there waits for the softmax, so that a phase of the barrier could pass it by.)
           if (j < tiles) umma::umma_commit<false>(umma::smem_u32(&sh.s_full[i][u & 1]), 0);
-          if (i == 1) umma::umma_commit<false>(umma::smem_u32(&sh.empty[stage]), 0);
+          if (i == S::kTiles - 1) umma::umma_commit<false>(umma::smem_u32(&sh.empty[stage]), 0);
         }
         __syncwarp();
       }
@@ -338,9 +346,10 @@ __device__ __forceinline__ float2 exp2_pair(uint64_t x) {
 
 // Weights of 32 columns (two blocks' scales), their sum over each block's V scale; the largest y = s + log2(vs) of them.
 // EVERY: the row sees all of its columns, else those in [low, high) of blocks that are there.
-template <bool EVERY>
-__device__ __forceinline__ void weights_of(const uint32_t (&r)[32], const float4 (&x)[2], float factor, float unbias, int low, int high, float bias, uint32_t (&p)[16],
-                                           float& l, float& top) {
+// PARTS: terms of a weight, the second one behind the first.  With two the FMA units' exponentials would be what limits the result.
+template <bool EVERY, int PARTS>
+__device__ __forceinline__ void weights_of(const uint32_t (&r)[32], const float4 (&x)[2], float factor, float unbias, int low, int high, float bias,
+                                           uint32_t (&p)[PARTS][16], float& l, float& top) {
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
     const float f = x[g].x * factor, add = fmaf(-unbias, f, x[g].y + bias);
@@ -352,7 +361,7 @@ __device__ __forceinline__ void weights_of(const uint32_t (&r)[32], const float4
       const float s[2] = {__uint_as_float(r[16 * g + k]), __uint_as_float(r[16 * g + k + 1])};
       const uint64_t y = fma2(pair_of(s[0], s[1]), ff, aa);
       float w[2];
-      if (EVERY && (kPolynomial >> (k / 2) & 1) != 0) {                 // (a NaN is lost there: the row's other columns of the block have it)
+      if (EVERY && PARTS == 1 && (kPolynomial >> (k / 2) & 1) != 0) {                 // (a NaN is lost there: the row's other columns of the block have it)
         const float2 e = exp2_pair(y);
         w[0] = e.x;
         w[1] = e.y;
@@ -371,7 +380,11 @@ __device__ __forceinline__ void weights_of(const uint32_t (&r)[32], const float4
         }
       }
       sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], pair_of(w[0], w[1]));
-      p[8 * g + k / 2] = pack_half(w[0], w[1]);
+      p[0][8 * g + k / 2] = pack_half(w[0], w[1]);
+      if (PARTS == 2) {
+        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&p[0][8 * g + k / 2]));
+        p[PARTS - 1][8 * g + k / 2] = pack_half(w[0] - back.x, w[1] - back.y);
+      }
     }
     const float2 both = halves_of(add2(sum[0], sum[1]));
     if (EVERY || both.x + both.y != 0.f) l = fmaf(both.x + both.y, x[g].z, l);
@@ -384,7 +397,7 @@ __device__ __forceinline__ void weights_of(const uint32_t (&r)[32], const float4
 template <class S, bool EVERY, typename Wait>
 __device__ __forceinline__ bool tile_weights(uint32_t tmem_s, uint32_t tmem_o, const float4* scales, float factor, float unbias, int low, int high, bool more,
                                              float& ref, float& l, Wait products_done) {
-  uint32_t r[2][32], p[2][16];
+  uint32_t r[2][32], p[2][S::PARTS][16];                                // p: of the first and the last 32 columns
   tmem_ld32(tmem_s, r[0]);
   float4 x[2][2];
 #pragma unroll
@@ -392,9 +405,9 @@ __device__ __forceinline__ bool tile_weights(uint32_t tmem_s, uint32_t tmem_o, c
   umma::tmem_ld_wait();
   tmem_ld32(tmem_s + 32u, r[1]);
   float bias = (ref == -INFINITY ? 0.f : -ref) + kUp, sum = 0.f, top = -INFINITY;
-  weights_of<EVERY>(r[0], x[0], factor, unbias, low, high, bias, p[0], sum, top);
+  weights_of<EVERY, S::PARTS>(r[0], x[0], factor, unbias, low, high, bias, p[0], sum, top);
   umma::tmem_ld_wait();
-  weights_of<EVERY>(r[1], x[1], factor, unbias, low - 32, high - 32, bias, p[1], sum, top);
+  weights_of<EVERY, S::PARTS>(r[1], x[1], factor, unbias, low - 32, high - 32, bias, p[1], sum, top);
   const bool grow = top > ref + kGrow || (ref == -INFINITY && top != -INFINITY);
   if (__any_sync(0xffffffffu, grow)) {
     const float old = ref;
@@ -419,20 +432,23 @@ __device__ __forceinline__ bool tile_weights(uint32_t tmem_s, uint32_t tmem_o, c
     float again = -INFINITY;
 #pragma unroll 1
     for (int c = 0; c < 2; ++c) {
-      uint32_t s[32], w[16];
+      uint32_t s[32], w[S::PARTS][16];
       tmem_ld32(tmem_s + uint32_t(32 * c), s);
       float4 y[2] = {scales[2 * c], scales[2 * c + 1]};
       umma::tmem_ld_wait();
-      weights_of<false>(s, y, factor, unbias, EVERY ? 0 : low - 32 * c, EVERY ? 32 : high - 32 * c, bias, w, sum, again);
+      weights_of<false, S::PARTS>(s, y, factor, unbias, EVERY ? 0 : low - 32 * c, EVERY ? 32 : high - 32 * c, bias, w, sum, again);
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        if (c == 0) p[0][k] = w[k]; else p[1][k] = w[k];
+      for (int k = 0; k < 16 * S::PARTS; ++k) {
+        if (c == 0) p[0][k / 16][k % 16] = w[k / 16][k % 16]; else p[1][k / 16][k % 16] = w[k / 16][k % 16];
       }
     }
   }
   l += sum;
-  umma::tmem_st16(tmem_s, p[0]);
-  umma::tmem_st16(tmem_s + 16u, p[1]);
+#pragma unroll
+  for (int t = 0; t < S::PARTS; ++t) {
+    umma::tmem_st16(tmem_s + 32u * t, p[0][t]);
+    umma::tmem_st16(tmem_s + 32u * t + 16u, p[1][t]);
+  }
   return true;
 }
 
@@ -447,18 +463,20 @@ struct Ends {
 };
 
 // q of a warp's 32 rows, from row r0 of the sequence, into its place in shared memory; factor, unbias: of the row of this lane.  It is copied there as it is
-// (D / 8 lanes have a row) and worked on in place by a thread a row: eight lanes' chunks lie in different banks by the swizzle, and nothing is shuffled (4000
+// (16 bytes a lane) and worked on in place by a thread a row: eight lanes' chunks lie in different banks by the swizzle, and nothing is shuffled (4000
 // to 5700 cycles an item went into shuffles).  What happens once an item is short loops: unrolled code is fetched more slowly than it runs.
 template <int TYPE, class S>
 __device__ __forceinline__ void open_rows(const AttnParams& a, const Ends e, uint32_t q_smem, int r0, float& factor, float& unbias) {
-  constexpr int kLanes = S::D / 8, kStep = 32 / kLanes, kSteps = 32 / kStep;      // of a row; rows at once
-  const int lane = threadIdx.x & 31, chunk = lane % kLanes, sub = lane / kLanes, row0 = 32 * ((threadIdx.x >> 5) & 3);
-  const bool wide = ((reinterpret_cast<uintptr_t>(a.q) | uint64_t(a.row_stride * 2) | uint64_t(a.head_stride * 2)) & 15) == 0, f16 = a.dtype == DINO_F16;
+  using T = std::conditional_t<S::PARTS == 2, uint32_t, uint16_t>;
+  constexpr int kChunks = S::D * S::PARTS / 8, kEach = 16 / int(sizeof(T));      // of a row, of 16 bytes; values of one
+  const int lane = threadIdx.x & 31, row0 = 32 * ((threadIdx.x >> 5) & 3);
+  const bool wide = ((reinterpret_cast<uintptr_t>(a.q) | uint64_t(a.row_stride * sizeof(T)) | uint64_t(a.head_stride * sizeof(T))) & 15) == 0, f16 = a.dtype == DINO_F16;
 #pragma unroll 4
-  for (int k = 0; k < kSteps; ++k) {
-    const int r = r0 + kStep * k + sub, token = a.by_group(min(r, e.r1 - 1)), head = e.head + r - token * a.group;
-    const uint16_t* src = static_cast<const uint16_t*>(a.q) + int64_t(e.row + token) * a.row_stride + int64_t(head) * a.head_stride + 8 * chunk;
-    const uint32_t to = q_smem + operand_at<kRows>(row0 + kStep * k + sub, chunk);
+  for (int k = 0; k < kChunks; ++k) {
+    const int at = 32 * k + lane, row = at / kChunks, chunk = at % kChunks;
+    const int r = r0 + row, token = a.by_group(min(r, e.r1 - 1)), head = e.head + r - token * a.group;
+    const T* src = static_cast<const T*>(a.q) + int64_t(e.row + token) * a.row_stride + int64_t(head) * a.head_stride + kEach * chunk;
+    const uint32_t to = q_smem + operand_at<kRows>(row0 + row, chunk);
     if (r >= e.r1) {
       st_shared16(to, 0u, 0u, 0u, 0u);
     } else if (wide) {
@@ -466,55 +484,84 @@ __device__ __forceinline__ void open_rows(const AttnParams& a, const Ends e, uin
     } else {
       uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = uint32_t(src[2 * j]) | (uint32_t(src[2 * j + 1]) << 16);
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (S::PARTS == 2) w[j] = src[j];
+        else w[j] = uint32_t(src[2 * j]) | (uint32_t(src[2 * j + 1]) << 16);
+      }
       st_shared16(to, w[0], w[1], w[2], w[3]);
     }
   }
   asm volatile("cp.async.wait_all;\n" ::: "memory");
   __syncwarp();
-  uint32_t largest = 0;                                                 // of the 16-bit magnitudes, whose order is that of the values
+  uint32_t largest = 0;                                                 // of the magnitudes, as bits: their order is that of the values
 #pragma unroll 4
-  for (int c = 0; c < S::D / 8; ++c) {
+  for (int c = 0; c < kChunks; ++c) {
     const uint4 x = lds128(q_smem + operand_at<kRows>(row0 + lane, c));
-    largest = __vmaxu2(largest, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
+    if (S::PARTS == 2) largest = max(max(largest, max(x.x & 0x7fffffffu, x.y & 0x7fffffffu)), max(x.z & 0x7fffffffu, x.w & 0x7fffffffu));
+    else largest = __vmaxu2(largest, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
   }
-  largest = max(largest & 0xffffu, largest >> 16);
-  const float top = f16 ? __half2float(__ushort_as_half(uint16_t(largest))) : __uint_as_float(largest << 16);
-  const uint32_t exponent = __float_as_uint(top) >> 23;
+  if (S::PARTS == 1) {
+    largest = max(largest & 0xffffu, largest >> 16);
+    largest = f16 ? __float_as_uint(__half2float(__ushort_as_half(uint16_t(largest)))) : largest << 16;
+  }
+  const uint32_t exponent = largest >> 23;
   const bool plain = exponent == 0 || exponent == 255;
   const int shift = plain ? 0 : min(max(127 + 12 - int(exponent), -126), 126);
   const float up = __uint_as_float(uint32_t(127 + shift) << 23), sign = a.scale < 0.f ? -up : up;      // scores' factors are not negative
   float total[2] = {0.f, 0.f};
-#pragma unroll 2
-  for (int c = 0; c < S::D / 8; ++c) {
-    const uint32_t at = q_smem + operand_at<kRows>(row0 + lane, c);
-    const uint4 x = lds128(at);
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    uint32_t h[4];
+  if constexpr (S::PARTS == 2) {                                        // 16 values: the float16 nearest to them, and what is left
+#pragma unroll 1
+    for (int c = 0; c < kChunks; c += 4) {
+      uint32_t h[8], rest[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 v = f16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[j])) : make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
-      h[j] = pack_half(v.x * sign, v.y * sign);
-      const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
-      total[j & 1] += back.x + back.y;
+      for (int k = 0; k < 4; ++k) {
+        const uint4 x = lds128(q_smem + operand_at<kRows>(row0 + lane, c + k));
+        const float v[4] = {__uint_as_float(x.x) * sign, __uint_as_float(x.y) * sign, __uint_as_float(x.z) * sign, __uint_as_float(x.w) * sign};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          h[2 * k + j] = pack_half(v[2 * j], v[2 * j + 1]);
+          const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h[2 * k + j]));
+          rest[2 * k + j] = pack_half(v[2 * j] - back.x, v[2 * j + 1] - back.y);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        st_shared16(q_smem + operand_at<kRows>(row0 + lane, c + k), h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]);
+        st_shared16(q_smem + operand_at<kRows>(row0 + lane, c + 2 + k), rest[4 * k], rest[4 * k + 1], rest[4 * k + 2], rest[4 * k + 3]);
+      }
     }
-    st_shared16(at, h[0], h[1], h[2], h[3]);
+  } else {
+#pragma unroll 2
+    for (int c = 0; c < kChunks; ++c) {
+      const uint32_t at = q_smem + operand_at<kRows>(row0 + lane, c);
+      const uint4 x = lds128(at);
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+      uint32_t h[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 v = f16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[j])) : make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+        h[j] = pack_half(v.x * sign, v.y * sign);
+        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+        total[j & 1] += back.x + back.y;
+      }
+      st_shared16(at, h[0], h[1], h[2], h[3]);
+    }
   }
   factor = fabsf(a.scale) * __uint_as_float(uint32_t(127 - shift) << 23);
-  unbias = Half2Of<TYPE>::kBias * (total[0] + total[1]);                // K's of int8 are that much too large
+  unbias = S::PARTS == 1 ? Half2Of<TYPE>::kBias * (total[0] + total[1]) : 0.f;      // K's of int8 are that much too large
   fence_async_smem();
   __syncwarp();
 }
 
-// O of a warp's 32 rows (row0: the first one's number in the item): results, or float32 sums of a piece.  Through the place of q, which nobody reads any more:
-// 256 bytes a row there, chunks of 16 bytes turned by the row's number, so that rows leave in whole lines.
+// O of a warp's 32 rows (row0: the first one's number in the item): results, or float32 sums of a piece.  Through the place of these rows' q, which nobody
+// reads any more (that of other rows may be the next item's already): 2 D bytes a row, so that rows leave in whole lines.
 template <class S>
 __device__ __forceinline__ void close_rows(const AttnParams& a, const Ends e, uint32_t q_smem, uint32_t tmem_o, int row0, float inverse) {
-  constexpr int D = S::D, kPiece = kItemRows * (D + 2);
-  const int lane = threadIdx.x & 31, rows = e.r1 - e.r0 - row0;      // of this warp's
-  const uint32_t mine = q_smem + uint32_t(((threadIdx.x >> 5) & 3) * 32 * D * 2);
-  auto at = [&](int row, int chunk) { return mine + uint32_t(row * D * 2) + uint32_t((chunk ^ (row & (D / 8 - 1))) << 4); };
-  if (e.piece < 0) {
+  constexpr int D = S::D, kLanes = D / 8, kStep = 32 / kLanes;          // of a row; rows at once
+  const int lane = threadIdx.x & 31, rows = e.r1 - e.r0 - row0;         // of this warp's
+  const int first = 32 * ((threadIdx.x >> 5) & 3);
+  auto at = [&](int row, int chunk) { return q_smem + operand_at<kRows>(first + row, chunk); };
+  if (S::PARTS == 1 && e.piece < 0) {
 #pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
       uint32_t o[32], h[16];
@@ -534,7 +581,6 @@ __device__ __forceinline__ void close_rows(const AttnParams& a, const Ends e, ui
       for (int k = 0; k < 4; ++k) st_shared16(at(lane, 4 * c + k), h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]);
     }
     __syncwarp();
-    constexpr int kLanes = D / 8, kStep = 32 / kLanes;
 #pragma unroll 4
     for (int k = 0; k < 32; k += kStep) {
       const int row = k + lane / kLanes, chunk = lane % kLanes;
@@ -543,34 +589,39 @@ __device__ __forceinline__ void close_rows(const AttnParams& a, const Ends e, ui
     __syncwarp();
     return;
   }
-  float* const part = a.partial + size_t(e.piece) * kPiece + size_t(row0) * D;
+  float* const part = a.partial + size_t(e.piece) * S::kPiece + size_t(row0) * D;
 #pragma unroll 1
   for (int half = 0; half < 2; ++half) {                                // D / 2 columns at a time
-#pragma unroll
+#pragma unroll 1
     for (int c = 0; c < D / 64; ++c) {
       uint32_t o[32];
       tmem_ld32(tmem_o + uint32_t(half * (D / 2) + 32 * c), o);
       umma::tmem_ld_wait();
+      if (S::PARTS == 2 && e.piece < 0) {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * inverse);
+      }
 #pragma unroll
       for (int k = 0; k < 8; ++k) st_shared16(at(lane, 8 * c + k), o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
     }
     __syncwarp();
-    constexpr int kLanes = D / 8, kStep = 32 / kLanes;
 #pragma unroll 4
     for (int k = 0; k < 32; k += kStep) {
       const int row = k + lane / kLanes, chunk = lane % kLanes;
-      if (row < rows) __stcg(reinterpret_cast<uint4*>(part + size_t(row) * D + half * (D / 2) + 4 * chunk), lds128(at(row, chunk)));
+      if (row >= rows) continue;
+      float* const to = S::PARTS == 2 && e.piece < 0 ? static_cast<float*>(a.out) + e.place(a, row0 + row) : part + size_t(row) * D;
+      __stcg(reinterpret_cast<uint4*>(to + half * (D / 2) + 4 * chunk), lds128(at(row, chunk)));
     }
     __syncwarp();
   }
 }
 
-// The results of a cut item from its pieces, by 256 threads.  First a row's largest y and its sum by a thread each (kept in the place of q), then the sums of
+// The results of a cut item from its pieces, by a thread for each row of an item.  First a row's largest y and its sum by a thread each (kept in the place of q), then the sums of
 // all columns, kPlaces of four columns and kPieces pieces under way at a time.
 template <class S, typename Meet> __device__ __forceinline__ bool join_rows(const AttnParams& a, const Ends e, int c0, int c1, int piece0, uint32_t q_smem, Meet meet) {
-  constexpr int D = S::D, kPiece = kItemRows * (D + 2), kPlaces = 8, kPieces = 2;
+  constexpr int D = S::D, kPlaces = 8, kPieces = 2;
   const int rows = e.r1 - e.r0, count = c1 - c0 + 1, tid = int(threadIdx.x);
-  auto piece = [&](int c) { return a.partial + size_t(c == 0 ? piece0 : 2 * (c0 + c)) * kPiece; };
+  auto piece = [&](int c) { return a.partial + size_t(c == 0 ? piece0 : 2 * (c0 + c)) * S::kPiece; };
   auto weight = [](float ref, float top) { return ref == -INFINITY ? 0.f : exp2_approx(ref - top); };
   if (tid < rows) {
     float top = -INFINITY, sum = 0.f;
@@ -578,7 +629,7 @@ template <class S, typename Meet> __device__ __forceinline__ bool join_rows(cons
     for (int c = 0; c < count; c += 4) {
       float2 ml[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) ml[k] = c + k < count ? __ldcg(reinterpret_cast<const float2*>(piece(c + k) + kItemRows * D) + tid) : make_float2(-INFINITY, 0.f);
+      for (int k = 0; k < 4; ++k) ml[k] = c + k < count ? __ldcg(reinterpret_cast<const float2*>(piece(c + k) + S::kItemRows * D) + tid) : make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float next = fmaxf(top, ml[k].x);
@@ -597,13 +648,13 @@ template <class S, typename Meet> __device__ __forceinline__ bool join_rows(cons
   };
   const int last = rows * (D / 4) - 1;
 #pragma unroll 1
-  for (int x0 = tid; x0 <= last; x0 += 256 * kPlaces) {
+  for (int x0 = tid; x0 <= last; x0 += S::kItemRows * kPlaces) {
     float4 v[kPlaces];
     float top[kPlaces];
 #pragma unroll
     for (int u = 0; u < kPlaces; ++u) {
       v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      top[u] = stats(min(x0 + 256 * u, last) / (D / 4)).x;
+      top[u] = stats(min(x0 + S::kItemRows * u, last) / (D / 4)).x;
     }
 #pragma unroll 1
     for (int c = 0; c < count; c += kPieces) {
@@ -614,9 +665,9 @@ template <class S, typename Meet> __device__ __forceinline__ bool join_rows(cons
         const float* const src = piece(min(c + k, count - 1));
 #pragma unroll
         for (int u = 0; u < kPlaces; ++u) {
-          const int x = min(x0 + 256 * u, last);
+          const int x = min(x0 + S::kItemRows * u, last);
           y[k][u] = __ldcg(reinterpret_cast<const float4*>(src) + x);
-          ref[k][u] = __ldcg(src + kItemRows * D + 2 * (x / (D / 4)));
+          ref[k][u] = __ldcg(src + S::kItemRows * D + 2 * (x / (D / 4)));
         }
       }
 #pragma unroll
@@ -631,9 +682,13 @@ template <class S, typename Meet> __device__ __forceinline__ bool join_rows(cons
     }
 #pragma unroll
     for (int u = 0; u < kPlaces; ++u) {
-      const int x = x0 + 256 * u;
+      const int x = x0 + S::kItemRows * u;
       if (x > last) break;
       const float inv = stats(x / (D / 4)).y;
+      if constexpr (S::PARTS == 2) {
+        __stcg(reinterpret_cast<float4*>(static_cast<float*>(a.out) + e.place(a, x / (D / 4)) + x % (D / 4) * 4), make_float4(v[u].x * inv, v[u].y * inv, v[u].z * inv, v[u].w * inv));
+        continue;
+      }
       uint2 h;
       if (a.dtype == DINO_F16) {
         h = make_uint2(pack_half(v[u].x * inv, v[u].y * inv), pack_half(v[u].z * inv, v[u].w * inv));
@@ -647,10 +702,10 @@ template <class S, typename Meet> __device__ __forceinline__ bool join_rows(cons
   return meet();                                                        // (the next item's q goes where the rows' sums are)
 }
 
-// ---- warps 0..7: tile i of the item, a row per thread
+// ---- warps 0..3 and, where there are two tiles of rows, 4..7: tile i of the item, a row per thread
 template <int TYPE, class S>
 __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, uint32_t q_smem) {
-  constexpr int D = S::D, kPiece = kItemRows * (D + 2);
+  constexpr int D = S::D;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = warp >> 2, my_row = 32 * (warp & 3) + lane;
   const uint32_t lanes = sh.tmem + (uint32_t(32 * (warp & 3)) << 16), tmem_s = lanes + uint32_t(i * 128), tmem_o = lanes + kO + uint32_t(i * D);
   int first = 0, meetings = 0;                                          // tiles so far
@@ -711,7 +766,7 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
     close_rows<S>(a, e, q_smem + uint32_t(i * S::kQ), tmem_o, i * kRows + 32 * (warp & 3), l == 0.f ? 0.f : 1.f / l);
     umma::tcgen05_fence_before();
     if (e.piece >= 0) {                                                 // cut: the last of its CTAs to arrive adds the pieces up, in order
-      if (mine) __stcg(reinterpret_cast<float2*>(a.partial + size_t(e.piece) * kPiece + kItemRows * D) + (i * kRows + my_row), make_float2(ref, l));
+      if (mine) __stcg(reinterpret_cast<float2*>(a.partial + size_t(e.piece) * S::kPiece + S::kItemRows * D) + (i * kRows + my_row), make_float2(ref, l));
       if (!meet()) return;
       if (threadIdx.x == 0) {
         int before = 0;
@@ -734,16 +789,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_many_kernel(const __gri
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared sh;
   const uint32_t smem = (umma::smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t q_smem = smem, k_smem = smem + 2 * S::kQ, v_smem = k_smem + kStages * S::kKv;
+  const uint32_t q_smem = smem, k_smem = smem + S::kTiles * S::kQ, v_smem = k_smem + S::kStages * S::kKv;
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSegments; ++i) {
       umma::mbar_init(umma::smem_u32(&sh.described[i]), 1);
-      umma::mbar_init(umma::smem_u32(&sh.closed[i]), 13);              // eight, four and one warps
+      umma::mbar_init(umma::smem_u32(&sh.closed[i]), 4 * S::kTiles + S::kConverters + 1);
     }
-    umma::mbar_init(umma::smem_u32(&sh.q_ready), 8);
-    for (int i = 0; i < kStages; ++i) {
-      umma::mbar_init(umma::smem_u32(&sh.full[i]), 4);
+    umma::mbar_init(umma::smem_u32(&sh.q_ready), 4 * S::kTiles);
+    for (int i = 0; i < S::kStages; ++i) {
+      umma::mbar_init(umma::smem_u32(&sh.full[i]), S::kConverters);
       umma::mbar_init(umma::smem_u32(&sh.empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -752,7 +807,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_many_kernel(const __gri
         umma::mbar_init(umma::smem_u32(&sh.p_ready[i][k]), 4);
       }
     }
-    umma::mbar_init(umma::smem_u32(&sh.together), 8);
+    umma::mbar_init(umma::smem_u32(&sh.together), 4 * S::kTiles);
     umma::mbar_init(umma::smem_u32(&sh.drain), 1);
     sh.lost = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -765,8 +820,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_many_kernel(const __gri
   const Walk first = walk_of<kThreads>(a, kLog2, kLeast, sh.walk);         // (its barriers: the inits and the allocation are visible)
   __syncthreads();
   umma::tcgen05_fence_after();
-  if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;\n");            // 2 x 176 + 96 + 64 = 4 x 128
+  // Two tiles of rows: 2 x 176 + 96 + 64 = 4 x 128 registers; one: 192 + 2 x 96 + 64 of them.
+  if (warp < 4 * S::kTiles) {
+    if constexpr (S::kTiles == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;\n");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 192;\n");
     softmax_rows<TYPE, S>(a, sh, q_smem);
   } else if (warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
@@ -794,13 +851,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_many_kernel(const __gri
   }
 }
 
-template <int TYPE, int D> int launch(AttnParams& a, cudaStream_t s) {
-  using S = Shape<D>;
-  a.row_tile = kItemRows;
-  a.row_tile_log2 = 8;
+template <int TYPE, int D, int PARTS> int launch(AttnParams& a, cudaStream_t s) {
+  using S = Shape<D, PARTS>;
+  a.row_tile = S::kItemRows;
+  a.row_tile_log2 = S::kTiles == 2 ? 8 : 7;
   a.ends = kEnds;
   const int ctas = stream::sm_count();
-  a.partial = attention_scratch(size_t(ctas) * 2 * kItemRows * (D + 2), ctas, s, &a.arrived);
+  a.partial = attention_scratch(size_t(ctas) * 2 * S::kPiece, ctas, s, &a.arrived);
   if (a.partial == nullptr) return RC_LAUNCH;
   static SmemOptIn opt;
   auto kern = attention_many_kernel<TYPE, S>;
