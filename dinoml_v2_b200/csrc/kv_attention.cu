@@ -23,8 +23,9 @@ struct AttnScratch {
 static ScratchSets<AttnScratch> g_sets;
 // Rows (tokens x heads of a cached head) of a sequence up to which the kernel of few rows takes it: it reads the cache once for 16 rows, the other one once for
 // 256, at a lower rate.  Measured (few, many; 8 cached heads of 128, int8): 64 sequences of 4000 tokens, 32 rows 310 and 358 us, 64 rows 574 and 354;
-// 16 of 2000, 20 rows 59 and 64, 36 rows 79 and 66.
-constexpr int kFewRows = 32;
+// 16 of 2000, 20 rows 59 and 64, 36 rows 79 and 66; heads of 256: 64 of 2000, 16 rows 276 and 220, 20 rows 490 and 223 (up to one reading of the cache the kernel
+// of few rows is kept: its weights have no smallest one); float32: 64 of 2000, 16 rows 126 and 190, 32 rows 213 and 201.
+static int few_rows(int dim) { return dim == 256 ? 16 : 32; }
 
 // Allocates outside of stream capture only: callers run a shape once before capturing a graph.
 float* attention_scratch(size_t floats, int ctas, cudaStream_t s, int** arrived) {
@@ -82,13 +83,13 @@ int cache_attention(const DinoB200KvCache* cache, const DinoB200KvBatch* batch, 
   const bool tensor = dtype != DINO_F32 || a.c.dim != 256;                   // (two terms of 256 values do not fit into shared memory)
   const int64_t most = a.p.starts == nullptr ? a.group : all_rows;          // rows of a sequence
   a.min_rows = 0;
-  a.max_rows = tensor ? kFewRows : INT32_MAX;
+  a.max_rows = tensor ? few_rows(a.c.dim) : INT32_MAX;
   const int tiles = rows <= 8 ? 1 : 2;
   if (a.p.starts != nullptr || most <= a.max_rows) {
     const int rc = cache->type == DINOML_B200_KV_INT8 ? attention_few_int8(a, tiles, s) : attention_few_e4m3(a, tiles, s);
     if (rc != RC_OK || most <= a.max_rows) return rc;
   }
-  a.min_rows = kFewRows + 1;
+  a.min_rows = a.max_rows + 1;
   a.max_rows = INT32_MAX;
   return attention_many(a, cache->type, s);
 }

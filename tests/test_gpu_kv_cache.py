@@ -123,6 +123,21 @@ def test_attention_of_chunks(dim, block, dtype, kind):
             _check_attention(q, cache, table, _ints(lengths), _ints(starts), window=1, scale=0.3, dtype=dtype)
 
 
+@pytest.mark.parametrize("dim,dtype", [(64, "bfloat16"), (128, "float16"), (256, "bfloat16"), (64, "float32"), (128, "float32")])
+def test_attention_of_short_prompts_one_after_the_other(dim, dtype):
+    """More of them than there are CTAs: every one begins items while its warps still have results of the ones before to store."""
+    sizes = [(64 + 7 * (i % 3), 64 + 5 * (i % 4) - 20) for i in range(120)]
+    lengths, counts = [n for n, _ in sizes], [m for _, m in sizes]
+    starts = [sum(counts[:i]) for i in range(len(counts) + 1)]
+    blocks = sum(-(-n // 32) for n in lengths)
+    cache, table = _random_cache(blocks, 4, 32, dim, "int8", 11), _table(lengths, 32, blocks, 12)
+    q, _, _ = _qkv(starts[-1], 4, 4, dim, dtype, 13)
+    first = kernels.kv_cache_attention(q, cache, table, _ints(lengths), _ints(starts))
+    for _ in range(10):
+        assert torch.equal(kernels.kv_cache_attention(q, cache, table, _ints(lengths), _ints(starts)), first)
+    _check_attention(q, cache, table, _ints(lengths), _ints(starts), dtype=dtype)
+
+
 @pytest.mark.parametrize("window", [1, 15, 16, 17, 64, 100, 129, 5000])
 def test_attention_windows(window):
     lengths = [1, 16, 63, 128, 500, 1111]
