@@ -150,18 +150,26 @@ __global__ void __launch_bounds__(NT, kThreads / NT) rms_norm_kernel(const T* x,
         for (int o = 16 / V; o > 0; o >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
         if (!here) return;
         const __half d = __float2half_rn(__fmul_rn(__uint_as_float(largest), 1.0f / 127.0f));
-        const float step8 = __half2float(d), up = __frcp_rn(step8);
+        const float step8 = __half2float(d);
         // blocks are multiples of two bytes
         uint16_t* block = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(y) + (row * width + i) / 32 * 34);
         if ((i & 31) == 0) block[0] = __half_as_ushort(d);
+        // The integer nearest to v / step, in the last bits of v * (1 / step) + 1.5 2^23.  With a reciprocal within 2 units of its last place v / step is at
+        // most 127.1 * 2^-22 < 2^-14 away: where that is further from half way between two integers than 1e-4 both have the same nearest one, elsewhere,
+        // and where the step is no normal float16 (so that values may be beyond 127 of it, or none is finite), the division decides.
+        constexpr float kRound = 12582912.f;
+        const float up = __fdividef(1.f, step8);
         uint32_t q[V];
+        float worst = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          // The integer nearest to v / step.  v times the rounded reciprocal is within 1.5 * 2^-23 of that, 2^-15 at 255 (the most that a rounded step gives):
-          // where it is further than that from half way between two integers both have the same nearest one, elsewhere the division decides.
-          const float near = v[j] * up, whole = rintf(near);
-          const float at = fabsf(near - whole) < 0.4999f ? whole : rintf(__fdiv_rn(v[j], step8));
-          q[j] = step8 > 0.f ? uint32_t(__float2int_rn(fminf(fmaxf(at, -127.f), 127.f))) & 0xffu : 0u;
+          const float t = fmaf(v[j], up, kRound);
+          q[j] = __float_as_uint(t) & 0xffu;
+          worst = fmaxf(worst, fabsf(fmaf(v[j], up, kRound - t)));
+        }
+        if (!(worst < 0.4999f && step8 >= 0x1p-14f && step8 <= 65504.f)) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) q[j] = step8 > 0.f ? uint32_t(__float2int_rn(fminf(fmaxf(__fdiv_rn(v[j], step8), -127.f), 127.f))) & 0xffu : 0u;
         }
 #pragma unroll
         for (int j = 0; j + 1 < V; j += 2) block[1 + ((i & 31) + j) / 2] = uint16_t(q[j] | (q[j + 1] << 8));
