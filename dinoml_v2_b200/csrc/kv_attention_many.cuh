@@ -5,12 +5,16 @@
 // have two places in tensor memory: the next ones are there when the softmax of a tile is done, which so never waits for products.
 //   * warps 0..3 and 4..7: softmax, a row of scores per thread, S_i from tensor memory, P_i back into the same columns;
 //   * warps 8..11: K and V of the next tiles, 8 bits in global memory to float16 in shared memory (swizzled as the MMA reads them);
+//   * heads of 256 and float32 (q and P in two float16 terms, the second one's MMAs behind the first's into the same sums): one tile of 128 rows, warps 4..7 convert too;
 //   * warp 12: issues the MMAs, S_i = Q_i K^T from shared memory and O_i += P_i V with P_i from tensor memory; V stays [token][channel], an MN-major operand;
 //   * warp 13: walks the CTA's items.
 // 8-bit values are exact in float16, q is brought to [2^12, 2^13) by a power of two per row, so products and their float32 sums are those of the stored
 // values.  The scale of a block's K multiplies the scores; that of its V goes into the exponent: with y = s + log2(vs), P = 2^(y - ref + 7) is
 // what V is multiplied by, and the softmax's sum takes P / vs in float32.  ref is the row's largest y when it was last set; O is rescaled only when y
 // outgrows it by 2^8, so that P stays below 2^15 and loses bits (as a float16 denormal) only below 2^-21 of that.
+//
+// Measured, 2048 tokens after 6144, 32 heads on 8 cached ones: heads of 128 286 us (840 TFLOP/s), of 256 556 us (866), of 64 240 us (500), float32 of 128 485 us. A tile of
+// 64 tokens takes 2015 cycles: MMAs 1415 of them (scores 940, 64 columns being bound by shared memory; P V 516), the softmax warps 1100 and the wait for scores.
 #pragma once
 #include <type_traits>
 
@@ -31,6 +35,7 @@ constexpr uint32_t kTmem = 512, kO = 256;                                     //
 constexpr int kEnds = 8, kLeast = 12;          // in tiles; units that a CTA takes at least
 constexpr float kGrow = 8.f, kUp = 7.f;
 constexpr unsigned kPolynomial = 0x11;      // of eight pairs of exponentials, those that the FMA units take: the special function units are the bound
+                                             // (none 380 us, these two 342, four 347, all 429 for the prompt above at an earlier state of the rest)
 
 // PARTS: float16 terms of a q and of a weight, 2 for float32 activations.  Shared memory has room for two tiles of rows where q takes 256 bytes a row, for
 // one tile beyond; the warps that had the other one are converters then.

@@ -1,9 +1,11 @@
 // Root-mean-square norm with the residual's addition: t = x + residual, y = t / sqrt(mean(t^2) + eps) * weight, in float32 with one rounding at the
 // end; y in the activation type or as Q8_0 blocks.
 //
-// Bound by bytes: x and the residual in, t and y out.  A CTA has a row and a thread keeps its values of t in registers between the sum of squares and the
-// products, so each is read once; rows that registers do not hold are read a second time (from L2).  NT threads of V values, R rounds: as few threads as hold a row
-// in 16 bytes each, since a CTA of few warps starts and meets sooner.
+// Bound by bytes: x and the residual in, t and y out; to Q8_0 by instructions beside them.  A CTA has a row and a thread keeps its values of t in registers between the sum
+// of squares and the products, so each is read once; rows that registers do not hold are read a second time (from L2).  NT threads of V values, R rounds: as few threads
+// as hold a row in 16 bytes each, since a CTA of few warps starts and meets sooner (a row of 4096: 6.2 us with 1024 threads of 4 values, 5.7 so, both with the call from Python).
+// 2048 rows of 8192 float16 with residual to Q8_0, and decoded again: 67.6 us with a CTA a row and 1024 threads, 47.4 with 512, 39.4 with the next row copied ahead, 37.2 with one
+// reciprocal a block instead of divisions.
 #include <algorithm>
 
 #include "kv_cache.cuh"
