@@ -190,31 +190,30 @@ __device__ __forceinline__ Walk walk_of(const AttnParams& a, int log2, int least
 // Two bytes of a cached word as two float16, exactly.
 template <int TYPE> struct Half2Of;
 template <> struct Half2Of<DINOML_B200_KV_INT8> {
-  static constexpr float kBias = 1152.f;                            // 1024 + value + 128 has the value + 128 in its last byte
-  template <bool BIASED, int LO, int HI> static __device__ __forceinline__ uint32_t pair(uint32_t w) {
+  // 1024 + value + 128 has the value + 128 in its last byte; 1152 is taken off again before any product: as part of the keys it would be in the scores' sums, whose
+  // rounding then goes with 1152 times the sum of q instead of with the score.
+  template <int LO, int HI> static __device__ __forceinline__ uint32_t pair(uint32_t w) {
     const uint32_t m = __byte_perm(w, 0x64646464u, 0x4040 | LO | (HI << 8));
-    if (BIASED) return m;
     const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&m), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t*>(&v);
   }
-  // bytes 0, 1 and 2, 3 (BIASED: + kBias); bytes 0, 2 and 1, 3
-  template <bool BIASED> static __device__ __forceinline__ void along(uint32_t w, uint32_t& a, uint32_t& b) {
+  // bytes 0, 1 and 2, 3; bytes 0, 2 and 1, 3
+  static __device__ __forceinline__ void along(uint32_t w, uint32_t& a, uint32_t& b) {
     w ^= 0x80808080u;
-    a = pair<BIASED, 0, 1>(w);
-    b = pair<BIASED, 2, 3>(w);
+    a = pair<0, 1>(w);
+    b = pair<2, 3>(w);
   }
   static __device__ __forceinline__ void across(uint32_t w, uint32_t& a, uint32_t& b) {
     w ^= 0x80808080u;
-    a = pair<false, 0, 2>(w);
-    b = pair<false, 1, 3>(w);
+    a = pair<0, 2>(w);
+    b = pair<1, 3>(w);
   }
 };
 template <> struct Half2Of<DINOML_B200_KV_E4M3> {
-  static constexpr float kBias = 0.f;
-  template <bool> static __device__ __forceinline__ void along(uint32_t w, uint32_t& a, uint32_t& b) {
+  static __device__ __forceinline__ void along(uint32_t w, uint32_t& a, uint32_t& b) {
     asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}\n" : "=r"(a), "=r"(b) : "r"(w));
   }
-  static __device__ __forceinline__ void across(uint32_t w, uint32_t& a, uint32_t& b) { along<false>(__byte_perm(w, w, 0x3120), a, b); }
+  static __device__ __forceinline__ void across(uint32_t w, uint32_t& a, uint32_t& b) { along(__byte_perm(w, w, 0x3120), a, b); }
 };
 
 __device__ __forceinline__ float exp2_approx(float x) {

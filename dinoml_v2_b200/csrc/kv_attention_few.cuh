@@ -11,8 +11,7 @@
 //     Token tok(g) stands in row g so that eight lanes touch all banks.
 //   * V comes by ldmatrix.trans on pairs of bytes: one register holds channels 2g, 2g + 1 of two tokens, a byte permutation makes a
 //     float16 pair along the tokens of each channel - the transposition is the conversion.  Rows g and g + 8 are channels 16c + 2g, 16c + 2g + 1.
-//   * 8-bit values are exact in float16.  (int8 with 16-bit rows: K + 1152 is, which spares a subtraction for each pair, and the scores' sums begin at
-//     -1152 times the sum of q: 2^-17 of a score at most, against the weights' 2^-11.)  q is brought to [2^12, 2^13) by a power of two for each row, which keeps every bit of it that matters
+//   * 8-bit values are exact in float16.  q is brought to [2^12, 2^13) by a power of two for each row, which keeps every bit of it that matters
 //     (bfloat16: all but values 2^-37 of the row's largest); float32 rows are two float16 terms (PARTS = 2).
 //   * The products of a tile start from zero, with weights relative to the tile's own maxima: p = 2^(s - top) (vs / vt), vs the scale of a block's V and vt
 //     the largest in the tile, is rounded to float16 as 2^14 p, and the result joins O in float32: the sums of a long cache are float32 additions.
@@ -147,7 +146,6 @@ template <class S> __device__ __forceinline__ void clear_unseen(uint32_t vtile, 
 
 // An item's rows as the computing warps need them, for two items in turn.
 template <class S> struct Rows8 {
-  float bias[S::R];                            // where the sums of a row's scores begin
   float factor[S::R];                          // of a row's scores: what q was divided by, the softmax scale, log2(e)
   int low[S::R], high[S::R];                   // positions that a row sees
 };
@@ -271,8 +269,7 @@ __device__ __forceinline__ void copy_tiles(const AttnParams& a, Shared<S>& sh, c
 
 // ---- the opening warp.  Rows of an item: q as operand fragments, what their scores are multiplied by, what they see.  Lane (g, t) has the fragments of
 // row g, 16 t .. 16 t + 15 of every 64 values, so it reads them, and eight rows are made at once.
-template <int TYPE, class S> __device__ __forceinline__ void open_rows(const AttnParams& a, Rows8<S>& out, const Segment& sg, uint2* qfrag) {
-  using H = Half2Of<TYPE>;
+template <class S> __device__ __forceinline__ void open_rows(const AttnParams& a, Rows8<S>& out, const Segment& sg, uint2* qfrag) {
   constexpr int D = S::D, NT = S::NT, PARTS = S::PARTS;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, rows = sg.item.r1 - sg.item.r0;
   const int size = a.dtype == DINO_F32 ? 4 : 2;
@@ -298,7 +295,6 @@ template <int TYPE, class S> __device__ __forceinline__ void open_rows(const Att
     const bool plain = e == 0 || e == 255;
     const int shift = plain ? 0 : min(max(127 + 12 - int(e), -126), 126);
     const float up = __uint_as_float(uint32_t(127 + shift) << 23), down = __uint_as_float(uint32_t(127 - shift) << 23);
-    float total = 0.f;                                                  // of the row's first terms
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
       float v[4];
@@ -309,15 +305,11 @@ template <int TYPE, class S> __device__ __forceinline__ void open_rows(const Att
         const uint32_t lo = pack_half(v[0], v[1]), hi = pack_half(v[2], v[3]);
         qfrag[((i * NT + n) * PARTS + part) * 32 + lane] = make_uint2(lo, hi);
         const float2 l = __half22float2(*reinterpret_cast<const __half2*>(&lo)), h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-        if (part == 0) total += (l.x + l.y) + (h.x + h.y);
         v[0] -= l.x; v[1] -= l.y; v[2] -= h.x; v[3] -= h.y;
       }
     }
-    total += __shfl_xor_sync(0xffffffffu, total, 1);
-    total += __shfl_xor_sync(0xffffffffu, total, 2);
     if (t == 0) {
       const int position = sg.s.first + token;
-      out.bias[r] = H::kBias != 0.f ? -H::kBias * total : 0.f;
       out.factor[r] = a.scale * down;
       out.high[r] = r < rows ? min(position + 1, sg.s.end) : 0;
       out.low[r] = a.window > 0 ? max(0, position - a.window + 1) : 0;
@@ -419,7 +411,7 @@ template <class S> __device__ __forceinline__ void join_at_end(const AttnParams&
   for (int i = 0; i < sh.joins; ++i) join_pieces<S>(a, sh.to_join[i], from, (S::W + 1) * 32);
 }
 
-template <int TYPE, class S>
+template <class S>
 __device__ __forceinline__ void open_and_close(const AttnParams& a, Shared<S>& sh, uint2* qfrag) {
   const int lane = threadIdx.x & 31;
   for (int segment = 0;; ++segment) {
@@ -427,7 +419,7 @@ __device__ __forceinline__ void open_and_close(const AttnParams& a, Shared<S>& s
     if (!warp_wait(a, sh, &sh.described[slot], uint32_t(segment / kSegments) & 1u)) return;
     const bool done = sh.segments[slot].tile0 == sh.segments[slot].tile1;
     if (segment >= 2 && !warp_wait(a, sh, &sh.written[segment & 1], uint32_t((segment - 2) >> 1) & 1u)) return;      // its place is free
-    if (!done) open_rows<TYPE, S>(a, sh.rows[segment & 1], sh.segments[slot], qfrag + (segment & 1) * (S::kQ / 8));
+    if (!done) open_rows<S>(a, sh.rows[segment & 1], sh.segments[slot], qfrag + (segment & 1) * (S::kQ / 8));
     __syncwarp();
     if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.opened[segment & 1]));
     if (segment >= 2) close_segment(a, sh, segment - 2, done);
@@ -449,7 +441,6 @@ __global__ void __launch_bounds__(S::kThreads, kCtasPerSm) attention_few_kernel(
                                                                                 const __grid_constant__ CUtensorMap v_map) {
   using H = Half2Of<TYPE>;
   constexpr int D = S::D, NT = S::NT, PARTS = S::PARTS, TK = S::TK, MT = S::MT, W = S::W;
-  constexpr bool kBiased = H::kBias != 0.f && PARTS == 1;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared<S> sh;
   static_assert(sizeof(sh) <= S::kStatic, "two CTAs per SM");
@@ -487,7 +478,7 @@ __global__ void __launch_bounds__(S::kThreads, kCtasPerSm) attention_few_kernel(
     return;
   }
   if (warp == W + 1) {
-    open_and_close<TYPE, S>(a, sh, qfrag);
+    open_and_close<S>(a, sh, qfrag);
     return;
   }
 
@@ -511,13 +502,12 @@ __global__ void __launch_bounds__(S::kThreads, kCtasPerSm) attention_few_kernel(
     // positions that every row sees: the first row ends first, the last one begins last
     const int all_high = min(sg.s.first + a.by_group(sg.item.r0) + 1, sg.s.end);
     const int all_low = a.window > 0 ? max(0, sg.s.first + a.by_group(sg.item.r1 - 1) - a.window + 1) : 0;
-    float factor[NT][2], begin[NT][2], m[NT][2], l[NT][2], o[S::DC][NT][4];
+    float factor[NT][2], m[NT][2], l[NT][2], o[S::DC][NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         factor[n][j] = of.factor[8 * n + 2 * t + j];
-        begin[n][j] = kBiased ? of.bias[8 * n + 2 * t + j] : 0.f;
         m[n][j] = -INFINITY;
         l[n][j] = 0.f;
       }
@@ -537,14 +527,6 @@ __global__ void __launch_bounds__(S::kThreads, kCtasPerSm) attention_few_kernel(
       const uint32_t ktile = ring + stage * uint32_t(2 * S::kHalf) + uint32_t((warp & 1) * TK * S::kRow);
       const float4* const box_of = sh.boxes[stage] + (warp & 1) * MT;
       float s[MT][NT][4];
-      if (kBiased) {
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[i][n][j] = begin[n][j & 1];
-      }
 #pragma unroll
       for (int kk = 0; kk < D / 64; ++kk) {
         uint4 raw[MT][2];
@@ -563,13 +545,13 @@ __global__ void __launch_bounds__(S::kThreads, kCtasPerSm) attention_few_kernel(
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
             uint32_t a0, a1, a2, a3;
-            H::template along<kBiased>(reinterpret_cast<const uint32_t*>(&raw[i][0])[i4], a0, a2);
-            H::template along<kBiased>(reinterpret_cast<const uint32_t*>(&raw[i][1])[i4], a1, a3);
+            H::along(reinterpret_cast<const uint32_t*>(&raw[i][0])[i4], a0, a2);
+            H::along(reinterpret_cast<const uint32_t*>(&raw[i][1])[i4], a1, a3);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
               for (int part = 0; part < PARTS; ++part) {
-                if (kk == 0 && i4 == 0 && part == 0 && !kBiased) mma16816_first(s[i][n], a0, a1, a2, a3, b[n][part].x, b[n][part].y);
+                if (kk == 0 && i4 == 0 && part == 0) mma16816_first(s[i][n], a0, a1, a2, a3, b[n][part].x, b[n][part].y);
                 else mma16816(s[i][n], a0, a1, a2, a3, b[n][part].x, b[n][part].y);
               }
           }

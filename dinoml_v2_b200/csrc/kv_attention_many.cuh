@@ -169,18 +169,17 @@ __device__ __forceinline__ void walk_items(const AttnParams& a, Shared& sh, Walk
   }
 }
 
-// A lane's values of a tile, to[0] and to[1] being the places of its first 16.  BIASED: K of int8 stays 1152 too large (Half2Of), which the rows' scores take
-// off again.
-template <int TYPE, class S, bool BIASED, int COPIES> __device__ __forceinline__ void store_operand(const uint4 (&x)[COPIES], uint32_t smem, const uint32_t (&to)[2]) {
+// A lane's values of a tile, to[0] and to[1] being the places of its first 16.
+template <int TYPE, int COPIES> __device__ __forceinline__ void store_operand(const uint4 (&x)[COPIES], uint32_t smem, const uint32_t (&to)[2]) {
   using H = Half2Of<TYPE>;
   constexpr int kStep = 16 / COPIES;
 #pragma unroll
   for (int i = 0; i < COPIES; ++i) {
     uint32_t h[8];
-    H::template along<BIASED>(x[i].x, h[0], h[1]);
-    H::template along<BIASED>(x[i].y, h[2], h[3]);
-    H::template along<BIASED>(x[i].z, h[4], h[5]);
-    H::template along<BIASED>(x[i].w, h[6], h[7]);
+    H::along(x[i].x, h[0], h[1]);
+    H::along(x[i].y, h[2], h[3]);
+    H::along(x[i].z, h[4], h[5]);
+    H::along(x[i].w, h[6], h[7]);
     const uint32_t turn = kStep == 4 && (i & 1) != 0 ? 64u : 0u;         // rows 4..7 of eight
     const uint32_t at = smem + uint32_t(i * kStep * 128);
     st_shared16((at + to[0]) ^ turn, h[0], h[1], h[2], h[3]);
@@ -250,10 +249,10 @@ __device__ __forceinline__ void convert_tiles(const AttnParams& a, Shared& sh, u
           sh.scales[at][warp] = make_float4(ks, __log2f(v), __fdividef(1.f, v), bh[kAhead] >= 0 ? 1.f : 0.f);
           reinterpret_cast<int*>(&sh.whole[at])[warp] = bh[kAhead] >= 0;
         }
-        store_operand<TYPE, S, S::PARTS == 1>(raw[0], k_smem + uint32_t(stage * S::kKv), to);
+        store_operand<TYPE>(raw[0], k_smem + uint32_t(stage * S::kKv), to);
       }
       load_k(tile0 + u + 1, bh[kAhead + 1]);
-      if (u >= kAhead && u < tiles + kAhead) store_operand<TYPE, S, false>(raw[1], v_smem + uint32_t(stage * S::kKv), to);
+      if (u >= kAhead && u < tiles + kAhead) store_operand<TYPE>(raw[1], v_smem + uint32_t(stage * S::kKv), to);
       if (u + 1 >= kAhead) load(raw[1], 1, tile0 + u + 1 - kAhead, bh[1]);
       fence_async_smem();
       __syncwarp();
@@ -353,11 +352,11 @@ __device__ __forceinline__ float2 exp2_pair(uint64_t x) {
 // EVERY: the row sees all of its columns, else those in [low, high) of blocks that are there.
 // PARTS: terms of a weight, the second one behind the first.  With two the FMA units' exponentials would be what limits the result.
 template <bool EVERY, int PARTS>
-__device__ __forceinline__ void weights_of(const uint32_t (&r)[32], const float4 (&x)[2], float factor, float unbias, int low, int high, float bias,
+__device__ __forceinline__ void weights_of(const uint32_t (&r)[32], const float4 (&x)[2], float factor, int low, int high, float bias,
                                            uint32_t (&p)[PARTS][16], float& l, float& top) {
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
-    const float f = x[g].x * factor, add = fmaf(-unbias, f, x[g].y + bias);
+    const float f = x[g].x * factor, add = x[g].y + bias;
     const uint64_t ff = pair_of(f, f), aa = pair_of(add, add);
     uint64_t sum[2] = {0u, 0u};
     float best = -INFINITY;
@@ -393,14 +392,14 @@ __device__ __forceinline__ void weights_of(const uint32_t (&r)[32], const float4
     }
     const float2 both = halves_of(add2(sum[0], sum[1]));
     if (EVERY || both.x + both.y != 0.f) l = fmaf(both.x + both.y, x[g].z, l);
-    if (EVERY || best != -INFINITY) top = fmaxf(top, fmaf(best - unbias, f, x[g].y));
+    if (EVERY || best != -INFINITY) top = fmaxf(top, fmaf(best, f, x[g].y));
   }
 }
 
 // A row's tile: weights into the scores' place, their sum to l.  They are taken relative to what was the largest so far, at once, and again where the tile has
 // outgrown that (O is brought along then, once products_done() says that the tile before is in it; false where that gives up): the first tiles do.
 template <class S, bool EVERY, typename Wait>
-__device__ __forceinline__ bool tile_weights(uint32_t tmem_s, uint32_t tmem_o, const float4* scales, float factor, float unbias, int low, int high, bool more,
+__device__ __forceinline__ bool tile_weights(uint32_t tmem_s, uint32_t tmem_o, const float4* scales, float factor, int low, int high, bool more,
                                              float& ref, float& l, Wait products_done) {
   uint32_t r[2][32], p[2][S::PARTS][16];                                // p: of the first and the last 32 columns
   tmem_ld32(tmem_s, r[0]);
@@ -410,9 +409,9 @@ __device__ __forceinline__ bool tile_weights(uint32_t tmem_s, uint32_t tmem_o, c
   umma::tmem_ld_wait();
   tmem_ld32(tmem_s + 32u, r[1]);
   float bias = (ref == -INFINITY ? 0.f : -ref) + kUp, sum = 0.f, top = -INFINITY;
-  weights_of<EVERY, S::PARTS>(r[0], x[0], factor, unbias, low, high, bias, p[0], sum, top);
+  weights_of<EVERY, S::PARTS>(r[0], x[0], factor, low, high, bias, p[0], sum, top);
   umma::tmem_ld_wait();
-  weights_of<EVERY, S::PARTS>(r[1], x[1], factor, unbias, low - 32, high - 32, bias, p[1], sum, top);
+  weights_of<EVERY, S::PARTS>(r[1], x[1], factor, low - 32, high - 32, bias, p[1], sum, top);
   const bool grow = top > ref + kGrow || (ref == -INFINITY && top != -INFINITY);
   if (__any_sync(0xffffffffu, grow)) {
     const float old = ref;
@@ -441,7 +440,7 @@ __device__ __forceinline__ bool tile_weights(uint32_t tmem_s, uint32_t tmem_o, c
       tmem_ld32(tmem_s + uint32_t(32 * c), s);
       float4 y[2] = {scales[2 * c], scales[2 * c + 1]};
       umma::tmem_ld_wait();
-      weights_of<false, S::PARTS>(s, y, factor, unbias, EVERY ? 0 : low - 32 * c, EVERY ? 32 : high - 32 * c, bias, w, sum, again);
+      weights_of<false, S::PARTS>(s, y, factor, EVERY ? 0 : low - 32 * c, EVERY ? 32 : high - 32 * c, bias, w, sum, again);
 #pragma unroll
       for (int k = 0; k < 16 * S::PARTS; ++k) {
         if (c == 0) p[0][k / 16][k % 16] = w[k / 16][k % 16]; else p[1][k / 16][k % 16] = w[k / 16][k % 16];
@@ -467,11 +466,11 @@ struct Ends {
   }
 };
 
-// q of a warp's 32 rows, from row r0 of the sequence, into its place in shared memory; factor, unbias: of the row of this lane.  It is copied there as it is
+// q of a warp's 32 rows, from row r0 of the sequence, into its place in shared memory; factor: of the row of this lane.  It is copied there as it is
 // (16 bytes a lane) and worked on in place by a thread a row: eight lanes' chunks lie in different banks by the swizzle, and nothing is shuffled (4000
 // to 5700 cycles an item went into shuffles).  What happens once an item is short loops: unrolled code is fetched more slowly than it runs.
-template <int TYPE, class S>
-__device__ __forceinline__ void open_rows(const AttnParams& a, const Ends e, uint32_t q_smem, int r0, float& factor, float& unbias) {
+template <class S>
+__device__ __forceinline__ void open_rows(const AttnParams& a, const Ends e, uint32_t q_smem, int r0, float& factor) {
   using T = std::conditional_t<S::PARTS == 2, uint32_t, uint16_t>;
   constexpr int kChunks = S::D * S::PARTS / 8, kEach = 16 / int(sizeof(T));      // of a row, of 16 bytes; values of one
   const int lane = threadIdx.x & 31, row0 = 32 * ((threadIdx.x >> 5) & 3);
@@ -513,7 +512,6 @@ __device__ __forceinline__ void open_rows(const AttnParams& a, const Ends e, uin
   const bool plain = exponent == 0 || exponent == 255;
   const int shift = plain ? 0 : min(max(127 + 12 - int(exponent), -126), 126);
   const float up = __uint_as_float(uint32_t(127 + shift) << 23), sign = a.scale < 0.f ? -up : up;      // scores' factors are not negative
-  float total[2] = {0.f, 0.f};
   if constexpr (S::PARTS == 2) {                                        // 16 values: the float16 nearest to them, and what is left
 #pragma unroll 1
     for (int c = 0; c < kChunks; c += 4) {
@@ -546,14 +544,11 @@ __device__ __forceinline__ void open_rows(const AttnParams& a, const Ends e, uin
       for (int j = 0; j < 4; ++j) {
         const float2 v = f16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[j])) : make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
         h[j] = pack_half(v.x * sign, v.y * sign);
-        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
-        total[j & 1] += back.x + back.y;
       }
       st_shared16(at, h[0], h[1], h[2], h[3]);
     }
   }
   factor = fabsf(a.scale) * __uint_as_float(uint32_t(127 - shift) << 23);
-  unbias = S::PARTS == 1 ? Half2Of<TYPE>::kBias * (total[0] + total[1]) : 0.f;      // K's of int8 are that much too large
   fence_async_smem();
   __syncwarp();
 }
@@ -708,7 +703,7 @@ template <class S, typename Meet> __device__ __forceinline__ bool join_rows(cons
 }
 
 // ---- warps 0..3 and, where there are two tiles of rows, 4..7: tile i of the item, a row per thread
-template <int TYPE, class S>
+template <class S>
 __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, uint32_t q_smem) {
   constexpr int D = S::D;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = warp >> 2, my_row = 32 * (warp & 3) + lane;
@@ -730,8 +725,8 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
     const int r = e.r0 + i * kRows + my_row;
     const bool mine = r < e.r1;
     const int token = a.by_group(mine ? r : e.r0);
-    float factor = 0.f, unbias = 0.f;
-    open_rows<TYPE, S>(a, e, q_smem + uint32_t(i * S::kQ), e.r0 + i * kRows + 32 * (warp & 3), factor, unbias);
+    float factor = 0.f;
+    open_rows<S>(a, e, q_smem + uint32_t(i * S::kQ), e.r0 + i * kRows + 32 * (warp & 3), factor);
     if (lane == 0) umma::mbar_arrive(umma::smem_u32(&sh.q_ready));
     const int position = sg.s.first + token;
     const int high = mine ? min(position + 1, sg.s.end) : 0, low = a.window > 0 ? max(0, position - a.window + 1) : 0;
@@ -751,8 +746,8 @@ __device__ __forceinline__ void softmax_rows(const AttnParams& a, Shared& sh, ui
       const bool every = token0 >= all_low && token0 + kTile <= all_high && (whole.x & whole.y & whole.z & whole.w) != 0;
       const uint32_t at = tmem_s + uint32_t((u & 1) * 64);
       auto products_done = [&] { return wait(a, sh, &sh.s_full[i][(u + 1) & 1], (scores >> ((u + 1) & 1)) & 1u); };      // the MMAs of the stage after this one
-      if (!(every ? tile_weights<S, true>(at, tmem_o, scales, factor, unbias, 0, 0, u > 0, ref, l, products_done)
-                  : tile_weights<S, false>(at, tmem_o, scales, factor, unbias, low - token0, high - token0, u > 0, ref, l, products_done))) {
+      if (!(every ? tile_weights<S, true>(at, tmem_o, scales, factor, 0, 0, u > 0, ref, l, products_done)
+                  : tile_weights<S, false>(at, tmem_o, scales, factor, low - token0, high - token0, u > 0, ref, l, products_done))) {
         lost = true;
         break;
       }
@@ -829,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_many_kernel(const __gri
   if (warp < 4 * S::kTiles) {
     if constexpr (S::kTiles == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 176;\n");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 192;\n");
-    softmax_rows<TYPE, S>(a, sh, q_smem);
+    softmax_rows<S>(a, sh, q_smem);
   } else if (warp < 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
     convert_tiles<TYPE, S>(a, sh, k_smem, v_smem);

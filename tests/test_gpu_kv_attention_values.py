@@ -1,0 +1,58 @@
+"""Attention over the 8-bit cache at values that a kernel can lose: keys of small codes under a large scale.
+Every case goes through the kernel of few rows and through the one of many.
+
+Bounds, from the arithmetic: an output is rounded once, u |out|; weights carry a rounding of 2^-11 (16-bit activations) and twice that of their scores, which are float32 sums
+of head_dim products of what q and the keys are - (head_dim + 8) 2^-24 of the sum of |q k|, whatever the block's scale is -, relative to sum p |v| and once more
+through the sum of the weights."""
+import pytest
+import torch
+
+from dinoml_v2_b200 import kernels
+from oracle import decoder as D
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+
+
+def _ints(values):
+    return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+
+def _prompt(tokens, block, singles=1):
+    """Table, lengths and starts of one prompt of `tokens` and of sequences of as many tokens with one new one each: the rows of the first take the kernel of
+    many rows, those of the others the one of few."""
+    need = -(-tokens // block)
+    return _ints([list(range(need))] * (1 + singles)), _ints([tokens] * (1 + singles)), _ints([0, *range(tokens, tokens + singles + 1)])
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("dim,mean", [(64, 30.0), (128, 8.0), (128, 30.0), (256, 8.0), (256, 30.0)])
+def test_small_codes_under_a_large_scale(dim, mean, dtype):
+    """One outlier sets the scale of every block, the other keys are a step or none; all of q has one sign.  q is zero in the outlier's channel, so the
+    scores are sums of small products.  All values are of one size: an output shows what its scores are off by."""
+    g = torch.Generator()
+    g.manual_seed(dim)
+    tokens, block, group, singles = 48, 16, 4, 40
+    cache = kernels.kv_cache(3, 1, block, dim, "int8")
+    base = torch.randint(-1, 2, (dim,), generator=g)
+    k = base.repeat(tokens, 1)
+    for j in range(tokens):
+        at = torch.randint(0, dim, (4,), generator=g)
+        k[j, at] = torch.randint(-1, 2, (4,), generator=g)
+    k[:, 5] = 0
+    k[::block, 5] = 127
+    cache.k.copy_(k.to(torch.int8).view(3, 1, block, dim))
+    cache.v.copy_((254 * torch.randint(0, 2, (3, 1, block, dim), generator=g) - 127).to(torch.int8))
+    cache.k_scale.fill_(100 / 127)
+    cache.v_scale.fill_(1 / 127)
+    q = (mean + torch.randn(tokens + singles, group, dim, generator=g)).to(getattr(torch, dtype))
+    q[:, :, 5] = 0
+    q = q.to(DEV)
+    table, lengths, starts = _prompt(tokens, block, singles)
+    out = kernels.kv_cache_attention(q, cache, table, lengths, starts)
+    assert kernels.device_status() == 0
+    ref, spread, terms = D.attention(q, cache, table, lengths, starts, dim ** -0.5, 0)
+    weights = 2.0 ** -11 + 2 * (dim + 8) * 2.0 ** -24 * terms[..., None]
+    bound = D.UNIT[dtype] * ref.abs() + 2 * weights * spread + D.SMALLEST[dtype]
+    off = (out.cpu().double() - ref).abs() / bound
+    assert (off <= 1).all(), (float(off[:tokens].max()), float(off[tokens:].max()))
