@@ -310,7 +310,8 @@ template <class S> __device__ __forceinline__ void open_rows(const AttnParams& a
     }
     if (t == 0) {
       const int position = sg.s.first + token;
-      out.factor[r] = a.scale * down;
+      // (an infinite or NaN q has no softmax, also where all of its scores are -inf and would look like those of a row that sees nothing)
+      out.factor[r] = e == 255 ? __uint_as_float(0x7fc00000u) : a.scale * down;
       out.high[r] = r < rows ? min(position + 1, sg.s.end) : 0;
       out.low[r] = a.window > 0 ? max(0, position - a.window + 1) : 0;
     }

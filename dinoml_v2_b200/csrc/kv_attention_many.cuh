@@ -548,7 +548,8 @@ __device__ __forceinline__ void open_rows(const AttnParams& a, const Ends e, uin
       st_shared16(at, h[0], h[1], h[2], h[3]);
     }
   }
-  factor = fabsf(a.scale) * __uint_as_float(uint32_t(127 - shift) << 23);
+  // (an infinite or NaN q: NaN, also where all of its scores are -inf and would look like those of a row that sees nothing)
+  factor = exponent == 255 ? __uint_as_float(0x7fc00000u) : fabsf(a.scale) * __uint_as_float(uint32_t(127 - shift) << 23);
   fence_async_smem();
   __syncwarp();
 }

@@ -1,5 +1,5 @@
-"""Attention over the 8-bit cache at values that a kernel can lose: keys of small codes under a large scale.
-Every case goes through the kernel of few rows and through the one of many.
+"""Attention over the 8-bit cache at values that a kernel can lose: keys of small codes under a large scale,
+infinite rows of q.  Every case goes through the kernel of few rows and through the one of many.
 
 Bounds, from the arithmetic: an output is rounded once, u |out|; weights carry a rounding of 2^-11 (16-bit activations) and twice that of their scores, which are float32 sums
 of head_dim products of what q and the keys are - (head_dim + 8) 2^-24 of the sum of |q k|, whatever the block's scale is -, relative to sum p |v| and once more
@@ -11,6 +11,7 @@ from dinoml_v2_b200 import kernels
 from oracle import decoder as D
 
 pytestmark = pytest.mark.gpu
+TYPES = ("int8", "float8_e4m3fn")
 DEV = torch.device("cuda:0")
 
 
@@ -56,3 +57,39 @@ def test_small_codes_under_a_large_scale(dim, mean, dtype):
     bound = D.UNIT[dtype] * ref.abs() + 2 * weights * spread + D.SMALLEST[dtype]
     off = (out.cpu().double() - ref).abs() / bound
     assert (off <= 1).all(), (float(off[:tokens].max()), float(off[tokens:].max()))
+
+
+def _cache_of_ones(blocks, heads, block, dim, kind, seed):
+    """Random codes; keys and values of order one."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    cache = kernels.kv_cache(blocks, heads, block, dim, kind)
+    for x, scale in zip(cache[:2], cache[2:]):
+        r = torch.randn(x.shape, device=DEV, generator=g)
+        x.copy_((r * 40).round().clamp(-127, 127) if kind == "int8" else (r * 100).clamp(-448, 448))
+        scale.fill_(1 / 32 if kind == "int8" else 1 / 128)
+    return cache
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("tokens", [1, 33, 80])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_infinite_q_is_nan(sign, tokens, kind, dtype):
+    """inf times keys is inf, -inf or NaN and its softmax is NaN, also where every score is -inf; other heads and rows are what they are without."""
+    for dim in (64, 128, 256):
+        cache = _cache_of_ones(5, 2, 16, dim, kind, 3)
+        cache.k.view(torch.uint8)[..., 9] = 0x38                 # of one sign in this channel (56, or e4m3's 1.0)
+        g = torch.Generator(device=DEV)
+        g.manual_seed(4)
+        q = torch.randn(tokens + 1, 4, dim, device=DEV, generator=g).to(getattr(torch, dtype))
+        table, lengths, starts = _prompt(tokens, 16)
+        clean = kernels.kv_cache_attention(q, cache, table, lengths, starts)
+        rows = sorted({0, tokens // 2, tokens})
+        bad = q.clone()
+        bad[rows, 3, 9] = sign * float("inf")
+        got = kernels.kv_cache_attention(bad, cache, table, lengths, starts)
+        assert kernels.device_status() == 0 and torch.isfinite(clean).all()
+        assert torch.isnan(got[rows, 3]).all()
+        got[rows, 3] = clean[rows, 3]
+        assert torch.equal(got, clean)
