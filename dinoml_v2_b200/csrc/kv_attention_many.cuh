@@ -327,6 +327,16 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(v) : "l"(a), "l"(b));
   return v;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float v;
+  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(v) : "f"(a), "f"(b));
+  return v;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float v;
   asm("max.f32 %0, %1, %2, %3;\n" : "=f"(v) : "f"(a), "f"(b), "f"(c));
@@ -334,18 +344,19 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // 2^x of two numbers below 2^7 without the special function unit: x = n + f with n the nearest integer (its bits are the last ones of x + 1.5 2^23), a
-// polynomial of degree four for 2^f on [-1/2, 1/2] (Remez exchange, relative error 2.6e-6), n added to its exponent.  Below 2^-126: 2^-126.
+// polynomial of degree four for 2^f on [-1/2, 1/2] (Remez exchange, relative error 2.6e-6), times 2^n (a product, not an addition to its exponent: a NaN stays one).
+// Below 2^-126: 2^-126.
 __device__ __forceinline__ float2 exp2_pair(uint64_t x) {
   const float2 raw = halves_of(x);
-  x = pair_of(fmaxf(raw.x, -126.f), fmaxf(raw.y, -126.f));
+  x = pair_of(max_or_nan(raw.x, -126.f), max_or_nan(raw.y, -126.f));
   constexpr float kRound = 12582912.f;
   const uint64_t t = add2(x, pair_of(kRound, kRound)), n = add2(t, pair_of(-kRound, -kRound)), f = fma2(n, pair_of(-1.f, -1.f), x);
   uint64_t p = fma2(f, pair_of(0.009570102207362652f, 0.009570102207362652f), pair_of(0.05591785907745361f, 0.05591785907745361f));
   p = fma2(p, f, pair_of(0.240247443318367f, 0.240247443318367f));
   p = fma2(p, f, pair_of(0.6931217908859253f, 0.6931217908859253f));
   p = fma2(p, f, pair_of(0.9999992847442627f, 0.9999992847442627f));
-  const float2 q = halves_of(p), e = halves_of(t);
-  return make_float2(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(e.x) << 23)), __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(e.y) << 23)));
+  const float2 e = halves_of(t);
+  return halves_of(mul2(p, pair_of(__uint_as_float((__float_as_uint(e.x) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(e.y) << 23) + 0x3f800000u))));
 }
 
 // Weights of 32 columns (two blocks' scales), their sum over each block's V scale; the largest y = s + log2(vs) of them.
@@ -365,7 +376,7 @@ __device__ __forceinline__ void weights_of(const uint32_t (&r)[32], const float4
       const float s[2] = {__uint_as_float(r[16 * g + k]), __uint_as_float(r[16 * g + k + 1])};
       const uint64_t y = fma2(pair_of(s[0], s[1]), ff, aa);
       float w[2];
-      if (EVERY && PARTS == 1 && (kPolynomial >> (k / 2) & 1) != 0) {                 // (a NaN is lost there: the row's other columns of the block have it)
+      if (EVERY && PARTS == 1 && (kPolynomial >> (k / 2) & 1) != 0) {
         const float2 e = exp2_pair(y);
         w[0] = e.x;
         w[1] = e.y;

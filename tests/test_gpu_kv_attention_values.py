@@ -1,5 +1,5 @@
 """Attention over the 8-bit cache at values that a kernel can lose: keys of small codes under a large scale,
-infinite rows of q.  Every case goes through the kernel of few rows and through the one of many.
+infinite rows of q, keys that stand for NaN.  Every case goes through the kernel of few rows and through the one of many.
 
 Bounds, from the arithmetic: an output is rounded once, u |out|; weights carry a rounding of 2^-11 (16-bit activations) and twice that of their scores, which are float32 sums
 of head_dim products of what q and the keys are - (head_dim + 8) 2^-24 of the sum of |q k|, whatever the block's scale is -, relative to sum p |v| and once more
@@ -93,3 +93,24 @@ def test_infinite_q_is_nan(sign, tokens, kind, dtype):
         assert torch.isnan(got[rows, 3]).all()
         got[rows, 3] = clean[rows, 3]
         assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_keys_of_nan_codes_are_nan(dim, dtype):
+    """An e4m3 NaN among the keys makes every row that sees it NaN, at every place of a tile."""
+    tokens = 200
+    cache = _cache_of_ones(13, 1, 16, dim, "float8_e4m3fn", 3)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(4)
+    q = torch.randn(tokens + 1, 2, dim, device=DEV, generator=g).to(getattr(torch, dtype))
+    table, lengths, starts = _prompt(tokens, 16)
+    clean = kernels.kv_cache_attention(q, cache, table, lengths, starts)
+    position = torch.cat([torch.arange(tokens), torch.tensor([tokens - 1])]).to(DEV)
+    for at in [*range(64, 80), 127, 128, 199]:
+        spoilt = [t.clone() for t in cache]
+        spoilt[0].view(torch.uint8)[at // 16, 0, at % 16, 21] = 0x7f
+        got = kernels.kv_cache_attention(q, spoilt, table, lengths, starts)
+        sees = position >= at
+        assert torch.isnan(got[sees]).all(), at
+        assert torch.equal(got[~sees], clean[~sees]), at
