@@ -267,6 +267,29 @@ __device__ __forceinline__ void copy_tiles(const AttnParams& a, Shared<S>& sh, c
   }
 }
 
+// Rows of the call that no sequence has - before the first one, behind the last one (a padded batch), those of starts that point outside - become zeros, by a
+// warp of every CTA.
+__device__ __forceinline__ void clear_rows_of_nobody(const AttnParams& a) {
+  if (a.p.starts == nullptr) return;
+  const int lane = threadIdx.x & 31, count = a.p.sequences, rows = a.p.rows;
+  const int per_row = a.heads * a.c.dim * (a.dtype == DINO_F32 ? 4 : 2) / 16;      // in 16 bytes
+  auto clear = [&](int low, int high, int first, int step) {
+    for (int64_t r = int64_t(low) + first; r < high; r += step)
+      for (int i = lane; i < per_row; i += 32) static_cast<uint4*>(a.out)[r * per_row + i] = make_uint4(0u, 0u, 0u, 0u);
+  };
+  clear(0, min(rows, min(fetch(a.p.starts), fetch(a.p.starts + 1))), int(blockIdx.x), int(gridDim.x));
+  clear(max(0, max(fetch(a.p.starts + count - 1), fetch(a.p.starts + count))), rows, int(blockIdx.x), int(gridDim.x));
+  for (int b0 = 32 * int(blockIdx.x); b0 < count; b0 += 32 * int(gridDim.x)) {
+    int s0 = 0, s1 = 0;
+    if (b0 + lane < count) {
+      s0 = fetch(a.p.starts + b0 + lane);
+      s1 = fetch(a.p.starts + b0 + lane + 1);
+    }
+    for (uint32_t bad = __ballot_sync(0xffffffffu, s0 < 0 || s1 < s0 || s1 > rows); bad != 0; bad &= bad - 1)      // (as in rows_of)
+      clear(max(0, __shfl_sync(0xffffffffu, s0, __ffs(bad) - 1)), min(rows, __shfl_sync(0xffffffffu, s1, __ffs(bad) - 1)), 0, 1);
+  }
+}
+
 // ---- the opening warp.  Rows of an item: q as operand fragments, what their scores are multiplied by, what they see.  Lane (g, t) has the fragments of
 // row g, 16 t .. 16 t + 15 of every 64 values, so it reads them, and eight rows are made at once.
 template <class S> __device__ __forceinline__ void open_rows(const AttnParams& a, Rows8<S>& out, const Segment& sg, uint2* qfrag) {
@@ -476,6 +499,7 @@ __global__ void __launch_bounds__(S::kThreads, kCtasPerSm) attention_few_kernel(
   const Walk first = walk_of<S::kThreads>(a, S::kLog2, W / 2, sh.walk);    // (its barriers: the inits are visible)
   if (warp == W) {
     copy_tiles(a, sh, &k_map, &v_map, ring, first);
+    clear_rows_of_nobody(a);
     return;
   }
   if (warp == W + 1) {

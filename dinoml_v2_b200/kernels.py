@@ -251,6 +251,13 @@ def _kv_rows(t: torch.Tensor, name: str, device, heads, head_dim: int) -> None:
         raise ValueError(f"{name} must be [rows, {heads or 'heads'}, {head_dim}] in {sorted(_TORCH_DTYPE)}, its last dimension contiguous")
 
 
+def _kv_zero(out, stream) -> None:
+    """Rows without a sequence."""
+    with torch.cuda.stream(stream):
+        for t in out:
+            t.zero_()
+
+
 def kv_cache_write(cache, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor | None = None, *,
                    stream=None):
     """Quantizes new tokens into the cache, in place, and returns it.  k, v: [rows, kv_heads, head_dim], any row and head strides.  Rows are packed:
@@ -280,7 +287,7 @@ def kv_cache_write(cache, k: torch.Tensor, v: torch.Tensor, block_table: torch.T
 def kv_cache_read(cache, block_table: torch.Tensor, starts: torch.Tensor | None, rows: int, dtype: str = "bfloat16", *, begins: torch.Tensor | None = None,
                   out=None, stream=None):
     """Dense (k, v), each [rows, kv_heads, head_dim]: row starts[b] + j is position begins[b] + j of sequence b (begins None: from the first token; starts
-    None: one row each).  `out`: two such tensors to fill."""
+    None: one row each).  Rows that no sequence has are zero.  `out`: two such tensors to fill."""
     done = _native_call("kv_read")(cache, block_table, starts, rows, dtype, begins, stream) if out is None else None
     if done is not None:                                                                  # None: not the plain case, checked below
         if type(done) is int:
@@ -303,6 +310,8 @@ def kv_cache_read(cache, block_table: torch.Tensor, starts: torch.Tensor | None,
         rc = _native.lib().dinoml_b200_kv_cache_read(ctypes.byref(struct), ctypes.byref(batch), begins_ptr, k.data_ptr(), v.data_ptr(),
                                                      _native.DINO_DTYPE[dtype], _stream_ptr(stream))
         _native.check(rc, "dinoml_b200_kv_cache_read")
+    else:
+        _kv_zero((k, v), stream)
     return k, v
 
 
@@ -310,7 +319,7 @@ def kv_cache_attention(q: torch.Tensor, cache, block_table: torch.Tensor, length
                        window: int = 0, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """softmax(scale * q K^T) V over the cache, causal: a row at position p of its sequence sees positions max(0, p - window + 1) .. p (window 0: all up to p).
     q [rows, heads, head_dim], any row and head strides; heads is a multiple of kv_heads, head h reads cached head h // (heads // kv_heads); rows, lengths and
-    starts as for `kv_cache_write`, whose tokens have to be in the cache.  scale None: head_dim ** -0.5.  A row that sees nothing is zero."""
+    starts as for `kv_cache_write`, whose tokens have to be in the cache.  scale None: head_dim ** -0.5.  A row that sees nothing is zero, and so is one that no sequence has."""
     done = _native_call("kv_attention")(q, cache, block_table, lengths, starts, scale, window, out, stream)
     if done is not None:                                                                  # None: not the plain case, checked below
         if type(done) is int:
@@ -334,6 +343,8 @@ def kv_cache_attention(q: torch.Tensor, cache, block_table: torch.Tensor, length
             ctypes.byref(struct), ctypes.byref(batch), q.data_ptr(), out.data_ptr(), _native.DINO_DTYPE[_DTYPE_NAME[q.dtype]], q.shape[1], q.stride(0),
             q.stride(1), struct.head_dim ** -0.5 if scale is None else float(scale), int(window), _stream_ptr(stream))
         _native.check(rc, "dinoml_b200_kv_cache_attention")
+    else:
+        _kv_zero((out,), stream)
     return out
 
 

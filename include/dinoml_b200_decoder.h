@@ -34,9 +34,11 @@ typedef struct DinoB200KvCache {
 } DinoB200KvCache;
 
 /* Which tokens a call is about.  Position p of sequence b is in slot p % block_size of block block_table[b * table_stride + p / block_size].
- * Rows of the call's dense tensors are packed: sequence b has rows starts[b] .. starts[b + 1] - 1 (starts[0] = 0, starts[sequences] = rows); with
+ * Rows of the call's dense tensors are packed: sequence b has rows starts[b] .. starts[b + 1] - 1; with
  * starts null every sequence has one row.  lengths[b] counts the tokens of the sequence, those of the call's rows among them: row starts[b] + j
- * is position lengths[b] - (starts[b + 1] - starts[b]) + j.  Rows at negative positions (an idle slot has length 0) are nobody's. */
+ * is position lengths[b] - (starts[b + 1] - starts[b]) + j.  Rows at negative positions (an idle slot has length 0) are
+ * nobody's, and so are those before starts[0] and behind starts[sequences] (a padded batch): they are not written to the cache, and zero in what a read or the
+ * attention gives. */
 typedef struct DinoB200KvBatch {
   const int* block_table;
   int64_t table_stride; /* elements */
