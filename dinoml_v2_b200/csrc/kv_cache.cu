@@ -235,7 +235,10 @@ __global__ void __launch_bounds__(32 * kReadWarps) kv_read_kernel(Cache c, Batch
   const Rows rows = rows_of(p, b);
   const int64_t position = int64_t(row) - rows.first + (begins != nullptr ? fetch(begins + b) : 0);
   int id = -1;
-  if (row >= rows.first && row < rows.first + rows.count && position >= 0 && position <= INT32_MAX) id = block_at(p, c.blocks, b, int(position >> c.block_log2));
+  if (row >= rows.first && row < rows.first + rows.count) {
+    if (position >= 0 && position <= INT32_MAX) id = block_at(p, c.blocks, b, int(position >> c.block_log2));
+    else flag_range(p.status);
+  }
   const int slot = int(position) & ((1 << c.block_log2) - 1), log2 = __ffs(c.dim) - 1, width = c.heads << log2;
   const int64_t to = row64 * width;
   for (int i = lane * N; i < width; i += 32 * N * kReadAhead) {

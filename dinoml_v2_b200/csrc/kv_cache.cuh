@@ -11,7 +11,7 @@
 namespace b200gguf {
 namespace kv {
 
-constexpr int ST_KV_RANGE = 10;      // device status: a block table entry, a length or a start pointed outside of the cache or of the rows
+constexpr int ST_KV_RANGE = 10;      // device status: a block table entry, a length, a start or a begin pointed outside of the cache or of the rows
 
 struct Cache {
   uint8_t* data[2];                  // keys, values

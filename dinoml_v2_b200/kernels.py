@@ -397,5 +397,5 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, residu
 
 def device_status() -> int:
     """Synchronizes and returns the status word written by bounded device-side waits (0 = none gave up; 16: one of the attention over the cache) and by the checks of
-    what only the device sees (10: a block table, lengths or starts pointed outside of the cache or of the rows).  Read once: it is 0 after that."""
+    what only the device sees (10: a block table, lengths, starts or begins pointed outside of the cache or of the rows).  Read once: it is 0 after that."""
     return int(_native.lib().dinoml_b200_gguf_device_status())

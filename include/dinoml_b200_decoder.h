@@ -4,7 +4,7 @@
  *
  * Conventions are those of dinoml_b200_gguf.h: device pointers, `stream` a cudaStream_t as void*, 0 = ok, 1 = null pointer, 2 = non-positive
  * dimension, 4 = launch failure, 6 = unsupported dtype or cache type, 7 = alignment, 8 = size outside what the kernels take; a message is
- * available from dino_get_last_error().  What only the device sees (block table, lengths, starts) is checked there: an entry that
+ * available from dino_get_last_error().  What only the device sees (block table, lengths, starts, begins) is checked there: an entry that
  * points outside of the cache or of the rows is left out of the operation, and dinoml_b200_gguf_device_status() answers 10.  16 there: a wait
  * inside of an attention kernel gave up, and its results are not to be used; reading the status empties the workspaces' counters.
  */

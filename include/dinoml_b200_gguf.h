@@ -111,7 +111,7 @@ DINOML_B200_API size_t dinoml_b200_gguf_prealloc_scratch_bytes(void);
 /* The tcgen05 kernel bounds every barrier wait; a wait that gives up records a code in a per-device
  * status word instead of hanging or trapping.  Synchronizes the device, returns the word (0 = never
  * happened; 1 / 2 / 3 / 4 = a stage-free / stage-ready / accumulator / partial-tile wait gave up; 6 = a peer never signalled
- * in dinoml_b200_peer_exchange; 10 = a block table entry, a length or a start pointed outside of a cache, 16 = a wait of the
+ * in dinoml_b200_peer_exchange; 10 = a block table entry, a length, a start or a begin pointed outside of a cache, 16 = a wait of the
  * attention over one gave up, dinoml_b200_decoder.h; < 0 = CUDA error) and
  * clears it together with the partial-tile flags.
  * No counterpart in the reference. */

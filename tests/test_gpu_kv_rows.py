@@ -66,3 +66,13 @@ def test_no_sequences_at_all():
     k, v = (torch.full((5, 2, 64), 7.0, device=DEV) for _ in range(2))
     kernels.kv_cache_read(cache, rows=5, dtype="float32", out=(k, v), **none)
     assert not k.any() and not v.any() and kernels.device_status() == 0
+
+
+def test_positions_before_the_first_token():
+    """A range that begins before the first token: zeros, told by the status word."""
+    cache, table = _cache(64)
+    k, v = kernels.kv_cache_read(cache, table, _ints([0, 5, 8]), 8, "float32", begins=_ints([-2, 0]))
+    assert kernels.device_status() == 10
+    want, _ = kernels.kv_cache_read(cache, table, _ints([0, 3, 6]), 6, "float32")
+    assert kernels.device_status() == 0
+    assert not k[:2].any() and not v[:2].any() and torch.equal(k[2:], want)
