@@ -638,9 +638,10 @@ __global__ void __launch_bounds__(S::kThreads, kCtasPerSm) attention_few_kernel(
       bool tiny = PARTS == 2;
 #pragma unroll
       for (int n = 0; n < NT; ++n) sum[n][0] = sum[n][1] = 0.f;
+      const float up = 0x1p14f * __frcp_rn(vt);                         // (2^14 vs may be past the largest float32)
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        const float f = __fdividef(vs[i] * 0x1p14f, vt);
+        const float f = vs[i] * up;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float p[4];

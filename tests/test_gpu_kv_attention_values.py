@@ -1,5 +1,6 @@
 """Attention over the 8-bit cache at values that a kernel can lose: keys of small codes under a large scale,
-infinite rows of q, keys that stand for NaN.  Every case goes through the kernel of few rows and through the one of many.
+infinite rows of q, keys that stand for NaN, values near the largest float32.
+Every case but the last goes through the kernel of few rows and through the one of many (which holds the scale of a block of values in exponents).
 
 Bounds, from the arithmetic: an output is rounded once, u |out|; weights carry a rounding of 2^-11 (16-bit activations) and twice that of their scores, which are float32 sums
 of head_dim products of what q and the keys are - (head_dim + 8) 2^-24 of the sum of |q k|, whatever the block's scale is -, relative to sum p |v| and once more
@@ -114,3 +115,21 @@ def test_keys_of_nan_codes_are_nan(dim, dtype):
         sees = position >= at
         assert torch.isnan(got[sees]).all(), at
         assert torch.equal(got[~sees], clean[~sees]), at
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_values_near_the_largest_float32(dtype, kind):
+    """A sequence of one token answers with its value, whatever its size is."""
+    for dim in (64, 128, 256):
+        g = torch.Generator(device=DEV)
+        g.manual_seed(dim)
+        x = torch.randn(1, 2, dim, device=DEV, generator=g).clamp(-3, 3).to(getattr(torch, dtype))
+        for size in (1e30, 3e36, 1e38):
+            cache = kernels.kv_cache(1, 2, 16, dim, kind)
+            v = x * size
+            kernels.kv_cache_write(cache, x, v, _ints([[0]]), _ints([1]))
+            held = kernels.kv_cache_read(cache, _ints([[0]]), None, 1, "float32")[1]
+            got = kernels.kv_cache_attention(x, cache, _ints([[0]]), _ints([1])).float()
+            assert kernels.device_status() == 0 and torch.isfinite(held).all()
+            assert ((got - held).abs() <= (D.UNIT[dtype] + 2.0 ** -11) * held.abs()).all(), size
