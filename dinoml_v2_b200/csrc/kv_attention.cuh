@@ -10,7 +10,6 @@ namespace stream { int sm_count(); }             // gemv_stream.cu
 namespace kv {
 
 constexpr float kLog2e = 1.4426950408889634f;
-enum : int { ST_KV_TIMEOUT = 16 };          // device status: a wait gave up
 constexpr uint32_t kPolls = 1u << 18;       // of a barrier before a wait gives up, a second or two: waits are within a CTA
 
 // n / d for 0 <= n < 2^31: the quotient is (mulhi(n, m) + n) >> s with s = ceil(log2 d), m = floor(2^32 (2^s - d) / d) + 1 (Granlund and Montgomery).

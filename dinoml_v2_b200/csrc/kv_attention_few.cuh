@@ -174,7 +174,7 @@ template <class S> __device__ __forceinline__ bool wait(const AttnParams& a, Sha
     if ((i & 255u) == 255u && *lost) return false;
   }
   *lost = 1;
-  atomicCAS(a.p.status, 0, ST_KV_TIMEOUT);
+  flag_timeout(a.p.status);
   return false;
 }
 template <class S> __device__ __forceinline__ bool warp_wait(const AttnParams& a, Shared<S>& sh, uint64_t* bar, uint32_t parity) {

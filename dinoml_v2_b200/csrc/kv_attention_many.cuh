@@ -79,7 +79,7 @@ __device__ __forceinline__ bool wait(const AttnParams& a, Shared& sh, uint64_t* 
   ok = __all_sync(0xffffffffu, ok) != 0;
   if (!ok && !*lost) {
     *lost = 1;
-    atomicCAS(a.p.status, 0, ST_KV_TIMEOUT);
+    flag_timeout(a.p.status);
   }
   return ok;
 }

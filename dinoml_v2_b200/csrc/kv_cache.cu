@@ -7,7 +7,7 @@
 namespace b200gguf {
 namespace kv {
 
-static __device__ int g_kv_status;
+static __device__ int g_kv_status[kStatusWords];
 
 static int* status_ptr() {
   static int* ptr[kGemvMaxDevices] = {};
@@ -292,14 +292,7 @@ int cache_read(const DinoB200KvCache* cache, const DinoB200KvBatch* batch, const
 
 }  // namespace kv
 
-// Status word of the cache's kernels on the current device (read once).
-int kv_device_status() {
-  int value = 0;
-  int* p = kv::status_ptr();
-  if (p == nullptr || cudaMemcpy(&value, p, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return 0;
-  if (value != 0) cudaMemset(p, 0, sizeof(int));
-  if (value == kv::ST_KV_TIMEOUT) kv::attention_reset();
-  return value;
-}
+// Status of the cache's kernels on the current device (read once).
+int kv_device_status() { return kv::take_status(kv::status_ptr(), kv::attention_reset); }
 
 }  // namespace b200gguf

@@ -7,11 +7,10 @@
 
 #include "../../include/dinoml_b200_decoder.h"
 #include "gguf_common.cuh"
+#include "kv_status.h"
 
 namespace b200gguf {
 namespace kv {
-
-constexpr int ST_KV_RANGE = 10;      // device status: a block table entry, a length, a start or a begin pointed outside of the cache or of the rows
 
 struct Cache {
   uint8_t* data[2];                  // keys, values
@@ -22,7 +21,7 @@ struct Batch {
   const int *table, *lengths, *starts;
   int64_t table_stride;
   int table_blocks, sequences, rows;
-  int* status;
+  int* status;                       // the words of kv_status.h
 };
 
 // Host: checks and the device's view of the two structs; a return code.
@@ -33,7 +32,8 @@ int batch_view(const DinoB200KvBatch* batch, bool needs_lengths, Batch* out);
 // A plain read.  (A read as of constant data may be moved ahead of a kernel's wait for the launch before it.)
 template <typename T> __device__ __forceinline__ T fetch(const T* p) { return *p; }
 
-__device__ __forceinline__ void flag_range(int* status) { atomicCAS(status, 0, ST_KV_RANGE); }
+__device__ __forceinline__ void flag_range(int* status) { atomicExch(status, ST_KV_RANGE); }
+__device__ __forceinline__ void flag_timeout(int* status) { atomicExch(status + 1, ST_KV_TIMEOUT); }
 
 // Block j of sequence b, -1 if there is none.
 __device__ __forceinline__ int block_at(const Batch& p, int blocks, int b, int j) {
