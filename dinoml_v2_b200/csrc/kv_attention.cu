@@ -4,22 +4,6 @@
 namespace b200gguf {
 namespace kv {
 
-// Pieces of cut items and a counter per CTA, per (device, stream).
-struct AttnScratch {
-  int* arrived = nullptr;
-  float* partial = nullptr;
-  size_t floats = 0;
-  std::vector<void*> outgrown;      // smaller workspaces that captured graphs may still use
-  bool made() const { return arrived != nullptr; }
-  bool empty(cudaStream_t s) { return arrived == nullptr || cudaMemsetAsync(arrived, 0, sizeof(int) * kMaxWorkers, s) == cudaSuccess; }
-  int word(cudaStream_t) { return 0; }
-  void give_back() {
-    if (arrived != nullptr) cudaFree(arrived);
-    if (partial != nullptr) cudaFree(partial);
-    for (void* p : outgrown) cudaFree(p);
-  }
-  static constexpr int kMaxWorkers = 1024;
-};
 static ScratchSets<AttnScratch> g_sets;
 // Rows (tokens x heads of a cached head) of a sequence up to which the kernel of few rows takes it: it reads the cache once for 16 rows, the other one once for
 // 256, at a lower rate.  Measured (few, many; 8 cached heads of 128, int8): 64 sequences of 4000 tokens, 32 rows 310 and 358 us, 64 rows 574 and 354;
@@ -53,7 +37,7 @@ void attention_reset() {
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess) return;
   std::lock_guard<std::mutex> lock(g_sets.mutex);
-  g_sets.for_each(dev, [](AttnScratch& set) { set.empty(nullptr); });
+  g_sets.empty_all(dev);
 }
 
 int cache_attention(const DinoB200KvCache* cache, const DinoB200KvBatch* batch, const void* q, void* out, int dtype, int heads, int64_t q_row_stride,

@@ -59,6 +59,23 @@ struct UmmaScratch {
   }
 };
 
+// Attention over the 8-bit cache: the pieces of items that several CTAs share, and a counter per CTA, zero between launches.  Its status belongs to the device.
+struct AttnScratch {
+  static constexpr int kMaxWorkers = 1024;
+  int* arrived = nullptr;
+  float* partial = nullptr;
+  size_t floats = 0;
+  std::vector<void*> outgrown;      // smaller workspaces that captured graphs may still use
+  bool made() const { return arrived != nullptr; }
+  bool empty(cudaStream_t s) { return arrived == nullptr || cudaMemsetAsync(arrived, 0, sizeof(int) * kMaxWorkers, s) == cudaSuccess; }
+  int word(cudaStream_t) { return 0; }
+  void give_back() {
+    if (arrived != nullptr) cudaFree(arrived);
+    if (partial != nullptr) cudaFree(partial);
+    for (void* p : outgrown) cudaFree(p);
+  }
+};
+
 template <typename Set>
 class ScratchSets {
  public:
@@ -99,6 +116,12 @@ class ScratchSets {
   template <typename F> void for_each(int dev, F f) {
     for (auto& entry : sets_)
       if (entry.first.first == dev && entry.second.made()) f(entry.second);
+  }
+  // The sets in use on a device are empty when this returns: before a launch on any stream, of which most do not wait for the one that empties.
+  bool empty_all(int dev) {
+    bool emptied = true;
+    for_each(dev, [&](Set& set) { emptied = set.empty(nullptr) && emptied; });
+    return cudaStreamSynchronize(nullptr) == cudaSuccess && emptied;
   }
   // Error code of a set whose stream is gone (read once).
   int take_kept_word(int dev) {
