@@ -1,43 +1,30 @@
 // Host side of attention over the 8-bit cache: checks, workspaces, which kernel takes a call.  The kernels are in kv_attention_few.cuh and kv_attention_many.cuh.
+#include "captured_sets.h"
 #include "kv_attention.cuh"
 
 namespace b200gguf {
 namespace kv {
 
-static ScratchSets<AttnScratch> g_sets;
+// (Never destroyed: a graph may be dropped while the process ends.)
+static AttnWorkspaces& workspaces() {
+  static AttnWorkspaces* all = new AttnWorkspaces;
+  return *all;
+}
 // Rows (tokens x heads of a cached head) of a sequence up to which the kernel of few rows takes it: it reads the cache once for 16 rows, the other one once for
 // 256, at a lower rate.  Measured (few, many; 8 cached heads of 128, int8): 64 sequences of 4000 tokens, 32 rows 310 and 358 us, 64 rows 574 and 354;
 // 16 of 2000, 20 rows 59 and 64, 36 rows 79 and 66; heads of 256: 64 of 2000, 16 rows 276 and 220, 20 rows 490 and 223 (up to one reading of the cache the kernel
 // of few rows is kept: its weights have no smallest one); float32: 64 of 2000, 16 rows 126 and 190, 32 rows 213 and 201.
 static int few_rows(int dim) { return dim == 256 ? 16 : 32; }
 
-// Allocates outside of stream capture only: callers run a shape once before capturing a graph.
 float* attention_scratch(size_t floats, int ctas, cudaStream_t s, int** arrived) {
   int dev = -1;
   if (ctas > AttnScratch::kMaxWorkers || cudaGetDevice(&dev) != cudaSuccess) return nullptr;
-  std::lock_guard<std::mutex> lock(g_sets.mutex);
-  AttnScratch& set = g_sets.at(dev, s);
-  if (set.arrived == nullptr) {
-    if (cudaMalloc(&set.arrived, sizeof(int) * AttnScratch::kMaxWorkers) != cudaSuccess) { set.arrived = nullptr; return nullptr; }
-    if (!set.empty(s)) return nullptr;
-  }
-  if (floats > set.floats) {
-    const size_t size = floats > 2 * set.floats ? floats : 2 * set.floats;
-    float* p = nullptr;
-    if (cudaMalloc(&p, size * sizeof(float)) != cudaSuccess) return nullptr;
-    if (set.partial != nullptr) set.outgrown.push_back(set.partial);
-    set.partial = p;
-    set.floats = size;
-  }
-  *arrived = set.arrived;
-  return set.partial;
+  return workspaces().get(dev, s, floats, arrived);
 }
 
 void attention_reset() {
   int dev = -1;
-  if (cudaGetDevice(&dev) != cudaSuccess) return;
-  std::lock_guard<std::mutex> lock(g_sets.mutex);
-  g_sets.empty_all(dev);
+  if (cudaGetDevice(&dev) == cudaSuccess) workspaces().reset(dev);
 }
 
 int cache_attention(const DinoB200KvCache* cache, const DinoB200KvBatch* batch, const void* q, void* out, int dtype, int heads, int64_t q_row_stride,

@@ -2,7 +2,6 @@
 // between them, 8-bit pairs as float16.
 #pragma once
 #include "kv_cache.cuh"
-#include "scratch_sets.h"
 #include "umma_frame.cuh"
 
 namespace b200gguf {

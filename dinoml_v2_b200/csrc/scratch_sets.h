@@ -65,7 +65,7 @@ struct AttnScratch {
   int* arrived = nullptr;
   float* partial = nullptr;
   size_t floats = 0;
-  std::vector<void*> outgrown;      // smaller workspaces that captured graphs may still use
+  std::vector<void*> outgrown;      // smaller workspaces that launches on their way may still use
   bool made() const { return arrived != nullptr; }
   bool empty(cudaStream_t s) { return arrived == nullptr || cudaMemsetAsync(arrived, 0, sizeof(int) * kMaxWorkers, s) == cudaSuccess; }
   int word(cudaStream_t) { return 0; }

@@ -64,7 +64,9 @@ DINOML_B200_API int dinoml_b200_kv_cache_read(const DinoB200KvCache* cache, cons
 /* out[row][head] = softmax(scale * q[row][head] K^T) V over the positions max(0, p - window + 1) .. p of the row's own sequence (window 0: 0 .. p),
  * p its position; head h reads cached head h / (heads / kv_heads).  q: [rows][heads][head_dim], strides in elements, head_dim contiguous; out
  * contiguous.  A row that sees nothing is zero.  Scores, softmax statistics and sums are float32.  The library keeps the workspace of sequences
- * that several CTAs share, per device and stream: run a shape once before capturing it. */
+ * that several CTAs share: one per device and stream, and for captured calls one per capture and stream, which is made during the capture and given back when the graph
+ * is destroyed.  So a graph may be replayed on any stream, beside other graphs and beside calls on the stream that it was captured on; two graphs that are
+ * instantiated from one capture have one workspace and must not overlap.  Run a call once before the first capture: kernels are loaded then. */
 DINOML_B200_API int dinoml_b200_kv_cache_attention(const DinoB200KvCache* cache, const DinoB200KvBatch* batch, const void* q, void* out, int dtype, int heads,
                                                    int64_t q_row_stride, int64_t q_head_stride, float scale, int window, void* stream);
 

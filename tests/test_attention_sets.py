@@ -1,4 +1,4 @@
-"""CPU tests of the attention's workspaces (csrc/scratch_sets.h), compiled against a fake CUDA runtime whose stream work is carried out when the stream is
+"""CPU tests of the attention's workspaces (csrc/scratch_sets.h, csrc/captured_sets.h), compiled against a fake CUDA runtime whose stream work is carried out when the stream is
 waited for."""
 import shutil
 import subprocess
@@ -54,6 +54,100 @@ int main() {
   std::puts("ok");
 }
 """
+CAPTURED = FAKE + r"""
+#include "captured_sets.h"
+using namespace b200gguf;
+
+struct Object { cudaHostFn_t destroy; void* data; int references; };
+struct Graph { std::vector<Object*> owned; };
+static std::map<cudaStream_t, std::pair<unsigned long long, Graph*>> capturing;
+static cudaStreamCaptureMode mode = cudaStreamCaptureModeGlobal;
+static bool fail_retain = false, fail_malloc = false;
+static void drop(Object* o, unsigned n) { if ((o->references -= int(n)) == 0) { o->destroy(o->data); delete o; } }
+extern "C" {
+cudaError_t cudaStreamGetCaptureInfo_v2(cudaStream_t s, cudaStreamCaptureStatus* status, unsigned long long* id, cudaGraph_t* graph, const cudaGraphNode_t**, size_t*) {
+  const auto it = capturing.find(s);
+  *status = it == capturing.end() ? cudaStreamCaptureStatusNone : cudaStreamCaptureStatusActive;
+  if (it != capturing.end()) { *id = it->second.first; *graph = reinterpret_cast<cudaGraph_t>(it->second.second); }
+  return cudaSuccess;
+}
+cudaError_t cudaThreadExchangeStreamCaptureMode(cudaStreamCaptureMode* m) { std::swap(*m, mode); return cudaSuccess; }
+cudaError_t cudaStreamCreateWithFlags(cudaStream_t* s, unsigned) { *s = reinterpret_cast<cudaStream_t>(size_t(999)); return cudaSuccess; }
+cudaError_t cudaStreamDestroy(cudaStream_t s) { assert(queued[s].empty()); return cudaSuccess; }
+cudaError_t cudaUserObjectCreate(cudaUserObject_t* o, void* p, cudaHostFn_t f, unsigned n, unsigned) {
+  *o = reinterpret_cast<cudaUserObject_t>(new Object{f, p, int(n)});
+  return cudaSuccess;
+}
+cudaError_t cudaUserObjectRelease(cudaUserObject_t o, unsigned n) { drop(reinterpret_cast<Object*>(o), n); return cudaSuccess; }
+cudaError_t cudaGraphRetainUserObject(cudaGraph_t g, cudaUserObject_t o, unsigned n, unsigned flags) {
+  assert(n == 1 && flags == cudaGraphUserObjectMove);
+  if (fail_retain) return cudaErrorUnknown;
+  reinterpret_cast<Graph*>(g)->owned.push_back(reinterpret_cast<Object*>(o));
+  return cudaSuccess;
+}
+}
+static void destroy(Graph& g) { for (Object* o : g.owned) drop(o, 1); g.owned.clear(); }
+
+struct Got { float* room; int* counters; };
+static Got get(AttnWorkspaces& all, cudaStream_t s, size_t floats = 100) {
+  const cudaStreamCaptureMode before = mode;
+  Got got{nullptr, nullptr};
+  got.room = all.get(0, s, floats, &got.counters);
+  assert(mode == before);
+  if (got.room != nullptr && capturing.count(s) == 0) cudaStreamSynchronize(s);      // (the launch behind it would wait)
+  if (got.room != nullptr) for (int i = 0; i < AttnScratch::kMaxWorkers; ++i) assert(got.counters[i] == 0);
+  return got;
+}
+
+int main() {
+  AttnWorkspaces all;
+  Graph one, two, three;
+  const Got eager = get(all, stream(1));
+  capturing[stream(1)] = {11, &one};
+  const Got a = get(all, stream(1)), again = get(all, stream(1), 50);
+  assert(a.room != eager.room && a.counters != eager.counters);                          // not the stream's own
+  assert(again.room == a.room && again.counters == a.counters);                          // ordered within a capture
+  const Got more = get(all, stream(1), 1000);
+  assert(more.room != a.room && more.counters == a.counters && live.count(a.room) == 1); // the smaller room stays: nodes have its address
+  capturing[stream(2)] = {11, &one};
+  const Got fork = get(all, stream(2));
+  assert(fork.room != more.room && fork.counters != a.counters);                         // a branch of the same capture
+  capturing.clear();
+  capturing[stream(1)] = {12, &two};
+  const Got b = get(all, stream(1));
+  assert(b.counters != a.counters && b.counters != eager.counters && b.counters != fork.counters);     // another graph of the same stream
+  capturing.clear();
+  assert(get(all, stream(1)).counters == eager.counters);
+  // A status read empties all of them.
+  a.counters[3] = fork.counters[4] = b.counters[5] = eager.counters[6] = 1;
+  all.reset(0);
+  assert(a.counters[3] == 0 && fork.counters[4] == 0 && b.counters[5] == 0 && eager.counters[6] == 0);
+  // Sets of graphs that are gone are used again, empty; nothing is allocated.
+  b.counters[7] = 9;
+  destroy(two);
+  const size_t before = live.size();
+  capturing[stream(3)] = {13, &three};
+  assert(get(all, stream(3)).counters == b.counters && live.size() == before);
+  // What can't be had leaves nothing behind.
+  capturing[stream(3)] = {14, &three};
+  fail_retain = true;
+  assert(get(all, stream(3)).room == nullptr);
+  fail_retain = false;
+  capturing.clear();
+  destroy(one);
+  destroy(three);
+  // A bounded number is kept.
+  std::vector<Graph> many(20);
+  for (int i = 0; i < 20; ++i) {
+    capturing[stream(4)] = {100ull + unsigned(i), &many[i]};
+    assert(get(all, stream(4)).room != nullptr);
+  }
+  for (Graph& g : many) destroy(g);
+  all.reset(0);
+  assert(live.size() <= 2 + 4 * 3);                                                      // the stream's, and four sets of up to three
+  std::puts("ok");
+}
+"""
 
 
 def _run(source, tmp_path):
@@ -71,3 +165,7 @@ def _run(source, tmp_path):
 
 def test_counters_are_empty_when_the_status_has_been_read(tmp_path):
     _run(EMPTIED, tmp_path)
+
+
+def test_captures_have_workspaces_of_their_own(tmp_path):
+    _run(CAPTURED, tmp_path)
