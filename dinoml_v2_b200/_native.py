@@ -103,6 +103,8 @@ def lib() -> ctypes.CDLL:
     L.dinoml_b200_kv_cache_attention.restype = ci
     L.dinoml_b200_rms_norm.argtypes = [vp, vp, vp, vp, vp, ci, ci, ci, ci, cf, ci, vp]
     L.dinoml_b200_rms_norm.restype = ci
+    L.dinoml_b200_release_stream.argtypes = [vp]
+    L.dinoml_b200_release_stream.restype = ci
     _lib = L
     return L
 

@@ -131,6 +131,11 @@ class AttnWorkspaces {
     *arrived = set.arrived;
     return set.partial;
   }
+  // `stream` is about to be destroyed and has no work left.
+  void release(cudaStream_t stream) {
+    std::lock_guard<std::mutex> lock(sets_.mutex);
+    sets_.release(stream);
+  }
   void reset(int dev) {
     {
       std::lock_guard<std::mutex> lock(sets_.mutex);

@@ -4,6 +4,9 @@
 
 namespace b200gguf {
 int set_error(int rc, const char* where);
+void stream_release_scratch(cudaStream_t s);
+void umma_release_scratch(cudaStream_t s);
+void attention_release_scratch(cudaStream_t s);
 namespace kv {
 int cache_write(const DinoB200KvCache* cache, const DinoB200KvBatch* batch, const void* k, const void* v, int dtype, int64_t k_row_stride,
                 int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride, cudaStream_t s);
@@ -41,6 +44,15 @@ int dinoml_b200_rms_norm(const void* x, const void* residual, const void* weight
                          float eps, int q8_0, void* stream) {
   return set_error(norm::rms_norm(x, residual, weight, y, total, dtype, weight_dtype, rows, width, eps, q8_0, static_cast<cudaStream_t>(stream)),
                    "dinoml_b200_rms_norm");
+}
+
+int dinoml_b200_release_stream(void* stream) {
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (cudaStreamSynchronize(s) != cudaSuccess) return set_error(RC_LAUNCH, "dinoml_b200_release_stream");
+  stream_release_scratch(s);
+  umma_release_scratch(s);
+  attention_release_scratch(s);
+  return set_error(RC_OK, "dinoml_b200_release_stream");
 }
 
 }  // extern "C"

@@ -66,4 +66,7 @@ int cache_attention(const DinoB200KvCache* cache, const DinoB200KvBatch* batch, 
 }
 
 }  // namespace kv
+
+void attention_release_scratch(cudaStream_t s) { kv::workspaces().release(s); }
+
 }  // namespace b200gguf

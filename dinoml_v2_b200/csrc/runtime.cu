@@ -53,6 +53,7 @@ int gemm_rcr(const void* a, const void* b, const void* bias, void* c, int qtype,
              int variant, cudaStream_t s);
 void stream_release_scratch(cudaStream_t s);      // workspaces the kernels keep for a stream
 void umma_release_scratch(cudaStream_t s);
+void attention_release_scratch(cudaStream_t s);
 bool stream_reserve_scratch(cudaStream_t s, cudaStream_t like);      // the workspaces of `s`, with room for what `like` has had room for
 bool umma_reserve_scratch(cudaStream_t s, cudaStream_t like);
 }  // namespace b200gguf
@@ -923,6 +924,7 @@ int dino_session_create(DinoModule* module, DinoSession** out) {
 static void release_workspaces(cudaStream_t stream) {
   b200gguf::stream_release_scratch(stream);
   b200gguf::umma_release_scratch(stream);
+  b200gguf::attention_release_scratch(stream);
 }
 
 // All captured graphs, and the side streams that no later run of this session uses without asking for them again: those of every

@@ -395,6 +395,11 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, residu
     return out, total
 
 
+def release_stream(stream) -> None:
+    """Gives back the workspaces that the library keeps for a stream (of the attention and of the linears), before the stream is destroyed.  Waits for the stream."""
+    _native.check(_native.lib().dinoml_b200_release_stream(_stream_ptr(stream)), "dinoml_b200_release_stream")
+
+
 def device_status() -> int:
     """Synchronizes and returns the status word written by bounded device-side waits (0 = none gave up; 16: one of the attention over the cache) and by the checks of
     what only the device sees (10: a block table, lengths, starts or begins pointed outside of the cache or of the rows).  Read once: it is 0 after that."""

@@ -77,6 +77,10 @@ DINOML_B200_API int dinoml_b200_kv_cache_attention(const DinoB200KvCache* cache,
 DINOML_B200_API int dinoml_b200_rms_norm(const void* x, const void* residual, const void* weight, void* y, void* total, int dtype, int weight_dtype, int rows,
                                          int width, float eps, int q8_0, void* stream);
 
+/* The workspaces that the library keeps for a stream of the caller's (those of the attention and of the linears) are emptied and wait for another stream, or are
+ * freed.  Waits for the stream; call it before the stream is destroyed, and after the graphs with linears that were captured on it.  Workspaces of streams that are not released live as long as the process. */
+DINOML_B200_API int dinoml_b200_release_stream(void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -136,6 +136,14 @@ int main() {
   capturing.clear();
   destroy(one);
   destroy(three);
+  // A stream that is released leaves its set, empty, to the next one.
+  const Got own = get(all, stream(5));
+  own.counters[2] = 1;
+  all.release(stream(5));
+  const Got next = get(all, stream(6));
+  assert(next.counters == own.counters && next.room == own.room);
+  all.release(stream(6));
+  all.release(stream(6));                                                                // (nothing left)
   // A bounded number is kept.
   std::vector<Graph> many(20);
   for (int i = 0; i < 20; ++i) {
@@ -144,7 +152,7 @@ int main() {
   }
   for (Graph& g : many) destroy(g);
   all.reset(0);
-  assert(live.size() <= 2 + 4 * 3);                                                      // the stream's, and four sets of up to three
+  assert(live.size() <= 2 + 2 + 4 * 3);                                                  // a stream's, a spare one, and four sets of up to three
   std::puts("ok");
 }
 """

@@ -1,5 +1,7 @@
 """Attention over the 8-bit cache in captured graphs and on several streams: calls that overlap on the GPU have workspaces of their own, so every result is, bit for bit, that of
 the call alone.  Sequences are long enough that several CTAs share an item and meet in the workspace."""
+from ctypes import addressof, c_void_p
+
 import pytest
 import torch
 
@@ -124,6 +126,24 @@ def test_graphs_that_are_gone_give_their_memory_back():
         del graph
         if i % 8 == 7:
             torch.cuda.synchronize()
+            free.append(torch.cuda.mem_get_info()[0])
+    assert free[0] - free[-1] < 32 << 20, free               # a set of this call is 39 MB
+    assert kernels.device_status() == 0
+
+
+def test_streams_that_are_released_give_their_memory_back():
+    call = _Call(2, [5000], [700])
+    free = []
+    for i in range(24):
+        handle = c_void_p()
+        assert int(torch.cuda.cudart().cudaStreamCreate(addressof(handle))) == 0
+        stream = torch.cuda.ExternalStream(handle.value)
+        for _ in range(2):
+            call.run(stream)
+        kernels.release_stream(stream)
+        call.check()
+        assert int(torch.cuda.cudart().cudaStreamDestroy(handle.value)) == 0
+        if i % 8 == 7:
             free.append(torch.cuda.mem_get_info()[0])
     assert free[0] - free[-1] < 32 << 20, free               # a set of this call is 39 MB
     assert kernels.device_status() == 0
