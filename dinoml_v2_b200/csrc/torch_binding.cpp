@@ -190,6 +190,9 @@ PyObject* py_dequantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 // ---- the operators between the linears.  A cache is a tuple of four tensors; the checks are those of kernels.py.
+// A launch goes to the current device.
+bool on_current_device(const at::Tensor& t) { return t.device().index() == c10::cuda::current_device(); }
+
 bool kv_cache_of(PyObject* o, DinoB200KvCache* out, const at::Tensor** first) {
   if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return false;
   const at::Tensor* t[4];
@@ -197,6 +200,7 @@ bool kv_cache_of(PyObject* o, DinoB200KvCache* out, const at::Tensor** first) {
     t[i] = cuda_tensor(PyTuple_GET_ITEM(o, i));
     if (t[i] == nullptr || t[i]->device() != t[0]->device()) return false;
   }
+  if (!on_current_device(*t[0])) return false;
   const at::ScalarType type = t[0]->scalar_type();
   if ((type != at::kChar && type != at::kFloat8_e4m3fn) || t[1]->scalar_type() != type || t[0]->dim() != 4 || t[1]->sizes() != t[0]->sizes()) return false;
   for (int i = 2; i < 4; ++i)
@@ -347,7 +351,7 @@ PyObject* py_rms_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (x == nullptr || weight == nullptr || !PyFloat_CheckExact(args[2]) || !PyBool_Check(args[4]) || !stream_of(args[5], &stream)) Py_RETURN_NONE;
     const int dtype = dino_dtype(x->scalar_type()), weight_dtype = dino_dtype(weight->scalar_type());
     const bool q8_0 = args[4] == Py_True;
-    if (dtype == 0 || x->dim() < 1 || x->size(-1) < 1 || (weight_dtype != dtype && weight_dtype != DINO_DTYPE_FLOAT32)) Py_RETURN_NONE;
+    if (!on_current_device(*x) || dtype == 0 || x->dim() < 1 || x->size(-1) < 1 || (weight_dtype != dtype && weight_dtype != DINO_DTYPE_FLOAT32)) Py_RETURN_NONE;
     const int64_t width = x->size(-1), rows = x->numel() / width;
     if (rows < 1 || rows > INT_MAX || width > INT_MAX || weight->dim() != 1 || weight->size(0) != width || weight->device() != x->device() || (q8_0 && width % 32)) Py_RETURN_NONE;
     if (args[3] != Py_None) {

@@ -26,6 +26,12 @@ def _require_cuda(t: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name} must be contiguous")
 
 
+def _require_current_device(t: torch.Tensor, name: str) -> None:
+    """A launch goes to the current device, whose kernels would take another device's addresses for their own."""
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
 _binding = None
 
 
@@ -214,6 +220,7 @@ def _kv_struct(cache) -> _native.KvCache:
         _require_cuda(t, name)
         if t.device != k.device:
             raise ValueError("the tensors of a cache must be on one device")
+    _require_current_device(k, "the cache")
     if k.dtype not in _KV_TYPE or k.dim() != 4 or v.dtype != k.dtype or v.shape != k.shape:
         raise ValueError("cache.k and cache.v must be int8 or float8_e4m3fn [blocks, kv_heads, block_size, head_dim] of one shape")
     if k.shape[2] not in _KV_BLOCK_SIZES or k.shape[3] not in _KV_HEAD_DIMS or k.shape[0] < 1 or k.shape[1] < 1:
@@ -359,6 +366,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, residu
             _native.check(done, "dinoml_b200_rms_norm")
         return done
     _require_cuda(x, "x")
+    _require_current_device(x, "x")
     _require_cuda(weight, "weight")
     if x.dtype not in _DTYPE_NAME or x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"x must be [..., width] in {sorted(_TORCH_DTYPE)}")

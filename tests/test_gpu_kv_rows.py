@@ -76,3 +76,15 @@ def test_positions_before_the_first_token():
     want, _ = kernels.kv_cache_read(cache, table, _ints([0, 3, 6]), 6, "float32")
     assert kernels.device_status() == 0
     assert not k[:2].any() and not v[:2].any() and torch.equal(k[2:], want)
+
+
+def test_tensors_of_another_device_are_refused(monkeypatch):
+    """(The current device stands in for the other one; the native path leaves such calls to the checks in Python.)"""
+    cache, table = _cache(64)
+    q = torch.ones(2, 2, 64, device=DEV, dtype=torch.float16)
+    monkeypatch.setattr(kernels, "_native_call", lambda name: lambda *args: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    for call, args in ((kernels.kv_cache_attention, (q, cache, table, _ints([3, 3]))), (kernels.kv_cache_write, (cache, q, q, table, _ints([3, 3]))),
+                       (kernels.kv_cache_read, (cache, table, None, 2)), (kernels.rms_norm, (q, torch.ones(64, device=DEV)))):
+        with pytest.raises(ValueError, match="current device"):
+            call(*args)
