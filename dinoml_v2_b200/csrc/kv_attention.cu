@@ -11,9 +11,9 @@ static AttnWorkspaces& workspaces() {
   return *all;
 }
 // Rows (tokens x heads of a cached head) of a sequence up to which the kernel of few rows takes it: it reads the cache once for 16 rows, the other one once for
-// 256, at a lower rate.  Measured (few, many; 8 cached heads of 128, int8): 64 sequences of 4000 tokens, 32 rows 310 and 358 us, 64 rows 574 and 354;
-// 16 of 2000, 20 rows 59 and 64, 36 rows 79 and 66; heads of 256: 64 of 2000, 16 rows 276 and 220, 20 rows 490 and 223 (up to one reading of the cache the kernel
-// of few rows is kept: its weights have no smallest one); float32: 64 of 2000, 16 rows 126 and 190, 32 rows 213 and 201.
+// 256, at a lower rate.  Measured (few, many; 64 sequences, 8 cached heads, int8): heads of 128, 4000 tokens, 16 rows 173 and 372 us, 32 rows 301 and 373, 36 rows 425 and 374,
+// 64 rows 557 and 378; of 64, 2000 tokens, 32 rows 128 and 184, 48 rows 175 and 184, 64 rows 222 and 184; of 256, 2000 tokens, 16 rows 231 and 226, 20 rows 321 and 230 (where
+// both take the same the kernel of few rows is kept: its weights have no smallest one); float32, heads of 128, 2000 tokens, 16 rows 129 and 193, 32 rows 216 and 204.
 static int few_rows(int dim) { return dim == 256 ? 16 : 32; }
 
 float* attention_scratch(size_t floats, int ctas, cudaStream_t s, int** arrived) {
@@ -55,7 +55,10 @@ int cache_attention(const DinoB200KvCache* cache, const DinoB200KvBatch* batch, 
   const int64_t most = a.p.starts == nullptr ? a.group : all_rows;          // rows of a sequence
   a.min_rows = 0;
   a.max_rows = tensor ? few_rows(a.c.dim) : INT32_MAX;
-  const int tiles = rows <= 8 ? 1 : 2;
+  // One tile of eight rows or two (one reading of the cache for 9 to 16 rows), by the mean rows of a sequence.  Measured (one, two; 32 sequences of 4000 tokens, 8 cached
+  // heads, int8, single tokens): heads of 64, 8 rows 46 and 59 us, 12 rows 81 and 60; of 128, 8 rows 61 and 83, 12 rows 103 and 86, float32 12 rows 132 and 104.
+  // Heads of 256 have no second tile: its sums leave a quarter of an SM two warps, 8 rows 113 and 239, 16 rows 202 and 251, float32 251 and 325.
+  const int tiles = rows <= 8 || a.c.dim == 256 ? 1 : 2;
   if (a.p.starts != nullptr || most <= a.max_rows) {
     const int rc = cache->type == DINOML_B200_KV_INT8 ? attention_few_int8(a, tiles, s) : attention_few_e4m3(a, tiles, s);
     if (rc != RC_OK || most <= a.max_rows) return rc;

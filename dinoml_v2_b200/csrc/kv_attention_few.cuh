@@ -36,9 +36,10 @@ template <int D_, int NT_, int PARTS_> struct Shape {
   static constexpr int TK = D == 256 ? 16 : 32;                           // tokens of a warp's half of a tile
   static constexpr int kTile = 2 * TK, kLog2 = D == 256 ? 5 : 6;
   static constexpr int MT = TK / 16, KS = D / 16, DC = D / 16;             // 16-token rows, 16-value steps, 16-channel rows
-  // Warps that compute, by the registers of their sums (D NT / 4): with the two others and two CTAs per SM a quarter of an SM has four, three or two
-  // warps, of 128, 168 or 255 registers.
-  static constexpr int W = D * NT <= 128 ? 6 : D * NT <= 256 ? 4 : 2;
+  // Warps that compute, by the registers of their sums (D NT / 4): with the two others and two CTAs per SM a quarter of an SM has four or three
+  // warps, of 128 or 168 registers.
+  static constexpr int W = D * NT <= 128 ? 6 : 4;
+  static_assert(D * NT <= 256);
   static constexpr int kThreads = (W + 2) * 32;
   static constexpr int kRow = D == 64 ? 64 : 128;                          // bytes of a row; heads of 256 are two such halves, one after the other
   static constexpr int kHalf = kTile * D;                                  // bytes of a tile's K, and of its V
@@ -837,12 +838,12 @@ template <int TYPE, int D, int NT, int PARTS> int launch(AttnParams& a, cudaStre
   return cudaLaunchKernelEx(&cfg, kern, a, k_map, v_map) == cudaSuccess ? RC_OK : RC_LAUNCH;
 }
 
-// `tiles` of eight rows: 1 or 2.
+// `tiles` of eight rows: 1 or 2 (heads of 256: 1).
 template <int TYPE, int PARTS> int launch_rows(AttnParams& a, int tiles, cudaStream_t s) {
   switch (a.c.dim) {
     case 64: return tiles == 1 ? launch<TYPE, 64, 1, PARTS>(a, s) : launch<TYPE, 64, 2, PARTS>(a, s);
     case 128: return tiles == 1 ? launch<TYPE, 128, 1, PARTS>(a, s) : launch<TYPE, 128, 2, PARTS>(a, s);
-    default: return tiles == 1 ? launch<TYPE, 256, 1, PARTS>(a, s) : launch<TYPE, 256, 2, PARTS>(a, s);
+    default: return launch<TYPE, 256, 1, PARTS>(a, s);
   }
 }
 template <int TYPE> int launch_shape(AttnParams& a, int tiles, cudaStream_t s) {
