@@ -1,4 +1,5 @@
 // Write and read of the 8-bit cache of keys and values (layout: kv_cache.cuh).
+#include <algorithm>
 #include <mutex>
 #include <type_traits>
 
@@ -69,9 +70,9 @@ __device__ __forceinline__ void wait_for_launch_before() {
 
 // ---- write ------------------------------------------------------------------------------------------------------------------
 // A unit is the new tokens of one sequence in one block, for one head of K or of V: the only writer of that block and head, so the scale and the
-// tokens that are there already need no atomics.  NT threads work on a unit: a warp where a call brings a token or two, a CTA where it brings
-// whole blocks.  A thread keeps the first kHeld pieces of 16 bytes that it has between the maximum and the rounding and reads the others again.  64 single
-// tokens of 8 heads of 128 and the read behind them: 9.3 us (tokens brought to a new scale four bytes at a time: 11.5); 12006 tokens in six prompts: 12 us alone.
+// tokens that are there already need no atomics.  NT threads work on a unit, a warp or a CTA (cache_write).  A thread keeps the first kHeld pieces of 16 bytes that
+// it has between the maximum and the rounding and reads the others again.  8 heads of 128, launches one after the other: 64 single tokens 3.6 us, 2671 tokens in five prompts 8.0,
+// 12006 in six 24.9 (74 MB, 3.0 TB/s).
 constexpr int kHeld = 4;
 struct Source {
   const void* x[2];
@@ -206,7 +207,14 @@ int cache_write(const DinoB200KvCache* cache, const DinoB200KvBatch* batch, cons
     const Source src{{k, v}, {k_row_stride, v_row_stride}, {k_head_stride, v_head_stride}, (every & 15) == 0};
     const int64_t pieces = p.starts == nullptr ? p.rows : int64_t(p.rows >> c.block_log2) + 2 * int64_t(p.sequences);
     const int64_t units = 2 * pieces * c.heads;
-    const bool few = p.rows < 8 * int64_t(p.sequences);
+    // A CTA is done with a unit sooner, a warp has 4 to 8 times as many of them under way.  So a unit is a warp's where there are more of them than one for every SM and two
+    // thirds of one more for every 128 values of a head that a unit brings.  Measured (a warp, a CTA; 8 heads of 128, bfloat16, blocks of 16): 1 sequence of 64 new tokens
+    // 8.1 and 3.5 us, 16 of 4 4.1 and 5.7, 64 of 1 3.6 and 6.8, 64 of 8 6.5 and 11.1, 128 of 16 12.8 and 28.6; blocks of 128, 64 new tokens: 16 sequences 29.1 and 6.9,
+    // 128 42.6 and 34.1.  Over 120 sizes, head sizes and types the rule's choice takes up to 1.06 times the better one.
+    const int sms = stream::sm_count();
+    if (sms <= 0) return RC_LAUNCH;
+    const int64_t tokens = std::min((int64_t(p.rows) + p.sequences - 1) / p.sequences, int64_t(1) << c.block_log2);
+    const bool few = 3 * units > sms * (3 + 2 * tokens * c.dim / 128);
     const int64_t ctas = few ? (units + 7) / 8 : units;
     if (pieces > INT32_MAX || ctas > INT32_MAX) return RC_RANGE;
     auto launch = [&](auto kern) { return start(kern, unsigned(ctas), s, c, p, src, int(pieces)); };
@@ -216,7 +224,7 @@ int cache_write(const DinoB200KvCache* cache, const DinoB200KvBatch* batch, cons
 }
 
 // ---- read -------------------------------------------------------------------------------------------------------------------
-// A warp has one row of K and V: 512 bytes of the result at a time, kReadAhead of them under way.  131072 tokens of 8 heads of 128, int8 to bfloat16: 80.6 us,
+// A warp has one row of K and V: 512 bytes of the result at a time, kReadAhead of them under way.  82062 tokens of 8 heads of 128 (four contexts), int8 to bfloat16: 80.6 us,
 // 6.26 TB/s (a CTA for eight rows with one piece of 16 bytes a thread under way: 98.7).
 constexpr int kReadWarps = 8, kReadAhead = 4;
 
