@@ -17,7 +17,6 @@ VARIANT_NAMES = {v: k for k, v in VARIANTS.items()}
 DINO_DTYPE = {"float16": 1, "float32": 2, "bfloat16": 6}
 ACTIVATIONS = {"silu": 1, "fast_gelu": 2}
 DEQUANT_DTYPE = {"float32": 0, "float16": 1, "bfloat16": 2}
-KV_TYPE = {"int8": 1, "float8_e4m3fn": 2}
 
 _lib = None
 _binding = None
