@@ -55,10 +55,13 @@ int cache_attention(const DinoB200KvCache* cache, const DinoB200KvBatch* batch, 
   const int64_t most = a.p.starts == nullptr ? a.group : all_rows;          // rows of a sequence
   a.min_rows = 0;
   a.max_rows = tensor ? few_rows(a.c.dim) : INT32_MAX;
-  // One tile of eight rows or two (one reading of the cache for 9 to 16 rows), by the mean rows of a sequence.  Measured (one, two; 32 sequences of 4000 tokens, 8 cached
+  // One tile of eight rows or two (one reading of the cache for 9 to 16 rows), by the mean rows of a sequence, or of a single token where the mean says that there are
+  // prompts, beside which single tokens are what is most common.  Measured (one, two; 32 sequences of 4000 tokens, 8 cached
   // heads, int8, single tokens): heads of 64, 8 rows 46 and 59 us, 12 rows 81 and 60; of 128, 8 rows 61 and 83, 12 rows 103 and 86, float32 12 rows 132 and 104.
   // Heads of 256 have no second tile: its sums leave a quarter of an SM two warps, 8 rows 113 and 239, 16 rows 202 and 251, float32 251 and 325.
-  const int tiles = rows <= 8 || a.c.dim == 256 ? 1 : 2;
+  // 64 single tokens of 4 rows and a prompt of 512: 137 and 160 us; 32 chunks of 3 tokens and a prompt of 512 (where this rule is wrong) 178 and 160.
+  const int64_t usual = rows > few_rows(a.c.dim) ? a.group : rows;
+  const int tiles = usual <= 8 || a.c.dim == 256 ? 1 : 2;
   if (a.p.starts != nullptr || most <= a.max_rows) {
     const int rc = cache->type == DINOML_B200_KV_INT8 ? attention_few_int8(a, tiles, s) : attention_few_e4m3(a, tiles, s);
     if (rc != RC_OK || most <= a.max_rows) return rc;
