@@ -26,8 +26,8 @@ namespace kv {
 namespace few {
 
 constexpr int kCtasPerSm = 2, kSegments = 4;
-// What an item costs beside its tiles (q, the join of its pieces), in tiles.  64 ragged sequences: 108.5 us with 0, 99.4 with 2, 96.2 with 6, 98.4 with 11;
-// four of 131072 tokens: 95.6, 86.3, 78.6, 78.8.
+// What an item costs beside its tiles (q, the join of its pieces), in tiles.  64 ragged sequences of up to 8192 tokens: 108.5 us with 0, 99.4 with 2, 96.2 with 6,
+// 98.4 with 11; three of 131072, 35361 and 26873 tokens: 95.6, 86.3, 78.6, 78.8.
 constexpr int kEnds = 6;
 
 template <int D_, int NT_, int PARTS_> struct Shape {

@@ -11,10 +11,12 @@
 // 8-bit values are exact in float16, q is brought to [2^12, 2^13) by a power of two per row, so products and their float32 sums are those of the stored
 // values.  The scale of a block's K multiplies the scores; that of its V goes into the exponent: with y = s + log2(vs), P = 2^(y - ref + 7) is
 // what V is multiplied by, and the softmax's sum takes P / vs in float32.  ref is the row's largest y when it was last set; O is rescaled only when y
-// outgrows it by 2^8, so that P stays below 2^15 and loses bits (as a float16 denormal) only below 2^-21 of that.
+// outgrows it by 2^8, so that P stays below 2^15 and loses bits (as a float16 denormal) only below 2^-21 of that: a channel in which all larger weights meet zeros is what
+// shows it.  (Twelve binades above ref and three of growth would keep weights down to 2^-26; 2048 tokens after 6144 took 329 us so instead of 310 on one GPU, chunks of up to 300
+// tokens 106 instead of 94, since O is rescaled more often.)  A scale of V below 2^-100 counts as 2^-100, so that its logarithm leaves the exponent room: values are then 4e-28 off at most.
 //
-// Measured, 2048 tokens after 6144, 32 heads on 8 cached ones: heads of 128 286 us (840 TFLOP/s), of 256 556 us (866), of 64 240 us (500), float32 of 128 485 us. A tile of
-// 64 tokens takes 2015 cycles: MMAs 1415 of them (scores 940, 64 columns being bound by shared memory; P V 516), the softmax warps 1100 and the wait for scores.
+// Measured, int8, blocks of 64, 2048 tokens after 6144, 32 heads on 8 cached ones, launches one after the other on three sets of inputs: heads of 128 292 us (822 TFLOP/s), of 256
+// 577 to 591 us (820), of 64 240 us (501), float32 of 128 512 to 530 us, of 64 393 us.  A tile of 64 tokens takes 2015 cycles: MMAs 1415 of them (scores 940, 64 columns being bound by shared memory; P V 516), the softmax warps 1100 and the wait for scores.
 #pragma once
 #include <type_traits>
 

@@ -5,7 +5,8 @@
 // of squares and the products, so each is read once; rows that registers do not hold are read a second time (from L2).  NT threads of V values, R rounds: as few threads
 // as hold a row in 16 bytes each, since a CTA of few warps starts and meets sooner (a row of 4096: 6.2 us with 1024 threads of 4 values, 5.7 so, both with the call from Python).
 // 2048 rows of 8192 float16 with residual to Q8_0, and decoded again: 67.6 us with a CTA a row and 1024 threads, 47.4 with 512, 39.4 with the next row copied ahead, 37.2 with one
-// reciprocal a block instead of divisions.
+// reciprocal a block instead of divisions.  The norm alone, launches one after the other: 30.0 us of these (119 MB, 3.9 TB/s); bfloat16 to bfloat16 with residual 23.1 us (134 MB, 5.8 TB/s),
+// 2048 rows of 4096 13.4 us, 8192 of 4096 48.5 us (5.5 TB/s), 2048 of 8192 float32 61.1 us (4.4 TB/s).
 #include <algorithm>
 
 #include "kv_cache.cuh"

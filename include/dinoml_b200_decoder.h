@@ -22,7 +22,8 @@ extern "C" {
 enum DinoB200KvType { DINOML_B200_KV_INT8 = 1, DINOML_B200_KV_E4M3 = 2 };
 
 /* A cache: `blocks` blocks of `block_size` tokens.  k, v: uint8[blocks][kv_heads][block_size][head_dim] (int8 or float8 e4m3), 16-byte
- * aligned; k_scale, v_scale: float[blocks][kv_heads].  A stored value stands for q * scale.  block_size is 16, 32, 64 or 128, head_dim 64, 128
+ * aligned; k_scale, v_scale: float[blocks][kv_heads].  A stored value stands for q * scale.  e4m3's codes for NaN are no values (a write gives none): a key
+ * with one makes the rows that see it NaN, a value may do so to its channel of rows of the call that do not.  block_size is 16, 32, 64 or 128, head_dim 64, 128
  * or 256. */
 typedef struct DinoB200KvCache {
   void* k;
