@@ -34,6 +34,24 @@ class KvBatch(ctypes.Structure):
                 ("starts", ctypes.c_void_p), ("sequences", ctypes.c_int), ("rows", ctypes.c_int)]
 
 
+class Heads(ctypes.Structure):
+    """DinoB200Heads (include/dinoml_b200_decoder.h)."""
+    _fields_ = [("x", ctypes.c_void_p), ("out", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("out_row_stride", ctypes.c_int64), ("out_head_stride", ctypes.c_int64), ("heads", ctypes.c_int)]
+
+
+class KvPool(ctypes.Structure):
+    """DinoB200KvPool (include/dinoml_b200_decoder.h)."""
+    _fields_ = [("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("lengths", ctypes.c_void_p), ("free_blocks", ctypes.c_void_p),
+                ("free_count", ctypes.c_void_p), ("table_blocks", ctypes.c_int), ("sequences", ctypes.c_int), ("blocks", ctypes.c_int), ("block_size", ctypes.c_int)]
+
+
+class SampleSettings(ctypes.Structure):
+    """DinoB200SampleSettings (include/dinoml_b200_decoder.h)."""
+    _fields_ = [("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p), ("top_p", ctypes.c_void_p), ("min_p", ctypes.c_void_p),
+                ("temperature_all", ctypes.c_float), ("top_k_all", ctypes.c_int), ("top_p_all", ctypes.c_float), ("min_p_all", ctypes.c_float)]
+
+
 def variant_code(variant) -> int:
     """"mma", "stream", ... or "stream:3" (family : tuning configuration) or an int code -> the C ABI's variant code."""
     if isinstance(variant, int):
@@ -102,6 +120,15 @@ def lib() -> ctypes.CDLL:
     L.dinoml_b200_kv_cache_attention.restype = ci
     L.dinoml_b200_rms_norm.argtypes = [vp, vp, vp, vp, vp, ci, ci, ci, ci, cf, ci, vp]
     L.dinoml_b200_rms_norm.restype = ci
+    L.dinoml_b200_embedding.argtypes = [vp, ci, vp, i64, vp, ci, ci, i64, i64, cf, vp]
+    L.dinoml_b200_embedding.restype = ci
+    heads = ctypes.POINTER(Heads)
+    L.dinoml_b200_rotary.argtypes = [heads, heads, vp, vp, ci, ci, ci, ci, ci, cf, cf, ci, vp]
+    L.dinoml_b200_rotary.restype = ci
+    L.dinoml_b200_kv_pool_step.argtypes = [ctypes.POINTER(KvPool), vp, vp, ci, vp, vp, vp, vp, vp]
+    L.dinoml_b200_kv_pool_step.restype = ci
+    L.dinoml_b200_sample.argtypes = [vp, i64, ci, ci, ci, vp, ctypes.POINTER(SampleSettings), vp, vp, vp]
+    L.dinoml_b200_sample.restype = ci
     L.dinoml_b200_release_stream.argtypes = [vp]
     L.dinoml_b200_release_stream.restype = ci
     _lib = L

@@ -1,9 +1,8 @@
 // extern "C" surface of the operators between the quantized linears (include/dinoml_b200_decoder.h).
 #include "../../include/dinoml_b200_decoder.h"
-#include "gguf_common.cuh"
+#include "decoder_entry.h"
 
 namespace b200gguf {
-int set_error(int rc, const char* where);
 void stream_release_scratch(cudaStream_t s);
 void umma_release_scratch(cudaStream_t s);
 void attention_release_scratch(cudaStream_t s);
@@ -21,19 +20,6 @@ int rms_norm(const void* x, const void* residual, const void* weight, void* y, v
 }  // namespace b200gguf
 
 using namespace b200gguf;
-
-// The workspaces' bookkeeping and the messages allocate on the host: no exception leaves an entry.
-template <typename F> static int entry(const char* where, F f) noexcept {
-  try {
-    return set_error(f(), where);
-  } catch (...) {
-  }
-  try {
-    return set_error(RC_LAUNCH, where);
-  } catch (...) {
-    return RC_LAUNCH;
-  }
-}
 
 extern "C" {
 

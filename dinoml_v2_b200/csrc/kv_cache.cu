@@ -10,7 +10,7 @@ namespace kv {
 
 static __device__ int g_kv_status[kStatusWords];
 
-static int* status_ptr() {
+int* status_words() {
   static int* ptr[kGemvMaxDevices] = {};
   static std::mutex mu;
   int dev = -1;
@@ -41,7 +41,7 @@ int batch_view(const DinoB200KvBatch* b, bool needs_lengths, Batch* out) {
   if (b->sequences <= 0 || b->rows <= 0 || b->table_blocks <= 0) return RC_DIMS;
   if (b->table_stride < b->table_blocks && b->sequences > 1) return RC_RANGE;
   if (b->starts == nullptr && b->rows != b->sequences) return RC_RANGE;
-  int* status = status_ptr();
+  int* status = status_words();
   if (status == nullptr) return RC_LAUNCH;
   *out = {b->block_table, b->lengths, b->starts, b->table_stride, b->table_blocks, b->sequences, b->rows, status};
   return RC_OK;
@@ -301,6 +301,6 @@ int cache_read(const DinoB200KvCache* cache, const DinoB200KvBatch* batch, const
 }  // namespace kv
 
 // Status of the cache's kernels on the current device (read once).
-int kv_device_status() { return kv::take_status(kv::status_ptr(), kv::attention_reset); }
+int kv_device_status() { return kv::take_status(kv::status_words(), kv::attention_reset); }
 
 }  // namespace b200gguf

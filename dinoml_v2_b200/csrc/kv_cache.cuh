@@ -27,6 +27,8 @@ struct Batch {
 // Host: checks and the device's view of the two structs; a return code.
 int cache_view(const DinoB200KvCache* cache, Cache* out);
 int batch_view(const DinoB200KvBatch* batch, bool needs_lengths, Batch* out);
+// The status words of the current device (null: there is none).
+int* status_words();
 
 #ifdef __CUDACC__
 // A plain read.  (A read as of constant data may be moved ahead of a kernel's wait for the launch before it.)

@@ -1,0 +1,741 @@
+// The next token of every row of logits from one given random number: temperature, top-k, top-p, min-p (include/dinoml_b200_decoder.h has the definition).
+//
+// Every filter keeps a beginning of one order - by value, the lowest index first among equals - and the choice is where the running sum of the weights in that order passes u times
+// the sum of the kept.  So a row is never sorted: what is wanted is a few places of the order, each found from sums over ranges of values.
+//
+// 16-bit logits have 65536 values, so that how often each is there says everything but the indices: a row is read once, into counts (a CTA's part of the row into 128 KB of its
+// shared memory, two 16-bit counts a word).  The weight of a value is computed once, in float64, and only where its count is not zero: a row of 128256 has some thousand different
+// values.  Sums over groups of 32 values, their running sums, and then each place by one warp: the group, the value in it, how many of its equals.  At the end the part of the row
+// that has the chosen one among its equals is searched for it.
+// float32 logits: ranges of values instead of values.  2048 ranges of equal width in (largest - x) / temperature, whose counts and sums of weights (whole numbers of 2^-45, so
+// that atomics in any order give the same) all CTAs add up; each place is then narrowed down by the bits of the values in its range until one value is left.
+//
+// A row is a cluster's: its CTAs have parts of it, the first one finds the places.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "dependent_launch.cuh"
+#include "kv_cache.cuh"
+
+namespace b200gguf {
+namespace stream { int sm_count(); }             // gemv_stream.cu
+namespace choice {
+namespace cg = cooperative_groups;
+
+constexpr int kThreads = 1024, kWarps = kThreads / 32, kGroups = 2048, kMaxVocabulary = 262144;
+constexpr int kPart16 = 65528;                   // of a row: counts of 16 bits, whole vectors
+constexpr int kPart32 = 32768;
+constexpr double kOne = 35184372088832.;         // 2^45
+
+struct Args {
+  const void* logits;
+  int64_t row_stride;
+  int vocabulary;
+  const float* uniforms;
+  DinoB200SampleSettings set;
+  int* tokens;
+  float* probabilities;
+  int* status;
+};
+
+struct Row {
+  float temperature, top_p, min_p, u;
+  int top_k;
+  bool valid, first;                             // settings are numbers; the first of the order is the answer
+};
+__device__ __forceinline__ Row row_of(const Args& a, int64_t row) {
+  Row r;
+  r.temperature = a.set.temperature != nullptr ? a.set.temperature[row] : a.set.temperature_all;
+  r.top_k = a.set.top_k != nullptr ? a.set.top_k[row] : a.set.top_k_all;
+  r.top_p = a.set.top_p != nullptr ? a.set.top_p[row] : a.set.top_p_all;
+  r.min_p = a.set.min_p != nullptr ? a.set.min_p[row] : a.set.min_p_all;
+  r.u = a.uniforms[row];
+  r.valid = r.temperature >= 0.f && r.top_p == r.top_p && r.min_p == r.min_p && r.u == r.u;
+  r.u = fminf(fmaxf(r.u, 0.f), 0x1.fffffep-1f);
+  r.first = r.temperature == 0.f || r.top_k == 1 || r.top_p <= 0.f || r.min_p > 1.f;
+  return r;
+}
+
+// Order of values as unsigned numbers, the largest value first; NaN before inf and behind -inf.
+template <typename T> struct Code;
+template <> struct Code<__nv_bfloat16> {
+  static constexpr uint32_t kInf = 0x007f, kMinusInf = 0xff80;
+  static __device__ __forceinline__ float value(uint32_t d) { return __uint_as_float(((d & 0x8000u) ? d : d ^ 0x7fffu) << 16); }
+};
+template <> struct Code<__half> {
+  static constexpr uint32_t kInf = 0x03ff, kMinusInf = 0xfc00;
+  static __device__ __forceinline__ float value(uint32_t d) { return __half2float(__ushort_as_half(uint16_t((d & 0x8000u) ? d : d ^ 0x7fffu))); }
+};
+template <> struct Code<float> {
+  static constexpr uint32_t kInf = 0x007fffff, kMinusInf = 0xff800000;
+  static __device__ __forceinline__ float value(uint32_t d) { return __uint_as_float((d & 0x80000000u) ? d : d ^ 0x7fffffffu); }
+  static __device__ __forceinline__ uint32_t of(float x) {
+    const uint32_t b = __float_as_uint(x + 0.f);           // (-0 becomes 0)
+    return (b & 0x80000000u) ? b : b ^ 0x7fffffffu;
+  }
+};
+// Two values at once.
+__device__ __forceinline__ uint32_t codes_of(uint32_t w) {
+  const uint32_t plus = (~w >> 15) & 0x00010001u;
+  uint32_t d = w ^ (plus * 0x7fffu);
+  if ((w & 0xffffu) == 0x8000u) d ^= 0xffffu;              // -0 is 0: 0x8000 -> 0x7fff
+  if ((w >> 16) == 0x8000u) d ^= 0xffff0000u;
+  return d;
+}
+
+template <typename T> struct Weight {
+  uint32_t first;                                // the largest value's code
+  double largest, inverse;
+  bool infinite;
+  __device__ __forceinline__ Weight(uint32_t first, float temperature)
+      : first(first), largest(double(Code<T>::value(first))), inverse(1. / double(temperature)), infinite(first == Code<T>::kInf) {}
+  __device__ __forceinline__ double operator()(uint32_t d) const {
+    return d == first ? 1. : infinite ? 0. : exp((double(Code<T>::value(d)) - largest) * inverse);
+  }
+};
+
+// The last code in [low, high] with holds(code), which holds for low and up to some code: by a converged warp.
+template <typename F> __device__ __forceinline__ uint32_t last_that(uint32_t low, uint32_t high, F holds) {
+  const uint32_t lane = threadIdx.x & 31;
+  uint64_t span = uint64_t(high) - low + 1;
+  while (span > 1) {
+    const uint64_t step = (span + 31) >> 5, at = lane * step;
+    const bool in = at < span && (lane == 0 || holds(uint32_t(low + at)));
+    const int hits = __popc(__ballot_sync(0xffffffffu, in));
+    low += uint32_t((hits - 1) * step);
+    span = min(step, span - (hits - 1) * step);
+  }
+  return low;
+}
+
+// The first of 2048 running sums that passes: by a converged warp; the last one if none does.
+template <typename F> __device__ __forceinline__ int first_of(F passes) {
+  const int lane = threadIdx.x & 31;
+  uint32_t hit = __ballot_sync(0xffffffffu, passes(lane * 64 + 63));
+  if (hit == 0) return kGroups - 1;
+  const int at = (__ffs(hit) - 1) * 64;
+  hit = __ballot_sync(0xffffffffu, passes(at + 2 * lane + 1));
+  const int pair = at + 2 * (__ffs(hit) - 1);
+  return passes(pair) ? pair : pair + 1;
+}
+
+template <typename V> __device__ __forceinline__ V warp_running(V v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+// Running sums of 2048 counts and masses in place, by all threads.
+template <typename M> __device__ __forceinline__ void running_sums(uint32_t* count, M* mass, uint32_t* warp_count, M* warp_mass) {
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const uint32_t c0 = count[2 * t], c1 = c0 + count[2 * t + 1];
+  const M m0 = mass[2 * t], m1 = m0 + mass[2 * t + 1];
+  const uint32_t c = warp_running(c1);
+  const M m = warp_running(m1);
+  if (lane == 31) {
+    warp_count[warp] = c;
+    warp_mass[warp] = m;
+  }
+  __syncthreads();
+  const uint32_t wc = warp_running(warp_count[lane]);
+  const M wm = warp_running(warp_mass[lane]);
+  uint32_t before_c = __shfl_sync(0xffffffffu, wc, (warp + 31) & 31);
+  M before_m = __shfl_sync(0xffffffffu, wm, (warp + 31) & 31);
+  if (warp == 0) {
+    before_c = 0;
+    before_m = M(0);
+  }
+  // (as a difference the own part would lose what a small group adds to a large sum)
+  const uint32_t up_c = __shfl_up_sync(0xffffffffu, c, 1);
+  const M up_m = __shfl_up_sync(0xffffffffu, m, 1);
+  const uint32_t base_c = before_c + (lane > 0 ? up_c : 0u);
+  const M base_m = before_m + (lane > 0 ? up_m : M(0));
+  count[2 * t] = base_c + c0;
+  count[2 * t + 1] = base_c + c1;
+  mass[2 * t] = base_m + m0;
+  mass[2 * t + 1] = base_m + m1;
+  __syncthreads();
+}
+
+__device__ __forceinline__ void answer(const Args& a, int64_t row, int token, float probability) {
+  a.tokens[row] = token;
+  if (a.probabilities != nullptr) a.probabilities[row] = probability;
+}
+
+// ---- 16-bit logits ------------------------------------------------------------------------------------------------------------------------------------
+struct Decision {
+  int owner, place;
+  uint32_t code;
+};
+struct Shared16 {
+  uint32_t counts[32768];                        // word d & 0x7fff: of code d in its upper half if d >= 0x8000, else in its lower half
+  double mass[kGroups];
+  uint32_t count[kGroups];
+  double warp_mass[kWarps];
+  uint32_t warp_count[kWarps];
+  uint32_t least, most;                          // codes of this part
+  Decision decision;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  Shared16& sh = *reinterpret_cast<Shared16*>(raw);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int ctas = int(cluster.num_blocks()), rank = int(cluster.block_rank());
+  const int64_t row = blockIdx.x / ctas;
+  for (int i = tid; i < 32768 / 4; i += kThreads) reinterpret_cast<uint4*>(sh.counts)[i] = make_uint4(0, 0, 0, 0);
+  if (tid == 0) {
+    sh.least = 0xffffu;
+    sh.most = 0;
+  }
+  wait_for_launch_before();
+  __syncthreads();
+  const Row set = row_of(a, row);
+
+  // This part of the row: values up to an address that is a multiple of 16, vectors of eight, the rest.
+  const int part = ((a.vocabulary + ctas - 1) / ctas + 7) & ~7;
+  const int begin = min(rank * part, a.vocabulary), length = min(part, a.vocabulary - begin);
+  const uint16_t* x = static_cast<const uint16_t*>(a.logits) + row * a.row_stride + begin;
+  const int head = min(int((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / 2, length);
+  const int vectors = (length - head) / 8, rest = length - head - 8 * vectors;
+  const uint4* wide = reinterpret_cast<const uint4*>(x + head);
+  uint32_t least = 0xffffffffu, most = 0;
+  auto add = [&](uint32_t two) {
+    const uint32_t d = codes_of(two);
+    least = __vminu2(least, d);
+    most = __vmaxu2(most, d);
+    atomicAdd(&sh.counts[d & 0x7fffu], (d & 0x8000u) ? 0x10000u : 1u);
+    atomicAdd(&sh.counts[(d >> 16) & 0x7fffu], (d >> 31) ? 0x10000u : 1u);
+  };
+  auto add_one = [&](uint32_t v) {
+    const uint32_t d = codes_of(v) & 0xffffu;
+    least = __vminu2(least, d | d << 16);
+    most = __vmaxu2(most, d | d << 16);
+    atomicAdd(&sh.counts[d & 0x7fffu], (d & 0x8000u) ? 0x10000u : 1u);
+  };
+  constexpr int kAhead = 4;
+  for (int v = tid; v < vectors; v += kAhead * kThreads) {
+    uint4 q[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (v + i * kThreads < vectors) q[i] = kv::fetch(wide + v + i * kThreads);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (v + i * kThreads >= vectors) break;
+      add(q[i].x);
+      add(q[i].y);
+      add(q[i].z);
+      add(q[i].w);
+    }
+  }
+  if (tid < head) add_one(x[tid]);
+  if (tid < rest) add_one(x[head + 8 * vectors + tid]);
+  least = __reduce_min_sync(0xffffffffu, min(least & 0xffffu, least >> 16));
+  most = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
+  if (lane == 0) {
+    atomicMin(&sh.least, least);
+    atomicMax(&sh.most, most);
+  }
+  cluster.sync();
+
+  least = 0xffffu;
+  most = 0;
+  if (lane < ctas) {
+    least = *cluster.map_shared_rank(&sh.least, lane);
+    most = *cluster.map_shared_rank(&sh.most, lane);
+  }
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  const uint32_t first = least;
+  if (!set.valid || first < Code<T>::kInf || most > Code<T>::kMinusInf || first >= Code<T>::kMinusInf) {
+    if (rank == 0 && tid == 0) {
+      if (!set.valid) kv::flag_range(a.status);
+      answer(a, row, -1, 0.f);
+    }
+    cluster.sync();                              // (others may be reading this part's codes)
+    return;
+  }
+  const Weight<T> weight(first, set.temperature);
+  Shared16* lead = cluster.map_shared_rank(&sh, 0);
+  if (!set.first) {
+    // Sums of groups: 32 words are a group of large and one of small values.  Neighbours go to different CTAs and warps, since the values lie close together.
+    for (int g = rank + ctas * warp; g < kGroups / 2; g += ctas * kWarps) {
+      uint32_t low = 0, high = 0;
+      for (int c = 0; c < ctas; ++c) {
+        const uint32_t w = cluster.map_shared_rank(sh.counts, c)[g * 32 + lane];
+        low += w & 0xffffu;
+        high += w >> 16;
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t d = uint32_t(g * 32 + lane) + half * 0x8000u, n = half == 0 ? low : d < Code<T>::kMinusInf ? high : 0u;
+        uint32_t count = 0;
+        double mass = 0.;
+        if (__any_sync(0xffffffffu, n != 0)) {
+          count = __reduce_add_sync(0xffffffffu, n);
+          mass = n != 0 ? double(n) * weight(d) : 0.;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+        }
+        if (lane == 0) {
+          lead->count[g + half * (kGroups / 2)] = count;
+          lead->mass[g + half * (kGroups / 2)] = mass;
+        }
+      }
+    }
+  }
+  cluster.sync();
+  if (rank == 0) {
+    if (!set.first) running_sums(sh.count, sh.mass, sh.warp_count, sh.warp_mass);
+    if (warp == 0) {
+      uint32_t code = first;
+      int place = 0;
+      double share = 1.;
+      if (!set.first) {
+        // One group: how often each of its values is there, its weight, running sums before and with it.
+        uint32_t n, n_with;
+        double w, m_before, m_with;
+        auto open = [&](int g) {
+          const int word = (g & (kGroups / 2 - 1)) * 32 + lane;
+          n = 0;
+          for (int c = 0; c < ctas; ++c) {
+            const uint32_t v = cluster.map_shared_rank(sh.counts, c)[word];
+            n += g < kGroups / 2 ? v & 0xffffu : v >> 16;
+          }
+          const uint32_t d = uint32_t(g * 32 + lane);
+          if (d >= Code<T>::kMinusInf) n = 0;
+          w = n != 0 ? weight(d) : 0.;
+          n_with = (g > 0 ? sh.count[g - 1] : 0u) + warp_running(n);
+          const double own = warp_running(double(n) * w), base = g > 0 ? sh.mass[g - 1] : 0.;
+          const double up = __shfl_up_sync(0xffffffffu, own, 1);
+          m_before = base + (lane > 0 ? up : 0.);
+          m_with = base + own;
+        };
+        auto pick = [&](bool passes) {           // the first lane that passes, or the last that has anything
+          const uint32_t hit = __ballot_sync(0xffffffffu, passes && n != 0), any = __ballot_sync(0xffffffffu, n != 0);
+          return hit != 0 ? __ffs(hit) - 1 : any != 0 ? 31 - __clz(any) : 0;
+        };
+        auto from = [&](auto v, int l) { return __shfl_sync(0xffffffffu, v, l); };
+        uint32_t end = 0xffffu, take = 0xffffffffu;      // kept: what comes before code `end`, and `take` of it
+        double kept = sh.mass[kGroups - 1];              // the sum of the kept
+        if (set.top_k > 0 && uint32_t(set.top_k) < sh.count[kGroups - 1]) {
+          const uint32_t k = uint32_t(set.top_k);
+          const int g = first_of([&](int i) { return sh.count[i] >= k; });
+          open(g);
+          const int l = pick(n_with >= k);
+          end = uint32_t(g * 32 + l);
+          take = k - from(n_with - n, l);
+          kept = from(m_before, l) + double(take) * from(w, l);
+        }
+        if (set.top_p < 1.f) {
+          const double wanted = double(set.top_p) * kept;
+          const int g = first_of([&](int i) { return sh.mass[i] >= wanted; });
+          open(g);
+          const int l = pick(m_with >= wanted);
+          const uint32_t e = uint32_t(g * 32 + l), c = from(n, l);
+          const double we = from(w, l), before = from(m_before, l), some = we > 0. ? ceil((wanted - before) / we) : 1.;
+          const uint32_t t = uint32_t(fmin(fmax(some, 1.), double(c)));
+          if (e < end || (e == end && t < take)) {
+            end = e;
+            take = t;
+            kept = before + double(t) * we;
+          }
+        }
+        if (set.min_p > 0.f) {
+          const uint32_t e = last_that(first, Code<T>::kMinusInf - 1, [&](uint32_t d) { return weight(d) >= double(set.min_p); });
+          if (e < end) {
+            open(int(e >> 5));
+            end = e;
+            take = 0xffffffffu;
+            kept = from(m_with, int(e & 31));
+          }
+        }
+        const double target = double(set.u) * kept;
+        const int g = first_of([&](int i) { return sh.mass[i] > target; });
+        open(g);
+        const int l = pick(m_with > target);
+        code = uint32_t(g * 32 + l);
+        const double wc = from(w, l), there = wc > 0. ? floor((target - from(m_before, l)) / wc) : 0.;
+        uint32_t most_place = from(n, l) - 1;
+        if (code == end && take <= most_place) most_place = take - 1;
+        place = int(fmin(fmax(there, 0.), double(most_place)));
+        share = wc / kept;
+      }
+      // Whose part has it: the equals of the parts before come first.
+      uint32_t mine = 0;
+      if (lane < ctas) {
+        const uint32_t v = cluster.map_shared_rank(sh.counts, lane)[code & 0x7fffu];
+        mine = (code & 0x8000u) ? v >> 16 : v & 0xffffu;
+      }
+      const uint32_t with = warp_running(mine), hit = __ballot_sync(0xffffffffu, int(with) > place);
+      const int owner = __ffs(hit) - 1, before = int(__shfl_sync(0xffffffffu, with - mine, owner & 31));
+      if (lane < ctas) *cluster.map_shared_rank(&sh.decision, lane) = Decision{owner, place - before, code};
+      if (lane == 0 && a.probabilities != nullptr) a.probabilities[row] = float(share);
+    }
+  }
+  cluster.sync();
+  const Decision what = sh.decision;
+  if (what.owner != rank) return;
+
+  // The place-th of its equals in this part.  A warp has a piece of the part; slots are the values before the vectors, the vectors, the rest.
+  const int slots = vectors + 2, each = (slots + kWarps - 1) / kWarps, from_slot = warp * each, to_slot = min(from_slot + each, slots);
+  auto hits_of = [&](int slot) -> uint32_t {     // bit i: value i of the slot is one
+    uint32_t hits = 0;
+    if (slot >= to_slot) return 0;
+    if (slot > 0 && slot <= vectors) {
+      const uint4 q = kv::fetch(wide + slot - 1);
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t d = codes_of(w[i]);
+        if ((d & 0xffffu) == what.code) hits |= 1u << (2 * i);
+        if ((d >> 16) == what.code) hits |= 2u << (2 * i);
+      }
+      return hits;
+    }
+    const int at = slot == 0 ? 0 : head + 8 * vectors, n = slot == 0 ? head : rest;
+    for (int i = 0; i < n; ++i)
+      if ((codes_of(x[at + i]) & 0xffffu) == what.code) hits |= 1u << i;
+    return hits;
+  };
+  uint32_t found = 0;
+  for (int s = from_slot; s < to_slot; s += 32) found += __popc(hits_of(s + lane));
+  found = __reduce_add_sync(0xffffffffu, found);
+  if (lane == 0) sh.warp_count[warp] = found;
+  __syncthreads();
+  const uint32_t with = warp_running(sh.warp_count[lane]);
+  const uint32_t place = uint32_t(what.place);
+  const uint32_t hit = __ballot_sync(0xffffffffu, with > place);
+  if (hit == 0 || __ffs(hit) - 1 != warp) return;
+  uint32_t left = place - (warp > 0 ? __shfl_sync(0xffffffffu, with, warp > 0 ? warp - 1 : 0) : 0u);
+  for (int s = from_slot; s < to_slot; s += 32) {
+    uint32_t hits = hits_of(s + lane);
+    const uint32_t c = __popc(hits), run = warp_running(c), all = __shfl_sync(0xffffffffu, run, 31);
+    if (left < all) {
+      if (run > left && run - c <= left) {
+        for (uint32_t skip = left - (run - c); skip > 0; --skip) hits &= hits - 1;
+        const int slot = s + lane, bit = __ffs(hits) - 1;
+        a.tokens[row] = begin + (slot == 0 ? 0 : head + 8 * (slot - 1)) + bit;
+      }
+      return;
+    }
+    left -= all;
+  }
+}
+
+// ---- float32 logits -----------------------------------------------------------------------------------------------------------------------------------
+struct Place {                                   // a range of codes, what comes before it, what is in it
+  uint32_t low, high;
+  uint32_t count_before, count;
+  unsigned long long mass_before, mass;
+};
+struct Shared32 {
+  uint32_t codes[kPart32];
+  unsigned long long mass[kGroups], range_mass[kGroups];      // sums of the 2048 ranges (the first CTA's: of all, running); of a range that is narrowed down
+  uint32_t count[kGroups], range_count[kGroups];
+  unsigned long long own_mass[kGroups];          // this part's
+  uint32_t own_count[kGroups];
+  unsigned long long warp_mass[kWarps];
+  uint32_t warp_count[kWarps];
+  uint32_t least, most;
+  Place place[2];                                // written in turn: a slow CTA may be reading the one before
+  unsigned long long sum_mass;
+  uint32_t sum_count;
+  uint32_t found[8];
+};
+
+__global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  Shared32& sh = *reinterpret_cast<Shared32*>(raw);
+  using C = Code<float>;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int ctas = int(cluster.num_blocks()), rank = int(cluster.block_rank());
+  const int64_t row = blockIdx.x / ctas;
+  for (int i = tid; i < kGroups; i += kThreads) {
+    sh.own_mass[i] = sh.range_mass[i] = 0;
+    sh.own_count[i] = sh.range_count[i] = 0;
+  }
+  if (tid == 0) {
+    sh.least = 0xffffffffu;
+    sh.most = 0;
+    sh.sum_mass = 0;
+    sh.sum_count = 0;
+  }
+  wait_for_launch_before();
+  __syncthreads();
+  const Row set = row_of(a, row);
+  const int part = (a.vocabulary + ctas - 1) / ctas;
+  const int begin = min(rank * part, a.vocabulary), length = min(part, a.vocabulary - begin);
+  const float* x = static_cast<const float*>(a.logits) + row * a.row_stride + begin;
+  uint32_t least = 0xffffffffu, most = 0;
+#pragma unroll 8
+  for (int i = tid; i < length; i += kThreads) {
+    const uint32_t d = C::of(kv::fetch(x + i));
+    sh.codes[i] = d;
+    least = min(least, d);
+    most = max(most, d);
+  }
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 0) {
+    atomicMin(&sh.least, least);
+    atomicMax(&sh.most, most);
+  }
+  cluster.sync();
+  least = 0xffffffffu;
+  most = 0;
+  if (lane < ctas) {
+    least = *cluster.map_shared_rank(&sh.least, lane);
+    most = *cluster.map_shared_rank(&sh.most, lane);
+  }
+  const uint32_t first = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (!set.valid || first < C::kInf || most > C::kMinusInf || first >= C::kMinusInf) {
+    if (rank == 0 && tid == 0) {
+      if (!set.valid) kv::flag_range(a.status);
+      answer(a, row, -1, 0.f);
+    }
+    cluster.sync();
+    return;
+  }
+  const Weight<float> weight(first, set.temperature);
+  Shared32* lead = cluster.map_shared_rank(&sh, 0);
+  Place found{first, first, 0, 1, 0, 1};
+  double kept = 1.;
+  uint32_t place = 0;
+  if (!set.first) {
+    // Ranges of equal width of (largest - x) / temperature: behind 44 all is one range, whose weights together are less than 2^-45 of the largest one's.
+    const float largest = C::value(first), per = float(kGroups) / 44.f / set.temperature;
+    auto range_of = [&](uint32_t d) -> int {
+      if (d == first) return 0;
+      return int(fminf(fmaxf((largest - C::value(d)) * per, 0.f), float(kGroups - 1)));      // (a NaN, inf - inf or 0 inf, is no number's: 0)
+    };
+    auto fixed = [&](uint32_t d) { return __double2ull_rn(weight(d) * kOne); };
+    for (int i = tid; i < length; i += kThreads) {
+      const uint32_t d = sh.codes[i];
+      if (d == C::kMinusInf) continue;
+      const int r = range_of(d);
+      atomicAdd(&sh.own_count[r], 1u);
+      atomicAdd(&sh.own_mass[r], fixed(d));
+    }
+    cluster.sync();
+    for (int i = rank * kThreads + tid; i < kGroups; i += ctas * kThreads) {
+      uint32_t c = 0;
+      unsigned long long m = 0;
+      for (int r = 0; r < ctas; ++r) {
+        const Shared32* other = cluster.map_shared_rank(&sh, r);
+        c += other->own_count[i];
+        m += other->own_mass[i];
+      }
+      lead->count[i] = c;
+      lead->mass[i] = m;
+    }
+    cluster.sync();
+    if (rank == 0) running_sums(sh.count, sh.mass, sh.warp_count, sh.warp_mass);
+    // The place where the running count reaches `count` (by_count) or the running sum reaches, or with `above` passes, `mass`.
+    int turn = 0;
+    auto descend = [&](bool by_count, uint32_t count, double mass, bool above) -> Place {
+      auto passes = [&](uint32_t c, unsigned long long m) { return by_count ? c >= count : above ? double(m) > mass : double(m) >= mass; };
+      if (rank == 0 && warp == 0) {
+        const int g = first_of([&](int i) { return passes(sh.count[i], sh.mass[i]); });
+        Place p;
+        p.low = g == 0 ? first : last_that(first, C::kMinusInf - 1, [&](uint32_t d) { return range_of(d) < g; }) + 1;
+        p.high = last_that(first, C::kMinusInf - 1, [&](uint32_t d) { return range_of(d) <= g; });
+        p.count_before = g > 0 ? sh.count[g - 1] : 0u;
+        p.mass_before = g > 0 ? sh.mass[g - 1] : 0ull;
+        p.count = sh.count[g] - p.count_before;
+        p.mass = sh.mass[g] - p.mass_before;
+        if (lane < ctas) *cluster.map_shared_rank(&sh.place[turn], lane) = p;
+      }
+      cluster.sync();
+      Place p = sh.place[turn];
+      turn ^= 1;
+      while (p.count > 1 && p.low < p.high && p.mass > 0) {      // (without weight it does not matter which of them)
+        const int shift = max(0, 32 - __clz(int(p.high - p.low)) - 11);
+        for (int i = tid; i < length; i += kThreads) {
+          const uint32_t d = sh.codes[i];
+          if (d < p.low || d > p.high) continue;
+          const uint32_t at = (d - p.low) >> shift;
+          atomicAdd(&lead->range_count[at], 1u);
+          atomicAdd(&lead->range_mass[at], fixed(d));
+        }
+        cluster.sync();
+        if (rank == 0) {
+          running_sums(sh.range_count, sh.range_mass, sh.warp_count, sh.warp_mass);
+          if (warp == 0) {
+            const int g = first_of([&](int i) { return passes(p.count_before + sh.range_count[i], p.mass_before + sh.range_mass[i]); });
+            const uint32_t c = g > 0 ? sh.range_count[g - 1] : 0u;
+            const unsigned long long m = g > 0 ? sh.range_mass[g - 1] : 0ull;
+            Place q;
+            q.low = p.low + (uint32_t(g) << shift);
+            q.high = min(p.high, q.low + ((1u << shift) - 1));
+            q.count_before = p.count_before + c;
+            q.mass_before = p.mass_before + m;
+            q.count = sh.range_count[g] - c;
+            q.mass = sh.range_mass[g] - m;
+            if (lane < ctas) *cluster.map_shared_rank(&sh.place[turn], lane) = q;
+          }
+          __syncthreads();
+          for (int i = tid; i < kGroups; i += kThreads) {
+            sh.range_mass[i] = 0;
+            sh.range_count[i] = 0;
+          }
+        }
+        cluster.sync();
+        p = sh.place[turn];
+        turn ^= 1;
+      }
+      return p;
+    };
+    cluster.sync();                              // (the running sums are there)
+    const uint32_t all_count = lead->count[kGroups - 1];
+    const unsigned long long all_mass = lead->mass[kGroups - 1];
+    uint32_t keep = all_count;                   // how many are kept
+    unsigned long long sum = all_mass;           // their weights
+    if (set.top_k > 0 && uint32_t(set.top_k) < all_count) {
+      const Place p = descend(true, uint32_t(set.top_k), 0., false);
+      keep = uint32_t(set.top_k);
+      sum = p.mass_before + p.mass / max(p.count, 1u) * (keep - p.count_before);
+    }
+    if (set.top_p < 1.f) {
+      const double wanted = double(set.top_p) * double(sum);
+      const Place p = descend(false, 0, wanted, false);
+      const unsigned long long w = p.mass / max(p.count, 1u);
+      const double some = w > 0 ? ceil((wanted - double(p.mass_before)) / double(w)) : 1.;
+      const uint32_t t = uint32_t(fmin(fmax(some, 1.), double(max(p.count, 1u))));
+      if (p.count_before + t < keep) {
+        keep = p.count_before + t;
+        sum = p.mass_before + w * t;
+      }
+    }
+    if (set.min_p > 0.f) {
+      const uint32_t e = last_that(first, C::kMinusInf - 1, [&](uint32_t d) { return weight(d) >= double(set.min_p); });
+      unsigned long long m = 0;
+      uint32_t c = 0;
+      for (int i = tid; i < length; i += kThreads) {
+        const uint32_t d = sh.codes[i];
+        if (d <= e) {
+          ++c;
+          m += fixed(d);
+        }
+      }
+      c = __reduce_add_sync(0xffffffffu, c);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+      if (lane == 0 && c > 0) {
+        atomicAdd(&lead->sum_count, c);
+        atomicAdd(&lead->sum_mass, m);
+      }
+      cluster.sync();
+      c = lead->sum_count;
+      m = lead->sum_mass;
+      if (c < keep) {
+        keep = c;
+        sum = m;
+      }
+    }
+    kept = double(sum);
+    const double target = double(set.u) * kept;
+    found = descend(false, 0, target, true);
+    const unsigned long long w = found.mass / max(found.count, 1u);
+    const double there = w > 0 ? floor((target - double(found.mass_before)) / double(w)) : 0.;
+    uint32_t most_place = max(found.count, 1u) - 1;
+    if (found.count_before + most_place >= keep) most_place = keep > found.count_before ? keep - found.count_before - 1 : 0u;
+    place = uint32_t(fmin(fmax(there, 0.), double(most_place)));
+    if (rank == 0 && tid == 0 && a.probabilities != nullptr) a.probabilities[row] = float(double(w) / kept);
+  } else if (rank == 0 && tid == 0 && a.probabilities != nullptr) {
+    a.probabilities[row] = 1.f;
+  }
+
+  // The place-th of its equals: a warp has a piece of the part.
+  const int each = (length + kWarps - 1) / kWarps, from_i = warp * each, to_i = min(from_i + each, length);
+  auto is_one = [&](int i) { return i < to_i && sh.codes[i] >= found.low && sh.codes[i] <= found.high; };
+  uint32_t hits = 0;
+  for (int i = from_i; i < to_i; i += 32) hits += __popc(__ballot_sync(0xffffffffu, is_one(i + lane)));
+  __syncthreads();
+  if (lane == 0) sh.warp_count[warp] = hits;
+  __syncthreads();
+  const uint32_t with = warp_running(sh.warp_count[lane]), own = __shfl_sync(0xffffffffu, with, 31);
+  if (warp == 0 && lane < ctas) cluster.map_shared_rank(sh.found, lane)[rank] = own;
+  cluster.sync();
+  for (int r = 0; r < rank; ++r) {
+    if (place < sh.found[r]) return;
+    place -= sh.found[r];
+  }
+  const uint32_t hit = __ballot_sync(0xffffffffu, with > place);
+  if (hit == 0 || __ffs(hit) - 1 != warp) return;
+  uint32_t left = place - (warp > 0 ? __shfl_sync(0xffffffffu, with, warp > 0 ? warp - 1 : 0) : 0u);
+  for (int i = from_i; i < to_i; i += 32) {
+    uint32_t here = __ballot_sync(0xffffffffu, is_one(i + lane));
+    const uint32_t c = __popc(here);
+    if (left < c) {
+      for (; left > 0; --left) here &= here - 1;
+      if (lane == 0) a.tokens[row] = begin + i + __ffs(here) - 1;
+      return;
+    }
+    left -= c;
+  }
+}
+
+template <typename K> static int allow(K kernel, size_t shared, std::atomic<uint64_t>& done) {
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return RC_LAUNCH;
+  if ((done.load(std::memory_order_acquire) >> dev & 1) == 0) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)) != cudaSuccess) return RC_LAUNCH;
+    done.fetch_or(uint64_t(1) << dev, std::memory_order_release);
+  }
+  return RC_OK;
+}
+
+template <typename T> static int launch16(const Args& a, int64_t rows, cudaStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  if (int rc = allow(sample16_kernel<T>, sizeof(Shared16), done)) return rc;
+  const int sms = stream::sm_count();
+  if (sms <= 0) return RC_LAUNCH;
+  unsigned ctas = 1;
+  while (ctas < 8 && (a.vocabulary + int(ctas) - 1) / int(ctas) > kPart16) ctas *= 2;
+  while (ctas < 8 && rows * ctas * 2 <= sms && a.vocabulary / int(ctas) > 4096) ctas *= 2;
+  return launch_dependent(sample16_kernel<T>, dim3(unsigned(rows * ctas)), kThreads, sizeof(Shared16), ctas, s, a);
+}
+
+static int launch32(const Args& a, int64_t rows, cudaStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  if (int rc = allow(sample32_kernel, sizeof(Shared32), done)) return rc;
+  const int sms = stream::sm_count();
+  if (sms <= 0) return RC_LAUNCH;
+  unsigned ctas = 1;
+  while (ctas < 8 && (a.vocabulary + int(ctas) - 1) / int(ctas) > kPart32) ctas *= 2;
+  while (ctas < 8 && rows * ctas * 2 <= sms && a.vocabulary / int(ctas) > 4096) ctas *= 2;
+  return launch_dependent(sample32_kernel, dim3(unsigned(rows * ctas)), kThreads, sizeof(Shared32), ctas, s, a);
+}
+
+}  // namespace choice
+
+int sample(const void* logits, int64_t row_stride, int dtype, int rows, int vocabulary, const float* uniforms, const DinoB200SampleSettings* settings, int* tokens,
+           float* probabilities, cudaStream_t s) {
+  using namespace choice;
+  if (logits == nullptr || uniforms == nullptr || settings == nullptr || tokens == nullptr) return RC_NULL;
+  if (rows <= 0 || vocabulary <= 0) return RC_DIMS;
+  if (vocabulary > kMaxVocabulary || rows > INT32_MAX / 8 || (rows > 1 && row_stride < vocabulary)) return RC_RANGE;
+  if (dtype != DINO_F16 && dtype != DINO_BF16 && dtype != DINO_F32) return RC_DTYPE;
+  if ((reinterpret_cast<uintptr_t>(logits) & (dtype == DINO_F32 ? 3 : 1)) != 0) return RC_ALIGN;
+  int* status = kv::status_words();
+  if (status == nullptr) return RC_LAUNCH;
+  const Args a{logits, row_stride, vocabulary, uniforms, *settings, tokens, probabilities, status};
+  switch (dtype) {
+    case DINO_F16: return launch16<__half>(a, rows, s);
+    case DINO_BF16: return launch16<__nv_bfloat16>(a, rows, s);
+    default: return launch32(a, rows, s);
+  }
+}
+
+}  // namespace b200gguf

@@ -14,6 +14,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <climits>
 #include <cstring>
 #include <memory>
@@ -379,6 +380,207 @@ PyObject* py_rms_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
+// An int32 or float32 tensor of one dimension, or null.
+const at::Tensor* vector_of(PyObject* o, at::ScalarType type, int64_t count, const at::Tensor& like) {
+  const at::Tensor* t = cuda_tensor(o);
+  return t != nullptr && t->scalar_type() == type && t->dim() == 1 && (count < 0 || t->size(0) == count) && t->device() == like.device() ? t : nullptr;
+}
+
+// kv_pool_step(pool, new, rows, drop, stream) -> (lengths, starts or None, positions, slots)
+PyObject* py_kv_pool_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 5) { PyErr_SetString(PyExc_TypeError, "kv_pool_step takes 5 arguments"); return nullptr; }
+  return guarded([&]() -> PyObject* {
+    PyObject* o = args[0];
+    void* stream = nullptr;
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 5 || !PyLong_CheckExact(PyTuple_GET_ITEM(o, 4)) || !THPVariable_Check(PyTuple_GET_ITEM(o, 0))) Py_RETURN_NONE;
+    const at::Tensor& table = THPVariable_Unpack(PyTuple_GET_ITEM(o, 0));
+    if (!table.defined() || !table.is_cuda() || table.layout() != at::kStrided || table.scalar_type() != at::kInt || table.dim() != 2 || !on_current_device(table)) Py_RETURN_NONE;
+    const int64_t sequences = table.size(0), columns = table.size(1);
+    const long block = PyLong_AsLong(PyTuple_GET_ITEM(o, 4));
+    if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+    if (sequences < 1 || sequences > 8192 || columns < 1 || table.stride(1) != 1 || (sequences > 1 && table.stride(0) < columns)) Py_RETURN_NONE;
+    if (block != 16 && block != 32 && block != 64 && block != 128) Py_RETURN_NONE;
+    const at::Tensor *lengths = vector_of(PyTuple_GET_ITEM(o, 1), at::kInt, sequences, table), *free = vector_of(PyTuple_GET_ITEM(o, 2), at::kInt, -1, table),
+                     *free_count = vector_of(PyTuple_GET_ITEM(o, 3), at::kInt, 1, table), *fresh = vector_of(args[1], at::kInt, sequences, table), *drop = nullptr;
+    if (lengths == nullptr || free == nullptr || free_count == nullptr || fresh == nullptr || free->size(0) < 1) Py_RETURN_NONE;
+    if (std::max(free->size(0), columns) > INT_MAX / block) Py_RETURN_NONE;
+    if (args[3] != Py_None && (drop = vector_of(args[3], at::kInt, sequences, table)) == nullptr) Py_RETURN_NONE;
+    const bool each = args[2] == Py_None;
+    if (!each && !PyLong_CheckExact(args[2])) Py_RETURN_NONE;
+    const int64_t rows = each ? sequences : PyLong_AsLongLong(args[2]);
+    if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+    if (rows < 1 || rows > INT_MAX || !stream_of(args[4], &stream)) Py_RETURN_NONE;
+    const auto options = table.options().requires_grad(false);
+    at::Tensor out[4];
+    out[0] = at::empty({sequences}, options);
+    if (!each) out[1] = at::empty({sequences + 1}, options);
+    out[2] = at::empty({rows}, options);
+    out[3] = at::empty({rows}, options);
+    const DinoB200KvPool pool{static_cast<int*>(table.mutable_data_ptr()), table.stride(0), static_cast<int*>(lengths->mutable_data_ptr()), static_cast<int*>(free->mutable_data_ptr()),
+                              static_cast<int*>(free_count->mutable_data_ptr()), int(columns), int(sequences), int(free->size(0)), int(block)};
+    const int *np = static_cast<const int*>(fresh->const_data_ptr()), *dp = drop != nullptr ? static_cast<const int*>(drop->const_data_ptr()) : nullptr;
+    int* p[4];
+    for (int i = 0; i < 4; ++i) p[i] = out[i].defined() ? static_cast<int*>(out[i].mutable_data_ptr()) : nullptr;
+    int rc = 0;
+    Py_BEGIN_ALLOW_THREADS
+    rc = dinoml_b200_kv_pool_step(&pool, np, dp, int(rows), p[0], p[1], p[2], p[3], stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) return PyLong_FromLong(rc);
+    PyObject* all = PyTuple_New(4);
+    for (int i = 0; i < 4 && all != nullptr; ++i) {
+      PyObject* t = Py_None;
+      if (out[i].defined()) t = THPVariable_Wrap(out[i]); else Py_INCREF(t);
+      if (t == nullptr) { Py_DECREF(all); return nullptr; }
+      PyTuple_SET_ITEM(all, i, t);
+    }
+    return all;
+  });
+}
+
+// rotary(q, k, positions, frequencies, q_weight, k_weight, eps, interleaved, magnitude, stream) -> (q, k), new tensors
+PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 10) { PyErr_SetString(PyExc_TypeError, "rotary takes 10 arguments"); return nullptr; }
+  return guarded([&]() -> PyObject* {
+    void* stream = nullptr;
+    const at::Tensor* x[2] = {};
+    for (int i = 0; i < 2; ++i) {
+      if (i == 1 && args[1] == Py_None) break;
+      if (!THPVariable_Check(args[i])) Py_RETURN_NONE;
+      const at::Tensor& t = THPVariable_Unpack(args[i]);
+      if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.dim() != 3 || t.size(0) < 1 || t.size(1) < 1 || t.size(1) > (1 << 18) || t.stride(2) != 1) Py_RETURN_NONE;
+      x[i] = &t;
+    }
+    const at::Tensor& q = *x[0];
+    const int dtype = dino_dtype(q.scalar_type());
+    const int64_t rows = q.size(0), dim = q.size(2);
+    if (!on_current_device(q) || dtype == 0 || rows > INT_MAX || dim < 2 || dim > 512 || dim % 2) Py_RETURN_NONE;
+    if (x[1] != nullptr && (x[1]->device() != q.device() || x[1]->scalar_type() != q.scalar_type() || x[1]->size(0) != rows || x[1]->size(2) != dim)) Py_RETURN_NONE;
+    const at::Tensor *positions = vector_of(args[2], at::kInt, rows, q), *frequencies = vector_of(args[3], at::kDouble, -1, q);
+    if (positions == nullptr || frequencies == nullptr || frequencies->size(0) < 1 || 2 * frequencies->size(0) > dim) Py_RETURN_NONE;
+    const at::Tensor* w[2] = {};
+    int weight_dtype = 0;
+    for (int i = 0; i < 2; ++i) {
+      if (args[4 + i] == Py_None) continue;
+      w[i] = cuda_tensor(args[4 + i]);
+      if (x[i] == nullptr || w[i] == nullptr || w[i]->dim() != 1 || w[i]->size(0) != dim || w[i]->device() != q.device()) Py_RETURN_NONE;
+      const int type = dino_dtype(w[i]->scalar_type());
+      if ((type != dtype && type != DINO_DTYPE_FLOAT32) || (weight_dtype != 0 && weight_dtype != type)) Py_RETURN_NONE;
+      weight_dtype = type;
+    }
+    if (!PyFloat_CheckExact(args[6]) || !PyBool_Check(args[7]) || !PyFloat_CheckExact(args[8]) || !stream_of(args[9], &stream)) Py_RETURN_NONE;
+    at::Tensor out[2];
+    DinoB200Heads sides[2] = {};
+    for (int i = 0; i < 2 && x[i] != nullptr; ++i) {
+      out[i] = at::empty(x[i]->sizes(), x[i]->options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+      sides[i] = {x[i]->const_data_ptr(), out[i].mutable_data_ptr(), w[i] != nullptr ? w[i]->const_data_ptr() : nullptr, x[i]->stride(0), x[i]->stride(1), x[i]->size(1) * dim, dim,
+                  int(x[i]->size(1))};
+    }
+    const int* pp = static_cast<const int*>(positions->const_data_ptr());
+    const double* fp = static_cast<const double*>(frequencies->const_data_ptr());
+    const int pairs = int(frequencies->size(0));
+    const float eps = float(PyFloat_AS_DOUBLE(args[6])), magnitude = float(PyFloat_AS_DOUBLE(args[8]));
+    const int interleaved = args[7] == Py_True ? 1 : 0;
+    int rc = 0;
+    Py_BEGIN_ALLOW_THREADS
+    rc = dinoml_b200_rotary(&sides[0], x[1] != nullptr ? &sides[1] : nullptr, pp, fp, pairs, dtype, weight_dtype != 0 ? weight_dtype : int(DINO_DTYPE_FLOAT32), int(rows), int(dim), eps,
+                            magnitude, interleaved, stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) return PyLong_FromLong(rc);
+    PyObject* pq = THPVariable_Wrap(out[0]);
+    PyObject* pk = Py_None;
+    if (x[1] != nullptr) pk = THPVariable_Wrap(out[1]); else Py_INCREF(pk);
+    PyObject* both = pq != nullptr && pk != nullptr ? PyTuple_Pack(2, pq, pk) : nullptr;
+    Py_XDECREF(pq);
+    Py_XDECREF(pk);
+    return both;
+  });
+}
+
+// embedding(tokens, table, qtype, dtype name, scale, stream) -> a new tensor
+PyObject* py_embedding(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 6) { PyErr_SetString(PyExc_TypeError, "embedding takes 6 arguments"); return nullptr; }
+  return guarded([&]() -> PyObject* {
+    const at::Tensor *tokens = cuda_tensor(args[0]), *table = cuda_tensor(args[1]);
+    const QTypeInfo* q = qtype_of(args[2]);
+    void* stream = nullptr;
+    if (tokens == nullptr || table == nullptr || q == nullptr || !PyUnicode_Check(args[3]) || !PyFloat_CheckExact(args[4]) || !stream_of(args[5], &stream)) Py_RETURN_NONE;
+    if ((tokens->scalar_type() != at::kInt && tokens->scalar_type() != at::kLong) || tokens->device() != table->device() || tokens->numel() < 1 || !on_current_device(*table)) Py_RETURN_NONE;
+    if (table->scalar_type() != at::kByte || table->dim() != 2 || table->size(0) < 1 || table->size(1) < 1 || table->size(1) % q->bytes) Py_RETURN_NONE;
+    at::ScalarType type = at::kFloat;
+    if (PyUnicode_CompareWithASCIIString(args[3], "bfloat16") == 0) type = at::kBFloat16;
+    else if (PyUnicode_CompareWithASCIIString(args[3], "float16") == 0) type = at::kHalf;
+    else if (PyUnicode_CompareWithASCIIString(args[3], "float32") != 0) Py_RETURN_NONE;
+    const int64_t width = table->size(1) / q->bytes * q->block;
+    c10::SmallVector<int64_t, 8> shape(tokens->sizes().begin(), tokens->sizes().end());
+    shape.push_back(width);
+    const at::Tensor out = at::empty(shape, table->options().dtype(type).requires_grad(false));
+    const void *ip = tokens->const_data_ptr(), *tp = table->const_data_ptr();
+    void* op = out.mutable_data_ptr();
+    const int64_t count = tokens->numel(), vocabulary = table->size(0);
+    const int bytes = int(tokens->element_size());
+    const float scale = float(PyFloat_AS_DOUBLE(args[4]));
+    int rc = 0;
+    Py_BEGIN_ALLOW_THREADS
+    rc = dinoml_b200_embedding(ip, bytes, tp, vocabulary, op, q->value, dino_dtype(type), count, width, scale, stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) return PyLong_FromLong(rc);
+    return THPVariable_Wrap(out);
+  });
+}
+
+// sample(logits, uniforms, temperature, top_k, top_p, min_p, stream) -> (tokens, probabilities)
+PyObject* py_sample(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 7) { PyErr_SetString(PyExc_TypeError, "sample takes 7 arguments"); return nullptr; }
+  return guarded([&]() -> PyObject* {
+    void* stream = nullptr;
+    if (!THPVariable_Check(args[0])) Py_RETURN_NONE;
+    const at::Tensor& logits = THPVariable_Unpack(args[0]);
+    if (!logits.defined() || !logits.is_cuda() || logits.layout() != at::kStrided || logits.dim() != 2 || !on_current_device(logits)) Py_RETURN_NONE;
+    const int dtype = dino_dtype(logits.scalar_type());
+    const int64_t rows = logits.size(0), columns = logits.size(1);
+    if (dtype == 0 || rows < 1 || rows > INT_MAX / 8 || columns < 1 || columns > 262144 || (columns > 1 && logits.stride(1) != 1) || (rows > 1 && logits.stride(0) < columns)) Py_RETURN_NONE;
+    const at::Tensor* uniforms = vector_of(args[1], at::kFloat, rows, logits);
+    if (uniforms == nullptr || !stream_of(args[6], &stream)) Py_RETURN_NONE;
+    DinoB200SampleSettings set{nullptr, nullptr, nullptr, nullptr, 1.f, 0, 1.f, 0.f};
+    const float** per_row[4] = {&set.temperature, nullptr, &set.top_p, &set.min_p};
+    float* all[4] = {&set.temperature_all, nullptr, &set.top_p_all, &set.min_p_all};
+    for (int i = 0; i < 4; ++i) {
+      PyObject* o = args[2 + i];
+      if (o == Py_None) {
+        if (i == 0) Py_RETURN_NONE;
+      } else if (THPVariable_Check(o)) {
+        const at::Tensor* t = vector_of(o, i == 1 ? at::kInt : at::kFloat, rows, logits);
+        if (t == nullptr) Py_RETURN_NONE;
+        if (i == 1) set.top_k = static_cast<const int*>(t->const_data_ptr()); else *per_row[i] = static_cast<const float*>(t->const_data_ptr());
+      } else if (i == 1) {
+        if (!PyLong_CheckExact(o)) Py_RETURN_NONE;
+        const long k = PyLong_AsLong(o);
+        if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+        set.top_k_all = int(std::min(std::max(k, 0l), long(INT_MAX)));
+      } else {
+        if (!PyFloat_CheckExact(o) || !(PyFloat_AS_DOUBLE(o) >= 0.)) Py_RETURN_NONE;
+        *all[i] = float(PyFloat_AS_DOUBLE(o));
+      }
+    }
+    const auto options = logits.options().requires_grad(false);
+    const at::Tensor tokens = at::empty({rows}, options.dtype(at::kInt)), probabilities = at::empty({rows}, options.dtype(at::kFloat));
+    const void* lp = logits.const_data_ptr();
+    const float* up = static_cast<const float*>(uniforms->const_data_ptr());
+    int* tp = static_cast<int*>(tokens.mutable_data_ptr());
+    float* pp = static_cast<float*>(probabilities.mutable_data_ptr());
+    const int64_t stride = logits.stride(0);
+    int rc = 0;
+    Py_BEGIN_ALLOW_THREADS
+    rc = dinoml_b200_sample(lp, stride, dtype, int(rows), int(columns), up, &set, tp, pp, stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) return PyLong_FromLong(rc);
+    PyObject *pt = THPVariable_Wrap(tokens), *pr = THPVariable_Wrap(probabilities), *both = pt != nullptr && pr != nullptr ? PyTuple_Pack(2, pt, pr) : nullptr;
+    Py_XDECREF(pt);
+    Py_XDECREF(pr);
+    return both;
+  });
+}
+
 // ---- sessions.  A Runner carries what Session.run_torch needs of the artifact: the names and dtypes of its inputs and outputs,
 // the output shapes as a walk over the nodes (a node's result is its input's shape with `columns` as the last dimension), and the
 // run entry of the library the artifact loaded (an artifact may carry its own copy).
@@ -521,6 +723,10 @@ PyMethodDef kMethods[] = {
     {"kv_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_kv_read)), METH_FASTCALL, nullptr},
     {"kv_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_kv_attention)), METH_FASTCALL, nullptr},
     {"rms_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_rms_norm)), METH_FASTCALL, nullptr},
+    {"kv_pool_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_kv_pool_step)), METH_FASTCALL, nullptr},
+    {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_rotary)), METH_FASTCALL, nullptr},
+    {"embedding", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_embedding)), METH_FASTCALL, nullptr},
+    {"sample", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_sample)), METH_FASTCALL, nullptr},
     {"make_runner", py_make_runner, METH_VARARGS, nullptr},
     {"run_torch", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_run_torch)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -403,6 +403,243 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, residu
     return out, total
 
 
+class KVPool(NamedTuple):
+    """Who has which blocks of a `KVCache`: block_table [sequences, table_blocks] (-1 behind a sequence's blocks), lengths [sequences] its tokens, free [blocks] a stack of
+    which the first free_count [1] are free, all int32 on the device.  `kv_pool_step` changes them in place; block_table is what the cache's calls take."""
+    block_table: torch.Tensor
+    lengths: torch.Tensor
+    free: torch.Tensor
+    free_count: torch.Tensor
+    block_size: int
+
+
+class KVStep(NamedTuple):
+    """One step's batch: lengths and starts as the cache's calls take them, positions and slots (block * block_size + place in it) of its rows, -1 of nobody's."""
+    lengths: torch.Tensor
+    starts: torch.Tensor | None
+    positions: torch.Tensor
+    slots: torch.Tensor
+
+
+_POOL_SEQUENCES = 8192
+
+
+def kv_pool(blocks: int, sequences: int, table_blocks: int, block_size: int, device="cuda") -> KVPool:
+    """A pool of a cache's `blocks` blocks, all free, for `sequences` sequences (8192 at most) of up to table_blocks blocks.  Blocks are handed out from 0 on."""
+    if block_size not in _KV_BLOCK_SIZES or blocks < 1 or table_blocks < 1 or not 1 <= sequences <= _POOL_SEQUENCES:
+        raise ValueError(f"a pool has blocks of {_KV_BLOCK_SIZES} tokens and 1 to {_POOL_SEQUENCES} sequences, got {block_size} and {sequences}")
+    if max(blocks, table_blocks) * block_size > 0x7fffffff:
+        raise ValueError("a pool has less than 2^31 tokens")
+    return KVPool(torch.full((sequences, table_blocks), -1, dtype=torch.int32, device=device), torch.zeros(sequences, dtype=torch.int32, device=device),
+                  torch.arange(blocks - 1, -1, -1, dtype=torch.int32, device=device), torch.full((1,), blocks, dtype=torch.int32, device=device), int(block_size))
+
+
+def kv_pool_step(pool, new: torch.Tensor, rows: int | None = None, *, drop: torch.Tensor | None = None, stream=None) -> KVStep:
+    """One step of all sequences, in place: sequence b loses drop[b] tokens at its end (None: none; a request that is done: as many as it has, or more) and gets new[b].  Blocks
+    go back before any is handed out; sequences that get as many as they lost get the same ones.  rows: of the packed batch, at least sum(new); those behind the last
+    sequence are nobody's.  rows None: one row per sequence, new[b] 0 or 1, and starts None.  A sequence whose new tokens do not fit goes without them (its lengths entry is 0,
+    it has no rows): the table's row is too short, or it wants blocks and those that the sequences up to it want are more than there are, or their rows more than `rows`."""
+    done = _native_call("kv_pool_step")(pool, new, rows, drop, stream)
+    if done is not None:                                                                  # None: not the plain case, checked below
+        if type(done) is int:
+            _native.check(done, "dinoml_b200_kv_pool_step")
+        return KVStep(*done)
+    table, lengths, free, free_count, block_size = pool
+    _require_cuda(lengths, "pool.lengths")
+    _require_current_device(lengths, "the pool")
+    device = lengths.device
+    if not table.is_cuda or table.dtype != torch.int32 or table.dim() != 2 or table.device != device or min(table.shape) < 1 or table.stride(1) != 1 \
+            or (table.shape[0] > 1 and table.stride(0) < table.shape[1]):
+        raise ValueError("pool.block_table must be int32 [sequences, blocks] on the device of the pool, its rows contiguous")
+    sequences = table.shape[0]
+    if sequences > _POOL_SEQUENCES or block_size not in _KV_BLOCK_SIZES:
+        raise ValueError(f"a pool has blocks of {_KV_BLOCK_SIZES} tokens and 1 to {_POOL_SEQUENCES} sequences, got {block_size} and {sequences}")
+    if free.dim() != 1 or free.shape[0] < 1:
+        raise ValueError("pool.free must be int32 [blocks]")
+    if max(free.shape[0], table.shape[1]) * block_size > 0x7fffffff:
+        raise ValueError("a pool has less than 2^31 tokens")
+    _kv_ints(lengths, "pool.lengths", sequences, device)
+    _kv_ints(free, "pool.free", free.shape[0], device)
+    _kv_ints(free_count, "pool.free_count", 1, device)
+    _kv_ints(new, "new", sequences, device)
+    drop_ptr = None if drop is None else _kv_ints(drop, "drop", sequences, device)
+    count = sequences if rows is None else int(rows)
+    if not 0 <= count <= 0x7fffffff:
+        raise ValueError(f"rows must be 0 to 2^31 - 1, got {rows}")
+    step = KVStep(torch.empty(sequences, dtype=torch.int32, device=device), None if rows is None else torch.empty(sequences + 1, dtype=torch.int32, device=device),
+                  *(torch.empty(count, dtype=torch.int32, device=device) for _ in range(2)))
+    spare = step.lengths.data_ptr()                                                       # no rows: nothing is written there, but addresses are wanted
+    struct = _native.KvPool(table.data_ptr(), table.stride(0), lengths.data_ptr(), free.data_ptr(), free_count.data_ptr(), table.shape[1], sequences, free.shape[0], block_size)
+    rc = _native.lib().dinoml_b200_kv_pool_step(
+        ctypes.byref(struct), new.data_ptr(), drop_ptr, count, step.lengths.data_ptr(), None if rows is None else step.starts.data_ptr(), step.positions.data_ptr() or spare,
+        step.slots.data_ptr() or spare, _stream_ptr(stream))
+    _native.check(rc, "dinoml_b200_kv_pool_step")
+    return step
+
+
+def rotary_frequencies(dim: int, base: float = 10000.0, *, scale: float = 1.0, factors=None, device="cuda") -> torch.Tensor:
+    """Angles per position of the dim / 2 pairs of a rotated head, float64: scale * base ** (-2 i / dim), divided by factors[i] where there are some (a GGUF file's
+    rope_freqs.weight)."""
+    if dim < 2 or dim % 2:
+        raise ValueError(f"pairs are of two values: dim {dim}")
+    out = scale * float(base) ** (-2.0 * torch.arange(dim // 2, dtype=torch.float64) / dim)
+    if factors is not None:
+        factors = torch.as_tensor(factors).cpu().to(torch.float64)
+        if factors.shape != out.shape:
+            raise ValueError(f"factors must be [{dim // 2}]")
+        out = out / factors
+    return out.to(device)
+
+
+def _rotary_side(x: torch.Tensor, weight, out, name: str, like: torch.Tensor) -> _native.Heads:
+    if not x.is_cuda or x.device != like.device or x.dim() != 3 or x.dtype != like.dtype or x.shape[0] != like.shape[0] or x.shape[2] != like.shape[2] or x.shape[1] < 1 \
+            or x.stride(2) != 1:
+        raise ValueError(f"{name} must be [rows, heads, head_dim], its last dimension contiguous, q and k of one dtype, device, number of rows and head_dim")
+    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(2) != 1:
+        raise ValueError(f"out of {name} must have its shape and dtype, its last dimension contiguous")
+    rows, heads, dim = x.shape
+    if not (out.stride(1) >= dim or heads == 1) or not (out.stride(0) >= dim or rows == 1) or not (
+            rows == 1 or heads == 1 or out.stride(0) >= (heads - 1) * out.stride(1) + dim or out.stride(1) >= (rows - 1) * out.stride(0) + dim):
+        raise ValueError(f"out of {name} must not overlap itself")
+    if rows and (out.data_ptr(), out.stride()) != (x.data_ptr(), x.stride()):
+        def span(t):
+            return t.data_ptr(), t.data_ptr() + ((rows - 1) * t.stride(0) + (heads - 1) * t.stride(1) + dim) * t.element_size()
+        if out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr() and span(out)[0] < span(x)[1] and span(x)[0] < span(out)[1]:
+            raise ValueError(f"out of {name} must be {name} itself or not overlap it")
+    if weight is not None:
+        _require_cuda(weight, f"{name}_weight")
+        if weight.shape != (dim,) or weight.dtype not in (torch.float32, x.dtype) or weight.device != x.device:
+            raise ValueError(f"{name}_weight must be [{dim}] in float32 or the dtype of {name}, on its device")
+    return _native.Heads(x.data_ptr(), out.data_ptr(), None if weight is None else weight.data_ptr(), x.stride(0), x.stride(1), out.stride(0), out.stride(1), heads)
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, frequencies: torch.Tensor, *, q_weight: torch.Tensor | None = None,
+           k_weight: torch.Tensor | None = None, eps: float = 1e-5, interleaved: bool = False, magnitude: float = 1.0, out=None, stream=None):
+    """(q, k) turned by position: pairs (a, b) of every head become magnitude * (a cos - b sin, b cos + a sin), angle positions[row] * frequencies[i] in float64.  Pair i is
+    (i, i + n) with n = len(frequencies), interleaved (2 i, 2 i + 1); values behind 2 n stay.  q_weight, k_weight [head_dim] (float32 or q's dtype): each head is first brought to
+    x / sqrt(mean(x^2) + eps) * weight.  float32 inside, one rounding at the end.  q [rows, heads, head_dim], k [rows, kv_heads, head_dim] (None: q alone), any row and head strides; head_dim
+    even, 512 at most; positions int32 [rows]; frequencies float64 (`rotary_frequencies`).  out: two tensors to fill, q and k themselves among them.  A row at a negative position is
+    nobody's: zero, or left as it was where it is written in place."""
+    done = _native_call("rotary")(q, k, positions, frequencies, q_weight, k_weight, eps, interleaved, magnitude, stream) if out is None else None
+    if done is not None:                                                                  # None: not the plain case, checked below
+        if type(done) is int:
+            _native.check(done, "dinoml_b200_rotary")
+        return done
+    if q.dim() != 3 or q.dtype not in _DTYPE_NAME or not q.is_cuda:
+        raise ValueError(f"q must be a CUDA tensor [rows, heads, head_dim] in {sorted(_TORCH_DTYPE)}")
+    _require_current_device(q, "q")
+    rows, _, dim = q.shape
+    if dim < 2 or dim % 2 or dim > 512:
+        raise ValueError(f"head_dim must be even and 512 at most, got {dim}")
+    _kv_ints(positions, "positions", rows, q.device)
+    _require_cuda(frequencies, "frequencies")
+    if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or 2 * frequencies.shape[0] > dim or frequencies.device != q.device:
+        raise ValueError(f"frequencies must be float64 [{dim // 2} at most] on the device of q")
+    if k is None and k_weight is not None:
+        raise ValueError("k_weight is k's: none is given")
+    given = (None, None) if out is None else tuple(out) if k is not None or isinstance(out, (tuple, list)) else (out, None)
+    if len(given) != 2 or (k is None and given[1] is not None):
+        raise ValueError("out must be two tensors, for q and for k")
+    q_out, k_out = (torch.empty(x.shape, dtype=x.dtype, device=x.device) if o is None and x is not None else o for x, o in zip((q, k), given))
+    side_q = _rotary_side(q, q_weight, q_out, "q", q)
+    side_k = None if k is None else _rotary_side(k, k_weight, k_out, "k", q)
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise ValueError("q_weight and k_weight must have one dtype")
+    if rows:
+        weight = q_weight if q_weight is not None else k_weight
+        rc = _native.lib().dinoml_b200_rotary(
+            ctypes.byref(side_q), None if side_k is None else ctypes.byref(side_k), positions.data_ptr(), frequencies.data_ptr() or None, frequencies.shape[0],
+            _native.DINO_DTYPE[_DTYPE_NAME[q.dtype]], _native.DINO_DTYPE["float32" if weight is None else _DTYPE_NAME[weight.dtype]], rows, dim, float(eps), float(magnitude),
+            int(bool(interleaved)), _stream_ptr(stream))
+        _native.check(rc, "dinoml_b200_rotary")
+    return q_out, k_out
+
+
+def embedding(tokens: torch.Tensor, table: torch.Tensor, qtype, dtype: str = "bfloat16", *, scale: float = 1.0, out: torch.Tensor | None = None,
+              stream=None) -> torch.Tensor:
+    """Rows of a GGUF table (uint8 [vocabulary, row_bytes]) for tokens (int32 or int64, any shape): tokens.shape + [width] in `dtype`, each value the dequantized float32 times
+    scale, rounded once.  Token -1 is nobody's, its row zero; so is that of any other token outside of the table, which `device_status()` tells."""
+    done = _native_call("embedding")(tokens, table, qtype, dtype, scale, stream) if out is None else None
+    if done is not None:                                                                  # None: not the plain case, checked below
+        if type(done) is int:
+            _native.check(done, "dinoml_b200_embedding")
+        return done
+    q = qtype_of(qtype)
+    _require_cuda(tokens, "tokens")
+    _require_cuda(table, "table")
+    _require_current_device(table, "the table")
+    if tokens.dtype not in (torch.int32, torch.int64) or tokens.device != table.device:
+        raise ValueError("tokens must be int32 or int64 on the device of the table")
+    if table.dtype != torch.uint8 or table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1 or table.shape[1] % q.block_bytes:
+        raise ValueError(f"table must be uint8 [vocabulary, row_bytes] with whole {q.name} blocks of {q.block_bytes} bytes")
+    if dtype not in _TORCH_DTYPE:
+        raise ValueError(f"dtype must be one of {sorted(_TORCH_DTYPE)}, got {dtype!r}")
+    width = table.shape[1] // q.block_bytes * q.block_size
+    shape = tuple(tokens.shape) + (width,)
+    if out is None:
+        out = torch.empty(shape, dtype=_TORCH_DTYPE[dtype], device=table.device)
+    _require_cuda(out, "out")
+    if tuple(out.shape) != shape or out.dtype != _TORCH_DTYPE[dtype] or out.device != table.device:
+        raise ValueError(f"out must be {dtype} {shape} on the device of the table")
+    if tokens.numel():
+        rc = _native.lib().dinoml_b200_embedding(tokens.data_ptr(), tokens.element_size(), table.data_ptr(), table.shape[0], out.data_ptr(), q.value,
+                                                 _native.DINO_DTYPE[dtype], tokens.numel(), width, float(scale), _stream_ptr(stream))
+        _native.check(rc, "dinoml_b200_embedding")
+    return out
+
+
+_SAMPLE_VOCABULARY = 262144
+
+
+def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=1.0, top_k=None, top_p=None, min_p=None, stream=None):
+    """(tokens int32 [rows], probabilities float32 [rows]): of every row of logits [rows, vocabulary] (262144 at most, any row stride) one token, chosen with its number of
+    uniforms float32 [rows] in [0, 1).  Tokens are ordered by logit, the lowest index first among equals, their weights are exp((logit - largest) / temperature); kept are the first
+    top_k (None or 0: all), of these the fewest whose weights are at least top_p of theirs (None or 1: all), of these those with at least min_p of the largest weight (None: all);
+    the token is the first whose running sum is above uniforms[row] times the sum of the kept, its probability its share of that sum.  Temperature 0 takes the first.  Each setting is a number
+    or a tensor [rows] (top_k int32, the others float32).  Logits of -inf are never chosen; a row with a NaN, without any other logit, or with a setting that is
+    none gives -1 and 0 (`device_status()` tells of the last)."""
+    done = _native_call("sample")(logits, uniforms, temperature, top_k, top_p, min_p, stream)
+    if done is not None:                                                                  # None: not the plain case, checked below
+        if type(done) is int:
+            _native.check(done, "dinoml_b200_sample")
+        return done
+    if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in _DTYPE_NAME or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError(f"logits must be a CUDA tensor [rows, vocabulary] in {sorted(_TORCH_DTYPE)}, its rows contiguous")
+    _require_current_device(logits, "logits")
+    rows, vocabulary = logits.shape
+    if vocabulary > _SAMPLE_VOCABULARY or (rows > 1 and logits.stride(0) < vocabulary):
+        raise ValueError(f"logits must have {_SAMPLE_VOCABULARY} columns at most, and rows that do not overlap")
+
+    def per_row(t, name, dtype):
+        _require_cuda(t, name)
+        if t.dtype != dtype or t.shape != (rows,) or t.device != logits.device:
+            raise ValueError(f"{name} must be {dtype} [{rows}] on the device of logits")
+        return t.data_ptr()
+
+    uniforms_ptr = per_row(uniforms, "uniforms", torch.float32)
+    settings = _native.SampleSettings(None, None, None, None, 1.0, 0, 1.0, 0.0)
+    for name, value, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if value is None:
+            if name == "temperature":
+                raise ValueError("temperature must be a number or a tensor")
+        elif isinstance(value, torch.Tensor):
+            setattr(settings, name, per_row(value, name, dtype))
+        elif name == "top_k":
+            if value != int(value):
+                raise ValueError(f"top_k must be a whole number, got {value}")
+            settings.top_k_all = min(max(int(value), 0), 0x7fffffff)
+        else:
+            if not value >= 0:
+                raise ValueError(f"{name} must not be negative, got {value}")
+            setattr(settings, name + "_all", float(value))
+    tokens, probabilities = (torch.empty(rows, dtype=t, device=logits.device) for t in (torch.int32, torch.float32))
+    if rows:
+        rc = _native.lib().dinoml_b200_sample(logits.data_ptr(), logits.stride(0), _native.DINO_DTYPE[_DTYPE_NAME[logits.dtype]], rows, vocabulary, uniforms_ptr,
+                                              ctypes.byref(settings), tokens.data_ptr(), probabilities.data_ptr(), _stream_ptr(stream))
+        _native.check(rc, "dinoml_b200_sample")
+    return tokens, probabilities
+
+
 def release_stream(stream) -> None:
     """Gives back the workspaces that the library keeps for a stream (of the attention and of the linears), before the stream is destroyed.  Waits for the stream."""
     _native.check(_native.lib().dinoml_b200_release_stream(_stream_ptr(stream)), "dinoml_b200_release_stream")
@@ -410,5 +647,6 @@ def release_stream(stream) -> None:
 
 def device_status() -> int:
     """Synchronizes and returns the status word written by bounded device-side waits (0 = none gave up; 16: one of the attention over the cache) and by the checks of
-    what only the device sees (10: a block table, lengths, starts or begins pointed outside of the cache or of the rows).  Read once: it is 0 after that."""
+    what only the device sees (10: a block table, lengths, starts or begins pointed outside of the cache or of the rows, a token outside of its table, a pool's numbers that cannot be, a row's
+    sampling settings that are none).  Read once: it is 0 after that."""
     return int(_native.lib().dinoml_b200_gguf_device_status())

@@ -1,11 +1,12 @@
 /*
  * C ABI of the operators that a decoder runs between its quantized linears, in libdinoml_b200_gguf.so: a paged cache of keys and
- * values in 8 bits (write, read, attention over it) and the root-mean-square norm with the residual's addition.
+ * values in 8 bits (write, read, attention over it), who has which of its blocks, the root-mean-square norm with the residual's addition, the rotation of queries
+ * and keys by position with their heads' norms; and at the two ends of a step the rows of a GGUF table for its tokens and the choice of the next ones.
  *
  * Conventions are those of dinoml_b200_gguf.h: device pointers, `stream` a cudaStream_t as void*, 0 = ok, 1 = null pointer, 2 = non-positive
  * dimension, 4 = launch failure, 6 = unsupported dtype or cache type, 7 = alignment, 8 = size outside what the kernels take; a message is
- * available from dino_get_last_error().  What only the device sees (block table, lengths, starts, begins) is checked there: an entry that
- * points outside of the cache or of the rows is left out of the operation, and dinoml_b200_gguf_device_status() answers 10.  16 there: a wait
+ * available from dino_get_last_error().  What only the device sees (block table, lengths, starts, begins, tokens, a row's settings) is checked there: an entry that
+ * points outside of the cache, the rows or the table, or that is no number where one is wanted, is left out of the operation, and dinoml_b200_gguf_device_status() answers 10.  16 there: a wait
  * inside of an attention kernel gave up, and its results are not to be used; reading the status empties the workspaces' counters.
  */
 #ifndef DINOML_B200_DECODER_H_
@@ -77,6 +78,68 @@ DINOML_B200_API int dinoml_b200_kv_cache_attention(const DinoB200KvCache* cache,
  * round(y / d)); width is then a multiple of 32. */
 DINOML_B200_API int dinoml_b200_rms_norm(const void* x, const void* residual, const void* weight, void* y, void* total, int dtype, int weight_dtype, int rows,
                                          int width, float eps, int q8_0, void* stream);
+
+/* Rows of a GGUF table ([vocabulary] rows of `width` values in blocks of `qtype`) for `count` tokens (token_bytes 4: int32, 8: int64): out [count][width] in `dtype`,
+ * 16-byte aligned; a value is the dequantized float32 times scale, in float32, rounded once.  Token -1 is nobody's: its row is zero; so is that of every other token
+ * outside of the table, which the status tells. */
+DINOML_B200_API int dinoml_b200_embedding(const void* tokens, int token_bytes, const void* table, int64_t vocabulary, void* out, int qtype, int dtype, int64_t count,
+                                          int64_t width, float scale, void* stream);
+
+/* Heads of one kind: x and out [rows][heads][head_dim], strides in elements, head_dim contiguous; out may be x with its strides, else they do not overlap.  weight
+ * [head_dim] (null: no norm). */
+typedef struct DinoB200Heads {
+  const void* x;
+  void* out;
+  const void* weight;
+  int64_t row_stride, head_stride, out_row_stride, out_head_stride;
+  int heads;
+} DinoB200Heads;
+
+/* t = x / sqrt(mean(x^2) + eps) * weight over each head (weight null: t = x); pairs of its first 2 `pairs` values are turned by the angle positions[row] * frequencies[i]:
+ * (a, b) -> magnitude * (a cos - b sin, b cos + a sin), pair i being (i, i + pairs), or with interleaved != 0 (2 i, 2 i + 1); the others stay.  The angle is float64 and so
+ * exact to 2^-30 at any position, the rest float32 with one rounding at the end.  k null: q alone.  head_dim is even, 512 at most.  A row at a negative position is nobody's: left as it
+ * was where out is x, else zero.  weight_dtype: float32 or `dtype`. */
+DINOML_B200_API int dinoml_b200_rotary(const DinoB200Heads* q, const DinoB200Heads* k, const int* positions, const double* frequencies, int pairs, int dtype,
+                                       int weight_dtype, int rows, int head_dim, float eps, float magnitude, int interleaved, void* stream);
+
+/* Who has which blocks of a cache.  block_table as in DinoB200KvBatch with -1 behind a sequence's blocks, lengths its tokens; free_blocks [blocks], the first
+ * free_count[0] of them are free, the last of these is the next one.  sequences is 8192 at most. */
+typedef struct DinoB200KvPool {
+  int* block_table;
+  int64_t table_stride; /* elements */
+  int* lengths;
+  int* free_blocks;
+  int* free_count;
+  int table_blocks, sequences, blocks, block_size;
+} DinoB200KvPool;
+
+/* One step of a pool, in place: every sequence loses drop[b] tokens at its end (null: none; all, if it has fewer) and then gets new_tokens[b].  Blocks without tokens go
+ * back first, the last sequence's last one before the others, so that sequences which get as many as they lost get the same ones.  A sequence whose tokens would not fit is left without
+ * its new ones: where the table's row is too short, where it wants blocks and the blocks that the sequences up to it want are more than there are, or where their rows are
+ * more than `rows`.  lengths [sequences]: the tokens of a sequence that got some, new ones among them, 0 of the others; starts [sequences + 1] and `rows` as in DinoB200KvBatch.
+ * starts null: one row per sequence (rows = sequences, new tokens 0 or 1).  positions, slots [rows]: a row's position and block * block_size + position % block_size; -1 of rows that are nobody's. */
+DINOML_B200_API int dinoml_b200_kv_pool_step(const DinoB200KvPool* pool, const int* new_tokens, const int* drop, int rows, int* lengths, int* starts, int* positions,
+                                             int* slots, void* stream);
+
+/* Settings of a choice: one for each row, or where the pointer is null one for all. */
+typedef struct DinoB200SampleSettings {
+  const float* temperature;
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all;
+  int top_k_all;
+  float top_p_all, min_p_all;
+} DinoB200SampleSettings;
+
+/* tokens[row]: one of [0, vocabulary), chosen with the given number uniforms[row] in [0, 1).  Order of the tokens: by logit, the lowest index first among equals (-0 is 0).  Weights
+ * w = exp((logit - largest) / temperature).  Kept are the first top_k (0 or less: all), of these the fewest whose weights are at least top_p of theirs (1: all), of these those with
+ * w >= min_p, the first in any case; the token is the first whose running sum is above uniforms[row] times the sum of the kept.  Temperature 0: the first token.  probabilities[row] (null:
+ * not wanted): w / sum of the kept; 1 with temperature 0.  Weights and sums are float64, or multiples of 2^-45 where the logits are float32.  A logit of -inf is never chosen, one of inf has all of the weight.  A row with a NaN, or
+ * with nothing but -inf, or whose settings are no numbers or its temperature negative (which the status tells) gives token -1, probability 0.  logits [rows][vocabulary], row_stride
+ * in elements; vocabulary is 262144 at most. */
+DINOML_B200_API int dinoml_b200_sample(const void* logits, int64_t row_stride, int dtype, int rows, int vocabulary, const float* uniforms,
+                                       const DinoB200SampleSettings* settings, int* tokens, float* probabilities, void* stream);
 
 /* The workspaces that the library keeps for a stream of the caller's (those of the attention and of the linears) are emptied and wait for another stream, or are
  * freed.  Waits for the stream; call it before the stream is destroyed, and after the graphs with linears that were captured on it.  Workspaces of streams that are not released live as long as the process. */
