@@ -159,7 +159,11 @@ __global__ void __launch_bounds__(NT) kv_pool_kernel(PoolArgs a) {
     }
     const int left = (kept[b] + round) >> a.block_log2, last = (kept[b] + rows + round) >> a.block_log2;
     int* row = a.table + int64_t(b) * a.table_stride;
-    for (int j = left + lane; j < last; j += 32) row[j] = __ldcg(a.free_blocks + (available - 1 - (taken[b] + j - left)));
+    for (int j = left + lane; j < last; j += 32) {
+      const int id = __ldcg(a.free_blocks + (available - 1 - (taken[b] + j - left)));
+      if (unsigned(id) >= unsigned(a.blocks)) flag_range(a.status);
+      row[j] = id;
+    }
   }
   if (rank == 0 && tid == 0) {
     a.free_count[0] = int(available - got[0]);
