@@ -1,5 +1,7 @@
 // Launches that start while the one before them in the stream ends; the kernel waits for that itself, before it reads or writes anything that another one may have.
 #pragma once
+#include <atomic>
+
 #include "gguf_common.cuh"
 
 namespace b200gguf {
@@ -21,6 +23,17 @@ inline int launch_dependent(void (*kernel)(P...), dim3 grid, unsigned threads, s
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? RC_OK : RC_LAUNCH;
+}
+
+// Lets a kernel have `shared` bytes of dynamic shared memory, once a device (`done` is the kernel's own).
+template <typename K> inline int allow_shared(K kernel, size_t shared, std::atomic<uint64_t>& done) {
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return RC_LAUNCH;
+  if ((done.load(std::memory_order_acquire) >> dev & 1) == 0) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)) != cudaSuccess) return RC_LAUNCH;
+    done.fetch_or(uint64_t(1) << dev, std::memory_order_release);
+  }
+  return RC_OK;
 }
 
 #ifdef __CUDACC__

@@ -214,8 +214,9 @@ int pool_step(const DinoB200KvPool* pool, const int* new_tokens, const int* drop
   const size_t shared = (4 * size_t(pool->sequences) + 1) * sizeof(int);
   const bool small = pool->sequences <= 256 && rows <= 1024;
   auto kernel = small ? kv_pool_kernel<256> : kv_pool_kernel<1024>;
-  if (shared > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int((4 * kPoolMaxSequences + 1) * sizeof(int))) != cudaSuccess)
-    return RC_LAUNCH;
+  static std::atomic<uint64_t> done{0};
+  if (!small)
+    if (int rc = allow_shared(kernel, (4 * size_t(kPoolMaxSequences) + 1) * sizeof(int), done)) return rc;
   return small ? launch_dependent(kernel, dim3(1), 256, shared, 1, s, a) : launch_dependent(kernel, dim3(kPoolCluster), 1024, shared, kPoolCluster, s, a);
 }
 

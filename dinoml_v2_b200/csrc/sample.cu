@@ -14,7 +14,6 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
-#include <atomic>
 
 #include "dependent_launch.cuh"
 #include "kv_cache.cuh"
@@ -686,19 +685,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
   }
 }
 
-template <typename K> static int allow(K kernel, size_t shared, std::atomic<uint64_t>& done) {
-  int dev = -1;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return RC_LAUNCH;
-  if ((done.load(std::memory_order_acquire) >> dev & 1) == 0) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)) != cudaSuccess) return RC_LAUNCH;
-    done.fetch_or(uint64_t(1) << dev, std::memory_order_release);
-  }
-  return RC_OK;
-}
-
 template <typename T> static int launch16(const Args& a, int64_t rows, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
-  if (int rc = allow(sample16_kernel<T>, sizeof(Shared16), done)) return rc;
+  if (int rc = allow_shared(sample16_kernel<T>, sizeof(Shared16), done)) return rc;
   const int sms = stream::sm_count();
   if (sms <= 0) return RC_LAUNCH;
   unsigned ctas = 1;
@@ -709,7 +698,7 @@ template <typename T> static int launch16(const Args& a, int64_t rows, cudaStrea
 
 static int launch32(const Args& a, int64_t rows, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
-  if (int rc = allow(sample32_kernel, sizeof(Shared32), done)) return rc;
+  if (int rc = allow_shared(sample32_kernel, sizeof(Shared32), done)) return rc;
   const int sms = stream::sm_count();
   if (sms <= 0) return RC_LAUNCH;
   unsigned ctas = 1;
