@@ -1,10 +1,12 @@
 // Rows of a GGUF table for the tokens of a step: out[i] = round(dequant(table[tokens[i]]) * scale).
 //
 // Bound by bytes, most of them the result's (8192 values of Q4_K are 4.6 KB read and 16 KB written, and a text's tokens repeat); a single token by its chain of reads (token, block,
-// result) and the launch.  A CTA has a token's row or a part of it, a thread eight values at a time: they are one store of 16 or 32 bytes, and neighbours read neighbouring bytes.
+// result) and the launch.  A thread has an item of a row (dequant_items.cuh: 32 weights of Q4_K in 16 bits), a CTA one row, or several short ones, at a time; it reads the next row's
+// item before it writes this one's.
 #include <algorithm>
 
 #include "dependent_launch.cuh"
+#include "dequant_items.cuh"
 #include "kv_cache.cuh"
 
 namespace b200gguf {
@@ -13,55 +15,106 @@ namespace embed {
 
 constexpr int kThreads = 256;
 
-template <int QT, typename T, typename I>
-__global__ void __launch_bounds__(kThreads) embedding_kernel(const I* tokens, const uint8_t* table, int64_t vocabulary, T* out, int64_t items, int parts, int units,
-                                                            int per_item, float scale, int* status) {
-  constexpr int kOf = QTraits<QT>::kBlock / 8, kBytes = QTraits<QT>::kBytes;      // units of a block
-  const int64_t row_bytes = int64_t(units / kOf) * kBytes;
-  wait_for_launch_before();
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int64_t i = parts == 1 ? item : item / parts;
-    const int begin = int(item - i * parts) * per_item, end = min(begin + per_item, units);
-    const int64_t token = int64_t(tokens[i]);
-    const bool in = token >= 0 && token < vocabulary;
-    if (!in && token != -1 && threadIdx.x == 0) kv::flag_range(status);
-    const uint8_t* row = table + (in ? token : 0) * row_bytes;
-    T* to = out + i * int64_t(units) * 8;
-#pragma unroll 4
-    for (int u = begin + int(threadIdx.x); u < end; u += kThreads) {
-      float w[8];
-      if (in) {
-        decode8<QT>(row + int64_t(u / kOf) * kBytes, u % kOf * 8, w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = __fmul_rn(w[j], scale);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = 0.f;
-      }
-      constexpr int N = 16 / int(sizeof(T));
-#pragma unroll
-      for (int j = 0; j < 8; j += N) {
-        kv::Pack<T> v;
-#pragma unroll
-        for (int m = 0; m < N; ++m) v.v[m] = kv::from_float<T>(w[j + m]);
-        *reinterpret_cast<uint4*>(to + int64_t(u) * 8 + j) = v.raw;
-      }
+template <typename I> struct Args {
+  const I* tokens;
+  const uint8_t* table;
+  void* out;
+  int64_t vocabulary, count, groups;             // groups: of tokens that a CTA has at once
+  int64_t first_edge, last_edge;                 // blocks of the table whose first or last aligned word holds bytes outside of it
+  int blocks, items, each, chunks;               // of a row: blocks, items; tokens of a group; turns that a CTA needs for a row
+  float scale;
+  bool wide;
+  int* status;
+};
+
+// A: alignment of the table that all of its blocks keep.
+template <int QT, typename T, typename I, int A>
+__global__ void __launch_bounds__(kThreads) embedding_kernel(Args<I> a) {
+  using G = ItemGeom<QT, run_of<QT, T>()>;
+  const int sub = a.each > 1 ? int(threadIdx.x) / a.items : 0, own = int(threadIdx.x) - sub * a.items;
+  const int64_t units = a.groups * a.chunks;
+  struct Job {
+    int64_t row;                                 // of the result; -1: nothing
+    int item;
+    bool in;                                     // the token is in the table
+    Item<QT, T, A> what;
+  };
+  auto load = [&](int64_t unit, Job& job) {
+    job.row = -1;
+    job.in = false;
+    if (unit >= units || sub >= a.each) return;
+    const int64_t group = a.chunks == 1 ? unit : unit / a.chunks;
+    const int at = own + int(unit - group * a.chunks) * kThreads;
+    const int64_t row = group * a.each + sub;
+    if (at >= a.items || row >= a.count) return;
+    const int64_t token = int64_t(a.tokens[row]);
+    job.row = row;
+    job.item = at;
+    job.in = token >= 0 && token < a.vocabulary;
+    if (job.in) {
+      const int64_t block = token * a.blocks + at / G::kItems;
+      job.what.load(a.table + block * QTraits<QT>::kBytes, at % G::kItems, block == a.first_edge || block == a.last_edge);
+    } else if (token != -1 && at == 0) {
+      kv::flag_range(a.status);
     }
+  };
+  auto store = [&](const Job& job) {
+    if (job.row < 0) return;
+    const int block = job.item / G::kItems, item = job.item % G::kItems;
+    T* to = static_cast<T*>(a.out) + (job.row * a.blocks + block) * QTraits<QT>::kBlock;
+    if (job.in) {
+      if (a.scale == 1.f) job.what.emit(to, item, a.wide); else job.what.template emit<true>(to, item, a.wide, a.scale);
+      return;
+    }
+    constexpr int R = run_of<QT, T>();
+#pragma unroll
+    for (int j = 0; j < G::kRuns; ++j)
+#pragma unroll
+      for (int i = 0; i < R * int(sizeof(T)); i += 16) *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(to + job.what.first(item, j)) + i) = make_uint4(0, 0, 0, 0);
+  };
+  wait_for_launch_before();
+  Job now, next;
+  int64_t unit = blockIdx.x;
+  load(unit, now);
+  while (true) {
+    unit += gridDim.x;
+    if (unit >= units) break;
+    load(unit, next);
+    store(now);
+    now = next;
   }
+  store(now);
+}
+
+template <int QT, typename T, typename I, int A>
+static int launch(Args<I> a, int64_t width, cudaStream_t s) {
+  using G = ItemGeom<QT, run_of<QT, T>()>;
+  const int sms = stream::sm_count();
+  if (sms <= 0) return RC_LAUNCH;
+  a.blocks = int(width / QTraits<QT>::kBlock);
+  if (int64_t(a.blocks) * G::kItems > INT32_MAX) return RC_RANGE;
+  a.items = a.blocks * G::kItems;
+  a.each = std::max(1, kThreads / a.items);
+  a.chunks = (a.items + kThreads - 1) / kThreads;
+  a.groups = (a.count + a.each - 1) / a.each;
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(a.table);
+  const int64_t blocks = a.vocabulary * a.blocks;
+  a.first_edge = begin & 3 ? 0 : -1;
+  a.last_edge = (begin + uintptr_t(blocks) * QTraits<QT>::kBytes) & 3 ? blocks - 1 : -1;
+  a.wide = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
+  return launch_dependent(embedding_kernel<QT, T, I, A>, dim3(unsigned(std::min<int64_t>(a.groups * a.chunks, 5 * int64_t(sms)))), kThreads, 0, 1, s, a);
 }
 
 template <int QT, typename T, typename I>
-static int launch(const void* tokens, const void* table, int64_t vocabulary, void* out, int64_t count, int64_t width, float scale, int* status, cudaStream_t s) {
-  const int sms = stream::sm_count();
-  if (sms <= 0) return RC_LAUNCH;
-  const int units = int(width / 8);
-  // A row in parts of one unit a thread where that leaves SMs without work, else in one.
-  const int parts = count < 4 * sms ? (units + kThreads - 1) / kThreads : 1;
-  const int per_item = parts == 1 ? units : kThreads;
-  const int64_t items = count * parts;
-  const unsigned ctas = unsigned(std::min<int64_t>(items, 8 * int64_t(sms)));
-  return launch_dependent(embedding_kernel<QT, T, I>, dim3(ctas), kThreads, 0, 1, s, static_cast<const I*>(tokens), static_cast<const uint8_t*>(table), vocabulary,
-                          static_cast<T*>(out), items, parts, units, per_item, scale, status);
+static int aligned(const Args<I>& a, int64_t width, cudaStream_t s) {
+  constexpr int kAlign = ItemGeom<QT, run_of<QT, T>()>::kAlign;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(a.table);
+  if constexpr (kAlign == 16)
+    if ((at & 15) == 0) return launch<QT, T, I, 16>(a, width, s);
+  if constexpr (kAlign >= 4)
+    if ((at & 3) == 0) return launch<QT, T, I, 4>(a, width, s);
+  if constexpr (QT == QTYPE_Q4_K) return RC_ALIGN;         // the entry has refused these
+  else return launch<QT, T, I, 1>(a, width, s);
 }
 
 }  // namespace embed
@@ -85,8 +138,19 @@ int embedding(const void* tokens, int token_bytes, const void* table, int64_t vo
     using T = decltype(t);
     auto of_type = [&](auto qt) -> int {
       constexpr int QT = decltype(qt)::value;
-      return token_bytes == 4 ? embed::launch<QT, T, int32_t>(tokens, table, vocabulary, out, count, width, scale, status, s)
-                              : embed::launch<QT, T, int64_t>(tokens, table, vocabulary, out, count, width, scale, status, s);
+      auto with = [&](auto i) {
+        using I = decltype(i);
+        embed::Args<I> a = {};
+        a.tokens = static_cast<const I*>(tokens);
+        a.table = static_cast<const uint8_t*>(table);
+        a.out = out;
+        a.vocabulary = vocabulary;
+        a.count = count;
+        a.scale = scale;
+        a.status = status;
+        return embed::aligned<QT, T, I>(a, width, s);
+      };
+      return token_bytes == 4 ? with(int32_t{}) : with(int64_t{});
     };
     switch (qtype) {
       case QTYPE_Q4_0: return of_type(std::integral_constant<int, QTYPE_Q4_0>{});
