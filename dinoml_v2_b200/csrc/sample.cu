@@ -24,13 +24,12 @@ namespace choice {
 namespace cg = cooperative_groups;
 
 constexpr int kThreads = 1024, kWarps = kThreads / 32, kGroups = 2048, kMaxVocabulary = 262144;
-constexpr int kPart16 = 65528;                   // of a row: counts of 16 bits, whole vectors
-constexpr int kPart32 = 32768;
+constexpr int kPart32 = 32768;                   // of a row, at most
 constexpr double kOne = 35184372088832.;         // 2^45
 
 struct Args {
   const void* logits;
-  int64_t row_stride;
+  int64_t row_stride, rows;
   int vocabulary;
   const float* uniforms;
   DinoB200SampleSettings set;
@@ -61,10 +60,14 @@ __device__ __forceinline__ Row row_of(const Args& a, int64_t row) {
 template <typename T> struct Code;
 template <> struct Code<__nv_bfloat16> {
   static constexpr uint32_t kInf = 0x007f, kMinusInf = 0xff80;
+  static constexpr int kMantissa = 7;
+  static __device__ __forceinline__ float spacing(int binade) { return ldexpf(1.f, max(binade, 1) - 134); }
   static __device__ __forceinline__ float value(uint32_t d) { return __uint_as_float(((d & 0x8000u) ? d : d ^ 0x7fffu) << 16); }
 };
 template <> struct Code<__half> {
   static constexpr uint32_t kInf = 0x03ff, kMinusInf = 0xfc00;
+  static constexpr int kMantissa = 10;
+  static __device__ __forceinline__ float spacing(int binade) { return ldexpf(1.f, max(binade, 1) - 25); }
   static __device__ __forceinline__ float value(uint32_t d) { return __half2float(__ushort_as_half(uint16_t((d & 0x8000u) ? d : d ^ 0x7fffu))); }
 };
 template <> struct Code<float> {
@@ -75,14 +78,9 @@ template <> struct Code<float> {
     return (b & 0x80000000u) ? b : b ^ 0x7fffffffu;
   }
 };
-// Two values at once.
-__device__ __forceinline__ uint32_t codes_of(uint32_t w) {
-  const uint32_t plus = (~w >> 15) & 0x00010001u;
-  uint32_t d = w ^ (plus * 0x7fffu);
-  if ((w & 0xffffu) == 0x8000u) d ^= 0xffffu;              // -0 is 0: 0x8000 -> 0x7fff
-  if ((w >> 16) == 0x8000u) d ^= 0xffff0000u;
-  return d;
-}
+// Two values at once.  -0, code 0x8000, comes right behind 0.
+constexpr uint32_t kZero = 0x7fff, kMinusZero = 0x8000;
+__device__ __forceinline__ uint32_t codes_of(uint32_t w) { return w ^ (((~w >> 15) & 0x00010001u) * 0x7fffu); }
 
 template <typename T> struct Weight {
   uint32_t first;                                // the largest value's code
@@ -130,11 +128,11 @@ template <typename V> __device__ __forceinline__ V warp_running(V v) {
   return v;
 }
 
-// Running sums of 2048 counts and masses in place, by all threads.
-template <typename M> __device__ __forceinline__ void running_sums(uint32_t* count, M* mass, uint32_t* warp_count, M* warp_mass) {
+// Running sums of 2048 counts and masses in place, by all threads; `times` makes the mass of a group of what is there.
+template <typename M, typename F> __device__ __forceinline__ void running_sums(uint32_t* count, M* mass, uint32_t* warp_count, M* warp_mass, F times) {
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const uint32_t c0 = count[2 * t], c1 = c0 + count[2 * t + 1];
-  const M m0 = mass[2 * t], m1 = m0 + mass[2 * t + 1];
+  const M m0 = times(2 * t, mass[2 * t]), m1 = m0 + times(2 * t + 1, mass[2 * t + 1]);
   const uint32_t c = warp_running(c1);
   const M m = warp_running(m1);
   if (lane == 31) {
@@ -168,267 +166,471 @@ __device__ __forceinline__ void answer(const Args& a, int64_t row, int token, fl
 }
 
 // ---- 16-bit logits ------------------------------------------------------------------------------------------------------------------------------------
+// A part is counted in turns of kTurn vectors of eight, behind which the counts that could pass 65535 in the next turn are set aside.
+constexpr int kTurn = 8064, kAside = 65535 - 8 * kTurn - 16, kMostAside = kMaxVocabulary / (kAside + 1) + 2;
+
 struct Decision {
   int owner, place;
   uint32_t code;
 };
 struct Shared16 {
   uint32_t counts[32768];                        // word d & 0x7fff: of code d in its upper half if d >= 0x8000, else in its lower half
-  double mass[kGroups];
+  double mass[kGroups];                          // of groups of 32 codes, then running; the first CTA's
   uint32_t count[kGroups];
+  double power[kWarps][32];                      // of a binade: the weights of a group's values relative to its first one's
+  double first_mass;                             // of the largest value's group
   double warp_mass[kWarps];
   uint32_t warp_count[kWarps];
   uint32_t least, most;                          // codes of this part
+  uint32_t all_least[8], all_most[8];            // of all parts
+  uint32_t some[8][2][kGroups / 64];             // of all parts: which groups have anything
+  uint32_t aside, aside_code[kMostAside], aside_count[kMostAside];
   Decision decision;
 };
 
-template <typename T>
+template <typename T, int ctas>
 __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
   extern __shared__ __align__(16) uint8_t raw[];
   Shared16& sh = *reinterpret_cast<Shared16*>(raw);
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int ctas = int(cluster.num_blocks()), rank = int(cluster.block_rank());
-  const int64_t row = blockIdx.x / ctas;
-  for (int i = tid; i < 32768 / 4; i += kThreads) reinterpret_cast<uint4*>(sh.counts)[i] = make_uint4(0, 0, 0, 0);
-  if (tid == 0) {
-    sh.least = 0xffffu;
-    sh.most = 0;
-  }
-  wait_for_launch_before();
-  __syncthreads();
-  const Row set = row_of(a, row);
-
-  // This part of the row: values up to an address that is a multiple of 16, vectors of eight, the rest.
+  const int rank = ctas > 1 ? int(cluster.block_rank()) : 0;
+  auto meet = [&] {
+    if (ctas > 1) cluster.sync(); else __syncthreads();
+  };
+  auto of_rank = [&](auto* p, int r) {           // p of another CTA
+    if constexpr (ctas > 1) return cluster.map_shared_rank(p, r); else return p;
+  };
   const int part = ((a.vocabulary + ctas - 1) / ctas + 7) & ~7;
   const int begin = min(rank * part, a.vocabulary), length = min(part, a.vocabulary - begin);
-  const uint16_t* x = static_cast<const uint16_t*>(a.logits) + row * a.row_stride + begin;
-  const int head = min(int((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / 2, length);
-  const int vectors = (length - head) / 8, rest = length - head - 8 * vectors;
-  const uint4* wide = reinterpret_cast<const uint4*>(x + head);
-  uint32_t least = 0xffffffffu, most = 0;
-  auto add = [&](uint32_t two) {
-    const uint32_t d = codes_of(two);
-    least = __vminu2(least, d);
-    most = __vmaxu2(most, d);
-    atomicAdd(&sh.counts[d & 0x7fffu], (d & 0x8000u) ? 0x10000u : 1u);
-    atomicAdd(&sh.counts[(d >> 16) & 0x7fffu], (d >> 31) ? 0x10000u : 1u);
-  };
-  auto add_one = [&](uint32_t v) {
-    const uint32_t d = codes_of(v) & 0xffffu;
-    least = __vminu2(least, d | d << 16);
-    most = __vmaxu2(most, d | d << 16);
-    atomicAdd(&sh.counts[d & 0x7fffu], (d & 0x8000u) ? 0x10000u : 1u);
-  };
-  constexpr int kAhead = 4;
-  for (int v = tid; v < vectors; v += kAhead * kThreads) {
-    uint4 q[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-      if (v + i * kThreads < vectors) q[i] = kv::fetch(wide + v + i * kThreads);
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      if (v + i * kThreads >= vectors) break;
-      add(q[i].x);
-      add(q[i].y);
-      add(q[i].z);
-      add(q[i].w);
+  bool waited = false;
+  for (int64_t row = blockIdx.x / ctas, step = gridDim.x / ctas; row < a.rows; row += step) {
+    for (int i = tid; i < 32768 / 4; i += kThreads) reinterpret_cast<uint4*>(sh.counts)[i] = make_uint4(0, 0, 0, 0);
+    if (rank == 0) {
+      for (int i = tid; i < kGroups; i += kThreads) {
+        sh.mass[i] = 0.;
+        sh.count[i] = 0;
+      }
     }
-  }
-  if (tid < head) add_one(x[tid]);
-  if (tid < rest) add_one(x[head + 8 * vectors + tid]);
-  least = __reduce_min_sync(0xffffffffu, min(least & 0xffffu, least >> 16));
-  most = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
-  if (lane == 0) {
-    atomicMin(&sh.least, least);
-    atomicMax(&sh.most, most);
-  }
-  cluster.sync();
+    if (tid == 0) {
+      sh.least = 0xffffu;
+      sh.most = 0;
+      sh.aside = 0;
+    }
+    if (!waited) wait_for_launch_before();
+    waited = true;
+    __syncthreads();
+    const Row set = row_of(a, row);
 
-  least = 0xffffu;
-  most = 0;
-  if (lane < ctas) {
-    least = *cluster.map_shared_rank(&sh.least, lane);
-    most = *cluster.map_shared_rank(&sh.most, lane);
-  }
-  least = __reduce_min_sync(0xffffffffu, least);
-  most = __reduce_max_sync(0xffffffffu, most);
-  const uint32_t first = least;
-  if (!set.valid || first < Code<T>::kInf || most > Code<T>::kMinusInf || first >= Code<T>::kMinusInf) {
-    if (rank == 0 && tid == 0) {
-      if (!set.valid) kv::flag_range(a.status);
-      answer(a, row, -1, 0.f);
-    }
-    cluster.sync();                              // (others may be reading this part's codes)
-    return;
-  }
-  const Weight<T> weight(first, set.temperature);
-  Shared16* lead = cluster.map_shared_rank(&sh, 0);
-  if (!set.first) {
-    // Sums of groups: 32 words are a group of large and one of small values.  Neighbours go to different CTAs and warps, since the values lie close together.
-    for (int g = rank + ctas * warp; g < kGroups / 2; g += ctas * kWarps) {
-      uint32_t low = 0, high = 0;
-      for (int c = 0; c < ctas; ++c) {
-        const uint32_t w = cluster.map_shared_rank(sh.counts, c)[g * 32 + lane];
-        low += w & 0xffffu;
-        high += w >> 16;
-      }
+    // This part of the row: values up to an address that is a multiple of 16, vectors of eight, the rest.
+    const uint16_t* x = static_cast<const uint16_t*>(a.logits) + row * a.row_stride + begin;
+    const int head = min(int((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / 2, length);
+    const int vectors = (length - head) / 8, rest = length - head - 8 * vectors;
+    const uint4* wide = reinterpret_cast<const uint4*>(x + head);
+    uint32_t least = 0xffffffffu, most = 0;
+    auto add = [&](uint32_t two) {
+      const uint32_t plus = (~two >> 15) & 0x00010001u, minus = plus ^ 0x00010001u, d = two ^ (plus * 0x7fffu);
+      least = __vminu2(least, d);
+      most = __vmaxu2(most, d);
+      // 1 in the lower half of a positive value's word, in the upper one of a negative's
+      atomicAdd(&sh.counts[d & 0x7fffu], __byte_perm(plus, minus, 0x1410));
+      atomicAdd(&sh.counts[d >> 16 & 0x7fffu], __byte_perm(plus, minus, 0x1612));
+    };
+    auto add_one = [&](uint32_t v) {
+      const uint32_t d = codes_of(v) & 0xffffu;
+      least = __vminu2(least, d | d << 16);
+      most = __vmaxu2(most, d | d << 16);
+      atomicAdd(&sh.counts[d & 0x7fffu], (d & 0x8000u) ? 0x10000u : 1u);
+    };
+    const int turns = max(1, (vectors + kTurn - 1) / kTurn);
+    for (int turn = 0; turn < turns; ++turn) {
+      const int end = min(vectors, (turn + 1) * kTurn);
+      // two vectors of a thread are counted while two more are on their way
+      uint4 q[2], r[2];
+      int v = turn * kTurn + tid;
+      auto load = [&](uint4 (&to)[2], int at) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t d = uint32_t(g * 32 + lane) + half * 0x8000u, n = half == 0 ? low : d < Code<T>::kMinusInf ? high : 0u;
-        uint32_t count = 0;
-        double mass = 0.;
-        if (__any_sync(0xffffffffu, n != 0)) {
-          count = __reduce_add_sync(0xffffffffu, n);
-          mass = n != 0 ? double(n) * weight(d) : 0.;
+        for (int i = 0; i < 2; ++i)
+          if (at + i * kThreads < end) to[i] = kv::fetch(wide + at + i * kThreads);
+      };
+      auto use = [&](const uint4 (&of)[2], int at) {
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+        for (int i = 0; i < 2; ++i) {
+          if (at + i * kThreads >= end) break;
+          add(of[i].x);
+          add(of[i].y);
+          add(of[i].z);
+          add(of[i].w);
         }
-        if (lane == 0) {
-          lead->count[g + half * (kGroups / 2)] = count;
-          lead->mass[g + half * (kGroups / 2)] = mass;
+      };
+      load(q, v);
+      for (; v < end; v += 4 * kThreads) {
+        load(r, v + 2 * kThreads);
+        use(q, v);
+        load(q, v + 4 * kThreads);
+        use(r, v + 2 * kThreads);
+      }
+      if (turn + 1 < turns) {
+        __syncthreads();
+        for (int i = tid; i < 32768 / 4; i += kThreads) {
+          const uint4 q = reinterpret_cast<const uint4*>(sh.counts)[i];
+          const uint32_t top = __vmaxu2(__vmaxu2(q.x, q.y), __vmaxu2(q.z, q.w));
+          if (max(top & 0xffffu, top >> 16) <= uint32_t(kAside)) continue;
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t w = sh.counts[4 * i + j / 2], n = j & 1 ? w >> 16 : w & 0xffffu, d = uint32_t(4 * i + j / 2) + (j & 1) * 0x8000u;
+            if (n <= uint32_t(kAside)) continue;
+            const uint32_t at = atomicAdd(&sh.aside, 1u);
+            sh.aside_code[at] = d == kMinusZero ? kZero : d;
+            sh.aside_count[at] = n;
+            sh.counts[4 * i + j / 2] = w - (j & 1 ? n << 16 : n);
+          }
+        }
+        __syncthreads();
+      }
+    }
+    if (tid < head) add_one(x[tid]);
+    if (tid < rest) add_one(x[head + 8 * vectors + tid]);
+    if (tid == 0 && row + step < a.rows) {       // the next row's part, while this one is worked on
+      const uint16_t* ahead = x + step * a.row_stride;
+      const int skip = min(int((16 - (reinterpret_cast<uintptr_t>(ahead) & 15)) & 15) / 2, length), bytes = (length - skip) / 8 * 16;
+      if (bytes > 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"(ahead + skip), "r"(bytes) : "memory");
+    }
+    least = __reduce_min_sync(0xffffffffu, min(least & 0xffffu, least >> 16));
+    most = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
+    if (lane == 0) {
+      atomicMin(&sh.least, least == kMinusZero ? kZero : least);
+      atomicMax(&sh.most, most);
+    }
+    __syncthreads();
+    if (tid == 0) {                              // -0 is 0
+      const uint32_t minus = sh.counts[kMinusZero & 0x7fffu] >> 16;
+      if (minus > 0) {
+        sh.counts[kMinusZero & 0x7fffu] -= minus << 16;
+        if (turns == 1) {
+          sh.counts[kZero] += minus;
+        } else {
+          sh.aside_code[sh.aside] = kZero;
+          sh.aside_count[sh.aside++] = minus;
         }
       }
     }
-  }
-  cluster.sync();
-  if (rank == 0) {
-    if (!set.first) running_sums(sh.count, sh.mass, sh.warp_count, sh.warp_mass);
-    if (warp == 0) {
-      uint32_t code = first;
-      int place = 0;
-      double share = 1.;
-      if (!set.first) {
-        // One group: how often each of its values is there, its weight, running sums before and with it.
-        uint32_t n, n_with;
-        double w, m_before, m_with;
-        auto open = [&](int g) {
-          const int word = (g & (kGroups / 2 - 1)) * 32 + lane;
-          n = 0;
-          for (int c = 0; c < ctas; ++c) {
-            const uint32_t v = cluster.map_shared_rank(sh.counts, c)[word];
-            n += g < kGroups / 2 ? v & 0xffffu : v >> 16;
-          }
-          const uint32_t d = uint32_t(g * 32 + lane);
-          if (d >= Code<T>::kMinusInf) n = 0;
-          w = n != 0 ? weight(d) : 0.;
-          n_with = (g > 0 ? sh.count[g - 1] : 0u) + warp_running(n);
-          const double own = warp_running(double(n) * w), base = g > 0 ? sh.mass[g - 1] : 0.;
-          const double up = __shfl_up_sync(0xffffffffu, own, 1);
-          m_before = base + (lane > 0 ? up : 0.);
-          m_with = base + own;
-        };
-        auto pick = [&](bool passes) {           // the first lane that passes, or the last that has anything
-          const uint32_t hit = __ballot_sync(0xffffffffu, passes && n != 0), any = __ballot_sync(0xffffffffu, n != 0);
-          return hit != 0 ? __ffs(hit) - 1 : any != 0 ? 31 - __clz(any) : 0;
-        };
-        auto from = [&](auto v, int l) { return __shfl_sync(0xffffffffu, v, l); };
-        uint32_t end = 0xffffu, take = 0xffffffffu;      // kept: what comes before code `end`, and `take` of it
-        double kept = sh.mass[kGroups - 1];              // the sum of the kept
-        if (set.top_k > 0 && uint32_t(set.top_k) < sh.count[kGroups - 1]) {
-          const uint32_t k = uint32_t(set.top_k);
-          const int g = first_of([&](int i) { return sh.count[i] >= k; });
-          open(g);
-          const int l = pick(n_with >= k);
-          end = uint32_t(g * 32 + l);
-          take = k - from(n_with - n, l);
-          kept = from(m_before, l) + double(take) * from(w, l);
-        }
-        if (set.top_p < 1.f) {
-          const double wanted = double(set.top_p) * kept;
-          const int g = first_of([&](int i) { return sh.mass[i] >= wanted; });
-          open(g);
-          const int l = pick(m_with >= wanted);
-          const uint32_t e = uint32_t(g * 32 + l), c = from(n, l);
-          const double we = from(w, l), before = from(m_before, l), some = we > 0. ? ceil((wanted - before) / we) : 1.;
-          const uint32_t t = uint32_t(fmin(fmax(some, 1.), double(c)));
-          if (e < end || (e == end && t < take)) {
-            end = e;
-            take = t;
-            kept = before + double(t) * we;
-          }
-        }
-        if (set.min_p > 0.f) {
-          const uint32_t e = last_that(first, Code<T>::kMinusInf - 1, [&](uint32_t d) { return weight(d) >= double(set.min_p); });
-          if (e < end) {
-            open(int(e >> 5));
-            end = e;
-            take = 0xffffffffu;
-            kept = from(m_with, int(e & 31));
-          }
-        }
-        const double target = double(set.u) * kept;
-        const int g = first_of([&](int i) { return sh.mass[i] > target; });
-        open(g);
-        const int l = pick(m_with > target);
-        code = uint32_t(g * 32 + l);
-        const double wc = from(w, l), there = wc > 0. ? floor((target - from(m_before, l)) / wc) : 0.;
-        uint32_t most_place = from(n, l) - 1;
-        if (code == end && take <= most_place) most_place = take - 1;
-        place = int(fmin(fmax(there, 0.), double(most_place)));
-        share = wc / kept;
+    if constexpr (ctas > 1) {
+      __syncthreads();
+      // Which groups have anything here, told to all: the others read no more of this part than that.
+      uint32_t any = 0;                          // a lane has a group of 32 words
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint4 q = reinterpret_cast<const uint4*>(sh.counts)[(warp * 32 + lane) * 8 + ((i + lane) & 7)];
+        any |= q.x | q.y | q.z | q.w;
       }
-      // Whose part has it: the equals of the parts before come first.
-      uint32_t mine = 0;
+      const uint32_t low = __ballot_sync(0xffffffffu, (any & 0xffffu) != 0), high = __ballot_sync(0xffffffffu, (any >> 16) != 0);
       if (lane < ctas) {
-        const uint32_t v = cluster.map_shared_rank(sh.counts, lane)[code & 0x7fffu];
-        mine = (code & 0x8000u) ? v >> 16 : v & 0xffffu;
+        Shared16* other = of_rank(&sh, lane);
+        other->some[rank][0][warp] = low;
+        other->some[rank][1][warp] = high;
+        if (warp == 0) {
+          other->all_least[rank] = sh.least;
+          other->all_most[rank] = sh.most;
+        }
       }
-      const uint32_t with = warp_running(mine), hit = __ballot_sync(0xffffffffu, int(with) > place);
-      const int owner = __ffs(hit) - 1, before = int(__shfl_sync(0xffffffffu, with - mine, owner & 31));
-      if (lane < ctas) *cluster.map_shared_rank(&sh.decision, lane) = Decision{owner, place - before, code};
-      if (lane == 0 && a.probabilities != nullptr) a.probabilities[row] = float(share);
+      cluster.sync();
+      least = __reduce_min_sync(0xffffffffu, lane < ctas ? sh.all_least[lane] : 0xffffu);
+      most = __reduce_max_sync(0xffffffffu, lane < ctas ? sh.all_most[lane] : 0u);
+    } else {
+      __syncthreads();
+      least = sh.least;
+      most = sh.most;
     }
-  }
-  cluster.sync();
-  const Decision what = sh.decision;
-  if (what.owner != rank) return;
 
-  // The place-th of its equals in this part.  A warp has a piece of the part; slots are the values before the vectors, the vectors, the rest.
-  const int slots = vectors + 2, each = (slots + kWarps - 1) / kWarps, from_slot = warp * each, to_slot = min(from_slot + each, slots);
-  auto hits_of = [&](int slot) -> uint32_t {     // bit i: value i of the slot is one
-    uint32_t hits = 0;
-    if (slot >= to_slot) return 0;
-    if (slot > 0 && slot <= vectors) {
-      const uint4 q = kv::fetch(wide + slot - 1);
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    const uint32_t first = least;
+    if (!set.valid || first < Code<T>::kInf || most > Code<T>::kMinusInf || first >= Code<T>::kMinusInf) {
+      if (rank == 0 && tid == 0) {
+        if (!set.valid) kv::flag_range(a.status);
+        answer(a, row, -1, 0.f);
+      }
+      meet();                                    // (others may be reading what the next row begins with)
+      continue;
+    }
+    const Weight<T> weight(first, set.temperature);
+    if (!set.first) {
+      Shared16* lead = of_rank(&sh, 0);
+      // Blocks of 32 groups are a CTA's each, in turn: it adds the other parts' counts to its own.  What passes 65535 is set aside.
+      if constexpr (ctas > 1) {
+        for (int i = warp; i < 1024 / ctas; i += kWarps) {
+          const int g = ((i >> 5) * ctas + rank) * 32 + (i & 31);                         // group of words
+          const uint32_t bit = 1u << (g & 31);
+          uint32_t low = 0, high = 0, others = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t d = codes_of(w[i]);
-        if ((d & 0xffffu) == what.code) hits |= 1u << (2 * i);
-        if ((d >> 16) == what.code) hits |= 2u << (2 * i);
+          for (int r = 0; r < ctas; ++r) {
+            const bool there = ((sh.some[r][0][g >> 5] | sh.some[r][1][g >> 5]) & bit) != 0;
+            if (!there) continue;
+            const uint32_t w = of_rank(sh.counts, r)[g * 32 + lane];
+            low += w & 0xffffu;
+            high += w >> 16;
+            others |= r != rank;
+          }
+          if (others == 0) continue;
+          sh.counts[g * 32 + lane] = min(low, 65535u) | min(high, 65535u) << 16;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t n = half ? high : low;
+            if (n <= 65535u) continue;
+            const uint32_t at = atomicAdd(&lead->aside, 1u);
+            lead->aside_code[at] = uint32_t(g * 32 + lane) + half * 0x8000u;
+            lead->aside_count[at] = n - 65535u;
+          }
+        }
       }
+      // Sums of groups of 32 values, a lane a group.  The values of a binade are equally far apart, so that the weights of a group are powers, w0 q^j, and q^j is the same for all groups of
+      // a binade: a lane adds up its counts times these, from a place on where no other lane has its bank, and w0 comes later (group_weight).  So exponentials are few: 32 of powers, one
+      // for a group.  The largest value's group is summed value by value, so that its weight is one.
+      constexpr int kMantissa = Code<T>::kMantissa;
+      // Powers of 32 binades: all of float16's; of bfloat16 those from the largest value's down 24 and up 7, where it is negative up 31.
+      const int lowest = kMantissa == 10 ? 0 : max(0, first < 0x8000u ? int((0x7fffu - first) >> kMantissa) - 24 : int((first & 0x7fffu) >> kMantissa));
+      auto step_of = [&](int binade) { return -double(Code<T>::spacing(binade)) * weight.inverse; };
+      sh.power[warp][lane] = exp(step_of(lowest + warp) * double(lane));
+      __syncthreads();
+      for (int task = warp; task < 64 / ctas; task += kWarps) {
+        const uint32_t half = task & 1, group0 = uint32_t((task >> 1) * ctas + rank) * 32, task0 = group0 * 32 + half * 0x8000u;
+        if (task0 > most || task0 + 1024 <= first || task0 >= Code<T>::kMinusInf) continue;
+        const uint32_t code0 = task0 + lane * 32;
+        const int binade = int((half ? code0 & 0x7fffu : 0x7fffu - code0) >> kMantissa);
+        const bool known = unsigned(binade - lowest) < 32u;
+        const double* power = sh.power[known ? binade - lowest : 0];
+        const uint32_t* counts = sh.counts + (group0 + lane) * 32;
+        const uint32_t shift = half * 16;
+        uint32_t n = 0;
+        double mass = 0.;
+        if (__any_sync(0xffffffffu, !known)) {             // (far from where the largest value is: bfloat16)
+          for (int i = 0; i < 32; ++i) {
+            const int j = (i + lane) & 31;
+            const uint32_t c = counts[j] >> shift & 0xffffu;
+            n += c;
+            if (c != 0) mass = ::fma(double(c), exp(step_of(binade) * double(j)), mass);
+          }
+        } else {
+#pragma unroll 8
+          for (int i = 0; i < 32; ++i) {
+            const int j = (i + lane) & 31;
+            const uint32_t c = counts[j] >> shift & 0xffffu;
+            n += c;
+            mass = ::fma(double(c), power[j], mass);
+          }
+        }
+        if (code0 < Code<T>::kMinusInf && n != 0) {
+          lead->count[code0 >> 5] = n;
+          lead->mass[code0 >> 5] = mass;
+        }
+        if (first >= task0 && first < task0 + 1024) {      // (the whole warp)
+          const uint32_t d = (first & ~31u) + lane, c = sh.counts[d & 0x7fffu] >> shift & 0xffffu;
+          double m = c != 0 ? double(c) * weight(d) : 0.;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+          if (lane == 0) lead->first_mass = m;
+        }
+      }
+    }
+    meet();
+    if (rank == 0) {
+      if (!set.first) {
+        const uint32_t aside = sh.aside;
+        if (aside > 0) {                         // what was set aside: few, and in the order of codes and counts, whoever came first
+          uint32_t code = 0, count = 0, before = 0;
+          if (tid < int(aside)) {
+            code = sh.aside_code[tid];
+            count = sh.aside_count[tid];
+            for (int i = 0; i < int(aside); ++i) {
+              const uint32_t c = sh.aside_code[i], n = sh.aside_count[i];
+              before += c < code || (c == code && (n < count || (n == count && i < tid))) ? 1u : 0u;
+            }
+          }
+          __syncthreads();
+          if (tid < int(aside)) {
+            sh.aside_code[before] = code;
+            sh.aside_count[before] = count;
+          }
+          __syncthreads();
+          if (tid == 0) {
+            for (uint32_t i = 0; i < aside; ++i) {
+              const uint32_t d = sh.aside_code[i];
+              if (d < first || d >= Code<T>::kMinusInf) continue;
+              const double times = double(sh.aside_count[i]);
+              sh.count[d >> 5] += sh.aside_count[i];
+              if (d >> 5 == first >> 5) sh.first_mass += times * weight(d);
+              else sh.mass[d >> 5] += times * exp(-double(Code<T>::spacing(int(((d & 0x8000u) ? d & 0x7fffu : 0x7fffu - d) >> Code<T>::kMantissa))) * weight.inverse * double(d & 31u));
+            }
+          }
+          __syncthreads();
+        }
+        auto group_weight = [&](int g, double powers) {    // (before the largest value there is nothing)
+          if (uint32_t(g) == first >> 5) return sh.first_mass;
+          return powers > 0. && !weight.infinite ? powers * exp((double(Code<T>::value(uint32_t(g) * 32)) - weight.largest) * weight.inverse) : 0.;
+        };
+        running_sums(sh.count, sh.mass, sh.warp_count, sh.warp_mass, group_weight);
+      }
+      if (warp == 0) {
+        uint32_t code = first;
+        int place = 0;
+        double share = 1.;
+        if (!set.first) {
+          // One group: how often each of its values is there, its weight, running sums before and with it.
+          uint32_t n, n_with;
+          double w, m_before, m_with;
+          auto open = [&](int g) {
+            const int word = (g & (kGroups / 2 - 1)) * 32 + lane;
+            const uint32_t d = uint32_t(g * 32 + lane);
+            const uint32_t v = of_rank(sh.counts, (word >> 10) % ctas)[word];
+            n = g < kGroups / 2 ? v & 0xffffu : v >> 16;
+            for (uint32_t i = 0; i < sh.aside; ++i)
+              if (sh.aside_code[i] == d) n += sh.aside_count[i];
+            if (d >= Code<T>::kMinusInf) n = 0;  // (and what stands for NaN is not there)
+            w = n != 0 ? weight(d) : 0.;
+            n_with = (g > 0 ? sh.count[g - 1] : 0u) + warp_running(n);
+            const double own = warp_running(double(n) * w), base = g > 0 ? sh.mass[g - 1] : 0.;
+            const double up = __shfl_up_sync(0xffffffffu, own, 1);
+            m_before = base + (lane > 0 ? up : 0.);
+            m_with = base + own;
+          };
+          auto pick = [&](bool passes) {         // the first lane that passes, or the last that has anything
+            const uint32_t hit = __ballot_sync(0xffffffffu, passes && n != 0), any = __ballot_sync(0xffffffffu, n != 0);
+            return hit != 0 ? __ffs(hit) - 1 : any != 0 ? 31 - __clz(any) : 0;
+          };
+          auto from = [&](auto v, int l) { return __shfl_sync(0xffffffffu, v, l); };
+          uint32_t end = 0xffffu, take = 0xffffffffu;      // kept: what comes before code `end`, and `take` of it
+          double kept = sh.mass[kGroups - 1];              // the sum of the kept
+          if (set.top_k > 0 && uint32_t(set.top_k) < sh.count[kGroups - 1]) {
+            const uint32_t k = uint32_t(set.top_k);
+            const int g = first_of([&](int i) { return sh.count[i] >= k; });
+            open(g);
+            const int l = pick(n_with >= k);
+            end = uint32_t(g * 32 + l);
+            take = k - from(n_with - n, l);
+            kept = from(m_before, l) + double(take) * from(w, l);
+          }
+          if (set.top_p < 1.f) {
+            const double wanted = double(set.top_p) * kept;
+            const int g = first_of([&](int i) { return sh.mass[i] >= wanted; });
+            open(g);
+            const int l = pick(m_with >= wanted);
+            const uint32_t e = uint32_t(g * 32 + l), c = from(n, l);
+            const double we = from(w, l), before = from(m_before, l), some = we > 0. ? ceil((wanted - before) / we) : 1.;
+            const uint32_t t = uint32_t(fmin(fmax(some, 1.), double(c)));
+            if (e < end || (e == end && t < take)) {
+              end = e;
+              take = t;
+              kept = before + double(t) * we;
+            }
+          }
+          if (set.min_p > 0.f) {
+            const uint32_t e = last_that(first, Code<T>::kMinusInf - 1, [&](uint32_t d) { return weight(d) >= double(set.min_p); });
+            if (e < end) {
+              open(int(e >> 5));
+              end = e;
+              take = 0xffffffffu;
+              kept = from(m_with, int(e & 31));
+            }
+          }
+          const double target = double(set.u) * kept;
+          const int g = first_of([&](int i) { return sh.mass[i] > target; });
+          open(g);
+          const int l = pick(m_with > target);
+          code = uint32_t(g * 32 + l);
+          const double wc = from(w, l), there = wc > 0. ? floor((target - from(m_before, l)) / wc) : 0.;
+          uint32_t most_place = from(n, l) - 1;
+          if (code == end && take <= most_place) most_place = take - 1;
+          place = int(fmin(fmax(there, 0.), double(most_place)));
+          share = wc / kept;
+        }
+        // Whose part has it: the equals of the parts before come first.
+        int owner = 0, before = 0;
+        if (ctas > 1) {
+          uint32_t mine = 0;
+          const int adder = int(code >> 10 & 31u) % ctas;          // which has all parts' there, unless nobody added
+          if (lane < ctas) {
+            const uint32_t v = of_rank(sh.counts, lane)[code & 0x7fffu];
+            mine = (code & 0x8000u) ? v >> 16 : v & 0xffffu;
+          }
+          if (!set.first) {
+            for (uint32_t i = 0; i < sh.aside; ++i)
+              if (sh.aside_code[i] == code && lane == adder) mine += sh.aside_count[i];
+            const uint32_t all = __shfl_sync(0xffffffffu, mine, adder), theirs = __reduce_add_sync(0xffffffffu, lane != adder ? mine : 0u);
+            if (lane == adder) mine = all - theirs;
+          }
+          const uint32_t with = warp_running(mine), hit = __ballot_sync(0xffffffffu, int(with) > place);
+          owner = __ffs(hit) - 1;
+          before = int(__shfl_sync(0xffffffffu, with - mine, owner & 31));
+        }
+        if (lane < ctas) *of_rank(&sh.decision, lane) = Decision{owner, place - before, code};
+        if (lane == 0 && a.probabilities != nullptr) a.probabilities[row] = float(share);
+      }
+    }
+    meet();
+    const Decision what = sh.decision;
+    if (what.owner != rank) continue;
+
+    // The place-th of its equals in this part.  A warp has a piece of the part; slots are the values before the vectors, the vectors, the rest.
+    const int slots = vectors + 2, each = (slots + kWarps - 1) / kWarps, from_slot = warp * each, to_slot = min(from_slot + each, slots);
+    // As they are in memory: one pattern, of zero two.
+    const uint32_t bits = (what.code & 0x8000u) ? what.code : what.code ^ 0x7fffu, here = bits * 0x10001u, also = bits == 0 ? 0x80008000u : here;
+    auto hits_of = [&](int slot) -> uint32_t {   // bit i: value i of the slot is one
+      uint32_t hits = 0;
+      if (slot >= to_slot) return 0;
+      if (slot > 0 && slot <= vectors) {
+        const uint4 q = kv::fetch(wide + slot - 1);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+        uint32_t zeros = 0;                      // a half that is zero takes a borrow
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t t = w[i] ^ here, u = w[i] ^ also;
+          zeros |= ((t - 0x00010001u) & ~t) | ((u - 0x00010001u) & ~u);
+        }
+        if ((zeros & 0x80008000u) == 0) return 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t t = w[i] ^ here, u = w[i] ^ also;
+          if ((t & 0xffffu) == 0 || (u & 0xffffu) == 0) hits |= 1u << (2 * i);
+          if ((t >> 16) == 0 || (u >> 16) == 0) hits |= 2u << (2 * i);
+        }
+        return hits;
+      }
+      const int at = slot == 0 ? 0 : head + 8 * vectors, n = slot == 0 ? head : rest;
+      for (int i = 0; i < n; ++i)
+        if (x[at + i] == (here & 0xffffu) || x[at + i] == (also & 0xffffu)) hits |= 1u << i;
       return hits;
+    };
+    uint32_t found = 0;
+    uint64_t seen = 0;                           // bit i: there was something in turn i
+#pragma unroll 4
+    for (int s = from_slot; s < to_slot; s += 32) {
+      const uint32_t hits = hits_of(s + lane);
+      found += __popc(hits);
+      seen |= uint64_t(hits != 0) << ((s - from_slot) >> 5);
     }
-    const int at = slot == 0 ? 0 : head + 8 * vectors, n = slot == 0 ? head : rest;
-    for (int i = 0; i < n; ++i)
-      if ((codes_of(x[at + i]) & 0xffffu) == what.code) hits |= 1u << i;
-    return hits;
-  };
-  uint32_t found = 0;
-  for (int s = from_slot; s < to_slot; s += 32) found += __popc(hits_of(s + lane));
-  found = __reduce_add_sync(0xffffffffu, found);
-  if (lane == 0) sh.warp_count[warp] = found;
-  __syncthreads();
-  const uint32_t with = warp_running(sh.warp_count[lane]);
-  const uint32_t place = uint32_t(what.place);
-  const uint32_t hit = __ballot_sync(0xffffffffu, with > place);
-  if (hit == 0 || __ffs(hit) - 1 != warp) return;
-  uint32_t left = place - (warp > 0 ? __shfl_sync(0xffffffffu, with, warp > 0 ? warp - 1 : 0) : 0u);
-  for (int s = from_slot; s < to_slot; s += 32) {
-    uint32_t hits = hits_of(s + lane);
-    const uint32_t c = __popc(hits), run = warp_running(c), all = __shfl_sync(0xffffffffu, run, 31);
-    if (left < all) {
-      if (run > left && run - c <= left) {
-        for (uint32_t skip = left - (run - c); skip > 0; --skip) hits &= hits - 1;
-        const int slot = s + lane, bit = __ffs(hits) - 1;
-        a.tokens[row] = begin + (slot == 0 ? 0 : head + 8 * (slot - 1)) + bit;
+    found = __reduce_add_sync(0xffffffffu, found);
+    seen = __reduce_or_sync(0xffffffffu, uint32_t(seen)) | uint64_t(__reduce_or_sync(0xffffffffu, uint32_t(seen >> 32))) << 32;
+    if (lane == 0) sh.warp_count[warp] = found;
+    __syncthreads();
+    const uint32_t with = warp_running(sh.warp_count[lane]), place = uint32_t(what.place), hit = __ballot_sync(0xffffffffu, with > place);
+    if (hit != 0 && __ffs(hit) - 1 == warp) {
+      uint32_t left = place - (warp > 0 ? __shfl_sync(0xffffffffu, with, warp > 0 ? warp - 1 : 0) : 0u);
+      for (; seen != 0; seen &= seen - 1) {
+        const int s = from_slot + (__ffsll(int64_t(seen)) - 1) * 32;
+        uint32_t hits = hits_of(s + lane);
+        const uint32_t c = __popc(hits), run = warp_running(c), all = __shfl_sync(0xffffffffu, run, 31);
+        if (left < all) {
+          if (run > left && run - c <= left) {
+            for (uint32_t skip = left - (run - c); skip > 0; --skip) hits &= hits - 1;
+            const int slot = s + lane, bit = __ffs(hits) - 1;
+            a.tokens[row] = begin + (slot == 0 ? 0 : head + 8 * (slot - 1)) + bit;
+          }
+          break;
+        }
+        left -= all;
       }
-      return;
     }
-    left -= all;
   }
 }
+static_assert(kMaxVocabulary / 8 + 2 <= 64 * 32 * kWarps, "turns of a search in 64 bits");
 
 // ---- float32 logits -----------------------------------------------------------------------------------------------------------------------------------
 struct Place {                                   // a range of codes, what comes before it, what is in it
@@ -539,7 +741,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
       lead->mass[i] = m;
     }
     cluster.sync();
-    if (rank == 0) running_sums(sh.count, sh.mass, sh.warp_count, sh.warp_mass);
+    auto as_it_is = [](int, unsigned long long m) { return m; };
+    if (rank == 0) running_sums(sh.count, sh.mass, sh.warp_count, sh.warp_mass, as_it_is);
     // The place where the running count reaches `count` (by_count) or the running sum reaches, or with `above` passes, `mass`.
     int turn = 0;
     auto descend = [&](bool by_count, uint32_t count, double mass, bool above) -> Place {
@@ -569,7 +772,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
         }
         cluster.sync();
         if (rank == 0) {
-          running_sums(sh.range_count, sh.range_mass, sh.warp_count, sh.warp_mass);
+          running_sums(sh.range_count, sh.range_mass, sh.warp_count, sh.warp_mass, as_it_is);
           if (warp == 0) {
             const int g = first_of([&](int i) { return passes(p.count_before + sh.range_count[i], p.mass_before + sh.range_mass[i]); });
             const uint32_t c = g > 0 ? sh.range_count[g - 1] : 0u;
@@ -685,15 +888,21 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
   }
 }
 
-template <typename T> static int launch16(const Args& a, int64_t rows, cudaStream_t s) {
+template <typename T, int C> static int launch16_of(const Args& a, int sms, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
-  if (int rc = allow_shared(sample16_kernel<T>, sizeof(Shared16), done)) return rc;
+  if (int rc = allow_shared(sample16_kernel<T, C>, sizeof(Shared16), done)) return rc;
+  // As many clusters as run at once; each takes rows in turn.
+  return launch_dependent(sample16_kernel<T, C>, dim3(unsigned(std::min<int64_t>(a.rows, std::max(1, sms / C)) * C)), kThreads, sizeof(Shared16), C, s, a);
+}
+template <typename T> static int launch16(const Args& a, cudaStream_t s) {
   const int sms = stream::sm_count();
   if (sms <= 0) return RC_LAUNCH;
-  unsigned ctas = 1;
-  while (ctas < 8 && (a.vocabulary + int(ctas) - 1) / int(ctas) > kPart16) ctas *= 2;
-  while (ctas < 8 && rows * ctas * 2 <= sms && a.vocabulary / int(ctas) > 4096) ctas *= 2;
-  return launch_dependent(sample16_kernel<T>, dim3(unsigned(rows * ctas)), kThreads, sizeof(Shared16), ctas, s, a);
+  // Several CTAs a row while there are fewer rows than SMs; then its parts are counted in one turn.
+  int ctas = 1;
+  while (ctas < 8 && a.rows * ctas * 2 <= sms && a.vocabulary / ctas > 4096) ctas *= 2;
+  if (ctas > 1)
+    while (ctas < 8 && (a.vocabulary + ctas - 1) / ctas + 7 > 8 * kTurn) ctas *= 2;
+  return ctas == 1 ? launch16_of<T, 1>(a, sms, s) : ctas == 2 ? launch16_of<T, 2>(a, sms, s) : ctas == 4 ? launch16_of<T, 4>(a, sms, s) : launch16_of<T, 8>(a, sms, s);
 }
 
 static int launch32(const Args& a, int64_t rows, cudaStream_t s) {
@@ -719,10 +928,10 @@ int sample(const void* logits, int64_t row_stride, int dtype, int rows, int voca
   if ((reinterpret_cast<uintptr_t>(logits) & (dtype == DINO_F32 ? 3 : 1)) != 0) return RC_ALIGN;
   int* status = kv::status_words();
   if (status == nullptr) return RC_LAUNCH;
-  const Args a{logits, row_stride, vocabulary, uniforms, *settings, tokens, probabilities, status};
+  const Args a{logits, row_stride, rows, vocabulary, uniforms, *settings, tokens, probabilities, status};
   switch (dtype) {
-    case DINO_F16: return launch16<__half>(a, rows, s);
-    case DINO_BF16: return launch16<__nv_bfloat16>(a, rows, s);
+    case DINO_F16: return launch16<__half>(a, s);
+    case DINO_BF16: return launch16<__nv_bfloat16>(a, s);
     default: return launch32(a, rows, s);
   }
 }

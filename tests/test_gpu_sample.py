@@ -214,3 +214,35 @@ def test_other_streams_and_graphs():
     graphs[0][0].replay()
     torch.cuda.synchronize()
     assert torch.equal(graphs[0][1][0][0], kernels.sample(x, u, top_p=0.9)[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_rows_of_large_vocabularies(dtype):
+    """More rows than run at once, parts that are counted in several turns, counts past 16 bits, the next row's parts beside each other."""
+    rows, vocabulary = 160, 140001
+    x, u = _logits(rows, vocabulary, dtype, 12)
+    x[3] = 0.5                                                                            # one value for all
+    x[5, 1000:] = torch.finfo(x.dtype).min                                                # a mask of the lowest value
+    x[7, :70000], x[7, 70000:] = 1.0, -1.0                                                # two, both past 65535
+    x[9, :] = -float("inf")
+    x[9, 139999] = -3.0
+    x[11, ::2], x[11, 1::2] = 0.0, -0.0
+    x[13, 0] = float("nan")
+    checked = [0, 1, 3, 5, 7, 9, 11, 13, 100, 147, 148, 149, 159]
+    for settings in ({}, {"top_k": 100000, "top_p": 0.9}, {"temperature": 3.0, "top_p": 0.99, "min_p": 0.001}):
+        _check(x, u, rows=checked, **settings)
+    first = kernels.sample(x, u, top_p=0.99, temperature=2.0)
+    for _ in range(3):
+        again = kernels.sample(x, u, top_p=0.99, temperature=2.0)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 20, 40])
+def test_equals_of_several_parts(rows, dtype):
+    """Counts past 16 bits only where the parts of a row meet; the chosen one in each of them."""
+    x = torch.full((rows, 200003), 2.0, dtype=getattr(torch, dtype), device=DEV)
+    x[:, 100000] = 3.0
+    u = torch.linspace(0, 0.999, rows, device=DEV)
+    for settings in ({}, {"top_k": 150000}, {"top_p": 0.6}, {"temperature": 0.5, "min_p": 0.1}):
+        _check(x, u, **settings)
