@@ -23,7 +23,7 @@ namespace stream { int sm_count(); }             // gemv_stream.cu
 namespace choice {
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 1024, kWarps = kThreads / 32, kGroups = 2048, kMaxVocabulary = 262144;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kGroups = 2048, kMaxVocabulary = 262144;
 constexpr int kPart32 = 32768;                   // of a row, at most
 constexpr double kOne = 35184372088832.;         // 2^45
 
@@ -130,33 +130,44 @@ template <typename V> __device__ __forceinline__ V warp_running(V v) {
 
 // Running sums of 2048 counts and masses in place, by all threads; `times` makes the mass of a group of what is there.
 template <typename M, typename F> __device__ __forceinline__ void running_sums(uint32_t* count, M* mass, uint32_t* warp_count, M* warp_mass, F times) {
+  constexpr int N = kGroups / kThreads;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const uint32_t c0 = count[2 * t], c1 = c0 + count[2 * t + 1];
-  const M m0 = times(2 * t, mass[2 * t]), m1 = m0 + times(2 * t + 1, mass[2 * t + 1]);
-  const uint32_t c = warp_running(c1);
-  const M m = warp_running(m1);
+  uint32_t c[N];
+  M m[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    c[i] = count[N * t + i];
+    m[i] = times(N * t + i, mass[N * t + i]);
+    if (i > 0) {
+      c[i] += c[i - 1];
+      m[i] += m[i - 1];
+    }
+  }
+  const uint32_t all_c = warp_running(c[N - 1]);
+  const M all_m = warp_running(m[N - 1]);
   if (lane == 31) {
-    warp_count[warp] = c;
-    warp_mass[warp] = m;
+    warp_count[warp] = all_c;
+    warp_mass[warp] = all_m;
   }
   __syncthreads();
-  const uint32_t wc = warp_running(warp_count[lane]);
-  const M wm = warp_running(warp_mass[lane]);
-  uint32_t before_c = __shfl_sync(0xffffffffu, wc, (warp + 31) & 31);
-  M before_m = __shfl_sync(0xffffffffu, wm, (warp + 31) & 31);
+  const uint32_t wc = warp_running(lane < kWarps ? warp_count[lane] : 0u);
+  const M wm = warp_running(lane < kWarps ? warp_mass[lane] : M(0));
+  uint32_t base_c = __shfl_sync(0xffffffffu, wc, (warp + 31) & 31);
+  M base_m = __shfl_sync(0xffffffffu, wm, (warp + 31) & 31);
   if (warp == 0) {
-    before_c = 0;
-    before_m = M(0);
+    base_c = 0;
+    base_m = M(0);
   }
   // (as a difference the own part would lose what a small group adds to a large sum)
-  const uint32_t up_c = __shfl_up_sync(0xffffffffu, c, 1);
-  const M up_m = __shfl_up_sync(0xffffffffu, m, 1);
-  const uint32_t base_c = before_c + (lane > 0 ? up_c : 0u);
-  const M base_m = before_m + (lane > 0 ? up_m : M(0));
-  count[2 * t] = base_c + c0;
-  count[2 * t + 1] = base_c + c1;
-  mass[2 * t] = base_m + m0;
-  mass[2 * t + 1] = base_m + m1;
+  const uint32_t up_c = __shfl_up_sync(0xffffffffu, all_c, 1);
+  const M up_m = __shfl_up_sync(0xffffffffu, all_m, 1);
+  base_c += lane > 0 ? up_c : 0u;
+  base_m += lane > 0 ? up_m : M(0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    count[N * t + i] = base_c + c[i];
+    mass[N * t + i] = base_m + m[i];
+  }
   __syncthreads();
 }
 
@@ -177,7 +188,7 @@ struct Shared16 {
   uint32_t counts[32768];                        // word d & 0x7fff: of code d in its upper half if d >= 0x8000, else in its lower half
   double mass[kGroups];                          // of groups of 32 codes, then running; the first CTA's
   uint32_t count[kGroups];
-  double power[kWarps][32];                      // of a binade: the weights of a group's values relative to its first one's
+  double power[32][32];                      // of a binade: the weights of a group's values relative to its first one's
   double first_mass;                             // of the largest value's group
   double warp_mass[kWarps];
   uint32_t warp_count[kWarps];
@@ -245,17 +256,18 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
     const int turns = max(1, (vectors + kTurn - 1) / kTurn);
     for (int turn = 0; turn < turns; ++turn) {
       const int end = min(vectors, (turn + 1) * kTurn);
-      // two vectors of a thread are counted while two more are on their way
-      uint4 q[2], r[2];
+      // some vectors of a thread are counted while as many more are on their way
+      constexpr int kAhead = 4;
+      uint4 q[kAhead], r[kAhead];
       int v = turn * kTurn + tid;
-      auto load = [&](uint4 (&to)[2], int at) {
+      auto load = [&](uint4 (&to)[kAhead], int at) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < kAhead; ++i)
           if (at + i * kThreads < end) to[i] = kv::fetch(wide + at + i * kThreads);
       };
-      auto use = [&](const uint4 (&of)[2], int at) {
+      auto use = [&](const uint4 (&of)[kAhead], int at) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kAhead; ++i) {
           if (at + i * kThreads >= end) break;
           add(of[i].x);
           add(of[i].y);
@@ -264,11 +276,11 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
         }
       };
       load(q, v);
-      for (; v < end; v += 4 * kThreads) {
-        load(r, v + 2 * kThreads);
+      for (; v < end; v += 2 * kAhead * kThreads) {
+        load(r, v + kAhead * kThreads);
         use(q, v);
-        load(q, v + 4 * kThreads);
-        use(r, v + 2 * kThreads);
+        load(q, v + 2 * kAhead * kThreads);
+        use(r, v + kAhead * kThreads);
       }
       if (turn + 1 < turns) {
         __syncthreads();
@@ -317,21 +329,24 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
     if constexpr (ctas > 1) {
       __syncthreads();
       // Which groups have anything here, told to all: the others read no more of this part than that.
-      uint32_t any = 0;                          // a lane has a group of 32 words
+      for (int block = warp; block < 32; block += kWarps) {
+        uint32_t any = 0;                        // a lane has a group of 32 words
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint4 q = reinterpret_cast<const uint4*>(sh.counts)[(warp * 32 + lane) * 8 + ((i + lane) & 7)];
-        any |= q.x | q.y | q.z | q.w;
-      }
-      const uint32_t low = __ballot_sync(0xffffffffu, (any & 0xffffu) != 0), high = __ballot_sync(0xffffffffu, (any >> 16) != 0);
-      if (lane < ctas) {
-        Shared16* other = of_rank(&sh, lane);
-        other->some[rank][0][warp] = low;
-        other->some[rank][1][warp] = high;
-        if (warp == 0) {
-          other->all_least[rank] = sh.least;
-          other->all_most[rank] = sh.most;
+        for (int i = 0; i < 8; ++i) {
+          const uint4 q = reinterpret_cast<const uint4*>(sh.counts)[(block * 32 + lane) * 8 + ((i + lane) & 7)];
+          any |= q.x | q.y | q.z | q.w;
         }
+        const uint32_t low = __ballot_sync(0xffffffffu, (any & 0xffffu) != 0), high = __ballot_sync(0xffffffffu, (any >> 16) != 0);
+        if (lane < ctas) {
+          Shared16* other = of_rank(&sh, lane);
+          other->some[rank][0][block] = low;
+          other->some[rank][1][block] = high;
+        }
+      }
+      if (tid < ctas) {
+        Shared16* other = of_rank(&sh, tid);
+        other->all_least[rank] = sh.least;
+        other->all_most[rank] = sh.most;
       }
       cluster.sync();
       least = __reduce_min_sync(0xffffffffu, lane < ctas ? sh.all_least[lane] : 0xffffu);
@@ -359,17 +374,20 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
         for (int i = warp; i < 1024 / ctas; i += kWarps) {
           const int g = ((i >> 5) * ctas + rank) * 32 + (i & 31);                         // group of words
           const uint32_t bit = 1u << (g & 31);
-          uint32_t low = 0, high = 0, others = 0;
+          uint32_t low = 0, high = 0, from = 0, w[ctas];
+#pragma unroll
+          for (int r = 0; r < ctas; ++r) from |= ((sh.some[r][0][g >> 5] | sh.some[r][1][g >> 5]) & bit) != 0 ? 1u << r : 0u;
+          if ((from & ~(1u << rank)) == 0) continue;
+#pragma unroll
+          for (int r = 0; r < ctas; ++r) {         // (all on their way before the first is used)
+            w[r] = 0;
+            if (from >> r & 1) w[r] = of_rank(sh.counts, r)[g * 32 + lane];
+          }
 #pragma unroll
           for (int r = 0; r < ctas; ++r) {
-            const bool there = ((sh.some[r][0][g >> 5] | sh.some[r][1][g >> 5]) & bit) != 0;
-            if (!there) continue;
-            const uint32_t w = of_rank(sh.counts, r)[g * 32 + lane];
-            low += w & 0xffffu;
-            high += w >> 16;
-            others |= r != rank;
+            low += w[r] & 0xffffu;
+            high += w[r] >> 16;
           }
-          if (others == 0) continue;
           sh.counts[g * 32 + lane] = min(low, 65535u) | min(high, 65535u) << 16;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
@@ -388,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
       // Powers of 32 binades: all of float16's; of bfloat16 those from the largest value's down 24 and up 7, where it is negative up 31.
       const int lowest = kMantissa == 10 ? 0 : max(0, first < 0x8000u ? int((0x7fffu - first) >> kMantissa) - 24 : int((first & 0x7fffu) >> kMantissa));
       auto step_of = [&](int binade) { return -double(Code<T>::spacing(binade)) * weight.inverse; };
-      sh.power[warp][lane] = exp(step_of(lowest + warp) * double(lane));
+      for (int i = warp; i < 32; i += kWarps) sh.power[i][lane] = exp(step_of(lowest + i) * double(lane));
       __syncthreads();
       for (int task = warp; task < 64 / ctas; task += kWarps) {
         const uint32_t half = task & 1, group0 = uint32_t((task >> 1) * ctas + rank) * 32, task0 = group0 * 32 + half * 0x8000u;
@@ -568,69 +586,83 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
     const Decision what = sh.decision;
     if (what.owner != rank) continue;
 
-    // The place-th of its equals in this part.  A warp has a piece of the part; slots are the values before the vectors, the vectors, the rest.
-    const int slots = vectors + 2, each = (slots + kWarps - 1) / kWarps, from_slot = warp * each, to_slot = min(from_slot + each, slots);
+    // The place-th of its equals in this part: among the values before the vectors, the vectors, the rest.  A warp has a piece of the vectors.
     // As they are in memory: one pattern, of zero two.
     const uint32_t bits = (what.code & 0x8000u) ? what.code : what.code ^ 0x7fffu, here = bits * 0x10001u, also = bits == 0 ? 0x80008000u : here;
-    auto hits_of = [&](int slot) -> uint32_t {   // bit i: value i of the slot is one
+    auto is_it = [&](uint32_t v) { return v == bits || v == (also & 0xffffu); };
+    auto may_hit = [&](const uint4& q) {         // a half that is zero takes a borrow
+      auto zeros = [](uint32_t t) { return (t - 0x00010001u) & ~t; };
+      return ((zeros(q.x ^ here) | zeros(q.y ^ here) | zeros(q.z ^ here) | zeros(q.w ^ here) | zeros(q.x ^ also) | zeros(q.y ^ also) | zeros(q.z ^ also) | zeros(q.w ^ also)) &
+              0x80008000u) != 0;
+    };
+    auto hits_of = [&](const uint4& q) -> uint32_t {       // bit i: value i is one
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
       uint32_t hits = 0;
-      if (slot >= to_slot) return 0;
-      if (slot > 0 && slot <= vectors) {
-        const uint4 q = kv::fetch(wide + slot - 1);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-        uint32_t zeros = 0;                      // a half that is zero takes a borrow
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t t = w[i] ^ here, u = w[i] ^ also;
-          zeros |= ((t - 0x00010001u) & ~t) | ((u - 0x00010001u) & ~u);
-        }
-        if ((zeros & 0x80008000u) == 0) return 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t t = w[i] ^ here, u = w[i] ^ also;
-          if ((t & 0xffffu) == 0 || (u & 0xffffu) == 0) hits |= 1u << (2 * i);
-          if ((t >> 16) == 0 || (u >> 16) == 0) hits |= 2u << (2 * i);
-        }
-        return hits;
-      }
-      const int at = slot == 0 ? 0 : head + 8 * vectors, n = slot == 0 ? head : rest;
-      for (int i = 0; i < n; ++i)
-        if (x[at + i] == (here & 0xffffu) || x[at + i] == (also & 0xffffu)) hits |= 1u << i;
+      for (int i = 0; i < 4; ++i) hits |= (is_it(w[i] & 0xffffu) ? 1u << (2 * i) : 0u) | (is_it(w[i] >> 16) ? 2u << (2 * i) : 0u);
       return hits;
     };
+    const int each = (vectors + kWarps - 1) / kWarps, from_v = min(warp * each, vectors), to_v = min(from_v + each, vectors);
     uint32_t found = 0;
     uint64_t seen = 0;                           // bit i: there was something in turn i
-#pragma unroll 4
-    for (int s = from_slot; s < to_slot; s += 32) {
-      const uint32_t hits = hits_of(s + lane);
-      found += __popc(hits);
-      seen |= uint64_t(hits != 0) << ((s - from_slot) >> 5);
+    constexpr int kAhead = 4;
+    for (int v = from_v, turn = 0; v < to_v; v += 32 * kAhead, turn += kAhead) {
+      uint4 q[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (v + 32 * i + lane < to_v) q[i] = kv::fetch(wide + v + 32 * i + lane);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (v + 32 * i + lane < to_v && may_hit(q[i])) {
+          const uint32_t n = __popc(hits_of(q[i]));
+          found += n;
+          seen |= uint64_t(n != 0) << (turn + i);
+        }
+      }
     }
     found = __reduce_add_sync(0xffffffffu, found);
     seen = __reduce_or_sync(0xffffffffu, uint32_t(seen)) | uint64_t(__reduce_or_sync(0xffffffffu, uint32_t(seen >> 32))) << 32;
     if (lane == 0) sh.warp_count[warp] = found;
     __syncthreads();
-    const uint32_t with = warp_running(sh.warp_count[lane]), place = uint32_t(what.place), hit = __ballot_sync(0xffffffffu, with > place);
-    if (hit != 0 && __ffs(hit) - 1 == warp) {
-      uint32_t left = place - (warp > 0 ? __shfl_sync(0xffffffffu, with, warp > 0 ? warp - 1 : 0) : 0u);
+    const uint32_t with = warp_running(lane < kWarps ? sh.warp_count[lane] : 0u);
+    const uint32_t begin_hits = __ballot_sync(0xffffffffu, lane < head && is_it(x[min(lane, length - 1)])), early = __popc(begin_hits);
+    uint32_t place = uint32_t(what.place);
+    if (place < early) {
+      if (tid == 0) {
+        uint32_t hits = begin_hits;
+        for (; place > 0; --place) hits &= hits - 1;
+        a.tokens[row] = begin + __ffs(hits) - 1;
+      }
+      continue;
+    }
+    place -= early;
+    const uint32_t hit = __ballot_sync(0xffffffffu, with > place);
+    if (hit == 0) {                              // behind the vectors
+      place -= __shfl_sync(0xffffffffu, with, 31);
+      uint32_t hits = __ballot_sync(0xffffffffu, lane < rest && is_it(x[min(head + 8 * vectors + lane, length - 1)]));
+      if (tid == 0) {
+        for (; place > 0; --place) hits &= hits - 1;
+        a.tokens[row] = begin + head + 8 * vectors + __ffs(hits) - 1;
+      }
+    } else if (__ffs(hit) - 1 == warp) {
+      place -= warp > 0 ? __shfl_sync(0xffffffffu, with, warp > 0 ? warp - 1 : 0) : 0u;
       for (; seen != 0; seen &= seen - 1) {
-        const int s = from_slot + (__ffsll(int64_t(seen)) - 1) * 32;
-        uint32_t hits = hits_of(s + lane);
+        const int v = from_v + (__ffsll(int64_t(seen)) - 1) * 32 + lane;
+        uint32_t hits = v < to_v ? hits_of(kv::fetch(wide + v)) : 0u;
         const uint32_t c = __popc(hits), run = warp_running(c), all = __shfl_sync(0xffffffffu, run, 31);
-        if (left < all) {
-          if (run > left && run - c <= left) {
-            for (uint32_t skip = left - (run - c); skip > 0; --skip) hits &= hits - 1;
-            const int slot = s + lane, bit = __ffs(hits) - 1;
-            a.tokens[row] = begin + (slot == 0 ? 0 : head + 8 * (slot - 1)) + bit;
+        if (place < all) {
+          if (run > place && run - c <= place) {
+            for (uint32_t skip = place - (run - c); skip > 0; --skip) hits &= hits - 1;
+            a.tokens[row] = begin + head + 8 * v + __ffs(hits) - 1;
           }
           break;
         }
-        left -= all;
+        place -= all;
       }
     }
   }
 }
-static_assert(kMaxVocabulary / 8 + 2 <= 64 * 32 * kWarps, "turns of a search in 64 bits");
+static_assert(kMaxVocabulary / 8 <= 64 * 32 * kWarps, "turns of a search in 64 bits");
 
 // ---- float32 logits -----------------------------------------------------------------------------------------------------------------------------------
 struct Place {                                   // a range of codes, what comes before it, what is in it
@@ -866,7 +898,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
   __syncthreads();
   if (lane == 0) sh.warp_count[warp] = hits;
   __syncthreads();
-  const uint32_t with = warp_running(sh.warp_count[lane]), own = __shfl_sync(0xffffffffu, with, 31);
+  const uint32_t with = warp_running(lane < kWarps ? sh.warp_count[lane] : 0u), own = __shfl_sync(0xffffffffu, with, 31);
   if (warp == 0 && lane < ctas) cluster.map_shared_rank(sh.found, lane)[rank] = own;
   cluster.sync();
   for (int r = 0; r < rank; ++r) {
