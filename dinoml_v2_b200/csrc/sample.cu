@@ -128,8 +128,8 @@ template <typename V> __device__ __forceinline__ V warp_running(V v) {
   return v;
 }
 
-// Running sums of 2048 counts and masses in place, by all threads; `times` makes the mass of a group of what is there.
-template <typename M, typename F> __device__ __forceinline__ void running_sums(uint32_t* count, M* mass, uint32_t* warp_count, M* warp_mass, F times) {
+// Running sums of 2048 counts and masses in place, by all threads.
+template <typename M> __device__ __forceinline__ void running_sums(uint32_t* count, M* mass, uint32_t* warp_count, M* warp_mass) {
   constexpr int N = kGroups / kThreads;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   uint32_t c[N];
@@ -137,7 +137,7 @@ template <typename M, typename F> __device__ __forceinline__ void running_sums(u
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     c[i] = count[N * t + i];
-    m[i] = times(N * t + i, mass[N * t + i]);
+    m[i] = mass[N * t + i];
     if (i > 0) {
       c[i] += c[i - 1];
       m[i] += m[i - 1];
@@ -177,8 +177,8 @@ __device__ __forceinline__ void answer(const Args& a, int64_t row, int token, fl
 }
 
 // ---- 16-bit logits ------------------------------------------------------------------------------------------------------------------------------------
-// A part is counted in turns of kTurn vectors of eight, behind which the counts that could pass 65535 in the next turn are set aside.
-constexpr int kTurn = 8064, kAside = 65535 - 8 * kTurn - 16, kMostAside = kMaxVocabulary / (kAside + 1) + 2;
+// A row that is one CTA's is counted in turns of kTurn vectors of eight, behind which the counts that could pass 65535 in the next turn are set aside; parts of a row have no more values.
+constexpr int kPart16 = 65528, kTurn = 15 * kThreads, kAside = 65535 - 8 * kTurn - 16, kMostAside = kMaxVocabulary / (kAside + 1) + 2;
 
 struct Decision {
   int owner, place;
@@ -189,7 +189,6 @@ struct Shared16 {
   double mass[kGroups];                          // of groups of 32 codes, then running; the first CTA's
   uint32_t count[kGroups];
   double power[32][32];                      // of a binade: the weights of a group's values relative to its first one's
-  double first_mass;                             // of the largest value's group
   double warp_mass[kWarps];
   uint32_t warp_count[kWarps];
   uint32_t least, most;                          // codes of this part
@@ -240,49 +239,60 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
     const uint4* wide = reinterpret_cast<const uint4*>(x + head);
     uint32_t least = 0xffffffffu, most = 0;
     auto add = [&](uint32_t two) {
-      const uint32_t plus = (~two >> 15) & 0x00010001u, minus = plus ^ 0x00010001u, d = two ^ (plus * 0x7fffu);
-      least = __vminu2(least, d);
-      most = __vmaxu2(most, d);
+      uint32_t minus;                            // ffff where a half is negative
+      asm("prmt.b32 %0, %1, 0, 0xbb99;" : "=r"(minus) : "r"(two));
+      const uint32_t d = two ^ (~minus & 0x7fff7fffu);
+      if (ctas > 1) {
+        least = __vminu2(least, d);
+        most = __vmaxu2(most, d);
+      }
       // 1 in the lower half of a positive value's word, in the upper one of a negative's
-      atomicAdd(&sh.counts[d & 0x7fffu], __byte_perm(plus, minus, 0x1410));
-      atomicAdd(&sh.counts[d >> 16 & 0x7fffu], __byte_perm(plus, minus, 0x1612));
+      atomicAdd(&sh.counts[d & 0x7fffu], (minus & 0xffffu) + 1u);
+      atomicAdd(&sh.counts[d >> 16 & 0x7fffu], (minus >> 16) + 1u);
     };
     auto add_one = [&](uint32_t v) {
       const uint32_t d = codes_of(v) & 0xffffu;
-      least = __vminu2(least, d | d << 16);
-      most = __vmaxu2(most, d | d << 16);
+      if (ctas > 1) {
+        least = __vminu2(least, d | d << 16);
+        most = __vmaxu2(most, d | d << 16);
+      }
       atomicAdd(&sh.counts[d & 0x7fffu], (d & 0x8000u) ? 0x10000u : 1u);
     };
-    const int turns = max(1, (vectors + kTurn - 1) / kTurn);
-    for (int turn = 0; turn < turns; ++turn) {
-      const int end = min(vectors, (turn + 1) * kTurn);
-      // some vectors of a thread are counted while as many more are on their way
-      constexpr int kAhead = 4;
-      uint4 q[kAhead], r[kAhead];
-      int v = turn * kTurn + tid;
-      auto load = [&](uint4 (&to)[kAhead], int at) {
+    // A step is a vector of every thread; a thread has kAhead of them on their way, those of the next turn too while the counts are looked through.
+    constexpr int kAhead = 5, kSteps = kTurn / kThreads;
+    static_assert(kSteps % kAhead == 0, "");
+    const int turns = ctas > 1 ? 1 : max(1, (vectors + kTurn - 1) / kTurn);
+    const uint4* next = wide + tid;
+    uint4 q[kAhead];
+    auto use = [&](const uint4& v) {
+      add(v.x);
+      add(v.y);
+      add(v.z);
+      add(v.w);
+    };
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i)
-          if (at + i * kThreads < end) to[i] = kv::fetch(wide + at + i * kThreads);
-      };
-      auto use = [&](const uint4 (&of)[kAhead], int at) {
+    for (int i = 0; i < kAhead; ++i)
+      if (tid + i * kThreads < vectors) q[i] = kv::fetch(next + i * kThreads);
+    int turn_left = kSteps, left = vectors - tid;      // steps of this turn; vectors at and behind the thread's next one
+    for (int all = vectors; all > 0; all -= kAhead * kThreads) {
+      next += kAhead * kThreads;
+      if (all >= 2 * kAhead * kThreads) {        // (everyone has all of these and of the next ones)
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-          if (at + i * kThreads >= end) break;
-          add(of[i].x);
-          add(of[i].y);
-          add(of[i].z);
-          add(of[i].w);
+          use(q[i]);
+          q[i] = kv::fetch(next + i * kThreads);
         }
-      };
-      load(q, v);
-      for (; v < end; v += 2 * kAhead * kThreads) {
-        load(r, v + kAhead * kThreads);
-        use(q, v);
-        load(q, v + 2 * kAhead * kThreads);
-        use(r, v + kAhead * kThreads);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          if (left > i * kThreads) use(q[i]);
+          if (left > (i + kAhead) * kThreads) q[i] = kv::fetch(next + i * kThreads);
+        }
       }
-      if (turn + 1 < turns) {
+      left -= kAhead * kThreads;
+      turn_left -= kAhead;
+      if (ctas == 1 && turn_left == 0 && all > kAhead * kThreads) {
+        turn_left = kSteps;
         __syncthreads();
         for (int i = tid; i < 32768 / 4; i += kThreads) {
           const uint4 q = reinterpret_cast<const uint4*>(sh.counts)[i];
@@ -309,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
     }
     least = __reduce_min_sync(0xffffffffu, min(least & 0xffffu, least >> 16));
     most = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
-    if (lane == 0) {
+    if (ctas > 1 && lane == 0) {
       atomicMin(&sh.least, least == kMinusZero ? kZero : least);
       atomicMax(&sh.most, most);
     }
@@ -326,23 +336,23 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
         }
       }
     }
-    if constexpr (ctas > 1) {
-      __syncthreads();
-      // Which groups have anything here, told to all: the others read no more of this part than that.
-      for (int block = warp; block < 32; block += kWarps) {
-        uint32_t any = 0;                        // a lane has a group of 32 words
+    __syncthreads();
+    // Which groups have anything here, told to all: the others read no more of this part than that.
+    for (int block = warp; block < 32; block += kWarps) {
+      uint32_t any = 0;                          // a lane has a group of 32 words
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint4 q = reinterpret_cast<const uint4*>(sh.counts)[(block * 32 + lane) * 8 + ((i + lane) & 7)];
-          any |= q.x | q.y | q.z | q.w;
-        }
-        const uint32_t low = __ballot_sync(0xffffffffu, (any & 0xffffu) != 0), high = __ballot_sync(0xffffffffu, (any >> 16) != 0);
-        if (lane < ctas) {
-          Shared16* other = of_rank(&sh, lane);
-          other->some[rank][0][block] = low;
-          other->some[rank][1][block] = high;
-        }
+      for (int i = 0; i < 8; ++i) {
+        const uint4 q = reinterpret_cast<const uint4*>(sh.counts)[(block * 32 + lane) * 8 + ((i + lane) & 7)];
+        any |= q.x | q.y | q.z | q.w;
       }
+      const uint32_t low = __ballot_sync(0xffffffffu, (any & 0xffffu) != 0), high = __ballot_sync(0xffffffffu, (any >> 16) != 0);
+      if (lane < ctas) {
+        Shared16* other = of_rank(&sh, lane);
+        other->some[rank][0][block] = low;
+        other->some[rank][1][block] = high;
+      }
+    }
+    if constexpr (ctas > 1) {
       if (tid < ctas) {
         Shared16* other = of_rank(&sh, tid);
         other->all_least[rank] = sh.least;
@@ -353,8 +363,24 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
       most = __reduce_max_sync(0xffffffffu, lane < ctas ? sh.all_most[lane] : 0u);
     } else {
       __syncthreads();
-      least = sh.least;
-      most = sh.most;
+      // The first and the last code that is there, what was set aside among them.
+      least = 0xffffu;
+      most = 0;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t word = sh.some[0][half][lane], there = __ballot_sync(0xffffffffu, word != 0);
+        if (there == 0) continue;
+        const uint32_t from = __shfl_sync(0xffffffffu, uint32_t(__ffs(word) - 1), __ffs(there) - 1) + 32 * (__ffs(there) - 1);
+        const uint32_t to = __shfl_sync(0xffffffffu, uint32_t(31 - __clz(word)), 31 - __clz(there)) + 32 * (31 - __clz(there));
+        const uint32_t in_from = __ballot_sync(0xffffffffu, (sh.counts[from * 32 + lane] >> (16 * half) & 0xffffu) != 0);
+        const uint32_t in_to = __ballot_sync(0xffffffffu, (sh.counts[to * 32 + lane] >> (16 * half) & 0xffffu) != 0);
+        least = min(least, half * 0x8000u + from * 32 + __ffs(in_from) - 1);
+        most = max(most, half * 0x8000u + to * 32 + 31 - __clz(in_to));
+      }
+      for (uint32_t i = 0; i < sh.aside; ++i) {
+        least = min(least, sh.aside_code[i]);
+        most = max(most, sh.aside_code[i]);
+      }
     }
 
     const uint32_t first = least;
@@ -371,40 +397,53 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
       Shared16* lead = of_rank(&sh, 0);
       // Blocks of 32 groups are a CTA's each, in turn: it adds the other parts' counts to its own.  What passes 65535 is set aside.
       if constexpr (ctas > 1) {
-        for (int i = warp; i < 1024 / ctas; i += kWarps) {
-          const int g = ((i >> 5) * ctas + rank) * 32 + (i & 31);                         // group of words
-          const uint32_t bit = 1u << (g & 31);
-          uint32_t low = 0, high = 0, from = 0, w[ctas];
-#pragma unroll
-          for (int r = 0; r < ctas; ++r) from |= ((sh.some[r][0][g >> 5] | sh.some[r][1][g >> 5]) & bit) != 0 ? 1u << r : 0u;
-          if ((from & ~(1u << rank)) == 0) continue;
-#pragma unroll
-          for (int r = 0; r < ctas; ++r) {         // (all on their way before the first is used)
-            w[r] = 0;
-            if (from >> r & 1) w[r] = of_rank(sh.counts, r)[g * 32 + lane];
-          }
+        static_assert(kWarps == 16, "groups w and w + 16 of a block are warp w's");
+        for (int block = rank; block < 32; block += ctas) {
+          uint32_t from[2] = {0, 0}, w[2][ctas];
 #pragma unroll
           for (int r = 0; r < ctas; ++r) {
-            low += w[r] & 0xffffu;
-            high += w[r] >> 16;
+            const uint32_t there = (sh.some[r][0][block] | sh.some[r][1][block]) >> warp;
+            from[0] |= (there & 1) << r;
+            from[1] |= (there >> 16 & 1) << r;
           }
-          sh.counts[g * 32 + lane] = min(low, 65535u) | min(high, 65535u) << 16;
+          if (((from[0] | from[1]) & ~(1u << rank)) == 0) continue;
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t n = half ? high : low;
-            if (n <= 65535u) continue;
-            const uint32_t at = atomicAdd(&lead->aside, 1u);
-            lead->aside_code[at] = uint32_t(g * 32 + lane) + half * 0x8000u;
-            lead->aside_count[at] = n - 65535u;
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < ctas; ++r) {     // (all on their way before the first is used)
+              w[i][r] = 0;
+              if (from[i] >> r & 1) w[i][r] = of_rank(sh.counts, r)[(block * 32 + warp + 16 * i) * 32 + lane];
+            }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int at = (block * 32 + warp + 16 * i) * 32 + lane;
+            uint32_t low = 0, high = 0;
+#pragma unroll
+            for (int r = 0; r < ctas; ++r) {
+              low += w[i][r] & 0xffffu;
+              high += w[i][r] >> 16;
+            }
+            if ((from[i] & ~(1u << rank)) != 0) sh.counts[at] = min(low, 65535u) | min(high, 65535u) << 16;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint32_t n = half ? high : low;
+              if (n <= 65535u) continue;
+              const uint32_t place = atomicAdd(&lead->aside, 1u);
+              lead->aside_code[place] = uint32_t(at) + half * 0x8000u;
+              lead->aside_count[place] = n - 65535u;
+            }
           }
         }
       }
       // Sums of groups of 32 values, a lane a group.  The values of a binade are equally far apart, so that the weights of a group are powers, w0 q^j, and q^j is the same for all groups of
-      // a binade: a lane adds up its counts times these, from a place on where no other lane has its bank, and w0 comes later (group_weight).  So exponentials are few: 32 of powers, one
+      // a binade: a lane adds up its counts times these, from a place on where no other lane has its bank, and multiplies by w0 at the end.  So exponentials are few: 32 of powers, one
       // for a group.  The largest value's group is summed value by value, so that its weight is one.
       constexpr int kMantissa = Code<T>::kMantissa;
       // Powers of 32 binades: all of float16's; of bfloat16 those from the largest value's down 24 and up 7, where it is negative up 31.
       const int lowest = kMantissa == 10 ? 0 : max(0, first < 0x8000u ? int((0x7fffu - first) >> kMantissa) - 24 : int((first & 0x7fffu) >> kMantissa));
+      auto group_weight = [&](uint32_t code0, double powers) {    // (before the largest value there is nothing)
+        return powers > 0. && !weight.infinite ? powers * exp((double(Code<T>::value(code0)) - weight.largest) * weight.inverse) : 0.;
+      };
       auto step_of = [&](int binade) { return -double(Code<T>::spacing(binade)) * weight.inverse; };
       for (int i = warp; i < 32; i += kWarps) sh.power[i][lane] = exp(step_of(lowest + i) * double(lane));
       __syncthreads();
@@ -435,16 +474,20 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
             mass = ::fma(double(c), power[j], mass);
           }
         }
-        if (code0 < Code<T>::kMinusInf && n != 0) {
+        if (code0 < Code<T>::kMinusInf && n != 0 && code0 >> 5 != first >> 5) {
           lead->count[code0 >> 5] = n;
-          lead->mass[code0 >> 5] = mass;
+          lead->mass[code0 >> 5] = group_weight(code0, mass);
         }
         if (first >= task0 && first < task0 + 1024) {      // (the whole warp)
           const uint32_t d = (first & ~31u) + lane, c = sh.counts[d & 0x7fffu] >> shift & 0xffffu;
           double m = c != 0 ? double(c) * weight(d) : 0.;
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
-          if (lane == 0) lead->first_mass = m;
+          const uint32_t all = __reduce_add_sync(0xffffffffu, c);
+          if (lane == 0) {
+            lead->count[first >> 5] = all;
+            lead->mass[first >> 5] = m;
+          }
         }
       }
     }
@@ -474,17 +517,12 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
               if (d < first || d >= Code<T>::kMinusInf) continue;
               const double times = double(sh.aside_count[i]);
               sh.count[d >> 5] += sh.aside_count[i];
-              if (d >> 5 == first >> 5) sh.first_mass += times * weight(d);
-              else sh.mass[d >> 5] += times * exp(-double(Code<T>::spacing(int(((d & 0x8000u) ? d & 0x7fffu : 0x7fffu - d) >> Code<T>::kMantissa))) * weight.inverse * double(d & 31u));
+              sh.mass[d >> 5] += times * weight(d);
             }
           }
           __syncthreads();
         }
-        auto group_weight = [&](int g, double powers) {    // (before the largest value there is nothing)
-          if (uint32_t(g) == first >> 5) return sh.first_mass;
-          return powers > 0. && !weight.infinite ? powers * exp((double(Code<T>::value(uint32_t(g) * 32)) - weight.largest) * weight.inverse) : 0.;
-        };
-        running_sums(sh.count, sh.mass, sh.warp_count, sh.warp_mass, group_weight);
+        running_sums(sh.count, sh.mass, sh.warp_count, sh.warp_mass);
       }
       if (warp == 0) {
         uint32_t code = first;
@@ -592,8 +630,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
     auto is_it = [&](uint32_t v) { return v == bits || v == (also & 0xffffu); };
     auto may_hit = [&](const uint4& q) {         // a half that is zero takes a borrow
       auto zeros = [](uint32_t t) { return (t - 0x00010001u) & ~t; };
-      return ((zeros(q.x ^ here) | zeros(q.y ^ here) | zeros(q.z ^ here) | zeros(q.w ^ here) | zeros(q.x ^ also) | zeros(q.y ^ also) | zeros(q.z ^ also) | zeros(q.w ^ also)) &
-              0x80008000u) != 0;
+      uint32_t any = zeros(q.x ^ here) | zeros(q.y ^ here) | zeros(q.z ^ here) | zeros(q.w ^ here);
+      if (bits == 0) any |= zeros(q.x ^ also) | zeros(q.y ^ also) | zeros(q.z ^ also) | zeros(q.w ^ also);
+      return (any & 0x80008000u) != 0;
     };
     auto hits_of = [&](const uint4& q) -> uint32_t {       // bit i: value i is one
       const uint32_t w[4] = {q.x, q.y, q.z, q.w};
@@ -605,19 +644,28 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
     const int each = (vectors + kWarps - 1) / kWarps, from_v = min(warp * each, vectors), to_v = min(from_v + each, vectors);
     uint32_t found = 0;
     uint64_t seen = 0;                           // bit i: there was something in turn i
-    constexpr int kAhead = 4;
-    for (int v = from_v, turn = 0; v < to_v; v += 32 * kAhead, turn += kAhead) {
-      uint4 q[kAhead];
+    constexpr int kLook = 8;
+    for (int v = from_v, turn = 0; v < to_v; v += 32 * kLook, turn += kLook) {
+      uint4 p[kLook];
+      if (v + 32 * kLook <= to_v) {
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i)
-        if (v + 32 * i + lane < to_v) q[i] = kv::fetch(wide + v + 32 * i + lane);
+        for (int i = 0; i < kLook; ++i) p[i] = kv::fetch(wide + v + 32 * i + lane);
+      } else {
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        if (v + 32 * i + lane < to_v && may_hit(q[i])) {
-          const uint32_t n = __popc(hits_of(q[i]));
-          found += n;
-          seen |= uint64_t(n != 0) << (turn + i);
+        for (int i = 0; i < kLook; ++i) {
+          p[i] = make_uint4(~here, ~here, ~here, ~here);   // (none)
+          if (v + 32 * i + lane < to_v) p[i] = kv::fetch(wide + v + 32 * i + lane);
         }
+      }
+      uint32_t may = 0;
+#pragma unroll
+      for (int i = 0; i < kLook; ++i) may |= may_hit(p[i]) ? 1u << i : 0u;
+      if (may == 0) continue;
+#pragma unroll
+      for (int i = 0; i < kLook; ++i) {
+        const uint32_t n = (may >> i & 1) && v + 32 * i + lane < to_v ? __popc(hits_of(p[i])) : 0u;
+        found += n;
+        seen |= uint64_t(n != 0) << (turn + i);
       }
     }
     found = __reduce_add_sync(0xffffffffu, found);
@@ -773,8 +821,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
       lead->mass[i] = m;
     }
     cluster.sync();
-    auto as_it_is = [](int, unsigned long long m) { return m; };
-    if (rank == 0) running_sums(sh.count, sh.mass, sh.warp_count, sh.warp_mass, as_it_is);
+    if (rank == 0) running_sums(sh.count, sh.mass, sh.warp_count, sh.warp_mass);
     // The place where the running count reaches `count` (by_count) or the running sum reaches, or with `above` passes, `mass`.
     int turn = 0;
     auto descend = [&](bool by_count, uint32_t count, double mass, bool above) -> Place {
@@ -804,7 +851,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
         }
         cluster.sync();
         if (rank == 0) {
-          running_sums(sh.range_count, sh.range_mass, sh.warp_count, sh.warp_mass, as_it_is);
+          running_sums(sh.range_count, sh.range_mass, sh.warp_count, sh.warp_mass);
           if (warp == 0) {
             const int g = first_of([&](int i) { return passes(p.count_before + sh.range_count[i], p.mass_before + sh.range_mass[i]); });
             const uint32_t c = g > 0 ? sh.range_count[g - 1] : 0u;
@@ -933,7 +980,7 @@ template <typename T> static int launch16(const Args& a, cudaStream_t s) {
   int ctas = 1;
   while (ctas < 8 && a.rows * ctas * 2 <= sms && a.vocabulary / ctas > 4096) ctas *= 2;
   if (ctas > 1)
-    while (ctas < 8 && (a.vocabulary + ctas - 1) / ctas + 7 > 8 * kTurn) ctas *= 2;
+    while (ctas < 8 && (a.vocabulary + ctas - 1) / ctas + 7 > kPart16) ctas *= 2;
   return ctas == 1 ? launch16_of<T, 1>(a, sms, s) : ctas == 2 ? launch16_of<T, 2>(a, sms, s) : ctas == 4 ? launch16_of<T, 4>(a, sms, s) : launch16_of<T, 8>(a, sms, s);
 }
 
