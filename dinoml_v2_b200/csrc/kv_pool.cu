@@ -23,7 +23,7 @@ struct PoolArgs {
 };
 
 // Sums of S numbers over all threads of the CTA before this one (in v), and over all (in all).
-template <int S, int NT> __device__ __forceinline__ void scan(int64_t (&v)[S], int64_t (&all)[S], int64_t (*shared)[NT / 32 + 1]) {
+template <int S, int NT> __device__ __forceinline__ void scan(int64_t (&v)[S], int64_t (&all)[S], int64_t (*shared)[NT / 32]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int64_t own[S];
 #pragma unroll
@@ -39,14 +39,15 @@ template <int S, int NT> __device__ __forceinline__ void scan(int64_t (&v)[S], i
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < S; ++i) {
-    int64_t before = 0, total = 0;
-    for (int w = 0; w < NT / 32; ++w) {
-      const int64_t x = shared[i][w];
-      if (w < warp) before += x;
-      total += x;
+    int64_t w = lane < NT / 32 ? shared[i][lane] : 0;
+#pragma unroll
+    for (int o = 1; o < NT / 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += u;
     }
-    v[i] += before - own[i];
-    all[i] = total;
+    const int64_t before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+    v[i] += (warp > 0 ? before : 0) - own[i];
+    all[i] = __shfl_sync(0xffffffffu, w, NT / 32 - 1);
   }
   __syncthreads();
 }
@@ -80,7 +81,7 @@ __device__ __forceinline__ void cluster_meet() {
 template <int NT>
 __global__ void __launch_bounds__(NT) kv_pool_kernel(PoolArgs a) {
   extern __shared__ int of[];                              // of each sequence: first row, tokens kept, blocks taken and given back before its own
-  __shared__ int64_t sums[3][NT / 32 + 1];
+  __shared__ int64_t sums[3][NT / 32];
   int *first_row = of, *kept = of + a.sequences + 1, *taken = kept + a.sequences, *gone = taken + a.sequences;
   uint32_t rank, ctas;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -170,30 +171,47 @@ __global__ void __launch_bounds__(NT) kv_pool_kernel(PoolArgs a) {
     if (a.starts != nullptr) a.starts[a.sequences] = int(got[1]);
   }
   // Positions and slots of the rows; the block of one comes from the stack where it was taken in this step.
-  for (int64_t row = int64_t(rank) * NT + tid; row < a.rows; row += int64_t(ctas) * NT) {
-    const int r = int(row);
-    int position = -1, slot = -1, b = r, at = 0;
-    if (a.starts != nullptr) {
-      if (r < int(got[1])) {
-        int low_b = 0, high_b = a.sequences;               // the last b with first_row[b] <= r (a sequence without rows has the next one's)
-        while (high_b - low_b > 1) {
-          const int mid = (low_b + high_b) >> 1;
-          if (first_row[mid] <= r) low_b = mid; else high_b = mid;
-        }
-        b = low_b;
-        at = r - first_row[b];
-        position = kept[b] + at;
+  // Some rows at once, whose searches and reads go side by side.
+  constexpr int kRows = 4;
+  const int64_t step = int64_t(ctas) * NT;
+  for (int64_t row = int64_t(rank) * NT + tid; row < a.rows; row += kRows * step) {
+    int b[kRows], position[kRows], id[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int64_t r = row + i * step;
+      b[i] = -1;
+      position[i] = -1;
+      if (r >= a.rows) continue;
+      if (a.starts == nullptr) {
+        if (first_row[r + 1] > first_row[r]) b[i] = int(r);
+      } else if (r < got[1]) {
+        b[i] = 0;
       }
-    } else if (first_row[b + 1] > first_row[b]) {
-      position = kept[b];
     }
-    if (position >= 0) {
-      const int j = position >> a.block_log2, left = (kept[b] + round) >> a.block_log2;
-      const int id = j < left ? a.table[int64_t(b) * a.table_stride + j] : __ldcg(a.free_blocks + (available - 1 - (taken[b] + j - left)));
-      slot = unsigned(id) < unsigned(a.blocks) ? (id << a.block_log2) + (position & round) : -1;
+    if (a.starts != nullptr) {                             // the last sequence whose first row is not behind it (one without rows has the next one's)
+      for (int span = a.sequences; span > 1;) {
+        const int half = span >> 1;
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+          if (b[i] >= 0 && first_row[b[i] + half] <= int(row + i * step)) b[i] += half;
+        span -= half;
+      }
     }
-    a.positions[r] = position;
-    a.slots[r] = slot;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      id[i] = -1;
+      if (b[i] < 0) continue;
+      position[i] = kept[b[i]] + (a.starts != nullptr ? int(row + i * step) - first_row[b[i]] : 0);
+      const int j = position[i] >> a.block_log2, left = (kept[b[i]] + round) >> a.block_log2;
+      id[i] = j < left ? a.table[int64_t(b[i]) * a.table_stride + j] : __ldcg(a.free_blocks + (available - 1 - (taken[b[i]] + j - left)));
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int64_t r = row + i * step;
+      if (r >= a.rows) break;
+      a.positions[r] = position[i];
+      a.slots[r] = unsigned(id[i]) < unsigned(a.blocks) ? (id[i] << a.block_log2) + (position[i] & round) : -1;
+    }
   }
 }
 

@@ -491,6 +491,26 @@ def rotary_frequencies(dim: int, base: float = 10000.0, *, scale: float = 1.0, f
     return out.to(device)
 
 
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two [rows, heads, head_dim] tensors share no memory, as far as their strides tell: other storages, one behind the other, or other columns of rows that are equally far apart."""
+    if not a.numel() or not b.numel() or a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
+        return True
+
+    def inside(t):                                                                        # values from a row's first to behind its last
+        return (t.shape[1] - 1) * t.stride(1) + t.shape[2]
+
+    def behind(t):
+        return t.storage_offset() + (t.shape[0] - 1) * t.stride(0) + inside(t)
+
+    if behind(a) <= b.storage_offset() or behind(b) <= a.storage_offset():
+        return True
+    pitch = a.stride(0)
+    if a.shape[0] < 2 or b.stride(0) != pitch or max(inside(a), inside(b)) > pitch:
+        return False
+    gap = (b.storage_offset() - a.storage_offset()) % pitch
+    return gap >= inside(a) and pitch - gap >= inside(b)
+
+
 def _rotary_side(x: torch.Tensor, weight, out, name: str, like: torch.Tensor) -> _native.Heads:
     if not x.is_cuda or x.device != like.device or x.dim() != 3 or x.dtype != like.dtype or x.shape[0] != like.shape[0] or x.shape[2] != like.shape[2] or x.shape[1] < 1 \
             or x.stride(2) != 1:
@@ -501,11 +521,8 @@ def _rotary_side(x: torch.Tensor, weight, out, name: str, like: torch.Tensor) ->
     if not (out.stride(1) >= dim or heads == 1) or not (out.stride(0) >= dim or rows == 1) or not (
             rows == 1 or heads == 1 or out.stride(0) >= (heads - 1) * out.stride(1) + dim or out.stride(1) >= (rows - 1) * out.stride(0) + dim):
         raise ValueError(f"out of {name} must not overlap itself")
-    if rows and (out.data_ptr(), out.stride()) != (x.data_ptr(), x.stride()):
-        def span(t):
-            return t.data_ptr(), t.data_ptr() + ((rows - 1) * t.stride(0) + (heads - 1) * t.stride(1) + dim) * t.element_size()
-        if out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr() and span(out)[0] < span(x)[1] and span(x)[0] < span(out)[1]:
-            raise ValueError(f"out of {name} must be {name} itself or not overlap it")
+    if (out.data_ptr(), out.stride()) != (x.data_ptr(), x.stride()) and not _apart(out, x):
+        raise ValueError(f"out of {name} must be {name} itself or not overlap it")
     if weight is not None:
         _require_cuda(weight, f"{name}_weight")
         if weight.shape != (dim,) or weight.dtype not in (torch.float32, x.dtype) or weight.device != x.device:
@@ -518,7 +535,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
     """(q, k) turned by position: pairs (a, b) of every head become magnitude * (a cos - b sin, b cos + a sin), angle positions[row] * frequencies[i] in float64.  Pair i is
     (i, i + n) with n = len(frequencies), interleaved (2 i, 2 i + 1); values behind 2 n stay.  q_weight, k_weight [head_dim] (float32 or q's dtype): each head is first brought to
     x / sqrt(mean(x^2) + eps) * weight.  float32 inside, one rounding at the end.  q [rows, heads, head_dim], k [rows, kv_heads, head_dim] (None: q alone), any row and head strides; head_dim
-    even, 512 at most; positions int32 [rows]; frequencies float64 (`rotary_frequencies`).  out: two tensors to fill, q and k themselves among them.  A row at a negative position is
+    even, 512 at most; positions int32 [rows]; frequencies float64 (`rotary_frequencies`).  out: two tensors to fill (None: a new one), q and k themselves among them.  A row at a negative position is
     nobody's: zero, or left as it was where it is written in place."""
     done = _native_call("rotary")(q, k, positions, frequencies, q_weight, k_weight, eps, interleaved, magnitude, stream) if out is None else None
     if done is not None:                                                                  # None: not the plain case, checked below
@@ -543,6 +560,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
     q_out, k_out = (torch.empty(x.shape, dtype=x.dtype, device=x.device) if o is None and x is not None else o for x, o in zip((q, k), given))
     side_q = _rotary_side(q, q_weight, q_out, "q", q)
     side_k = None if k is None else _rotary_side(k, k_weight, k_out, "k", q)
+    if k is not None and not (_apart(q_out, k) and _apart(k_out, q) and _apart(q_out, k_out)):
+        raise ValueError("what is written for one of q and k must not overlap the other")
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         raise ValueError("q_weight and k_weight must have one dtype")
     if rows:

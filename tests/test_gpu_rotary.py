@@ -160,6 +160,24 @@ def test_refusals():
     assert y.shape == (0, 4, 64) and z.shape == (0, 2, 64)
 
 
+def test_results_that_would_overlap():
+    """q and k are columns of one tensor, and so are their results; what one of them still reads is not written."""
+    f = kernels.rotary_frequencies(64)
+    q, k, p, _ = _inputs(5, 4, 4, 64, "bfloat16")
+    want = kernels.rotary(q, k, p, f)
+    for out in ((k, None), (None, q), (k, q)):
+        with pytest.raises(ValueError):
+            kernels.rotary(q, k, p, f, out=out)
+    both = torch.empty(5, 12, 64, dtype=q.dtype, device=DEV)
+    for out in ((both[:, :4], both[:, 2:6]), (both[:, 8:], both[:, 8:])):
+        with pytest.raises(ValueError):
+            kernels.rotary(q, k, p, f, out=out)
+    for out in ((both[:, :4], both[:, 8:]), (both[:, 8:], both[:, 4:8]), (q, both[:, :4]), (q, k)):
+        q2, k2 = q.clone(), k.clone()
+        got = kernels.rotary(q2, k2, p, f, out=tuple(q2 if t is q else k2 if t is k else t for t in out))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_other_streams_and_graphs():
     q, k, positions, weights = _inputs(17, 8, 2, 128, "bfloat16")
     f = kernels.rotary_frequencies(128)
