@@ -644,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
     const int each = (vectors + kWarps - 1) / kWarps, from_v = min(warp * each, vectors), to_v = min(from_v + each, vectors);
     uint32_t found = 0;
     uint64_t seen = 0;                           // bit i: there was something in turn i
-    constexpr int kLook = 8;
+    constexpr int kLook = 4;
     for (int v = from_v, turn = 0; v < to_v; v += 32 * kLook, turn += kLook) {
       uint4 p[kLook];
       if (v + 32 * kLook <= to_v) {
