@@ -713,21 +713,46 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
 static_assert(kMaxVocabulary / 8 <= 64 * 32 * kWarps, "turns of a search in 64 bits");
 
 // ---- float32 logits -----------------------------------------------------------------------------------------------------------------------------------
+// round(2^45 e^x) for x <= 0: by 2^n e^r with |r| <= ln(2) / 2 and Taylor's sum for e^r to r^12 (the next term is 2^-52), n ln(2) in two parts of which the first is exact.
+__device__ __forceinline__ unsigned long long fixed_exp(double x) {
+  if (!(x > -32.)) return 0;                     // (e^-32 2^45 is less than a half)
+  const double n = rint(x * 1.4426950408889634074), r = ::fma(-n, -1.904654299957768e-9, ::fma(-n, double(0.693147182464599609375f), x));
+  double p = 1. / 479001600.;
+  p = ::fma(p, r, 1. / 39916800.);
+  p = ::fma(p, r, 1. / 3628800.);
+  p = ::fma(p, r, 1. / 362880.);
+  p = ::fma(p, r, 1. / 40320.);
+  p = ::fma(p, r, 1. / 5040.);
+  p = ::fma(p, r, 1. / 720.);
+  p = ::fma(p, r, 1. / 120.);
+  p = ::fma(p, r, 1. / 24.);
+  p = ::fma(p, r, 1. / 6.);
+  p = ::fma(p, r, 0.5);
+  p = ::fma(p, r, 1.);
+  p = ::fma(p, r, 1.);
+  const double scale = __hiloint2double((1023 + 45 + int(n)) << 20, 0);
+  return (unsigned long long)__double_as_longlong(::fma(p, scale, 4503599627370496.)) & 0xfffffffffffffull;      // 2^52 + a whole number
+}
+
 struct Place {                                   // a range of codes, what comes before it, what is in it
   uint32_t low, high;
   uint32_t count_before, count;
   unsigned long long mass_before, mass;
+  __device__ __forceinline__ bool open() const { return count > 1 && low < high && mass > 0; }      // (without weight it does not matter which of them)
 };
+constexpr int kList = 2048;                      // values that the first CTA narrows down by itself
 struct Shared32 {
   uint32_t codes[kPart32];
   unsigned long long mass[kGroups], range_mass[kGroups];      // sums of the 2048 ranges (the first CTA's: of all, running); of a range that is narrowed down
   uint32_t count[kGroups], range_count[kGroups];
   unsigned long long own_mass[kGroups];          // this part's
   uint32_t own_count[kGroups];
+  uint32_t list_code[kList], list_index[kList];  // the values of a range, the first CTA's
   unsigned long long warp_mass[kWarps];
   uint32_t warp_count[kWarps];
-  uint32_t least, most;
-  Place place[2];                                // written in turn: a slow CTA may be reading the one before
+  uint32_t least, most, list;
+  uint32_t all_least[8], all_most[8];
+  Place place[2], own;                           // written in turn: a slow CTA may be reading the one before
   unsigned long long sum_mass;
   uint32_t sum_count;
   uint32_t found[8];
@@ -748,6 +773,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
   if (tid == 0) {
     sh.least = 0xffffffffu;
     sh.most = 0;
+    sh.list = 0;
     sh.sum_mass = 0;
     sh.sum_count = 0;
   }
@@ -771,47 +797,50 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
     atomicMin(&sh.least, least);
     atomicMax(&sh.most, most);
   }
-  cluster.sync();
-  least = 0xffffffffu;
-  most = 0;
-  if (lane < ctas) {
-    least = *cluster.map_shared_rank(&sh.least, lane);
-    most = *cluster.map_shared_rank(&sh.most, lane);
+  __syncthreads();
+  if (tid < ctas) {
+    Shared32* other = cluster.map_shared_rank(&sh, tid);
+    other->all_least[rank] = sh.least;
+    other->all_most[rank] = sh.most;
   }
-  const uint32_t first = __reduce_min_sync(0xffffffffu, least);
-  most = __reduce_max_sync(0xffffffffu, most);
+  cluster.sync();
+  const uint32_t first = __reduce_min_sync(0xffffffffu, lane < ctas ? sh.all_least[lane] : 0xffffffffu);
+  most = __reduce_max_sync(0xffffffffu, lane < ctas ? sh.all_most[lane] : 0u);
   if (!set.valid || first < C::kInf || most > C::kMinusInf || first >= C::kMinusInf) {
     if (rank == 0 && tid == 0) {
       if (!set.valid) kv::flag_range(a.status);
       answer(a, row, -1, 0.f);
     }
-    cluster.sync();
     return;
   }
   const Weight<float> weight(first, set.temperature);
   Shared32* lead = cluster.map_shared_rank(&sh, 0);
-  Place found{first, first, 0, 1, 0, 1};
-  double kept = 1.;
-  uint32_t place = 0;
+  Place found{first, first, 0, 1, 0, 1};         // where the chosen one is
+  uint32_t place = 0;                            // and which of the equals there (the first CTA's)
+  bool listed = false;
   if (!set.first) {
-    // Ranges of equal width of (largest - x) / temperature: behind 44 all is one range, whose weights together are less than 2^-45 of the largest one's.
-    const float largest = C::value(first), per = float(kGroups) / 44.f / set.temperature;
+    // Ranges of equal width of (largest - x) / temperature: behind 32 a weight is less than half of 2^-45.
+    const float largest = C::value(first), per = float(kGroups) / 32.f / set.temperature;
     auto range_of = [&](uint32_t d) -> int {
       if (d == first) return 0;
       return int(fminf(fmaxf((largest - C::value(d)) * per, 0.f), float(kGroups - 1)));      // (a NaN, inf - inf or 0 inf, is no number's: 0)
     };
-    auto fixed = [&](uint32_t d) { return __double2ull_rn(weight(d) * kOne); };
+    auto fixed = [&](uint32_t d) {
+      return d == first ? (unsigned long long)kOne : weight.infinite ? 0ull : fixed_exp((double(C::value(d)) - weight.largest) * weight.inverse);
+    };
     for (int i = tid; i < length; i += kThreads) {
       const uint32_t d = sh.codes[i];
       if (d == C::kMinusInf) continue;
       const int r = range_of(d);
+      const unsigned long long m = fixed(d);
       atomicAdd(&sh.own_count[r], 1u);
-      atomicAdd(&sh.own_mass[r], fixed(d));
+      if (m != 0) atomicAdd(&sh.own_mass[r], m);
     }
     cluster.sync();
     for (int i = rank * kThreads + tid; i < kGroups; i += ctas * kThreads) {
       uint32_t c = 0;
       unsigned long long m = 0;
+#pragma unroll 8
       for (int r = 0; r < ctas; ++r) {
         const Shared32* other = cluster.map_shared_rank(&sh, r);
         c += other->own_count[i];
@@ -822,74 +851,120 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
     }
     cluster.sync();
     if (rank == 0) running_sums(sh.count, sh.mass, sh.warp_count, sh.warp_mass);
-    // The place where the running count reaches `count` (by_count) or the running sum reaches, or with `above` passes, `mass`.
+    // What is kept: how many, their weights.  The first CTA's; the others follow the places that it gives.
+    uint32_t keep = 0;
+    unsigned long long sum = 0;
+    if (rank == 0) {
+      keep = sh.count[kGroups - 1];
+      sum = sh.mass[kGroups - 1];
+    }
     int turn = 0;
-    auto descend = [&](bool by_count, uint32_t count, double mass, bool above) -> Place {
+    auto tell = [&](const Place& p) {            // the first CTA's first warp
+      if (lane < ctas) *cluster.map_shared_rank(&sh.place[turn], lane) = p;
+    };
+    auto told = [&] {
+      cluster.sync();
+      const Place p = sh.place[turn];
+      turn ^= 1;
+      return p;
+    };
+    // The part of place p that the running sums of its 2048 parts (range_count, range_mass) say; by the first CTA, which gives the sums back as zeros.
+    auto narrow = [&](const Place& p, int shift, auto passes) {
+      running_sums(sh.range_count, sh.range_mass, sh.warp_count, sh.warp_mass);
+      Place q = p;
+      if (warp == 0) {
+        const int g = first_of([&](int i) { return passes(p.count_before + sh.range_count[i], p.mass_before + sh.range_mass[i]); });
+        const uint32_t c = g > 0 ? sh.range_count[g - 1] : 0u;
+        const unsigned long long m = g > 0 ? sh.range_mass[g - 1] : 0ull;
+        q.low = p.low + (uint32_t(g) << shift);
+        q.high = min(p.high, q.low + ((1u << shift) - 1));
+        q.count_before = p.count_before + c;
+        q.mass_before = p.mass_before + m;
+        q.count = sh.range_count[g] - c;
+        q.mass = sh.range_mass[g] - m;
+      }
+      __syncthreads();
+      for (int i = tid; i < kGroups; i += kThreads) {
+        sh.range_mass[i] = 0;
+        sh.range_count[i] = 0;
+      }
+      return q;                                  // (of the first warp)
+    };
+    auto shift_of = [](const Place& p) { return max(0, 32 - __clz(int(p.high - p.low)) - 11); };
+    // The place where the running count reaches `count` (by_count) or the running sum reaches, or with `above` passes, `mass`; nowhere if `none`.  All that the first CTA says is the first's.
+    auto descend = [&](bool none, bool by_count, uint32_t count, double mass, bool above) -> Place {
       auto passes = [&](uint32_t c, unsigned long long m) { return by_count ? c >= count : above ? double(m) > mass : double(m) >= mass; };
       if (rank == 0 && warp == 0) {
         const int g = first_of([&](int i) { return passes(sh.count[i], sh.mass[i]); });
-        Place p;
-        p.low = g == 0 ? first : last_that(first, C::kMinusInf - 1, [&](uint32_t d) { return range_of(d) < g; }) + 1;
-        p.high = last_that(first, C::kMinusInf - 1, [&](uint32_t d) { return range_of(d) <= g; });
-        p.count_before = g > 0 ? sh.count[g - 1] : 0u;
-        p.mass_before = g > 0 ? sh.mass[g - 1] : 0ull;
-        p.count = sh.count[g] - p.count_before;
-        p.mass = sh.mass[g] - p.mass_before;
-        if (lane < ctas) *cluster.map_shared_rank(&sh.place[turn], lane) = p;
+        Place p{first, first, 0, 0, 0, 0};
+        if (!none) {
+          p.low = g == 0 ? first : last_that(first, C::kMinusInf - 1, [&](uint32_t d) { return range_of(d) < g; }) + 1;
+          p.high = last_that(first, C::kMinusInf - 1, [&](uint32_t d) { return range_of(d) <= g; });
+          p.count_before = g > 0 ? sh.count[g - 1] : 0u;
+          p.mass_before = g > 0 ? sh.mass[g - 1] : 0ull;
+          p.count = sh.count[g] - p.count_before;
+          p.mass = sh.mass[g] - p.mass_before;
+        }
+        if (lane == 0) sh.list = 0;
+        tell(p);
       }
-      cluster.sync();
-      Place p = sh.place[turn];
-      turn ^= 1;
-      while (p.count > 1 && p.low < p.high && p.mass > 0) {      // (without weight it does not matter which of them)
-        const int shift = max(0, 32 - __clz(int(p.high - p.low)) - 11);
+      Place p = told();
+      listed = p.open() && p.count <= uint32_t(kList);
+      if (listed) {                              // few: the first CTA takes them all and goes on by itself
         for (int i = tid; i < length; i += kThreads) {
           const uint32_t d = sh.codes[i];
           if (d < p.low || d > p.high) continue;
-          const uint32_t at = (d - p.low) >> shift;
-          atomicAdd(&lead->range_count[at], 1u);
-          atomicAdd(&lead->range_mass[at], fixed(d));
+          const uint32_t at = atomicAdd(&lead->list, 1u);
+          lead->list_code[at] = d;
+          lead->list_index[at] = uint32_t(begin + i);
+        }
+        cluster.sync();
+        if (rank != 0) return p;
+        const int n = int(sh.list);
+        while (p.open()) {
+          const int shift = shift_of(p);
+          for (int i = tid; i < n; i += kThreads) {
+            const uint32_t d = sh.list_code[i];
+            if (d < p.low || d > p.high) continue;
+            atomicAdd(&sh.range_count[(d - p.low) >> shift], 1u);
+            atomicAdd(&sh.range_mass[(d - p.low) >> shift], fixed(d));
+          }
+          __syncthreads();
+          const Place q = narrow(p, shift, passes);
+          if (tid == 0) sh.own = q;
+          __syncthreads();
+          p = sh.own;
+        }
+        return p;
+      }
+      while (p.open()) {
+        const int shift = shift_of(p);
+        for (int i = tid; i < length; i += kThreads) {
+          const uint32_t d = sh.codes[i];
+          if (d < p.low || d > p.high) continue;
+          atomicAdd(&lead->range_count[(d - p.low) >> shift], 1u);
+          atomicAdd(&lead->range_mass[(d - p.low) >> shift], fixed(d));
         }
         cluster.sync();
         if (rank == 0) {
-          running_sums(sh.range_count, sh.range_mass, sh.warp_count, sh.warp_mass);
-          if (warp == 0) {
-            const int g = first_of([&](int i) { return passes(p.count_before + sh.range_count[i], p.mass_before + sh.range_mass[i]); });
-            const uint32_t c = g > 0 ? sh.range_count[g - 1] : 0u;
-            const unsigned long long m = g > 0 ? sh.range_mass[g - 1] : 0ull;
-            Place q;
-            q.low = p.low + (uint32_t(g) << shift);
-            q.high = min(p.high, q.low + ((1u << shift) - 1));
-            q.count_before = p.count_before + c;
-            q.mass_before = p.mass_before + m;
-            q.count = sh.range_count[g] - c;
-            q.mass = sh.range_mass[g] - m;
-            if (lane < ctas) *cluster.map_shared_rank(&sh.place[turn], lane) = q;
-          }
-          __syncthreads();
-          for (int i = tid; i < kGroups; i += kThreads) {
-            sh.range_mass[i] = 0;
-            sh.range_count[i] = 0;
-          }
+          const Place q = narrow(p, shift, passes);
+          if (warp == 0) tell(q);
         }
-        cluster.sync();
-        p = sh.place[turn];
-        turn ^= 1;
+        p = told();
       }
       return p;
     };
-    cluster.sync();                              // (the running sums are there)
-    const uint32_t all_count = lead->count[kGroups - 1];
-    const unsigned long long all_mass = lead->mass[kGroups - 1];
-    uint32_t keep = all_count;                   // how many are kept
-    unsigned long long sum = all_mass;           // their weights
-    if (set.top_k > 0 && uint32_t(set.top_k) < all_count) {
-      const Place p = descend(true, uint32_t(set.top_k), 0., false);
-      keep = uint32_t(set.top_k);
-      sum = p.mass_before + p.mass / max(p.count, 1u) * (keep - p.count_before);
+    if (set.top_k > 0) {
+      const uint32_t k = uint32_t(set.top_k);
+      const Place p = descend(rank == 0 && k >= keep, true, k, 0., false);
+      if (k < keep) {
+        keep = k;
+        sum = p.mass_before + p.mass / max(p.count, 1u) * (k - p.count_before);
+      }
     }
     if (set.top_p < 1.f) {
       const double wanted = double(set.top_p) * double(sum);
-      const Place p = descend(false, 0, wanted, false);
+      const Place p = descend(false, false, 0, wanted, false);
       const unsigned long long w = p.mass / max(p.count, 1u);
       const double some = w > 0 ? ceil((wanted - double(p.mass_before)) / double(w)) : 1.;
       const uint32_t t = uint32_t(fmin(fmax(some, 1.), double(max(p.count, 1u))));
@@ -917,28 +992,41 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
         atomicAdd(&lead->sum_mass, m);
       }
       cluster.sync();
-      c = lead->sum_count;
-      m = lead->sum_mass;
-      if (c < keep) {
-        keep = c;
-        sum = m;
+      if (rank == 0 && sh.sum_count < keep) {
+        keep = sh.sum_count;
+        sum = sh.sum_mass;
       }
     }
-    kept = double(sum);
-    const double target = double(set.u) * kept;
-    found = descend(false, 0, target, true);
-    const unsigned long long w = found.mass / max(found.count, 1u);
-    const double there = w > 0 ? floor((target - double(found.mass_before)) / double(w)) : 0.;
-    uint32_t most_place = max(found.count, 1u) - 1;
-    if (found.count_before + most_place >= keep) most_place = keep > found.count_before ? keep - found.count_before - 1 : 0u;
-    place = uint32_t(fmin(fmax(there, 0.), double(most_place)));
-    if (rank == 0 && tid == 0 && a.probabilities != nullptr) a.probabilities[row] = float(double(w) / kept);
+    const double kept = double(sum), target = double(set.u) * kept;
+    found = descend(false, false, 0, target, true);
+    if (rank == 0) {
+      const unsigned long long w = found.mass / max(found.count, 1u);
+      const double there = w > 0 ? floor((target - double(found.mass_before)) / double(w)) : 0.;
+      uint32_t most_place = max(found.count, 1u) - 1;
+      if (found.count_before + most_place >= keep) most_place = keep > found.count_before ? keep - found.count_before - 1 : 0u;
+      place = uint32_t(fmin(fmax(there, 0.), double(most_place)));
+      if (tid == 0 && a.probabilities != nullptr) a.probabilities[row] = float(double(w) / kept);
+    }
   } else if (rank == 0 && tid == 0 && a.probabilities != nullptr) {
     a.probabilities[row] = 1.f;
   }
 
+  if (listed) {                                  // the first CTA has all that it may be: the one with `place` of its equals before it
+    if (rank != 0) return;
+    const int n = int(sh.list);
+    for (int i = tid; i < n; i += kThreads) {
+      const uint32_t d = sh.list_code[i], index = sh.list_index[i];
+      if (d < found.low || d > found.high) continue;
+      uint32_t before = 0;
+      if (found.count > 1)
+        for (int j = 0; j < n; ++j) before += sh.list_code[j] >= found.low && sh.list_code[j] <= found.high && sh.list_index[j] < index ? 1u : 0u;
+      if (before == place) a.tokens[row] = int(index);
+    }
+    return;
+  }
   // The place-th of its equals: a warp has a piece of the part.
-  const int each = (length + kWarps - 1) / kWarps, from_i = warp * each, to_i = min(from_i + each, length);
+  if (rank == 0 && tid == 0) sh.sum_count = place;
+  const int each = (length + kWarps - 1) / kWarps, from_i = min(warp * each, length), to_i = min(from_i + each, length);
   auto is_one = [&](int i) { return i < to_i && sh.codes[i] >= found.low && sh.codes[i] <= found.high; };
   uint32_t hits = 0;
   for (int i = from_i; i < to_i; i += 32) hits += __popc(__ballot_sync(0xffffffffu, is_one(i + lane)));
@@ -948,10 +1036,12 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
   const uint32_t with = warp_running(lane < kWarps ? sh.warp_count[lane] : 0u), own = __shfl_sync(0xffffffffu, with, 31);
   if (warp == 0 && lane < ctas) cluster.map_shared_rank(sh.found, lane)[rank] = own;
   cluster.sync();
-  for (int r = 0; r < rank; ++r) {
-    if (place < sh.found[r]) return;
-    place -= sh.found[r];
-  }
+  place = lead->sum_count;
+  uint32_t before = 0;
+  for (int r = 0; r < rank; ++r) before += sh.found[r];
+  cluster.sync();                                // (all have read what the first CTA says)
+  if (place < before) return;
+  place -= before;
   const uint32_t hit = __ballot_sync(0xffffffffu, with > place);
   if (hit == 0 || __ffs(hit) - 1 != warp) return;
   uint32_t left = place - (warp > 0 ? __shfl_sync(0xffffffffu, with, warp > 0 ? warp - 1 : 0) : 0u);
