@@ -713,10 +713,12 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
 static_assert(kMaxVocabulary / 8 <= 64 * 32 * kWarps, "turns of a search in 64 bits");
 
 // ---- float32 logits -----------------------------------------------------------------------------------------------------------------------------------
-// round(2^45 e^x) for x <= 0: by 2^n e^r with |r| <= ln(2) / 2 and Taylor's sum for e^r to r^12 (the next term is 2^-52), n ln(2) in two parts of which the first is exact.
+// round(2^45 e^x) for x <= 0: by 2^n e^r with |r| <= ln(2) / 2 and Taylor's sum for e^r to r^12 (the next term is 2^-52), n ln(2) in two parts of which the first is exact,
+// n from the last bits of x / ln(2) + 1.5 2^52.
 __device__ __forceinline__ unsigned long long fixed_exp(double x) {
-  if (!(x > -32.)) return 0;                     // (e^-32 2^45 is less than a half)
-  const double n = rint(x * 1.4426950408889634074), r = ::fma(-n, -1.904654299957768e-9, ::fma(-n, double(0.693147182464599609375f), x));
+  const bool some = x > -32.;                    // (e^-32 2^45 is less than a half)
+  x = some ? x : 0.;
+  const double t = ::fma(x, 1.4426950408889634074, 6755399441055744.), n = t - 6755399441055744., r = ::fma(-n, -1.904654299957768e-9, ::fma(-n, double(0.693147182464599609375f), x));
   double p = 1. / 479001600.;
   p = ::fma(p, r, 1. / 39916800.);
   p = ::fma(p, r, 1. / 3628800.);
@@ -730,8 +732,8 @@ __device__ __forceinline__ unsigned long long fixed_exp(double x) {
   p = ::fma(p, r, 0.5);
   p = ::fma(p, r, 1.);
   p = ::fma(p, r, 1.);
-  const double scale = __hiloint2double((1023 + 45 + int(n)) << 20, 0);
-  return (unsigned long long)__double_as_longlong(::fma(p, scale, 4503599627370496.)) & 0xfffffffffffffull;      // 2^52 + a whole number
+  const double scale = __hiloint2double((1023 + 45 + __double2loint(t)) << 20, 0);
+  return some ? (unsigned long long)__double_as_longlong(::fma(p, scale, 4503599627370496.)) & 0xfffffffffffffull : 0ull;      // 2^52 + a whole number
 }
 
 struct Place {                                   // a range of codes, what comes before it, what is in it
@@ -745,8 +747,7 @@ struct Shared32 {
   uint32_t codes[kPart32];
   unsigned long long mass[kGroups], range_mass[kGroups];      // sums of the 2048 ranges (the first CTA's: of all, running); of a range that is narrowed down
   uint32_t count[kGroups], range_count[kGroups];
-  unsigned long long own_mass[kGroups];          // this part's
-  uint32_t own_count[kGroups];
+  uint32_t own_mass[3][kGroups], own_count[kGroups];      // this part's; the mass as sums of 15, 15 and 16 bits of each weight, whose 32768 do not pass 32 (a sum of 64 bits is no single atomic)
   uint32_t list_code[kList], list_index[kList];  // the values of a range, the first CTA's
   unsigned long long warp_mass[kWarps];
   uint32_t warp_count[kWarps];
@@ -767,7 +768,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
   const int ctas = int(cluster.num_blocks()), rank = int(cluster.block_rank());
   const int64_t row = blockIdx.x / ctas;
   for (int i = tid; i < kGroups; i += kThreads) {
-    sh.own_mass[i] = sh.range_mass[i] = 0;
+    sh.own_mass[0][i] = sh.own_mass[1][i] = sh.own_mass[2][i] = 0;
+    sh.range_mass[i] = 0;
     sh.own_count[i] = sh.range_count[i] = 0;
   }
   if (tid == 0) {
@@ -828,13 +830,27 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
     auto fixed = [&](uint32_t d) {
       return d == first ? (unsigned long long)kOne : weight.infinite ? 0ull : fixed_exp((double(C::value(d)) - weight.largest) * weight.inverse);
     };
-    for (int i = tid; i < length; i += kThreads) {
-      const uint32_t d = sh.codes[i];
-      if (d == C::kMinusInf) continue;
-      const int r = range_of(d);
-      const unsigned long long m = fixed(d);
-      atomicAdd(&sh.own_count[r], 1u);
-      if (m != 0) atomicAdd(&sh.own_mass[r], m);
+    constexpr int kTogether = 4;                 // values whose chains of instructions go side by side
+    for (int i = tid; i < length; i += kTogether * kThreads) {
+      uint32_t d[kTogether];
+      int r[kTogether];
+      unsigned long long m[kTogether];
+#pragma unroll
+      for (int j = 0; j < kTogether; ++j) d[j] = i + j * kThreads < length ? sh.codes[i + j * kThreads] : C::kMinusInf;
+#pragma unroll
+      for (int j = 0; j < kTogether; ++j) {
+        r[j] = range_of(d[j]);
+        m[j] = fixed(d[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < kTogether; ++j) {
+        if (d[j] == C::kMinusInf) continue;
+        const uint32_t low = uint32_t(m[j]) & 0x7fffu, middle = uint32_t(m[j] >> 15) & 0x7fffu, high = uint32_t(m[j] >> 30);
+        atomicAdd(&sh.own_count[r[j]], 1u);
+        if (low != 0) atomicAdd(&sh.own_mass[0][r[j]], low);
+        if (middle != 0) atomicAdd(&sh.own_mass[1][r[j]], middle);
+        if (high != 0) atomicAdd(&sh.own_mass[2][r[j]], high);
+      }
     }
     cluster.sync();
     for (int i = rank * kThreads + tid; i < kGroups; i += ctas * kThreads) {
@@ -844,7 +860,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
       for (int r = 0; r < ctas; ++r) {
         const Shared32* other = cluster.map_shared_rank(&sh, r);
         c += other->own_count[i];
-        m += other->own_mass[i];
+        m += other->own_mass[0][i] + ((unsigned long long)(other->own_mass[1][i]) << 15) + ((unsigned long long)(other->own_mass[2][i]) << 30);
       }
       lead->count[i] = c;
       lead->mass[i] = m;
