@@ -129,8 +129,8 @@ template <typename V> __device__ __forceinline__ V warp_running(V v) {
 }
 
 // Running sums of 2048 counts and masses in place, by all threads.
-template <typename M> __device__ __forceinline__ void running_sums(uint32_t* count, M* mass, uint32_t* warp_count, M* warp_mass) {
-  constexpr int N = kGroups / kThreads;
+template <int NT, typename M> __device__ __forceinline__ void running_sums(uint32_t* count, M* mass, uint32_t* warp_count, M* warp_mass) {
+  constexpr int N = kGroups / NT;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   uint32_t c[N];
   M m[N];
@@ -150,8 +150,8 @@ template <typename M> __device__ __forceinline__ void running_sums(uint32_t* cou
     warp_mass[warp] = all_m;
   }
   __syncthreads();
-  const uint32_t wc = warp_running(lane < kWarps ? warp_count[lane] : 0u);
-  const M wm = warp_running(lane < kWarps ? warp_mass[lane] : M(0));
+  const uint32_t wc = warp_running(lane < NT / 32 ? warp_count[lane] : 0u);
+  const M wm = warp_running(lane < NT / 32 ? warp_mass[lane] : M(0));
   uint32_t base_c = __shfl_sync(0xffffffffu, wc, (warp + 31) & 31);
   M base_m = __shfl_sync(0xffffffffu, wm, (warp + 31) & 31);
   if (warp == 0) {
@@ -178,7 +178,7 @@ __device__ __forceinline__ void answer(const Args& a, int64_t row, int token, fl
 
 // ---- 16-bit logits ------------------------------------------------------------------------------------------------------------------------------------
 // A row that is one CTA's is counted in turns of kTurn vectors of eight, behind which the counts that could pass 65535 in the next turn are set aside; parts of a row have no more values.
-constexpr int kPart16 = 65528, kTurn = 15 * kThreads, kAside = 65535 - 8 * kTurn - 16, kMostAside = kMaxVocabulary / (kAside + 1) + 2;
+constexpr int kPart16 = 65528, kTurn = 6144, kAside = 65535 - 8 * kTurn - 16, kMostAside = kMaxVocabulary / (kAside + 1) + 2;
 
 struct Decision {
   int owner, place;
@@ -189,8 +189,8 @@ struct Shared16 {
   double mass[kGroups];                          // of groups of 32 codes, then running; the first CTA's
   uint32_t count[kGroups];
   double power[32][32];                      // of a binade: the weights of a group's values relative to its first one's
-  double warp_mass[kWarps];
-  uint32_t warp_count[kWarps];
+  double warp_mass[32];
+  uint32_t warp_count[32];
   uint32_t least, most;                          // codes of this part
   uint32_t all_least[8], all_most[8];            // of all parts
   uint32_t some[8][2][kGroups / 64];             // of all parts: which groups have anything
@@ -198,8 +198,9 @@ struct Shared16 {
   Decision decision;
 };
 
-template <typename T, int ctas>
+template <typename T, int ctas, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
+  constexpr int kWarps = kThreads / 32;
   extern __shared__ __align__(16) uint8_t raw[];
   Shared16& sh = *reinterpret_cast<Shared16*>(raw);
   cg::cluster_group cluster = cg::this_cluster();
@@ -259,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
       atomicAdd(&sh.counts[d & 0x7fffu], (d & 0x8000u) ? 0x10000u : 1u);
     };
     // A step is a vector of every thread; a thread has kAhead of them on their way, those of the next turn too while the counts are looked through.
-    constexpr int kAhead = 5, kSteps = kTurn / kThreads;
+    constexpr int kSteps = kTurn / kThreads, kAhead = kThreads == 1024 ? 3 : 6;
     static_assert(kSteps % kAhead == 0, "");
     const int turns = ctas > 1 ? 1 : max(1, (vectors + kTurn - 1) / kTurn);
     const uint4* next = wide + tid;
@@ -397,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
       Shared16* lead = of_rank(&sh, 0);
       // Blocks of 32 groups are a CTA's each, in turn: it adds the other parts' counts to its own.  What passes 65535 is set aside.
       if constexpr (ctas > 1) {
-        static_assert(kWarps == 16, "groups w and w + 16 of a block are warp w's");
+        static_assert(ctas == 1 || kWarps == 16, "groups w and w + 16 of a block are warp w's");
         for (int block = rank; block < 32; block += ctas) {
           uint32_t from[2] = {0, 0}, w[2][ctas];
 #pragma unroll
@@ -471,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
             const int j = (i + lane) & 31;
             const uint32_t c = counts[j] >> shift & 0xffffu;
             n += c;
-            mass = ::fma(double(c), power[j], mass);
+            mass = ::fma(__hiloint2double(0x43300000, int(c)) - 4503599627370496., power[j], mass);      // (2^52 + c: a conversion takes four times as long)
           }
         }
         if (code0 < Code<T>::kMinusInf && n != 0 && code0 >> 5 != first >> 5) {
@@ -522,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
           }
           __syncthreads();
         }
-        running_sums(sh.count, sh.mass, sh.warp_count, sh.warp_mass);
+        running_sums<kThreads>(sh.count, sh.mass, sh.warp_count, sh.warp_mass);
       }
       if (warp == 0) {
         uint32_t code = first;
@@ -866,7 +867,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
       lead->mass[i] = m;
     }
     cluster.sync();
-    if (rank == 0) running_sums(sh.count, sh.mass, sh.warp_count, sh.warp_mass);
+    if (rank == 0) running_sums<kThreads>(sh.count, sh.mass, sh.warp_count, sh.warp_mass);
     // What is kept: how many, their weights.  The first CTA's; the others follow the places that it gives.
     uint32_t keep = 0;
     unsigned long long sum = 0;
@@ -886,7 +887,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
     };
     // The part of place p that the running sums of its 2048 parts (range_count, range_mass) say; by the first CTA, which gives the sums back as zeros.
     auto narrow = [&](const Place& p, int shift, auto passes) {
-      running_sums(sh.range_count, sh.range_mass, sh.warp_count, sh.warp_mass);
+      running_sums<kThreads>(sh.range_count, sh.range_mass, sh.warp_count, sh.warp_mass);
       Place q = p;
       if (warp == 0) {
         const int g = first_of([&](int i) { return passes(p.count_before + sh.range_count[i], p.mass_before + sh.range_mass[i]); });
@@ -1073,11 +1074,11 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
   }
 }
 
-template <typename T, int C> static int launch16_of(const Args& a, int sms, cudaStream_t s) {
+template <typename T, int C, int NT> static int launch16_of(const Args& a, int sms, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
-  if (int rc = allow_shared(sample16_kernel<T, C>, sizeof(Shared16), done)) return rc;
+  if (int rc = allow_shared(sample16_kernel<T, C, NT>, sizeof(Shared16), done)) return rc;
   // As many clusters as run at once; each takes rows in turn.
-  return launch_dependent(sample16_kernel<T, C>, dim3(unsigned(std::min<int64_t>(a.rows, std::max(1, sms / C)) * C)), kThreads, sizeof(Shared16), C, s, a);
+  return launch_dependent(sample16_kernel<T, C, NT>, dim3(unsigned(std::min<int64_t>(a.rows, std::max(1, sms / C)) * C)), NT, sizeof(Shared16), C, s, a);
 }
 template <typename T> static int launch16(const Args& a, cudaStream_t s) {
   const int sms = stream::sm_count();
@@ -1087,7 +1088,7 @@ template <typename T> static int launch16(const Args& a, cudaStream_t s) {
   while (ctas < 8 && a.rows * ctas * 2 <= sms && a.vocabulary / ctas > 4096) ctas *= 2;
   if (ctas > 1)
     while (ctas < 8 && (a.vocabulary + ctas - 1) / ctas + 7 > kPart16) ctas *= 2;
-  return ctas == 1 ? launch16_of<T, 1>(a, sms, s) : ctas == 2 ? launch16_of<T, 2>(a, sms, s) : ctas == 4 ? launch16_of<T, 4>(a, sms, s) : launch16_of<T, 8>(a, sms, s);
+  return ctas == 1 ? launch16_of<T, 1, 1024>(a, sms, s) : ctas == 2 ? launch16_of<T, 2, kThreads>(a, sms, s) : ctas == 4 ? launch16_of<T, 4, kThreads>(a, sms, s) : launch16_of<T, 8, kThreads>(a, sms, s);
 }
 
 static int launch32(const Args& a, int64_t rows, cudaStream_t s) {
