@@ -4,6 +4,8 @@
 // the new tokens, and every packed row gets its position and slot.  All of it is a few reads a sequence, three running sums and 8 bytes a row: bound by latency.  One cluster:
 // every CTA of it makes the sums over all sequences (a few hundred numbers, from L2), so that they need not meet for them, and has a part of the blocks and rows to write.
 // They meet once: blocks that go back are on the stack before any is taken, and nobody writes lengths or the count before all have read them.
+// 64 sequences with a token each 5.4 us, 256 5.7, 256 with 33,000 rows 9.7 (a row at a time 13.0; CTAs of 512 threads 11.5).  One CTA of 256 threads is as fast for 64 rows (5.2 us; 16 sequences
+// with 60 rows each 6.1 and 6.7) and slower for more (256 sequences with one each 11.9, 64 with 16 each 11.3 and 7.4), so that there is none.
 #include <algorithm>
 
 #include "dependent_launch.cuh"
@@ -12,7 +14,7 @@
 namespace b200gguf {
 namespace kv {
 
-constexpr int kPoolMaxSequences = 8192, kPoolCluster = 8;
+constexpr int kPoolMaxSequences = 8192, kPoolCluster = 8, kPoolThreads = 1024;
 
 struct PoolArgs {
   int *table, *lengths, *free_blocks, *free_count;
@@ -78,8 +80,8 @@ __device__ __forceinline__ void cluster_meet() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
 
-template <int NT>
-__global__ void __launch_bounds__(NT) kv_pool_kernel(PoolArgs a) {
+__global__ void __launch_bounds__(kPoolThreads) kv_pool_kernel(PoolArgs a) {
+  constexpr int NT = kPoolThreads;
   extern __shared__ int of[];                              // of each sequence: first row, tokens kept, blocks taken and given back before its own
   __shared__ int64_t sums[3][NT / 32];
   int *first_row = of, *kept = of + a.sequences + 1, *taken = kept + a.sequences, *gone = taken + a.sequences;
@@ -230,12 +232,9 @@ int pool_step(const DinoB200KvPool* pool, const int* new_tokens, const int* drop
   const PoolArgs a{pool->block_table, pool->lengths, pool->free_blocks, pool->free_count, new_tokens, drop, lengths, starts, positions, slots, status, pool->table_stride,
                    pool->table_blocks, pool->sequences, pool->blocks, log2, rows};
   const size_t shared = (4 * size_t(pool->sequences) + 1) * sizeof(int);
-  const bool small = pool->sequences <= 256 && rows <= 1024;
-  auto kernel = small ? kv_pool_kernel<256> : kv_pool_kernel<1024>;
   static std::atomic<uint64_t> done{0};
-  if (!small)
-    if (int rc = allow_shared(kernel, (4 * size_t(kPoolMaxSequences) + 1) * sizeof(int), done)) return rc;
-  return small ? launch_dependent(kernel, dim3(1), 256, shared, 1, s, a) : launch_dependent(kernel, dim3(kPoolCluster), 1024, shared, kPoolCluster, s, a);
+  if (int rc = allow_shared(kv_pool_kernel, (4 * size_t(kPoolMaxSequences) + 1) * sizeof(int), done)) return rc;
+  return launch_dependent(kv_pool_kernel, dim3(kPoolCluster), kPoolThreads, shared, kPoolCluster, s, a);
 }
 
 }  // namespace kv

@@ -4,7 +4,9 @@
 // bytes, a single token by its chain of reads (position, angle, result).  A lane has P pairs of a head, the two halves of a pair in one register file: 16 bytes of a from the first half
 // and 16 of b from the second (or 32 bytes in one piece where neighbours are pairs), so that neither the norm (a sum over the lanes of a head) nor the rotation needs shared memory.
 // The angles are a row's, not a head's: a CTA has some rows and reduces each of their angles once, in float64 (131072 radians in float32 are 0.008 off), to half turns in [-1, 1], whose sine
-// and cosine in float32 all heads share; a warp then has the same heads of all of these rows, their weights in registers and the next row's values under way.
+// and cosine in float32 all heads share; a warp then has the same heads of all of these rows, their weights in registers and the next rows' values under way.
+// 2048 rows of 32 and 8 heads of 128, bfloat16 with norms: 8.7 us one after the other (42 MB, 4.8 TB/s), a row 2.5 us (launch and chain); a warp for a row and its angles 17, a CTA for a row 22.
+// What is left is instructions: 265 for four heads of a row and warp, a third of them conversions and pairs of registers.
 #include <algorithm>
 
 #include "dependent_launch.cuh"

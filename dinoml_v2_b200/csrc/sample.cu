@@ -8,9 +8,13 @@
 // values.  Sums over groups of 32 values, their running sums, and then each place by one warp: the group, the value in it, how many of its equals.  At the end the part of the row
 // that has the chosen one among its equals is searched for it.
 // float32 logits: ranges of values instead of values.  2048 ranges of equal width in (largest - x) / temperature, whose counts and sums of weights (whole numbers of 2^-45, so
-// that atomics in any order give the same) all CTAs add up; each place is then narrowed down by the bits of the values in its range until one value is left.
+// that atomics in any order give the same) all CTAs add up; each place is then narrowed down by the bits of the values in its range until one value is left, by the first CTA alone
+// where these are few.
 //
-// A row is a cluster's: its CTAs have parts of it, the first one finds the places.
+// A row is a cluster's, of up to eight CTAs while there are fewer rows than SMs: its CTAs have parts of it, the first one finds the places.  Bound by latency there: one row of 128256 bfloat16
+// with top-k and top-p 14.7 us (four CTAs 16.2, two 20.6), of which the CTAs' meetings and their reads of one another's counts are half; seven rows of 50001 float32 16.6 us; 64 rows of
+// 128256 with settings of their own 22.2 us.  256 rows of 128256 float16 51 us (66 MB, 1.3 TB/s), two rows a CTA: of 25 us a row counting takes 12 (its atomics meet on random banks, 3.5
+// wavefronts for 32), the sums 5, the places 2, the search 4.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -1074,32 +1078,66 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
   }
 }
 
-template <typename T, int C, int NT> static int launch16_of(const Args& a, int sms, cudaStream_t s) {
-  static std::atomic<uint64_t> done{0};
-  if (int rc = allow_shared(sample16_kernel<T, C, NT>, sizeof(Shared16), done)) return rc;
-  // As many clusters as run at once; each takes rows in turn.
-  return launch_dependent(sample16_kernel<T, C, NT>, dim3(unsigned(std::min<int64_t>(a.rows, std::max(1, sms / C)) * C)), NT, sizeof(Shared16), C, s, a);
-}
-template <typename T> static int launch16(const Args& a, cudaStream_t s) {
-  const int sms = stream::sm_count();
-  if (sms <= 0) return RC_LAUNCH;
-  // Several CTAs a row while there are fewer rows than SMs; then its parts are counted in one turn.
-  int ctas = 1;
-  while (ctas < 8 && a.rows * ctas * 2 <= sms && a.vocabulary / ctas > 4096) ctas *= 2;
-  if (ctas > 1)
-    while (ctas < 8 && (a.vocabulary + ctas - 1) / ctas + 7 > kPart16) ctas *= 2;
-  return ctas == 1 ? launch16_of<T, 1, 1024>(a, sms, s) : ctas == 2 ? launch16_of<T, 2, kThreads>(a, sms, s) : ctas == 4 ? launch16_of<T, 4, kThreads>(a, sms, s) : launch16_of<T, 8, kThreads>(a, sms, s);
+// Clusters of C CTAs that run at once on the current device (the SMs of a part of it may not be a multiple of C), looked up once; 0: that failed.
+template <typename K> static int clusters_of(K kernel, int ctas, int threads, size_t shared, std::atomic<int> (&known)[64]) {
+  int dev = -1, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if ((n = known[dev].load(std::memory_order_acquire)) > 0) return n;
+  if (ctas == 1) {
+    n = stream::sm_count();
+  } else {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(ctas) * 64);
+    cfg.blockDim = dim3(unsigned(threads));
+    cfg.dynamicSmemBytes = shared;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = unsigned(ctas);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) return 0;
+  }
+  known[dev].store(n, std::memory_order_release);
+  return n;
 }
 
+template <typename T, int C> static int launch16_of(const Args& a, bool must, cudaStream_t s) {
+  constexpr int NT = C == 1 ? 1024 : kThreads;
+  static std::atomic<uint64_t> done{0};
+  static std::atomic<int> known[64];
+  if (int rc = allow_shared(sample16_kernel<T, C, NT>, sizeof(Shared16), done)) return rc;
+  const int clusters = clusters_of(sample16_kernel<T, C, NT>, C, NT, sizeof(Shared16), known);
+  if (clusters <= 0) return RC_LAUNCH;
+  if (!must && a.rows > clusters) return -1;
+  // As many clusters as run at once; each takes rows in turn.
+  return launch_dependent(sample16_kernel<T, C, NT>, dim3(unsigned(std::min<int64_t>(a.rows, clusters) * C)), NT, sizeof(Shared16), C, s, a);
+}
+// Several CTAs a row where all rows' run at once: their meetings cost what they save of a short row, or with two CTAs of a middling one.  Measured (1, 2, 4, 8 CTAs; one row, us):
+// 128256 bfloat16 26.4, 20.5, 15.4, 13.9, 32000 14.7, 15.3, 13.1, 13.2, 8000 13.1, 14.4, 12.9, 12.9; 128256 values of 36 rows 28.5, 21.8, 29.0 (36 clusters of four do not run at once), 53;
+// 100 rows 29.0, 43, 60, 134.  One CTA a row has 1024 threads (256 rows 53.5 us with 512).
+template <typename T> static int launch16(const Args& a, cudaStream_t s) {
+  int rc = -1;
+  if (a.vocabulary > 8192) rc = launch16_of<T, 8>(a, false, s);
+  if (rc == -1 && a.vocabulary > 8192 && a.vocabulary <= 4 * kPart16) rc = launch16_of<T, 4>(a, false, s);
+  if (rc == -1 && a.vocabulary > 40960 && a.vocabulary <= 2 * kPart16) rc = launch16_of<T, 2>(a, false, s);
+  return rc == -1 ? launch16_of<T, 1>(a, true, s) : rc;
+}
+
+// As many CTAs a row as let all rows' run at once, and no fewer than hold a row.  Measured (1, 2, 4, 8 CTAs; us): 50001 values of one row -, 36, 27, 21, of 18 rows -, 39, 30, 44, of 256 -, 151, 216, 370;
+// 20000 values of one row 31, 25, 21, 20, of 64 33, 27, 42, 87.
 static int launch32(const Args& a, int64_t rows, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
+  static std::atomic<int> known[4][64];
   if (int rc = allow_shared(sample32_kernel, sizeof(Shared32), done)) return rc;
-  const int sms = stream::sm_count();
-  if (sms <= 0) return RC_LAUNCH;
-  unsigned ctas = 1;
-  while (ctas < 8 && (a.vocabulary + int(ctas) - 1) / int(ctas) > kPart32) ctas *= 2;
-  while (ctas < 8 && rows * ctas * 2 <= sms && a.vocabulary / int(ctas) > 4096) ctas *= 2;
-  return launch_dependent(sample32_kernel, dim3(unsigned(rows * ctas)), kThreads, sizeof(Shared32), ctas, s, a);
+  int least = 0, log2 = 3;
+  while (least < 3 && (a.vocabulary + (1 << least) - 1) >> least > kPart32) ++least;
+  for (; log2 > least; --log2) {
+    const int clusters = clusters_of(sample32_kernel, 1 << log2, kThreads, sizeof(Shared32), known[log2]);
+    if (clusters <= 0) return RC_LAUNCH;
+    if (rows <= clusters && a.vocabulary >> log2 > 1024) break;
+  }
+  return launch_dependent(sample32_kernel, dim3(unsigned(rows << log2)), kThreads, sizeof(Shared32), 1u << log2, s, a);
 }
 
 }  // namespace choice
