@@ -202,6 +202,35 @@ struct Shared16 {
   Decision decision;
 };
 
+// What was set aside, added to its groups by all threads: few, and in the order of codes and counts, whoever came first.
+template <typename T> __device__ __forceinline__ void add_aside(Shared16& sh, const Weight<T>& weight) {
+  const int tid = threadIdx.x, aside = int(sh.aside);
+  uint32_t code = 0, count = 0, before = 0;
+  if (tid < aside) {
+    code = sh.aside_code[tid];
+    count = sh.aside_count[tid];
+    for (int i = 0; i < aside; ++i) {
+      const uint32_t c = sh.aside_code[i], n = sh.aside_count[i];
+      before += c < code || (c == code && (n < count || (n == count && i < tid))) ? 1u : 0u;
+    }
+  }
+  __syncthreads();
+  if (tid < aside) {
+    sh.aside_code[before] = code;
+    sh.aside_count[before] = count;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    for (int i = 0; i < aside; ++i) {
+      const uint32_t d = sh.aside_code[i];
+      if (d < weight.first || d >= Code<T>::kMinusInf) continue;
+      sh.count[d >> 5] += sh.aside_count[i];
+      sh.mass[d >> 5] += double(sh.aside_count[i]) * weight(d);
+    }
+  }
+  __syncthreads();
+}
+
 template <typename T, int ctas, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
   constexpr int kWarps = kThreads / 32;
@@ -264,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
       atomicAdd(&sh.counts[d & 0x7fffu], (d & 0x8000u) ? 0x10000u : 1u);
     };
     // A step is a vector of every thread; a thread has kAhead of them on their way, those of the next turn too while the counts are looked through.
-    constexpr int kSteps = kTurn / kThreads, kAhead = kThreads == 1024 ? 3 : 6;
+    constexpr int kSteps = kTurn / kThreads, kAhead = kThreads == 1024 ? 2 : 6;
     static_assert(kSteps % kAhead == 0, "");
     const int turns = ctas > 1 ? 1 : max(1, (vectors + kTurn - 1) / kTurn);
     const uint4* next = wide + tid;
@@ -453,8 +482,11 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
       for (int i = warp; i < 32; i += kWarps) sh.power[i][lane] = exp(step_of(lowest + i) * double(lane));
       __syncthreads();
       for (int task = warp; task < 64 / ctas; task += kWarps) {
-        const uint32_t half = task & 1, group0 = uint32_t((task >> 1) * ctas + rank) * 32, task0 = group0 * 32 + half * 0x8000u;
-        if (task0 > most || task0 + 1024 <= first || task0 >= Code<T>::kMinusInf) continue;
+        const uint32_t half = task & 1, block = uint32_t((task >> 1) * ctas + rank), group0 = block * 32, task0 = group0 * 32 + half * 0x8000u;
+        uint32_t any = 0;
+#pragma unroll
+        for (int r = 0; r < ctas; ++r) any |= sh.some[r][half][block];
+        if (any == 0 || task0 >= Code<T>::kMinusInf) continue;
         const uint32_t code0 = task0 + lane * 32;
         const int binade = int((half ? code0 & 0x7fffu : 0x7fffu - code0) >> kMantissa);
         const bool known = unsigned(binade - lowest) < 32u;
@@ -499,34 +531,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
     meet();
     if (rank == 0) {
       if (!set.first) {
-        const uint32_t aside = sh.aside;
-        if (aside > 0) {                         // what was set aside: few, and in the order of codes and counts, whoever came first
-          uint32_t code = 0, count = 0, before = 0;
-          if (tid < int(aside)) {
-            code = sh.aside_code[tid];
-            count = sh.aside_count[tid];
-            for (int i = 0; i < int(aside); ++i) {
-              const uint32_t c = sh.aside_code[i], n = sh.aside_count[i];
-              before += c < code || (c == code && (n < count || (n == count && i < tid))) ? 1u : 0u;
-            }
-          }
-          __syncthreads();
-          if (tid < int(aside)) {
-            sh.aside_code[before] = code;
-            sh.aside_count[before] = count;
-          }
-          __syncthreads();
-          if (tid == 0) {
-            for (uint32_t i = 0; i < aside; ++i) {
-              const uint32_t d = sh.aside_code[i];
-              if (d < first || d >= Code<T>::kMinusInf) continue;
-              const double times = double(sh.aside_count[i]);
-              sh.count[d >> 5] += sh.aside_count[i];
-              sh.mass[d >> 5] += times * weight(d);
-            }
-          }
-          __syncthreads();
-        }
+        if (sh.aside > 0) add_aside<T>(sh, weight);
         running_sums<kThreads>(sh.count, sh.mass, sh.warp_count, sh.warp_mass);
       }
       if (warp == 0) {
