@@ -12,8 +12,8 @@
 // where these are few.
 //
 // A row is a cluster's, of up to eight CTAs while there are fewer rows than SMs: its CTAs have parts of it, the first one finds the places.  Bound by latency there: one row of 128256 bfloat16
-// with top-k and top-p 14.7 us (four CTAs 16.2, two 20.6), of which the CTAs' meetings and their reads of one another's counts are half; seven rows of 50001 float32 16.6 us; 64 rows of
-// 128256 with settings of their own 22.2 us.  256 rows of 128256 float16 51 us (66 MB, 1.3 TB/s), two rows a CTA: of 25 us a row counting takes 12 (its atomics meet on random banks, 3.5
+// with top-k and top-p 14.0 us, of which the CTAs' meetings and their reads of one another's counts are half; seven rows of 50001 float32 16.5 us; 64 rows of
+// 128256 with settings of their own 21.7 us.  256 rows of 128256 float16 51 us (66 MB, 1.3 TB/s), two rows a CTA: of 25 us a row counting takes 12 (its atomics meet on random banks, 3.5
 // wavefronts for 32), the sums 5, the places 2, the search 4.
 #include <cooperative_groups.h>
 
@@ -1119,18 +1119,18 @@ template <typename T, int C> static int launch16_of(const Args& a, bool must, cu
   return launch_dependent(sample16_kernel<T, C, NT>, dim3(unsigned(std::min<int64_t>(a.rows, clusters) * C)), NT, sizeof(Shared16), C, s, a);
 }
 // Several CTAs a row where all rows' run at once: their meetings cost what they save of a short row, or with two CTAs of a middling one.  Measured (1, 2, 4, 8 CTAs; one row, us):
-// 128256 bfloat16 26.4, 20.5, 15.4, 13.9, 32000 14.7, 15.3, 13.1, 13.2, 8000 13.1, 14.4, 12.9, 12.9; 128256 values of 36 rows 28.5, 21.8, 29.0 (36 clusters of four do not run at once), 53;
-// 100 rows 29.0, 43, 60, 134.  One CTA a row has 1024 threads (256 rows 53.5 us with 512).
+// 128256 bfloat16 25.1, 20.0, 15.4, 13.6, 32000 13.2, 14.6, 13.1, 12.9, 12000 10.6, 12.6, 11.8, 12.1; 128256 values of 36 rows 28.5, 22.3, 29.7 (36 clusters of four do not run at once), 42;
+// 100 rows 27.9, 41, 60, 94.  One CTA a row has 1024 threads (256 rows of 128256 51 us, 53.5 with 512).
 template <typename T> static int launch16(const Args& a, cudaStream_t s) {
   int rc = -1;
-  if (a.vocabulary > 8192) rc = launch16_of<T, 8>(a, false, s);
-  if (rc == -1 && a.vocabulary > 8192 && a.vocabulary <= 4 * kPart16) rc = launch16_of<T, 4>(a, false, s);
-  if (rc == -1 && a.vocabulary > 40960 && a.vocabulary <= 2 * kPart16) rc = launch16_of<T, 2>(a, false, s);
+  if (a.vocabulary > 28672) rc = launch16_of<T, 8>(a, false, s);
+  if (rc == -1 && a.vocabulary > 28672 && a.vocabulary <= 4 * kPart16) rc = launch16_of<T, 4>(a, false, s);
+  if (rc == -1 && a.vocabulary > 53248 && a.vocabulary <= 2 * kPart16) rc = launch16_of<T, 2>(a, false, s);
   return rc == -1 ? launch16_of<T, 1>(a, true, s) : rc;
 }
 
-// As many CTAs a row as let all rows' run at once, and no fewer than hold a row.  Measured (1, 2, 4, 8 CTAs; us): 50001 values of one row -, 36, 27, 21, of 18 rows -, 39, 30, 44, of 256 -, 151, 216, 370;
-// 20000 values of one row 31, 25, 21, 20, of 64 33, 27, 42, 87.
+// As many CTAs a row as let all rows' run at once, of 1024 values at least, and no fewer than hold a row.  Measured (1, 2, 4, 8 CTAs; us): 50001 values of one row -, 38, 28, 23, of 18 rows -, 40, 29, 44, of
+// 256 -, 150, 215, 370; 20000 values of one row 31, 25, 21, 20, of 74 33, 27, 58, 90; 300 of one row 12.1, 13.6, 14.1, 14.6.
 static int launch32(const Args& a, int64_t rows, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
   static std::atomic<int> known[4][64];
