@@ -8,6 +8,7 @@
  * available from dino_get_last_error().  What only the device sees (block table, lengths, starts, begins, tokens, a row's settings) is checked there: an entry that
  * points outside of the cache, the rows or the table, or that is no number where one is wanted, is left out of the operation, and dinoml_b200_gguf_device_status() answers 10.  16 there: a wait
  * inside of an attention kernel gave up, and its results are not to be used; reading the status empties the workspaces' counters.
+ * All calls can be captured; run each once before the first capture: kernels are loaded then.
  */
 #ifndef DINOML_B200_DECODER_H_
 #define DINOML_B200_DECODER_H_
