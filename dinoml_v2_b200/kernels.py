@@ -438,7 +438,8 @@ def kv_pool_step(pool, new: torch.Tensor, rows: int | None = None, *, drop: torc
     """One step of all sequences, in place: sequence b loses drop[b] tokens at its end (None: none; a request that is done: as many as it has, or more) and gets new[b].  Blocks
     go back before any is handed out; sequences that get as many as they lost get the same ones.  rows: of the packed batch, at least sum(new); those behind the last
     sequence are nobody's.  rows None: one row per sequence, new[b] 0 or 1, and starts None.  A sequence whose new tokens do not fit goes without them (its lengths entry is 0,
-    it has no rows): the table's row is too short, or it wants blocks and those that the sequences up to it want are more than there are, or their rows more than `rows`."""
+    it has no rows): the table's row is too short, or it wants blocks and those that the sequences up to it want are more than there are, or their rows more than `rows`.  The rows of those
+    behind it come that much earlier: what a row is given (its token, say) goes by step.starts and positions, not by the running sum of `new`."""
     done = _native_call("kv_pool_step")(pool, new, rows, drop, stream)
     if done is not None:                                                                  # None: not the plain case, checked below
         if type(done) is int:

@@ -29,6 +29,15 @@ class Request(NamedTuple):
     min_p: float = 0.0
 
 
+def tokens_of_rows(step: kernels.KVStep, new: torch.Tensor, packed: torch.Tensor) -> torch.Tensor:
+    """The token of each row of a step, -1 of nobody's: `packed` has new[b] tokens of every sequence one after the other, the step only the rows of sequences that got theirs, so that a
+    sequence behind one that went without begins earlier there."""
+    row = torch.arange(len(packed), dtype=torch.int32, device=packed.device)
+    b = torch.searchsorted(step.starts[1:].contiguous(), row, right=True).clamp(max=len(new) - 1)
+    source = (new.cumsum(0) - new)[b] + row - step.starts[b]
+    return torch.where(step.positions >= 0, packed[source.clamp(max=len(packed) - 1)], -1).to(packed.dtype)
+
+
 class Server:
     """`slots` requests at a time, of at most `most` tokens each, that share `blocks` blocks of cache."""
 
@@ -76,8 +85,16 @@ class Server:
         chosen, _ = kernels.sample(logits, self.uniforms, **self.settings)
         self.tokens.copy_(torch.where(step.lengths > 0, chosen, self.tokens))
 
+    def check(self, r: Request) -> None:
+        """A prompt and what is generated after it, but for the last token, have to fit a slot's blocks: the pool would leave such a request out of every step."""
+        room = self.pool.block_table.shape[1] * self.c.block
+        if not r.prompt or r.most < 1 or len(r.prompt) + r.most - 1 > room:
+            raise ValueError(f"a request has a prompt and generates a token at least, of {room} tokens at most in all: got {len(r.prompt)} and {r.most}")
+
     def admit(self, requests: dict[int, Request]) -> None:
-        """Takes requests into their slots, in the place of whoever had them, and chooses their first tokens."""
+        """Takes requests into their slots, in the place of whoever had them, and chooses their first tokens.  One that finds no blocks has no tokens in the pool after that."""
+        for r in requests.values():
+            self.check(r)
         new, drop, packed = [0] * self.slots, [0] * self.slots, []
         for slot in sorted(requests):
             r = requests[slot]
@@ -88,7 +105,7 @@ class Server:
             self.active[slot] = 1
         new, drop, packed = (torch.tensor(v, dtype=torch.int32, device=self.device) for v in (new, drop, packed))
         step = kernels.kv_pool_step(self.pool, new, len(packed), drop=drop)
-        x = self.forward(packed, step)
+        x = self.forward(tokens_of_rows(step, new, packed), step)
         last = (step.starts[1:] - 1).clamp(min=0).long()                                  # (a slot that took no part has no row; its choice is not used)
         self.uniforms.uniform_(generator=self.generator)
         self.choose(x[last], step)
@@ -128,6 +145,8 @@ class Server:
 def serve(server: Server, requests: list[Request], captured: bool = True) -> list[list[int]]:
     """Generated tokens of each request: as many at a time as there are slots and blocks, the next one whenever one is done.  Where no request finds a block any more the one that came
     last gives its blocks up and begins again later."""
+    for r in requests:
+        server.check(r)
     out, waiting, running, full = [[] for _ in requests], list(range(len(requests))), {}, False
     while waiting or running:
         free = [s for s in range(server.slots) if s not in running]

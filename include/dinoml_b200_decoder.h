@@ -118,6 +118,7 @@ typedef struct DinoB200KvPool {
  * back first, the last sequence's last one before the others, so that sequences which get as many as they lost get the same ones.  A sequence whose tokens would not fit is left without
  * its new ones: where the table's row is too short, where it wants blocks and the blocks that the sequences up to it want are more than there are, or where their rows are
  * more than `rows`.  lengths [sequences]: the tokens of a sequence that got some, new ones among them, 0 of the others; starts [sequences + 1] and `rows` as in DinoB200KvBatch.
+ * The rows of sequences behind one that got nothing come that much earlier: a row's token goes by starts and positions, not by the running sum of new_tokens.
  * starts null: one row per sequence (rows = sequences, new tokens 0 or 1).  positions, slots [rows]: a row's position and block * block_size + position % block_size; -1 of rows that are nobody's. */
 DINOML_B200_API int dinoml_b200_kv_pool_step(const DinoB200KvPool* pool, const int* new_tokens, const int* drop, int rows, int* lengths, int* starts, int* positions,
                                              int* slots, void* stream);
