@@ -7,9 +7,9 @@
 // shared memory, two 16-bit counts a word).  The weight of a value is computed once, in float64, and only where its count is not zero: a row of 128256 has some thousand different
 // values.  Sums over groups of 32 values, their running sums, and then each place by one warp: the group, the value in it, how many of its equals.  At the end the part of the row
 // that has the chosen one among its equals is searched for it.
-// float32 logits: ranges of values instead of values.  2048 ranges of equal width in (largest - x) / temperature, whose counts and sums of weights (whole numbers of 2^-45, so
-// that atomics in any order give the same) all CTAs add up; each place is then narrowed down by the bits of the values in its range until one value is left, by the first CTA alone
-// where these are few.
+// float32 logits: ranges of values instead of values.  2048 ranges of equal width in (largest - x) / temperature, whose counts and sums of weights (whole numbers of a unit of the
+// range) all CTAs add up; running sums over the ranges are float64, in one order; each place is then narrowed down by the bits of the values in its range until one value is left, by the
+// first CTA alone where these are few.
 //
 // A row is a cluster's, of up to eight CTAs while there are fewer rows than SMs: its CTAs have parts of it, the first one finds the places.  Bound by latency there: one row of 128256 bfloat16
 // with top-k and top-p 14.0 us, of which the CTAs' meetings and their reads of one another's counts are half; seven rows of 50001 float32 16.5 us; 64 rows of
@@ -29,7 +29,6 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32, kGroups = 2048, kMaxVocabulary = 262144;
 constexpr int kPart32 = 32768;                   // of a row, at most
-constexpr double kOne = 35184372088832.;         // 2^45
 
 struct Args {
   const void* logits;
@@ -723,11 +722,22 @@ __global__ void __launch_bounds__(kThreads, 1) sample16_kernel(Args a) {
 static_assert(kMaxVocabulary / 8 <= 64 * 32 * kWarps, "turns of a search in 64 bits");
 
 // ---- float32 logits -----------------------------------------------------------------------------------------------------------------------------------
-// round(2^45 e^x) for x <= 0: by 2^n e^r with |r| <= ln(2) / 2 and Taylor's sum for e^r to r^12 (the next term is 2^-52), n ln(2) in two parts of which the first is exact,
-// n from the last bits of x / ln(2) + 1.5 2^52.
-__device__ __forceinline__ unsigned long long fixed_exp(double x) {
-  const bool some = x > -32.;                    // (e^-32 2^45 is less than a half)
-  x = some ? x : 0.;
+// A weight as the whole numbers that are added up, so that atomics in any order give the same: round(2^(45 + s) e^x), with an s for each range that puts its weights between 0.49 and 1.008
+// times 2^45.  That is 44 bits of every weight, however small, and 2^18 of them do not pass 64.  (Multiples of 2^-45 for all ranges left a weight of 2^-40 with 6 bits.)  Behind x = -32 there is one
+// range for all, in multiples of 2^-91: less than 2^-28 of the whole together, so that no number u and no float32 top_p below one has its border there.
+constexpr double kPer = kGroups / 32.;           // ranges of one in x
+__device__ __forceinline__ int scale_of(int range) { return range * 1477 >> 16; }        // (log2(e) / kPer from below)
+__device__ __forceinline__ double unit_of(int range) { return __hiloint2double((1023 - 45 - scale_of(range)) << 20, 0); }
+static_assert(kGroups == 2048, "scale_of");
+
+struct Weighed {
+  int range;
+  unsigned long long weight;                     // times unit_of(range)
+};
+// From x <= 0.  e^x by 2^n e^r with |r| <= ln(2) / 2 and Taylor's sum for e^r to r^12 (the next term is 2^-52), n ln(2) in two parts of which the first is exact, n from the last bits of
+// x / ln(2) + 1.5 2^52; the range in the same way.
+__device__ __forceinline__ int range_of(double x) { return min(__double2loint(::fma(x, -kPer, 6755399441055744.)), kGroups - 1); }
+__device__ __forceinline__ Weighed weighed_of(double x) {
   const double t = ::fma(x, 1.4426950408889634074, 6755399441055744.), n = t - 6755399441055744., r = ::fma(-n, -1.904654299957768e-9, ::fma(-n, double(0.693147182464599609375f), x));
   double p = 1. / 479001600.;
   p = ::fma(p, r, 1. / 39916800.);
@@ -742,24 +752,30 @@ __device__ __forceinline__ unsigned long long fixed_exp(double x) {
   p = ::fma(p, r, 0.5);
   p = ::fma(p, r, 1.);
   p = ::fma(p, r, 1.);
-  const double scale = __hiloint2double((1023 + 45 + __double2loint(t)) << 20, 0);
-  return some ? (unsigned long long)__double_as_longlong(::fma(p, scale, 4503599627370496.)) & 0xfffffffffffffull : 0ull;      // 2^52 + a whole number
+  const int range = range_of(x);
+  const double scale = __hiloint2double((1023 + 45 + scale_of(range) + __double2loint(t)) << 20, 0);
+  return {range, (unsigned long long)__double_as_longlong(::fma(p, scale, 4503599627370496.)) & 0xfffffffffffffull};      // 2^52 + a whole number
 }
 
 struct Place {                                   // a range of codes, what comes before it, what is in it
   uint32_t low, high;
   uint32_t count_before, count;
-  unsigned long long mass_before, mass;
+  double mass_before, unit;
+  unsigned long long mass;                       // times unit
   __device__ __forceinline__ bool open() const { return count > 1 && low < high && mass > 0; }      // (without weight it does not matter which of them)
+  __device__ __forceinline__ unsigned long long one() const { return mass / max(count, 1u); }       // of a place of equals
 };
 constexpr int kList = 2048;                      // values that the first CTA narrows down by itself
 struct Shared32 {
   uint32_t codes[kPart32];
-  unsigned long long mass[kGroups], range_mass[kGroups];      // sums of the 2048 ranges (the first CTA's: of all, running); of a range that is narrowed down
+  double mass[kGroups];                          // sums of the 2048 ranges (the first CTA's: of all, running)
+  unsigned long long range_mass[kGroups];        // of a range that is narrowed down, times its unit
   uint32_t count[kGroups], range_count[kGroups];
-  uint32_t own_mass[3][kGroups], own_count[kGroups];      // this part's; the mass as sums of 15, 15 and 16 bits of each weight, whose 32768 do not pass 32 (a sum of 64 bits is no single atomic)
+  uint32_t own_mass[3][kGroups], own_count[kGroups];      // this part's; the mass as sums of 15, 15 and 16 bits of each weight, whose 32768 do not pass 32 (a sum of 64 bits is no single atomic);
+                                                 // the first CTA's after that: 32 and 32 bits of every range's sum of all parts
   uint32_t list_code[kList], list_index[kList];  // the values of a range, the first CTA's
   unsigned long long warp_mass[kWarps];
+  double warp_sum[kWarps];
   uint32_t warp_count[kWarps];
   uint32_t least, most, list;
   uint32_t all_least[8], all_most[8];
@@ -827,39 +843,34 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
   }
   const Weight<float> weight(first, set.temperature);
   Shared32* lead = cluster.map_shared_rank(&sh, 0);
-  Place found{first, first, 0, 1, 0, 1};         // where the chosen one is
+  Place found{first, first, 0, 1, 0., 1., 1};    // where the chosen one is
   uint32_t place = 0;                            // and which of the equals there (the first CTA's)
   bool listed = false;
   if (!set.first) {
-    // Ranges of equal width of (largest - x) / temperature: behind 32 a weight is less than half of 2^-45.
-    const float largest = C::value(first), per = float(kGroups) / 32.f / set.temperature;
-    auto range_of = [&](uint32_t d) -> int {
-      if (d == first) return 0;
-      return int(fminf(fmaxf((largest - C::value(d)) * per, 0.f), float(kGroups - 1)));      // (a NaN, inf - inf or 0 inf, is no number's: 0)
+    // (largest - logit) / temperature of every value, which its range and its weight go by.  A NaN (inf - inf, 0 inf) is the largest value's or has no weight.
+    auto x_of = [&](uint32_t d) {
+      const double x = (double(C::value(d)) - weight.largest) * weight.inverse;
+      return d == first ? 0. : x > -64. ? x : -64.;        // (e^-64 2^91 is less than a half)
     };
-    auto fixed = [&](uint32_t d) {
-      return d == first ? (unsigned long long)kOne : weight.infinite ? 0ull : fixed_exp((double(C::value(d)) - weight.largest) * weight.inverse);
-    };
+    auto range = [&](uint32_t d) { return range_of(x_of(d)); };
+    auto weighed = [&](uint32_t d) { return weighed_of(x_of(d)); };
     constexpr int kTogether = 4;                 // values whose chains of instructions go side by side
     for (int i = tid; i < length; i += kTogether * kThreads) {
       uint32_t d[kTogether];
-      int r[kTogether];
-      unsigned long long m[kTogether];
+      Weighed m[kTogether];
 #pragma unroll
       for (int j = 0; j < kTogether; ++j) d[j] = i + j * kThreads < length ? sh.codes[i + j * kThreads] : C::kMinusInf;
 #pragma unroll
-      for (int j = 0; j < kTogether; ++j) {
-        r[j] = range_of(d[j]);
-        m[j] = fixed(d[j]);
-      }
+      for (int j = 0; j < kTogether; ++j) m[j] = weighed(d[j]);
 #pragma unroll
       for (int j = 0; j < kTogether; ++j) {
         if (d[j] == C::kMinusInf) continue;
-        const uint32_t low = uint32_t(m[j]) & 0x7fffu, middle = uint32_t(m[j] >> 15) & 0x7fffu, high = uint32_t(m[j] >> 30);
-        atomicAdd(&sh.own_count[r[j]], 1u);
-        if (low != 0) atomicAdd(&sh.own_mass[0][r[j]], low);
-        if (middle != 0) atomicAdd(&sh.own_mass[1][r[j]], middle);
-        if (high != 0) atomicAdd(&sh.own_mass[2][r[j]], high);
+        const int r = m[j].range;
+        const uint32_t low = uint32_t(m[j].weight) & 0x7fffu, middle = uint32_t(m[j].weight >> 15) & 0x7fffu, high = uint32_t(m[j].weight >> 30);
+        atomicAdd(&sh.own_count[r], 1u);
+        if (low != 0) atomicAdd(&sh.own_mass[0][r], low);
+        if (middle != 0) atomicAdd(&sh.own_mass[1][r], middle);
+        if (high != 0) atomicAdd(&sh.own_mass[2][r], high);
       }
     }
     cluster.sync();
@@ -873,13 +884,15 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
         m += other->own_mass[0][i] + ((unsigned long long)(other->own_mass[1][i]) << 15) + ((unsigned long long)(other->own_mass[2][i]) << 30);
       }
       lead->count[i] = c;
-      lead->mass[i] = m;
+      lead->mass[i] = double(m) * unit_of(i);
+      lead->own_mass[0][i] = uint32_t(m);        // (range i is this thread's alone, and all parts' are read)
+      lead->own_mass[1][i] = uint32_t(m >> 32);
     }
     cluster.sync();
-    if (rank == 0) running_sums<kThreads>(sh.count, sh.mass, sh.warp_count, sh.warp_mass);
+    if (rank == 0) running_sums<kThreads>(sh.count, sh.mass, sh.warp_count, sh.warp_sum);
     // What is kept: how many, their weights.  The first CTA's; the others follow the places that it gives.
     uint32_t keep = 0;
-    unsigned long long sum = 0;
+    double sum = 0.;
     if (rank == 0) {
       keep = sh.count[kGroups - 1];
       sum = sh.mass[kGroups - 1];
@@ -899,13 +912,14 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
       running_sums<kThreads>(sh.range_count, sh.range_mass, sh.warp_count, sh.warp_mass);
       Place q = p;
       if (warp == 0) {
-        const int g = first_of([&](int i) { return passes(p.count_before + sh.range_count[i], p.mass_before + sh.range_mass[i]); });
+        // (or the last that has anything: the sums of the ranges and of a range's parts have roundings of their own)
+        const int g = first_of([&](int i) { return sh.range_count[i] >= p.count || passes(p.count_before + sh.range_count[i], p.mass_before + double(sh.range_mass[i]) * p.unit); });
         const uint32_t c = g > 0 ? sh.range_count[g - 1] : 0u;
         const unsigned long long m = g > 0 ? sh.range_mass[g - 1] : 0ull;
         q.low = p.low + (uint32_t(g) << shift);
         q.high = min(p.high, q.low + ((1u << shift) - 1));
         q.count_before = p.count_before + c;
-        q.mass_before = p.mass_before + m;
+        q.mass_before = p.mass_before + double(m) * p.unit;
         q.count = sh.range_count[g] - c;
         q.mass = sh.range_mass[g] - m;
       }
@@ -919,17 +933,18 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
     auto shift_of = [](const Place& p) { return max(0, 32 - __clz(int(p.high - p.low)) - 11); };
     // The place where the running count reaches `count` (by_count) or the running sum reaches, or with `above` passes, `mass`; nowhere if `none`.  All that the first CTA says is the first's.
     auto descend = [&](bool none, bool by_count, uint32_t count, double mass, bool above) -> Place {
-      auto passes = [&](uint32_t c, unsigned long long m) { return by_count ? c >= count : above ? double(m) > mass : double(m) >= mass; };
+      auto passes = [&](uint32_t c, double m) { return by_count ? c >= count : above ? m > mass : m >= mass; };
       if (rank == 0 && warp == 0) {
-        const int g = first_of([&](int i) { return passes(sh.count[i], sh.mass[i]); });
-        Place p{first, first, 0, 0, 0, 0};
+        const int g = first_of([&](int i) { return sh.count[i] == sh.count[kGroups - 1] || passes(sh.count[i], sh.mass[i]); });
+        Place p{first, first, 0, 0, 0., 0., 0};
         if (!none) {
-          p.low = g == 0 ? first : last_that(first, C::kMinusInf - 1, [&](uint32_t d) { return range_of(d) < g; }) + 1;
-          p.high = last_that(first, C::kMinusInf - 1, [&](uint32_t d) { return range_of(d) <= g; });
+          p.low = g == 0 ? first : last_that(first, C::kMinusInf - 1, [&](uint32_t d) { return range(d) < g; }) + 1;
+          p.high = last_that(first, C::kMinusInf - 1, [&](uint32_t d) { return range(d) <= g; });
           p.count_before = g > 0 ? sh.count[g - 1] : 0u;
-          p.mass_before = g > 0 ? sh.mass[g - 1] : 0ull;
+          p.mass_before = g > 0 ? sh.mass[g - 1] : 0.;
           p.count = sh.count[g] - p.count_before;
-          p.mass = sh.mass[g] - p.mass_before;
+          p.mass = sh.own_mass[0][g] | (unsigned long long)(sh.own_mass[1][g]) << 32;
+          p.unit = unit_of(g);
         }
         if (lane == 0) sh.list = 0;
         tell(p);
@@ -953,7 +968,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
             const uint32_t d = sh.list_code[i];
             if (d < p.low || d > p.high) continue;
             atomicAdd(&sh.range_count[(d - p.low) >> shift], 1u);
-            atomicAdd(&sh.range_mass[(d - p.low) >> shift], fixed(d));
+            atomicAdd(&sh.range_mass[(d - p.low) >> shift], weighed(d).weight);
           }
           __syncthreads();
           const Place q = narrow(p, shift, passes);
@@ -969,7 +984,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
           const uint32_t d = sh.codes[i];
           if (d < p.low || d > p.high) continue;
           atomicAdd(&lead->range_count[(d - p.low) >> shift], 1u);
-          atomicAdd(&lead->range_mass[(d - p.low) >> shift], fixed(d));
+          atomicAdd(&lead->range_mass[(d - p.low) >> shift], weighed(d).weight);
         }
         cluster.sync();
         if (rank == 0) {
@@ -985,30 +1000,32 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
       const Place p = descend(rank == 0 && k >= keep, true, k, 0., false);
       if (k < keep) {
         keep = k;
-        sum = p.mass_before + p.mass / max(p.count, 1u) * (k - p.count_before);
+        sum = p.mass_before + double(p.one() * (k - p.count_before)) * p.unit;
       }
     }
     if (set.top_p < 1.f) {
-      const double wanted = double(set.top_p) * double(sum);
+      const double wanted = double(set.top_p) * sum;
       const Place p = descend(false, false, 0, wanted, false);
-      const unsigned long long w = p.mass / max(p.count, 1u);
-      const double some = w > 0 ? ceil((wanted - double(p.mass_before)) / double(w)) : 1.;
+      const double w = double(p.one()) * p.unit, some = w > 0. ? ceil((wanted - p.mass_before) / w) : 1.;
       const uint32_t t = uint32_t(fmin(fmax(some, 1.), double(max(p.count, 1u))));
       if (p.count_before + t < keep) {
         keep = p.count_before + t;
-        sum = p.mass_before + w * t;
+        sum = p.mass_before + w * double(t);
       }
     }
     if (set.min_p > 0.f) {
+      // the last one with that weight: what is kept are the ranges before its own and of that one what comes up to it
       const uint32_t e = last_that(first, C::kMinusInf - 1, [&](uint32_t d) { return weight(d) >= double(set.min_p); });
+      const int g = range(e);
       unsigned long long m = 0;
       uint32_t c = 0;
       for (int i = tid; i < length; i += kThreads) {
         const uint32_t d = sh.codes[i];
-        if (d <= e) {
-          ++c;
-          m += fixed(d);
-        }
+        if (d > e) continue;
+        const Weighed q = weighed(d);
+        if (q.range != g) continue;
+        ++c;
+        m += q.weight;
       }
       c = __reduce_add_sync(0xffffffffu, c);
 #pragma unroll
@@ -1018,20 +1035,20 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
         atomicAdd(&lead->sum_mass, m);
       }
       cluster.sync();
-      if (rank == 0 && sh.sum_count < keep) {
-        keep = sh.sum_count;
-        sum = sh.sum_mass;
+      const uint32_t some = rank == 0 ? (g > 0 ? sh.count[g - 1] : 0u) + sh.sum_count : 0u;
+      if (rank == 0 && some < keep) {
+        keep = some;
+        sum = (g > 0 ? sh.mass[g - 1] : 0.) + double(sh.sum_mass) * unit_of(g);
       }
     }
-    const double kept = double(sum), target = double(set.u) * kept;
+    const double target = double(set.u) * sum;
     found = descend(false, false, 0, target, true);
     if (rank == 0) {
-      const unsigned long long w = found.mass / max(found.count, 1u);
-      const double there = w > 0 ? floor((target - double(found.mass_before)) / double(w)) : 0.;
+      const double w = double(found.one()) * found.unit, there = w > 0. ? floor((target - found.mass_before) / w) : 0.;
       uint32_t most_place = max(found.count, 1u) - 1;
       if (found.count_before + most_place >= keep) most_place = keep > found.count_before ? keep - found.count_before - 1 : 0u;
       place = uint32_t(fmin(fmax(there, 0.), double(most_place)));
-      if (tid == 0 && a.probabilities != nullptr) a.probabilities[row] = float(double(w) / kept);
+      if (tid == 0 && a.probabilities != nullptr) a.probabilities[row] = float(w / sum);
     }
   } else if (rank == 0 && tid == 0 && a.probabilities != nullptr) {
     a.probabilities[row] = 1.f;

@@ -137,7 +137,8 @@ typedef struct DinoB200SampleSettings {
 /* tokens[row]: one of [0, vocabulary), chosen with the given number uniforms[row] in [0, 1).  Order of the tokens: by logit, the lowest index first among equals (-0 is 0).  Weights
  * w = exp((logit - largest) / temperature).  Kept are the first top_k (0 or less: all), of these the fewest whose weights are at least top_p of theirs (1: all), of these those with
  * w >= min_p, the first in any case; the token is the first whose running sum is above uniforms[row] times the sum of the kept.  Temperature 0: the first token.  probabilities[row] (null:
- * not wanted): w / sum of the kept; 1 with temperature 0.  Weights and sums are float64, or multiples of 2^-45 where the logits are float32.  A logit of -inf is never chosen, one of inf has all of the weight.  A row with a NaN, or
+ * not wanted): w / sum of the kept; 1 with temperature 0.  Weights and sums are float64; where the logits are float32 a weight has 44 bits, and those below e^-32 are
+ * multiples of 2^-91.  A logit of -inf is never chosen, one of inf has all of the weight.  A row with a NaN, or
  * with nothing but -inf, or whose settings are no numbers or its temperature negative (which the status tells) gives token -1, probability 0.  logits [rows][vocabulary], row_stride
  * in elements; vocabulary is 262144 at most. */
 DINOML_B200_API int dinoml_b200_sample(const void* logits, int64_t row_stride, int dtype, int rows, int vocabulary, const float* uniforms,
