@@ -21,6 +21,7 @@
 
 #include "dependent_launch.cuh"
 #include "kv_cache.cuh"
+#include "sample_clusters.h"
 
 namespace b200gguf {
 namespace stream { int sm_count(); }             // gemv_stream.cu
@@ -1100,13 +1101,13 @@ __global__ void __launch_bounds__(kThreads, 1) sample32_kernel(Args a) {
   }
 }
 
-// Clusters of C CTAs that run at once on the current device (the SMs of a part of it may not be a multiple of C), looked up once; 0: that failed.
+// Clusters of `ctas` CTAs that run at once on the current device (the SMs of a part of it may not be a multiple of that), looked up once (known: one more); negative: that failed.
 template <typename K> static int clusters_of(K kernel, int ctas, int threads, size_t shared, std::atomic<int> (&known)[64]) {
   int dev = -1, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-  if ((n = known[dev].load(std::memory_order_acquire)) > 0) return n;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
+  if ((n = known[dev].load(std::memory_order_acquire)) > 0) return n - 1;
   if (ctas == 1) {
-    n = stream::sm_count();
+    if ((n = stream::sm_count()) <= 0) return -1;
   } else {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(ctas) * 64);
@@ -1118,48 +1119,42 @@ template <typename K> static int clusters_of(K kernel, int ctas, int threads, si
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) return 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 0) return -1;
   }
-  known[dev].store(n, std::memory_order_release);
+  known[dev].store(n + 1, std::memory_order_release);
   return n;
 }
 
-template <typename T, int C> static int launch16_of(const Args& a, bool must, cudaStream_t s) {
-  constexpr int NT = C == 1 ? 1024 : kThreads;
+// One CTA a row has 1024 threads (256 rows of 128256 51 us, 53.5 with 512).
+template <int C> constexpr int threads16() { return C == 1 ? 1024 : kThreads; }
+template <typename T, int C> static int fits16() {
   static std::atomic<uint64_t> done{0};
   static std::atomic<int> known[64];
-  if (int rc = allow_shared(sample16_kernel<T, C, NT>, sizeof(Shared16), done)) return rc;
-  const int clusters = clusters_of(sample16_kernel<T, C, NT>, C, NT, sizeof(Shared16), known);
-  if (clusters <= 0) return RC_LAUNCH;
-  if (!must && a.rows > clusters) return -1;
-  // As many clusters as run at once; each takes rows in turn.
-  return launch_dependent(sample16_kernel<T, C, NT>, dim3(unsigned(std::min<int64_t>(a.rows, clusters) * C)), NT, sizeof(Shared16), C, s, a);
+  if (allow_shared(sample16_kernel<T, C, threads16<C>()>, sizeof(Shared16), done)) return -1;
+  return clusters_of(sample16_kernel<T, C, threads16<C>()>, C, threads16<C>(), sizeof(Shared16), known);
 }
-// Several CTAs a row where all rows' run at once: their meetings cost what they save of a short row, or with two CTAs of a middling one.  Measured (1, 2, 4, 8 CTAs; one row, us):
-// 128256 bfloat16 25.1, 20.0, 15.4, 13.6, 32000 13.2, 14.6, 13.1, 12.9, 12000 10.6, 12.6, 11.8, 12.1; 128256 values of 36 rows 28.5, 22.3, 29.7 (36 clusters of four do not run at once), 42;
-// 100 rows 27.9, 41, 60, 94.  One CTA a row has 1024 threads (256 rows of 128256 51 us, 53.5 with 512).
 template <typename T> static int launch16(const Args& a, cudaStream_t s) {
-  int rc = -1;
-  if (a.vocabulary > 28672) rc = launch16_of<T, 8>(a, false, s);
-  if (rc == -1 && a.vocabulary > 28672 && a.vocabulary <= 4 * kPart16) rc = launch16_of<T, 4>(a, false, s);
-  if (rc == -1 && a.vocabulary > 53248 && a.vocabulary <= 2 * kPart16) rc = launch16_of<T, 2>(a, false, s);
-  return rc == -1 ? launch16_of<T, 1>(a, true, s) : rc;
+  const SampleClusters c = sample_clusters_16(a.vocabulary, a.rows, kPart16, [](int ctas) { return ctas == 8 ? fits16<T, 8>() : ctas == 4 ? fits16<T, 4>() : ctas == 2 ? fits16<T, 2>() : fits16<T, 1>(); });
+  auto go = [&](auto of) {                       // as many clusters as run at once; each takes rows in turn
+    constexpr int C = decltype(of)::value;
+    return launch_dependent(sample16_kernel<T, C, threads16<C>()>, dim3(unsigned(std::min<int64_t>(a.rows, c.at_once) * C)), threads16<C>(), sizeof(Shared16), C, s, a);
+  };
+  switch (c.ctas) {
+    case 8: return go(std::integral_constant<int, 8>{});
+    case 4: return go(std::integral_constant<int, 4>{});
+    case 2: return go(std::integral_constant<int, 2>{});
+    case 1: return go(std::integral_constant<int, 1>{});
+    default: return RC_LAUNCH;
+  }
 }
 
-// As many CTAs a row as let all rows' run at once, of 1024 values at least, and no fewer than hold a row.  Measured (1, 2, 4, 8 CTAs; us): 50001 values of one row -, 38, 28, 23, of 18 rows -, 40, 29, 44, of
-// 256 -, 150, 215, 370; 20000 values of one row 31, 25, 21, 20, of 74 33, 27, 58, 90; 300 of one row 12.1, 13.6, 14.1, 14.6.
-static int launch32(const Args& a, int64_t rows, cudaStream_t s) {
+static int launch32(const Args& a, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
-  static std::atomic<int> known[4][64];
+  static std::atomic<int> known[9][64];
   if (int rc = allow_shared(sample32_kernel, sizeof(Shared32), done)) return rc;
-  int least = 0, log2 = 3;
-  while (least < 3 && (a.vocabulary + (1 << least) - 1) >> least > kPart32) ++least;
-  for (; log2 > least; --log2) {
-    const int clusters = clusters_of(sample32_kernel, 1 << log2, kThreads, sizeof(Shared32), known[log2]);
-    if (clusters <= 0) return RC_LAUNCH;
-    if (rows <= clusters && a.vocabulary >> log2 > 1024) break;
-  }
-  return launch_dependent(sample32_kernel, dim3(unsigned(rows << log2)), kThreads, sizeof(Shared32), 1u << log2, s, a);
+  const SampleClusters c = sample_clusters_32(a.vocabulary, a.rows, kPart32, [](int ctas) { return clusters_of(sample32_kernel, ctas, kThreads, sizeof(Shared32), known[ctas]); });
+  if (c.ctas == 0) return RC_LAUNCH;
+  return launch_dependent(sample32_kernel, dim3(unsigned(a.rows * c.ctas)), kThreads, sizeof(Shared32), unsigned(c.ctas), s, a);
 }
 
 }  // namespace choice
@@ -1178,7 +1173,7 @@ int sample(const void* logits, int64_t row_stride, int dtype, int rows, int voca
   switch (dtype) {
     case DINO_F16: return launch16<__half>(a, s);
     case DINO_BF16: return launch16<__nv_bfloat16>(a, s);
-    default: return launch32(a, rows, s);
+    default: return launch32(a, s);
   }
 }
 
