@@ -11,12 +11,16 @@ struct SampleClusters {
 
 // fits(c): clusters of c CTAs that run at once on the device: 0 where not one does (a part of a GPU may have fewer SMs together), negative where that could not be found out.
 
-// 16-bit logits.  Several CTAs a row where all rows' run at once: their meetings cost what they save of a short row, or with two CTAs of a middling one.  Measured (1, 2, 4, 8 CTAs; one row, us):
-// 128256 bfloat16 25.1, 20.0, 15.4, 13.6, 32000 13.2, 14.6, 13.1, 12.9, 12000 10.6, 12.6, 11.8, 12.1; 128256 values of 36 rows 28.5, 22.3, 29.7 (36 clusters of four do not run at once), 42;
-// 100 rows 27.9, 41, 60, 94.
+// 16-bit logits.  Several CTAs a row where all rows' run at once: their meetings cost what they save of a short row.  Measured (bfloat16, top_p, us a launch; 1, 2, 4, 8 CTAs a row):
+//   one row of 20000 11.2, 12.8, 11.8, 12.0; 24000 12.6, 14.4, 13.0, 12.8; 28672 13.1, 14.7, 13.3, 13.0; 40000 12.9, 13.9, 12.0, 12.2; 128256 23.5, 19.2, 15.3, 13.6
+//   33 rows of 24000 12.9, 14.4, 13.2, -; 28672 13.8, 14.9, 13.6, -; 40000 14.6, 15.6, 13.7, -; 128256 27.5, 22.3, 16.1, 40.5 (clusters of eight run in three turns then)
+//   74 rows of 45056 15.7, 16.7, -, -; 48000 16.5, 16.5; 50257 18.1, 17.6; 56000 18.1, 17.4; 128256 28.4, 23.0, 46.5, 67.9
+// So four and eight from 28672 on, two where one CTA would count in a second turn (8 * 6144 values).
+// A part holds no more values than a 16-bit count: two parts end at 131056, four at 262112, and behind that fewer rows run with several CTAs (40 rows of 128256 22.2, of 131072 27.5, of 151936
+// 30.8; 20 rows of 262112 21.8, of 262144 46.9).
 template <typename Fits> inline SampleClusters sample_clusters_16(int vocabulary, int64_t rows, int part, Fits fits) {
   for (int ctas = 8; ctas > 1; ctas /= 2) {
-    if (vocabulary <= (ctas == 2 ? 53248 : 28672) || vocabulary > int64_t(ctas) * part) continue;
+    if (vocabulary <= (ctas == 2 ? 49152 : 28672) || vocabulary > int64_t(ctas) * part) continue;
     const int64_t n = fits(ctas);
     if (n < 0) return {0, 0};
     if (rows <= n) return {ctas, n};

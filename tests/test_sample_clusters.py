@@ -30,6 +30,7 @@ int main() {
   };
   // the whole device, as before
   assert(of16(whole, 128256, 1) == 8 && of16(whole, 128256, 17) == 8 && of16(whole, 128256, 18) == 4 && of16(whole, 128256, 36) == 2 && of16(whole, 128256, 75) == 1);
+  assert(of16(whole, 28672, 1) == 1 && of16(whole, 28680, 1) == 8 && of16(whole, 49152, 74) == 1 && of16(whole, 50257, 74) == 2 && of16(whole, 131056, 74) == 2 && of16(whole, 131072, 74) == 1);
   assert(of16(whole, 12000, 1) == 1 && of16(whole, 262144, 18) == 1 && of16(whole, 262112, 18) == 4);
   assert(of32(whole, 50001, 7) == 8 && of32(whole, 50001, 18) == 4 && of32(whole, 50001, 256) == 2 && of32(whole, 300, 1) == 1 && of32(whole, 262144, 500) == 8);
   // a part of one
