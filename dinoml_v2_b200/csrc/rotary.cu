@@ -3,7 +3,7 @@
 // t = x / sqrt(mean(x^2) + eps) * w over a head, then pairs (a, b) -> m (a cos - b sin, b cos + a sin), the angle position * frequency.  A value is read and written once: bound by
 // bytes, a single token by its chain of reads (position, angle, result).  A lane has P pairs of a head, the two halves of a pair in one register file: 16 bytes of a from the first half
 // and 16 of b from the second (or 32 bytes in one piece where neighbours are pairs), so that neither the norm (a sum over the lanes of a head) nor the rotation needs shared memory.
-// The angles are a row's, not a head's: a CTA has some rows and reduces each of their angles once, in float64 (131072 radians in float32 are 0.008 off), to half turns in [-1, 1], whose sine
+// The angles are a row's, not a head's: a CTA has some rows and reduces each of their angles once, the float64 product without a further loss (131072 radians in float32 are 0.008 off), to half turns in [-1, 1], whose sine
 // and cosine in float32 all heads share; a warp then has the same heads of all of these rows, their weights in registers and the next rows' values under way.
 // 2048 rows of 32 and 8 heads of 128, bfloat16 with norms: 8.7 us one after the other (42 MB, 4.8 TB/s), a row 2.5 us (launch and chain); a warp for a row and its angles 17, a CTA for a row 22.
 // What is left is instructions: 265 for four heads of a row and warp, a third of them conversions and pairs of registers.
@@ -206,8 +206,10 @@ __global__ void __launch_bounds__(32 * kWarps, N == 1 && WIDE ? 2 : 1) rotary_ke
           const int position = g.positions[tile + r];
           if (p == 0) place[r] = position;
           if (p >= g.pairs) continue;
-          // half turns in [-1, 1], in two floats: the second is a rounding's rest, by which sine and cosine are moved to first order
-          const double all = double(position) * g.frequencies[p] * 0.15915494309189533577, part = 2. * (all - rint(all));
+          // Turns by 1 / (2 pi) in two parts and the product's rounding: of an angle of 2^31 the turns alone would be 2^-22 off.  Then half turns in [-1, 1], in two floats: the second is a
+          // rounding's rest, by which sine and cosine are moved to first order.  (A product that is not fused into the difference: its rounding is what `rest` has.)
+          const double angle = double(position) * g.frequencies[p], all = __dmul_rn(angle, 0.15915494309189533577), rest = ::fma(angle, -9.839338337591243e-18, ::fma(angle, 0.15915494309189533577, -all));
+          const double part = 2. * (all - rint(all) + rest);
           const float high = float(part), low = float(part - double(high)) * 3.14159265358979f;
           float sin, cos;
           sincospif(high, &sin, &cos);

@@ -97,8 +97,8 @@ typedef struct DinoB200Heads {
 } DinoB200Heads;
 
 /* t = x / sqrt(mean(x^2) + eps) * weight over each head (weight null: t = x); pairs of its first 2 `pairs` values are turned by the angle positions[row] * frequencies[i]:
- * (a, b) -> magnitude * (a cos - b sin, b cos + a sin), pair i being (i, i + pairs), or with interleaved != 0 (2 i, 2 i + 1); the others stay.  The angle is float64 and so
- * exact to 2^-30 at any position, the rest float32 with one rounding at the end.  k null: q alone.  head_dim is even, 512 at most.  A row at a negative position is nobody's: left as it
+ * (a, b) -> magnitude * (a cos - b sin, b cos + a sin), pair i being (i, i + pairs), or with interleaved != 0 (2 i, 2 i + 1); the others stay.  The angle is that
+ * product in float64, its turns reduced to 2^-50 of one at any position; the rest is float32 with one rounding at the end.  k null: q alone.  head_dim is even, 512 at most.  A row at a negative position is nobody's: left as it
  * was where out is x, else zero.  weight_dtype: float32 or `dtype`. */
 DINOML_B200_API int dinoml_b200_rotary(const DinoB200Heads* q, const DinoB200Heads* k, const int* positions, const double* frequencies, int pairs, int dtype,
                                        int weight_dtype, int rows, int head_dim, float eps, float magnitude, int interleaved, void* stream);
