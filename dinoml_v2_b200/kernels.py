@@ -493,22 +493,24 @@ def rotary_frequencies(dim: int, base: float = 10000.0, *, scale: float = 1.0, f
 
 
 def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two [rows, heads, head_dim] tensors share no memory, as far as their strides tell: other storages, one behind the other, or other columns of rows that are equally far apart."""
-    if not a.numel() or not b.numel() or a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
+    """Whether two [rows, heads, head_dim] tensors of one dtype share no memory, as far as their addresses and strides tell: one behind the other, or other columns of rows that are equally far
+    apart.  (Their storages may be two over one memory.)"""
+    if not a.numel() or not b.numel():
         return True
+    size = a.element_size()
 
-    def inside(t):                                                                        # values from a row's first to behind its last
-        return (t.shape[1] - 1) * t.stride(1) + t.shape[2]
+    def inside(t):                                                                        # bytes from a row's first value to behind its last
+        return ((t.shape[1] - 1) * t.stride(1) + t.shape[2]) * size
 
     def behind(t):
-        return t.storage_offset() + (t.shape[0] - 1) * t.stride(0) + inside(t)
+        return t.data_ptr() + (t.shape[0] - 1) * t.stride(0) * size + inside(t)
 
-    if behind(a) <= b.storage_offset() or behind(b) <= a.storage_offset():
+    if behind(a) <= b.data_ptr() or behind(b) <= a.data_ptr():
         return True
-    pitch = a.stride(0)
-    if a.shape[0] < 2 or b.stride(0) != pitch or max(inside(a), inside(b)) > pitch:
+    pitch = a.stride(0) * size
+    if a.shape[0] < 2 or b.stride(0) != a.stride(0) or max(inside(a), inside(b)) > pitch:
         return False
-    gap = (b.storage_offset() - a.storage_offset()) % pitch
+    gap = (b.data_ptr() - a.data_ptr()) % pitch
     return gap >= inside(a) and pitch - gap >= inside(b)
 
 
