@@ -42,7 +42,7 @@ template <int QT, typename T> constexpr int items_per_thread() { return QT == QT
 // The other types with odd blocks have shorter pieces and lose by it: Q8_0 f16 23.4 -> 24.5, Q3_K 19.3 -> 20.7, MXFP4 19.2 -> 20.9, Q4_0 equal.
 template <int QT, typename T, int A>
 __global__ void __launch_bounds__(kDequantThreads)
-dequant_kernel(const uint8_t* __restrict__ in, T* __restrict__ out, int64_t total_items, int64_t first_edge, int64_t last_edge, bool wide) {
+dequant_kernel(const uint8_t* in, T* __restrict__ out, int64_t total_items, int64_t first_edge, int64_t last_edge, bool wide) {
   using G = ItemGeom<QT, run_of<QT, T>()>;
   constexpr int kPer = items_per_thread<QT, T>();
   asm volatile("griddepcontrol.wait;\n" ::: "memory");          // the packed bytes may be the preceding kernel's output
@@ -56,7 +56,7 @@ dequant_kernel(const uint8_t* __restrict__ in, T* __restrict__ out, int64_t tota
 #pragma unroll
     for (int i = 0; i < (kVec + kDequantThreads - 1) / kDequantThreads; ++i) {
       const int at = i * kDequantThreads + threadIdx.x;
-      if (at < vecs) *reinterpret_cast<uint4*>(stage + 16 * at) = __ldg(reinterpret_cast<const uint4*>(src) + at);
+      if (at < vecs) *reinterpret_cast<uint4*>(stage + 16 * at) = reinterpret_cast<const uint4*>(src)[at];
     }
     for (int at = 16 * vecs + threadIdx.x; at < bytes; at += kDequantThreads) stage[at] = src[at];
     __syncthreads();

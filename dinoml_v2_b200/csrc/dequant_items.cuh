@@ -19,15 +19,17 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8], bool wi
   }
 }
 
+// Packed bytes are read as any others, not as constant data: both kernels are resident while the launch before them may still write the bytes, and wait for it first.
+// (As constant data the same times; the embedding's 8192 rows of 8192 NVFP4 to float32 60 us, 64 so.)
 // N words of packed bytes from p.  A: alignment of p.  1: any address; the aligned words around p are shifted into place, except where
 // `edge` says that such a word holds bytes outside the buffer.  0: any address in shared memory (with four bytes after the last).
 template <int N, int A>
-__device__ __forceinline__ void load_words(const uint8_t* __restrict__ p, bool edge, uint32_t (&v)[N]) {
+__device__ __forceinline__ void load_words(const uint8_t* p, bool edge, uint32_t (&v)[N]) {
   if constexpr (A == 16 && N == 4) {
-    const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint4 q = *reinterpret_cast<const uint4*>(p);
     v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
   } else if constexpr (A == 16 && N == 2) {
-    const uint2 q = __ldg(reinterpret_cast<const uint2*>(p));
+    const uint2 q = *reinterpret_cast<const uint2*>(p);
     v[0] = q.x; v[1] = q.y;
   } else if constexpr (A == 0) {
     const int off = int(__cvta_generic_to_shared(p)) & 3;
@@ -39,7 +41,7 @@ __device__ __forceinline__ void load_words(const uint8_t* __restrict__ p, bool e
     for (int i = 0; i < N; ++i) v[i] = __funnelshift_r(r[i], r[i + 1], 8 * off);
   } else if constexpr (A >= 4) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
+    for (int i = 0; i < N; ++i) v[i] = reinterpret_cast<const uint32_t*>(p)[i];
   } else {
     if (edge) {
 #pragma unroll
@@ -51,8 +53,8 @@ __device__ __forceinline__ void load_words(const uint8_t* __restrict__ p, bool e
     const uint32_t* w = reinterpret_cast<const uint32_t*>(p - off);
     uint32_t r[N + 1];
 #pragma unroll
-    for (int i = 0; i < N; ++i) r[i] = __ldg(w + i);
-    r[N] = off ? __ldg(w + N) : 0u;
+    for (int i = 0; i < N; ++i) r[i] = w[i];
+    r[N] = off ? w[N] : 0u;
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = __funnelshift_r(r[i], r[i + 1], 8 * off);
   }
@@ -97,7 +99,7 @@ template <int QT, typename T, int A> struct Item {
   static constexpr bool kHigh = QT == QTYPE_Q5_K || QT == QTYPE_Q6_K || QT == QTYPE_Q3_K;
   uint32_t q[kQ], h[kHigh ? N : 1], s[4];
 
-  __device__ __forceinline__ void load(const uint8_t* __restrict__ b, int item, bool edge) {
+  __device__ __forceinline__ void load(const uint8_t* b, int item, bool edge) {
     if constexpr (QT == QTYPE_Q4_0) {
       s[0] = uint32_t(b[0]) | uint32_t(b[1]) << 8;
       load_words<N, A>(b + 2 + R * item, edge, q);
