@@ -6,7 +6,8 @@
 // The angles are a row's, not a head's: a CTA has some rows and reduces each of their angles once, the float64 product without a further loss (131072 radians in float32 are 0.008 off), to half turns in [-1, 1], whose sine
 // and cosine in float32 all heads share; a warp then has the same heads of all of these rows, their weights in registers and the next rows' values under way.
 // 2048 rows of 32 and 8 heads of 128, bfloat16 with norms: 8.7 us one after the other (42 MB, 4.8 TB/s), a row 2.5 us (launch and chain); a warp for a row and its angles 17, a CTA for a row 22.
-// What is left is instructions: 265 for four heads of a row and warp, a third of them conversions and pairs of registers.
+// What is left is latency: twenty warps an SM (96 registers a thread), each with a chain of 265 instructions for four heads of a row, a third of them conversions and pairs of registers, keep
+// the issue slots half busy.
 #include <algorithm>
 
 #include "dependent_launch.cuh"

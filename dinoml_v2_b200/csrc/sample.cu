@@ -12,7 +12,8 @@
 // first CTA alone where these are few.
 //
 // A row is a cluster's, of up to eight CTAs while there are fewer rows than SMs: its CTAs have parts of it, the first one finds the places.  Bound by latency there: one row of 128256 bfloat16
-// with top-k and top-p 14.0 us, of which the CTAs' meetings and their reads of one another's counts are half; seven rows of 50001 float32 16.5 us; 64 rows of
+// with top-k and top-p 14.0 us, 12 of them behind the launch: counting 1.4, bitmaps and the first meeting 1.8, reads of one another's counts 2.0, powers and sums 0.7, the second meeting, which
+// waits for the slowest CTA, 2.0, running sums 0.9, places 2.6, the last meeting 0.5, the rest the search.  Seven rows of 50001 float32 16.2 us; 64 rows of
 // 128256 with settings of their own 21.7 us.  256 rows of 128256 float16 51 us (66 MB, 1.3 TB/s), two rows a CTA: of 25 us a row counting takes 12 (its atomics meet on random banks, 3.5
 // wavefronts for 32), the sums 5, the places 2, the search 4.
 #include <cooperative_groups.h>
