@@ -32,7 +32,9 @@ class Request(NamedTuple):
 def tokens_of_rows(step: kernels.KVStep, new: torch.Tensor, packed: torch.Tensor) -> torch.Tensor:
     """The token of each row of a step, -1 of nobody's: `packed` has new[b] tokens of every sequence one after the other, the step only the rows of sequences that got theirs, so that a
     sequence behind one that went without begins earlier there."""
-    row = torch.arange(len(packed), dtype=torch.int32, device=packed.device)
+    if not len(packed):
+        return torch.full_like(step.positions, -1)
+    row = torch.arange(len(step.positions), dtype=torch.int32, device=packed.device)
     b = torch.searchsorted(step.starts[1:].contiguous(), row, right=True).clamp(max=len(new) - 1)
     source = (new.cumsum(0) - new)[b] + row - step.starts[b]
     return torch.where(step.positions >= 0, packed[source.clamp(max=len(packed) - 1)], -1).to(packed.dtype)

@@ -48,6 +48,15 @@ def test_tokens_reach_their_sequences(blocks, sequences, columns, held, new, fit
     assert _reached(rows, starts.tolist(), positions.tolist()) == [[1000 * b + i for i in range(n)] if ok else [] for b, (n, ok) in enumerate(zip(new, fits))]
 
 
+def test_rows_to_spare():
+    model = E.Pool(20, 2, 8, 16)
+    step = kernels.KVStep(*(torch.tensor(t, dtype=torch.int32) for t in model.step([200, 3], 210)))
+    rows = _example().tokens_of_rows(step, torch.tensor([200, 3], dtype=torch.int32), torch.tensor(_packed([200, 3]), dtype=torch.int32))
+    assert rows.tolist() == [1000, 1001, 1002] + [-1] * 207
+    step = kernels.KVStep(*(torch.tensor(t, dtype=torch.int32) for t in model.step([0, 0], 4)))
+    assert _example().tokens_of_rows(step, torch.zeros(2, dtype=torch.int32), torch.zeros(0, dtype=torch.int32)).tolist() == [-1] * 4
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("blocks,sequences,columns,held,new,fits", CASES)
 def test_tokens_reach_their_sequences_on_the_device(blocks, sequences, columns, held, new, fits):
